@@ -23,7 +23,9 @@
  *     are the only blocking calls.
  *   - all tensors are dense row-major; float tensors are IEEE fp32,
  *     index tensors int32 (the runner clips ONNX int64 to int32:
- *     src/descriptor_runner/core/runnerImpl.ts:167-198).
+ *     src/descriptor_runner/core/runnerImpl.ts:167-198); the 8-bit serving
+ *     operators at the end of this file also take e4m3 tensors, a byte an
+ *     element.
  *   - strides are in ELEMENTS, not bytes.
  *   - the library is not re-entrant: call it from one thread at a time
  *     (the descriptor runner is single-threaded:
@@ -198,6 +200,11 @@ int wdh_read(wdh_buf h, size_t src_offset, void *dst, size_t bytes);
  * src/shader/wasm/src/kernels/standard/copy.cpp:6-8. */
 int wdh_copy(wdh_buf dst, size_t dst_offset, wdh_buf src, size_t src_offset,
              size_t bytes);
+/* The device address of a buffer, for programs that read or fill it with other libraries of the same process (a
+ * torch tensor over it, say).  The library's work runs on streams of its own: wdh_sync before others read what it
+ * wrote, and other streams' writes have to be over before a call of this library uses them.  The address is valid
+ * until wdh_free.  No counterpart in the reference. */
+int wdh_address(wdh_buf h, uint64_t *address);
 /* Waits for the work of the current lane (see wdh_set_lane). */
 int wdh_sync(void);
 
@@ -468,6 +475,63 @@ int wdh_gather(wdh_buf Data, wdh_buf Indices, wdh_buf Y, int64_t outer,
 int wdh_strided_copy(wdh_buf X, int64_t x_offset, wdh_buf Y, int64_t y_offset,
                      int ndim, const int32_t *shape, const int64_t *x_strides,
                      const int64_t *y_strides);
+
+/* ---- 8-bit serving of language models -------------------------------------
+ * No counterpart in the reference, whose operators are fp32 only.  Activations, the residual stream and all results
+ * are fp32; what large products and attention read is held in e4m3: 8-bit floating point with 4 exponent and 3 fraction
+ * bits as the OCP specification and ONNX FLOAT8E4M3FN define it (largest value 448, no infinities, NaN = 0x7f or 0xff).
+ * An element stands for its e4m3 value times the scale of its block.  Rounding is to nearest even; a block's scale
+ * follows its finite elements, and what is not finite is held as NaN.  All of them can be recorded (wdh_graph_begin);
+ * Table, Lens and Starts are read on the device, so that a replay may find other sequences in them.
+ * Results of a call do not depend on anything but its operands: no atomics, fixed orders of addition. */
+#define WDH_FP8_BLOCK 128   /* elements along a row that share a scale  */
+#define WDH_CACHE_PAGE 64   /* tokens of a page of the cache            */
+
+/* Root-mean-square normalisation of `outer` rows of `len` elements:
+ *   s = X (+ Skip);  y = s / sqrt(mean(s^2) + eps) (* Gamma)
+ * Sum (0 = not wanted) gets s, Y (or 0) gets y; Q and QScale (both or neither) get y in e4m3 [outer, len] with scales
+ * [outer, ceil(len / 128)]: scale = max(largest finite |y| of the block / 448, 2^-100).  At least one of Y and Q.
+ * Skip and Gamma may be 0.  Sum may be X or Skip itself (the residual stream updated in place); no other result may share
+ * a buffer with an operand.  Replaces, in one pass, Add + the ONNX RMSNormalization chain (binary7.ts:24-75,
+ * reduce.ts:369-405) and the quantisation behind it.  len <= 2^30. */
+int wdh_rmsnorm(wdh_buf X, wdh_buf Skip, wdh_buf Gamma, wdh_buf Sum, wdh_buf Y, wdh_buf Q, wdh_buf QScale,
+                int64_t outer, int len, float eps);
+/* X [rows, cols] to e4m3: Q [rows, cols], QScale [ceil(rows / block_rows), ceil(cols / 128)] with scales as above for
+ * blocks of block_rows x 128.  block_rows: 1 (activations, what wdh_gemm_fp8 takes as A) or 128 (weights, its W). */
+int wdh_quantize_fp8(wdh_buf X, wdh_buf Q, wdh_buf QScale, int64_t rows, int cols, int block_rows);
+/* Y[i, j] = sum_b AScale[i, b] WScale[j / 128, b] sum_{x in block b} A[i, x] W[j, x]  (+ Bias[j]) (+ R[i, j]), then the
+ * epilogue.  A [m, k] and W [n, k] are e4m3, both with k contiguous; scales [m, ceil(k/128)] and [ceil(n/128), ceil(k/128)]
+ * are any fp32 numbers.  Bias and R may be 0; R may be Y.  Sums are held in fp32.  k = 0 leaves Bias and R. */
+int wdh_gemm_fp8(wdh_buf A, wdh_buf AScale, wdh_buf W, wdh_buf WScale, wdh_buf Bias, wdh_buf Y, int64_t m, int n, int k,
+                 int epilogue, wdh_buf R);
+
+/* The cache: KPages [pages, kv_heads, 64, d] and VPages [pages, kv_heads, d, 64] in e4m3, KScales and VScales
+ * [pages, kv_heads] in fp32; d = 32, 64 or 128.  Table [seqs, max_pages]: the page of each 64 tokens of a sequence; Lens
+ * [seqs]: how many tokens a sequence has, those of this call counted; Starts [seqs + 1]: rows Starts[s] .. Starts[s+1]-1 of
+ * the call's `tokens` rows are sequence s's last tokens, in order.  All int32 on the device.  A sequence whose numbers do not
+ * fit (rows outside the call, more rows than tokens, more tokens than max_pages hold) is left out as one without rows is.
+ * Rows of K, V and Q are `stride` elements apart from element `offset` of their buffer on (both multiples of 4): the
+ * three parts of one projection's result can be read where they are.
+ *
+ * Appending: new tokens go behind the earlier ones, keys and values each with the least power of two c >= 2^-100 as scale
+ * that holds the page's largest finite element (<= 448 c); where a page held earlier tokens, their scale only grows, and they
+ * are rounded again to the new one (exact but for values that become subnormal).  Slots behind the last token and pages that
+ * no new token lies on are left as they are; a page number outside the cache is skipped.  Two sequences of a call must
+ * not append to the same page (they may share full pages of a common prefix). */
+int wdh_cache_append(wdh_buf K, int64_t k_offset, int64_t k_stride, wdh_buf V, int64_t v_offset, int64_t v_stride,
+                     wdh_buf KPages, wdh_buf KScales, wdh_buf VPages, wdh_buf VScales, wdh_buf Table, wdh_buf Lens,
+                     wdh_buf Starts, int seqs, int tokens, int kv_heads, int d, int pages, int max_pages);
+/* Attention over the cache: for each row of the call (heads queries of d elements, kv_heads of the cache shared by
+ * heads / kv_heads neighbouring queries each)
+ *   Y[row, h] = sum_j softmax_j(alpha q.k_j) v_j  over the tokens j of its sequence up to and with the row's own,
+ * which wdh_cache_append has to have written before.  Prompts, parts of prompts and single tokens may be mixed in a call.
+ * Y [tokens, heads * d] is dense; rows that belong to no sequence are left as they are.  A token on a page whose number is
+ * outside the cache makes the rows that see it NaN; slots behind a sequence's tokens and tokens behind a row do not touch
+ * it, whatever they hold.  Where one call's rows do not fill the chip the tokens are cut into parts whose results are
+ * joined by a second launch, in a workspace from the pool. */
+int wdh_cache_attention(wdh_buf Q, int64_t q_offset, int64_t q_stride, wdh_buf KPages, wdh_buf KScales, wdh_buf VPages,
+                        wdh_buf VScales, wdh_buf Table, wdh_buf Lens, wdh_buf Starts, wdh_buf Y, int seqs, int tokens,
+                        int heads, int kv_heads, int d, int pages, int max_pages, float alpha);
 
 #ifdef __cplusplus
 }

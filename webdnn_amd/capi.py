@@ -33,6 +33,7 @@ SIGNATURES = {
     "wdh_write": (_c.c_int, [c_buf, _c.c_size_t, _c.c_void_p, _c.c_size_t]),
     "wdh_read": (_c.c_int, [c_buf, _c.c_size_t, _c.c_void_p, _c.c_size_t]),
     "wdh_copy": (_c.c_int, [c_buf, _c.c_size_t, c_buf, _c.c_size_t, _c.c_size_t]),
+    "wdh_address": (_c.c_int, [c_buf, _u64p]),
     "wdh_sync": (_c.c_int, []),
     "wdh_set_lane": (_c.c_int, [_c.c_int]),
     "wdh_branch_begin": (_c.c_int, []),
@@ -76,6 +77,11 @@ SIGNATURES = {
     "wdh_gather": (_c.c_int, [c_buf, c_buf, c_buf, _c.c_int64, _c.c_int, _c.c_int64, _c.c_int64]),
     "wdh_cast": (_c.c_int, [_c.c_int, _c.c_int, c_buf, c_buf, _c.c_size_t]),
     "wdh_strided_copy": (_c.c_int, [c_buf, _c.c_int64, c_buf, _c.c_int64, _c.c_int, _i32p, _i64p, _i64p]),
+    "wdh_rmsnorm": (_c.c_int, [c_buf] * 7 + [_c.c_int64, _c.c_int, _c.c_float]),
+    "wdh_quantize_fp8": (_c.c_int, [c_buf, c_buf, c_buf, _c.c_int64, _c.c_int, _c.c_int]),
+    "wdh_gemm_fp8": (_c.c_int, [c_buf] * 6 + [_c.c_int64, _c.c_int, _c.c_int, _c.c_int, c_buf]),
+    "wdh_cache_append": (_c.c_int, [c_buf, _c.c_int64, _c.c_int64, c_buf, _c.c_int64, _c.c_int64] + [c_buf] * 7 + [_c.c_int] * 6),
+    "wdh_cache_attention": (_c.c_int, [c_buf, _c.c_int64, _c.c_int64] + [c_buf] * 8 + [_c.c_int] * 7 + [_c.c_float]),
 }
 
 

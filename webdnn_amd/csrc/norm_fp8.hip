@@ -1,0 +1,269 @@
+// Root-mean-square normalisation of rows (with the residual's addition before it and an 8-bit output behind it) and
+// quantisation to e4m3 in blocks.
+//
+// The reference has no such operators; in its terms the first is the chain Add, Mul, ReduceMean, Add, Sqrt, Div, Mul
+// (src/descriptor_runner/operators/cpu/operators/standard/binary7.ts:24-75, reduce.ts:369-405, unary.ts:10-32):
+//   s = x + r,  y = (s * t) * g  with  t = 1 / sqrt(mean(s^2) + eps).
+// Squares are summed in double (a row of values near 1e20 keeps a finite mean), t is rounded to fp32 once.
+// 8 bits: c = max(largest finite |y| of a block / 448, 2^-100), q = e4m3(y * (1/c)).
+//
+// Bound: memory.  Every element is read once and written once: a row stays in registers between its sum and its use.
+#include "common.h"
+#include "fastdiv.h"
+#include "fp8.h"
+
+namespace {
+
+using namespace wdh::fp8;
+
+struct NormParams {
+  const float *X, *R, *G;
+  float *S, *Y;
+  unsigned char *Q;
+  float *QS;
+  long long outer;
+  int len, blocks;
+  float eps;
+};
+
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// One piece (elements idx .. idx+3 of `row`) on its way out; the 32 lanes of a half wavefront hold the 128 elements of a block.
+__device__ __forceinline__ void finish_piece(const NormParams &p, long long row, int idx, bool live, float t, f32x4 v, f32x4 g) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = v[e] * t;
+  if (p.G)
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = v[e] * g[e];
+  if (p.Y && live) store4(p.Y + row * p.len, idx, p.len, v);
+  if (!p.Q) return;
+  float amax = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) amax = fmaxf(amax, idx + e < p.len ? finite_abs(v[e]) : 0.0f);
+  const float c = block_scale(half_max(amax));
+  if (!live) return;
+  store4_bytes(p.Q + row * p.len, idx, p.len, pack4(v, 1.0f / c));
+  if ((threadIdx.x & 31) == 0 && idx < p.len) p.QS[row * p.blocks + idx / BLOCK] = c;
+}
+
+// WAVES wavefronts to a row, NP pieces of four elements to a lane: a row of up to 256 * WAVES * NP elements in registers.
+template <int WAVES, int NP>
+__global__ __launch_bounds__(256) void rmsnorm_rows(NormParams p) {
+  constexpr int ROWS = 4 / WAVES;
+  __shared__ double part[4];
+  const int wave = threadIdx.x >> 6, t = threadIdx.x % (64 * WAVES);
+  for (long long row0 = (long long)blockIdx.x * ROWS; row0 < p.outer; row0 += (long long)gridDim.x * ROWS) {
+    const bool live = row0 + wave / WAVES < p.outer;
+    const long long row = live ? row0 + wave / WAVES : p.outer - 1;  // idle wavefronts repeat the last row and store nothing
+    const float *x = p.X + row * p.len;
+    f32x4 v[NP], g[NP];
+#pragma unroll
+    for (int i = 0; i < NP; i++) v[i] = load4(x, 4 * (t + 64 * WAVES * i), p.len);
+    if (p.R) {
+      const float *r = p.R + row * p.len;
+      f32x4 w[NP];
+#pragma unroll
+      for (int i = 0; i < NP; i++) w[i] = load4(r, 4 * (t + 64 * WAVES * i), p.len);
+#pragma unroll
+      for (int i = 0; i < NP; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[i][e] = v[i][e] + w[i][e];
+    }
+#pragma unroll
+    for (int i = 0; i < NP; i++) g[i] = p.G ? load4(p.G, 4 * (t + 64 * WAVES * i), p.len) : f32x4{1.f, 1.f, 1.f, 1.f};
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < NP; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum = fma((double)v[i][e], (double)v[i][e], sum);
+    sum = wave_sum_d(sum);
+    if constexpr (WAVES > 1) {
+      if ((threadIdx.x & 63) == 0) part[wave] = sum;
+      __syncthreads();
+      sum = ((part[0] + part[1]) + part[2]) + part[3];
+      __syncthreads();  // (the next row's sums go to the same places)
+    }
+    const float inv = (float)(1.0 / sqrt(sum / (double)p.len + (double)p.eps));
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int idx = 4 * (t + 64 * WAVES * i);
+      if (p.S && live) store4(p.S + row * p.len, idx, p.len, v[i]);
+      finish_piece(p, row, idx, live, inv, v[i], g[i]);
+    }
+  }
+}
+
+// Rows longer than the registers hold: a workgroup goes over its row twice.  (S may be X or R: a lane reads back its own sums.)
+__global__ __launch_bounds__(256) void rmsnorm_stream(NormParams p) {
+  __shared__ double part[4];
+  const int wave = threadIdx.x >> 6, t = threadIdx.x;
+  for (long long row = blockIdx.x; row < p.outer; row += gridDim.x) {
+    const float *x = p.X + row * p.len, *r = p.R ? p.R + row * p.len : nullptr;
+    auto piece = [&](int idx) {
+      f32x4 v = load4(x, idx, p.len);
+      if (r) {
+        const f32x4 w = load4(r, idx, p.len);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = v[e] + w[e];
+      }
+      return v;
+    };
+    double sum = 0.0;
+    for (long long idx = 4 * t; idx < p.len; idx += 1024) {
+      const f32x4 v = piece((int)idx);
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum = fma((double)v[e], (double)v[e], sum);
+      if (p.S) store4(p.S + row * p.len, idx, p.len, v);
+    }
+    sum = wave_sum_d(sum);
+    if ((threadIdx.x & 63) == 0) part[wave] = sum;
+    __syncthreads();
+    sum = ((part[0] + part[1]) + part[2]) + part[3];
+    __syncthreads();
+    const float inv = (float)(1.0 / sqrt(sum / (double)p.len + (double)p.eps));
+    for (long long idx0 = 0; idx0 < p.len; idx0 += 1024) {  // (whole wavefronts take part in a block's maximum)
+      const int idx = (int)(idx0 + 4 * t < p.len ? idx0 + 4 * t : (long long)p.len);
+      f32x4 v = {0.f, 0.f, 0.f, 0.f}, g = {1.f, 1.f, 1.f, 1.f};
+      if (idx < p.len) {
+        v = p.S ? load4(p.S + row * p.len, idx, p.len) : piece(idx);
+        if (p.G) g = load4(p.G, idx, p.len);
+      }
+      finish_piece(p, row, idx, idx < p.len, inv, v, g);
+    }
+  }
+}
+
+// A scale for each 1 x 128 block: half a wavefront to a block.
+constexpr int UNROLL = 4;  // blocks a half wavefront has in flight
+__global__ __launch_bounds__(256) void quantize_rows(const float *__restrict__ X, unsigned char *__restrict__ Q, float *__restrict__ QS, int cols,
+                                                     wdh::FastDiv blocks, long long units) {
+  const int sub = threadIdx.x & 31;
+  const long long unit0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * UNROLL;
+  f32x4 v[UNROLL];
+  long long at[UNROLL];
+  int idx[UNROLL];
+#pragma unroll
+  for (int j = 0; j < UNROLL; j++) {
+    const int unit = (int)(unit0 + j < units ? unit0 + j : units - 1), row = wdh::fdiv(unit, blocks);
+    idx[j] = (unit - row * blocks.d) * BLOCK + 4 * sub;
+    at[j] = (long long)row * cols;
+    v[j] = idx[j] < cols ? load4(X + at[j], idx[j], cols) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int j = 0; j < UNROLL; j++) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) amax = fmaxf(amax, finite_abs(v[j][e]));
+    const float c = block_scale(half_max(amax));
+    if (unit0 + j >= units) continue;
+    store4_bytes(Q + at[j], idx[j], cols, pack4(v[j], 1.0f / c));
+    if (sub == 0) QS[unit0 + j] = c;
+  }
+}
+
+// A scale for each 128 x 128 block: a workgroup to a block, which stays in registers.
+__global__ __launch_bounds__(256) void quantize_tiles(const float *__restrict__ X, unsigned char *__restrict__ Q, float *__restrict__ QS, long long rows,
+                                                      int cols, int blocks) {
+  __shared__ float part[4];
+  const long long br = blockIdx.x / blocks;
+  const int bc = (int)(blockIdx.x - br * blocks), idx = bc * BLOCK + 4 * (threadIdx.x & 31);
+  f32x4 v[16];
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const long long row = br * BLOCK + (threadIdx.x >> 5) + 8 * i;
+    v[i] = row < rows && idx < cols ? load4(X + row * cols, idx, cols) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; i++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) amax = fmaxf(amax, finite_abs(v[i][e]));
+  amax = wdh::rowmath::wave_max(amax);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = amax;
+  __syncthreads();
+  const float c = block_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))), inv = 1.0f / c;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const long long row = br * BLOCK + (threadIdx.x >> 5) + 8 * i;
+    if (row < rows) store4_bytes(Q + row * cols, idx, cols, pack4(v[i], inv));
+  }
+  if (threadIdx.x == 0) QS[blockIdx.x] = c;
+}
+
+}  // namespace
+
+using wdh::fail;
+
+extern "C" int wdh_rmsnorm(wdh_buf hX, wdh_buf hSkip, wdh_buf hGamma, wdh_buf hSum, wdh_buf hY, wdh_buf hQ, wdh_buf hQScale,
+                           int64_t outer, int len, float eps) {
+  WDH_REQUIRE_INIT();
+  WDH_REQUIRE_COMPUTE_LANE();
+  if (outer < 0 || len < 0) return fail(WDH_EINVAL, "wdh_rmsnorm: negative extent");
+  if (!hY && !hQ) return fail(WDH_EINVAL, "wdh_rmsnorm: neither Y nor Q given");
+  if (!hQ != !hQScale) return fail(WDH_EINVAL, "wdh_rmsnorm: Q and QScale go together");
+  if (!(eps >= 0.0f)) return fail(WDH_EINVAL, "wdh_rmsnorm: epsilon %g", (double)eps);
+  if (outer == 0 || len == 0) return WDH_OK;
+  if (len > (1 << 30) || outer > (1LL << 46) / len) return fail(WDH_EINVAL, "wdh_rmsnorm: too many elements");
+  const size_t count = (size_t)outer * len, blocks = ((size_t)len + BLOCK - 1) / BLOCK;
+  void *px, *pr = nullptr, *pg = nullptr, *ps = nullptr, *py = nullptr, *pq = nullptr, *pqs = nullptr;
+  if (!wdh::operand(hX, count * 4, "wdh_rmsnorm: X", &px)) return WDH_EINVAL;
+  if (hSkip && !wdh::operand(hSkip, count * 4, "wdh_rmsnorm: Skip", &pr)) return WDH_EINVAL;
+  if (hGamma && !wdh::operand(hGamma, (size_t)len * 4, "wdh_rmsnorm: Gamma", &pg)) return WDH_EINVAL;
+  if (hSum && !wdh::operand(hSum, count * 4, "wdh_rmsnorm: Sum", &ps)) return WDH_EINVAL;
+  if (hY && !wdh::operand(hY, count * 4, "wdh_rmsnorm: Y", &py)) return WDH_EINVAL;
+  if (hQ && !wdh::operand(hQ, count, "wdh_rmsnorm: Q", &pq)) return WDH_EINVAL;
+  if (hQScale && !wdh::operand(hQScale, (size_t)outer * blocks * 4, "wdh_rmsnorm: QScale", &pqs)) return WDH_EINVAL;
+  const wdh_buf out[4] = {hY, hQ, hQScale, hSum}, in[3] = {hX, hSkip, hGamma};
+  for (int i = 0; i < 4; i++) {
+    for (int j = 0; j < 3; j++)  // (a row is read whole before it is written, so the sum may take the place of X or Skip)
+      if (out[i] && out[i] == in[j] && !(i == 3 && j < 2)) return fail(WDH_EINVAL, "wdh_rmsnorm: a result aliases an input");
+    for (int j = 0; j < i; j++)
+      if (out[i] && out[i] == out[j]) return fail(WDH_EINVAL, "wdh_rmsnorm: two results share a buffer");
+  }
+  NormParams p;
+  p.X = (const float *)px; p.R = (const float *)pr; p.G = (const float *)pg; p.S = (float *)ps; p.Y = (float *)py;
+  p.Q = (unsigned char *)pq; p.QS = (float *)pqs;
+  p.outer = outer; p.len = len; p.blocks = (int)blocks; p.eps = eps;
+  hipStream_t st = wdh::stream();
+  const long long most = 1 << 20;  // (workgroups; more rows than that are taken in turns)
+  const long long quarters = (outer + 3) / 4;
+  const dim3 four((unsigned)(quarters < most ? quarters : most)), one((unsigned)(outer < most ? outer : most)), wg(256);
+  if (len <= 256) hipLaunchKernelGGL((rmsnorm_rows<1, 1>), four, wg, 0, st, p);
+  else if (len <= 512) hipLaunchKernelGGL((rmsnorm_rows<1, 2>), four, wg, 0, st, p);
+  else if (len <= 1024) hipLaunchKernelGGL((rmsnorm_rows<4, 1>), one, wg, 0, st, p);
+  else if (len <= 2048) hipLaunchKernelGGL((rmsnorm_rows<4, 2>), one, wg, 0, st, p);
+  else if (len <= 4096) hipLaunchKernelGGL((rmsnorm_rows<4, 4>), one, wg, 0, st, p);
+  else if (len <= 8192) hipLaunchKernelGGL((rmsnorm_rows<4, 8>), one, wg, 0, st, p);
+  else hipLaunchKernelGGL(rmsnorm_stream, one, wg, 0, st, p);
+  WDH_LAUNCH_CHECK();
+  return WDH_OK;
+}
+
+extern "C" int wdh_quantize_fp8(wdh_buf hX, wdh_buf hQ, wdh_buf hQScale, int64_t rows, int cols, int block_rows) {
+  WDH_REQUIRE_INIT();
+  WDH_REQUIRE_COMPUTE_LANE();
+  if (rows < 0 || cols < 0) return fail(WDH_EINVAL, "wdh_quantize_fp8: negative extent");
+  if (block_rows != 1 && block_rows != BLOCK)
+    return fail(WDH_EINVAL, "wdh_quantize_fp8: blocks of %d rows (1 and %d are built)", block_rows, BLOCK);
+  if (rows == 0 || cols == 0) return WDH_OK;
+  if (cols > (1 << 30) || rows > (1LL << 46) / cols) return fail(WDH_EINVAL, "wdh_quantize_fp8: too many elements");
+  const long long blocks = ((long long)cols + BLOCK - 1) / BLOCK, units = (rows + block_rows - 1) / block_rows * blocks;
+  if (units > (block_rows == 1 ? 0x7fffffffLL : 0xffffffffLL / 256)) return fail(WDH_EINVAL, "wdh_quantize_fp8: too many blocks");
+  void *px, *pq, *pqs;
+  if (!wdh::operand(hX, (size_t)rows * cols * 4, "wdh_quantize_fp8: X", &px)) return WDH_EINVAL;
+  if (!wdh::operand(hQ, (size_t)rows * cols, "wdh_quantize_fp8: Q", &pq)) return WDH_EINVAL;
+  if (!wdh::operand(hQScale, (size_t)units * 4, "wdh_quantize_fp8: QScale", &pqs)) return WDH_EINVAL;
+  if (hQ == hX || hQScale == hX || hQ == hQScale) return fail(WDH_EINVAL, "wdh_quantize_fp8: operands share a buffer");
+  if (block_rows == 1)
+    hipLaunchKernelGGL(quantize_rows, dim3((unsigned)((units + 8 * UNROLL - 1) / (8 * UNROLL))), dim3(256), 0, wdh::stream(), (const float *)px,
+                       (unsigned char *)pq, (float *)pqs, cols, wdh::make_fastdiv(blocks), units);
+  else
+    hipLaunchKernelGGL(quantize_tiles, dim3((unsigned)units), dim3(256), 0, wdh::stream(), (const float *)px, (unsigned char *)pq, (float *)pqs,
+                       (long long)rows, cols, (int)blocks);
+  WDH_LAUNCH_CHECK();
+  return WDH_OK;
+}

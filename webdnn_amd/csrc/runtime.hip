@@ -761,6 +761,15 @@ int wdh_copy(wdh_buf dst, size_t dst_offset, wdh_buf src, size_t src_offset,
   return WDH_OK;
 }
 
+int wdh_address(wdh_buf h, uint64_t *address) {
+  WDH_REQUIRE_INIT();
+  if (!address) return fail(WDH_EINVAL, "wdh_address: address is NULL");
+  void *p = wdh::resolve(h, nullptr);
+  if (!p) return WDH_EINVAL;
+  *address = (uint64_t)(uintptr_t)p;
+  return WDH_OK;
+}
+
 int wdh_set_lane(int lane) {
   WDH_REQUIRE_INIT();
   WDH_NOT_WHILE_CAPTURING("wdh_set_lane");

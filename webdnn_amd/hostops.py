@@ -22,7 +22,8 @@ import numpy as np
 from . import capi
 from .capi import HipError, call
 
-_DTYPES = {"float32": np.float32, "int32": np.int32}
+# (numpy has no 8-bit floating point: e4m3 tensors travel as their bytes)
+_DTYPES = {"float32": np.float32, "int32": np.int32, "float8e4m3fn": np.uint8}
 
 
 class OperatorError(ValueError):
@@ -87,7 +88,7 @@ class HipTensor:
         self.length = int(np.prod(self.dims, dtype=np.int64)) if self.dims else 1
         self.data_type = data_type
         if shared is None:
-            handle = capi.load().wdh_alloc(self.length * 4)
+            handle = capi.load().wdh_alloc(self.length * np.dtype(_DTYPES[data_type]).itemsize)
             if handle == 0:
                 raise HipError("wdh_alloc", -3, capi.last_error())
             shared = {"handle": handle, "refs": 0}
@@ -118,6 +119,16 @@ class HipTensor:
         out = np.empty(self.dims, dtype=_DTYPES[self.data_type])
         call("wdh_read", self.handle, 0, out.ctypes.data_as(ctypes.c_void_p), out.nbytes)
         return out
+
+    @property
+    def __cuda_array_interface__(self):
+        """The tensor's memory for other libraries of this process (`torch.as_tensor(tensor, device="cuda")` is a view of it; e4m3 tensors
+        are bytes there).  The library works on streams of its own: `context.sync()` before the other side reads.  torch has to
+        have brought the HIP runtime up (its first use of the GPU) before `HipContext.initialize`."""
+        address = ctypes.c_uint64()
+        call("wdh_address", self.handle, ctypes.byref(address))
+        return {"shape": tuple(self.dims), "typestr": np.dtype(_DTYPES[self.data_type]).str, "strides": None, "version": 2,
+                "data": (address.value if self.length else 0, False)}
 
     def dispose(self):
         if self._disposed:
@@ -170,12 +181,14 @@ class HipContext:
         return HipTensor(self, dims, data_type)
 
     def move_tensor(self, array):
-        """CPU (numpy) -> hip, like moveTensor = emptyTensor + setData."""
+        """CPU (numpy) -> hip, like moveTensor = emptyTensor + setData.  Bytes (uint8) are e4m3 values."""
         array = np.asarray(array)
         if array.dtype == np.float32:
             dt = "float32"
         elif array.dtype == np.int32:
             dt = "int32"
+        elif array.dtype == np.uint8:
+            dt = "float8e4m3fn"
         else:
             raise OperatorError("moveTensor: dtype %s not supported" % array.dtype)
         t = self.empty_tensor(array.shape, dt)
@@ -805,4 +818,168 @@ def cast(ctx, x, to):
     y = ctx.empty_tensor(x.dims, dt)
     call("wdh_cast", 0 if x.data_type == "float32" else 1, 0 if dt == "float32" else 1,
          x.handle, y.handle, x.length)
+    return y
+
+
+# ---- 8-bit serving of language models (e4m3 with block scales; include/webdnn_hip.h) ------------------
+FP8_BLOCK, CACHE_PAGE = 128, 64
+
+
+def _fp8_blocks(n):
+    return -(-n // FP8_BLOCK)
+
+
+def _result(ctx, given, dims, data_type="float32"):
+    """The buffer a result goes to: the caller's, if it has one of that shape and type."""
+    dims = [int(d) for d in dims]
+    if given is None:
+        return ctx.empty_tensor(dims, data_type)
+    if given.dims != dims or given.data_type != data_type:
+        raise OperatorError("out: %s of shape %s expected, got %s of %s" % (data_type, dims, given.data_type, given.dims))
+    return given
+
+
+def _require(what, tensor, dims, data_type="float32"):
+    if tensor.data_type != data_type or tensor.dims != list(dims):
+        raise OperatorError("%s: %s of shape %s expected, got %s of %s" % (what, data_type, list(dims), tensor.data_type, tensor.dims))
+
+
+def _handle(tensor):
+    return tensor.handle if tensor is not None else 0
+
+
+def _rms_rows(x, scale, skip):
+    _require_f32(x, scale, skip)
+    if x.ndim < 1:
+        raise OperatorError("RMSNormalization: a scalar has no rows")
+    length = x.dims[-1]
+    if scale is not None and scale.dims != [length]:
+        raise OperatorError("RMSNormalization: scale must have the normalised length")
+    if skip is not None and skip.dims != x.dims:
+        raise OperatorError("RMSNormalization: skip must have the input's shape")
+    return x.length // length if length else 0, length
+
+
+def rms_normalization(ctx, x, scale=None, skip=None, epsilon=1e-5, out=None):
+    """ONNX RMSNormalization over the last axis; with `skip`, of x + skip, which is then the first of two results.
+    out = (sum or None, y): buffers for the results (sum may be x or skip)."""
+    outer, length = _rms_rows(x, scale, skip)
+    total, y = out if out is not None else (None, None)
+    if skip is not None or total is not None:
+        total = _result(ctx, total, x.dims)
+    y = _result(ctx, y, x.dims)
+    call("wdh_rmsnorm", x.handle, _handle(skip), _handle(scale), _handle(total), y.handle, 0, 0, outer, length, epsilon)
+    return (total, y) if total is not None else y
+
+
+def rms_normalization_fp8(ctx, x, scale=None, skip=None, epsilon=1e-5, out=None):
+    """The same with the normalised rows in e4m3: (q, scales), or (sum, q, scales) with `skip`; scales [rows..., ceil(len/128)].
+    out = (sum or None, q, scales)."""
+    outer, length = _rms_rows(x, scale, skip)
+    total, q, scales = out if out is not None else (None, None, None)
+    if skip is not None or total is not None:
+        total = _result(ctx, total, x.dims)
+    q = _result(ctx, q, x.dims, "float8e4m3fn")
+    scales = _result(ctx, scales, x.dims[:-1] + [_fp8_blocks(length)])
+    call("wdh_rmsnorm", x.handle, _handle(skip), _handle(scale), _handle(total), 0, q.handle, scales.handle, outer, length, epsilon)
+    return (total, q, scales) if total is not None else (q, scales)
+
+
+def quantize_fp8(ctx, x, block_rows=1, out=None):
+    """x [rows, cols] in e4m3 with a scale for each block of block_rows x 128: (q, scales).  block_rows 1 for activations, 128 for weights."""
+    _require_f32(x)
+    if x.ndim != 2:
+        raise OperatorError("quantize_fp8: a matrix is expected")
+    if block_rows not in (1, FP8_BLOCK):
+        raise OperatorError("quantize_fp8: blocks of 1 or %d rows" % FP8_BLOCK)
+    rows, cols = x.dims
+    q, scales = out if out is not None else (None, None)
+    q = _result(ctx, q, x.dims, "float8e4m3fn")
+    scales = _result(ctx, scales, [-(-rows // block_rows), _fp8_blocks(cols)])
+    call("wdh_quantize_fp8", x.handle, q.handle, scales.handle, rows, cols, block_rows)
+    return q, scales
+
+
+def matmul_fp8(ctx, a, a_scales, w, w_scales, bias=None, residual=None, epilogue=None, out=None):
+    """a [m, k] times the transpose of w [n, k], both e4m3 with the scales of quantize_fp8 (1 and 128 rows to a block)."""
+    _require_f32(bias, residual)
+    if a.ndim != 2 or w.ndim != 2 or a.dims[1] != w.dims[1]:
+        raise OperatorError("matmul_fp8: shapes %s and %s" % (a.dims, w.dims))
+    (m, k), n = a.dims, w.dims[0]
+    _require("matmul_fp8: a", a, [m, k], "float8e4m3fn")
+    _require("matmul_fp8: w", w, [n, k], "float8e4m3fn")
+    _require("matmul_fp8: a_scales", a_scales, [m, _fp8_blocks(k)])
+    _require("matmul_fp8: w_scales", w_scales, [-(-n // FP8_BLOCK), _fp8_blocks(k)])
+    if bias is not None:
+        _require("matmul_fp8: bias", bias, [n])
+    if residual is not None:
+        _require("matmul_fp8: residual", residual, [m, n])
+    y = _result(ctx, out, [m, n])
+    call("wdh_gemm_fp8", a.handle, a_scales.handle, w.handle, w_scales.handle, _handle(bias), y.handle, m, n, k, EPI[epilogue], _handle(residual))
+    return y
+
+
+class KvCache:
+    """Keys and values in e4m3, in pages of 64 tokens: k [pages, heads, 64, d], v [pages, heads, d, 64], scales [pages, heads].
+    Which pages are whose is the caller's table."""
+
+    def __init__(self, ctx, k, k_scales, v, v_scales):
+        if k.ndim != 4:
+            raise OperatorError("KvCache: k is [pages, heads, %d, d]" % CACHE_PAGE)
+        self.pages, self.heads, _, self.d = k.dims
+        _require("KvCache: k", k, [self.pages, self.heads, CACHE_PAGE, self.d], "float8e4m3fn")
+        _require("KvCache: v", v, [self.pages, self.heads, self.d, CACHE_PAGE], "float8e4m3fn")
+        _require("KvCache: k_scales", k_scales, [self.pages, self.heads])
+        _require("KvCache: v_scales", v_scales, [self.pages, self.heads])
+        self.k, self.k_scales, self.v, self.v_scales = k, k_scales, v, v_scales
+
+    @classmethod
+    def empty(cls, ctx, pages, heads, d):
+        return cls(ctx, ctx.empty_tensor([pages, heads, CACHE_PAGE, d], "float8e4m3fn"), ctx.empty_tensor([pages, heads]),
+                   ctx.empty_tensor([pages, heads, d, CACHE_PAGE], "float8e4m3fn"), ctx.empty_tensor([pages, heads]))
+
+    def dispose(self):
+        for t in (self.k, self.k_scales, self.v, self.v_scales):
+            t.dispose()
+
+
+def _sequences(table, lens, starts):
+    if table.ndim != 2:
+        raise OperatorError("cache: table is [sequences, pages]")
+    _require("cache: table", table, table.dims, "int32")
+    _require("cache: lens", lens, [table.dims[0]], "int32")
+    _require("cache: starts", starts, [table.dims[0] + 1], "int32")
+    return table.dims
+
+
+def _rows_at(what, t, columns, width):
+    """Columns `columns` .. `columns` + width of the rows of t: (row stride, rows)."""
+    _require_f32(t)
+    if t.ndim != 2 or columns < 0 or columns + width > t.dims[1]:
+        raise OperatorError("%s: rows %s do not hold %d elements from %d on" % (what, t.dims, width, columns))
+    return t.dims[1], t.dims[0]
+
+
+def cache_append(ctx, cache, k, v, table, lens, starts, k_column=0, v_column=0):
+    """Rows of k and v ([tokens, heads * d], or columns k_column.. and v_column.. of wider rows) behind their sequences' earlier tokens.
+    table [sequences, pages], lens [sequences] (the new tokens counted) and starts [sequences + 1] are int32 tensors."""
+    seqs, most = _sequences(table, lens, starts)
+    width = cache.heads * cache.d
+    (ks, tokens), (vs, v_tokens) = _rows_at("cache_append: k", k, k_column, width), _rows_at("cache_append: v", v, v_column, width)
+    if tokens != v_tokens:
+        raise OperatorError("cache_append: %d keys and %d values" % (tokens, v_tokens))
+    call("wdh_cache_append", k.handle, k_column, ks, v.handle, v_column, vs, cache.k.handle, cache.k_scales.handle, cache.v.handle,
+         cache.v_scales.handle, table.handle, lens.handle, starts.handle, seqs, tokens, cache.heads, cache.d, cache.pages, most)
+
+
+def cache_attention(ctx, cache, q, heads, alpha, table, lens, starts, q_column=0, out=None):
+    """Attention of q's rows ([tokens, heads * d], or columns q_column.. of wider rows) over their sequences in the cache, each over the
+    tokens up to its own: [tokens, heads * d]."""
+    seqs, most = _sequences(table, lens, starts)
+    if heads <= 0 or not cache.heads or heads % cache.heads:
+        raise OperatorError("cache_attention: %d heads on %d of the cache" % (heads, cache.heads))
+    stride, tokens = _rows_at("cache_attention: q", q, q_column, heads * cache.d)
+    y = _result(ctx, out, [tokens, heads * cache.d])
+    call("wdh_cache_attention", q.handle, q_column, stride, cache.k.handle, cache.k_scales.handle, cache.v.handle, cache.v_scales.handle,
+         table.handle, lens.handle, starts.handle, y.handle, seqs, tokens, heads, cache.heads, cache.d, cache.pages, most, float(alpha))
     return y

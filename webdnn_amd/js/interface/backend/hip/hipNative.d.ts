@@ -87,4 +87,17 @@ export interface HipNative {
   /** from / to: 0 float32, 1 int32 */
   cast(from: number, to: number, X: Handle, Y: Handle, length: number): void;
   stridedCopy(X: Handle, xOffset: number, Y: Handle, yOffset: number, shape: IntList, xStrides: IntList, yStrides: IntList): void;
+  // ---- 8-bit serving (e4m3 tensors are one byte an element; 0 = absent) ----
+  /** Sum = X + Skip; Y = its root-mean-square normalisation times Gamma; Q, QScale = that in e4m3, a scale for 128 elements */
+  rmsnorm(X: Handle, Skip: Handle, Gamma: Handle, Sum: Handle, Y: Handle, Q: Handle, QScale: Handle, outer: number, len: number, epsilon: number): void;
+  /** blockRows: 1 (activations) or 128 (weights) */
+  quantizeFp8(X: Handle, Q: Handle, QScale: Handle, rows: number, cols: number, blockRows: number): void;
+  gemmFp8(A: Handle, AScale: Handle, W: Handle, WScale: Handle, Bias: Handle, Y: Handle, m: number, n: number, k: number,
+          epilogue: number, R: Handle): void;
+  cacheAppend(K: Handle, kOffset: number, kStride: number, V: Handle, vOffset: number, vStride: number, KPages: Handle, KScales: Handle,
+              VPages: Handle, VScales: Handle, Table: Handle, Lens: Handle, Starts: Handle, seqs: number, tokens: number,
+              kvHeads: number, d: number, pages: number, maxPages: number): void;
+  cacheAttention(Q: Handle, qOffset: number, qStride: number, KPages: Handle, KScales: Handle, VPages: Handle, VScales: Handle,
+                 Table: Handle, Lens: Handle, Starts: Handle, Y: Handle, seqs: number, tokens: number, heads: number,
+                 kvHeads: number, d: number, pages: number, maxPages: number, alpha: number): void;
 }

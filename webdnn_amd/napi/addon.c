@@ -402,6 +402,50 @@ FN(js_layernorm) {
   return make_undefined(env);
 }
 
+FN(js_rmsnorm) { /* (X, Skip, Gamma, Sum, Y, Q, QScale, outer, len, eps); 0 = absent */
+  ARGS("wdh_rmsnorm", 10);
+  I64(0, X); I64(1, R); I64(2, G); I64(3, S); I64(4, Y); I64(5, Q); I64(6, QS); I64(7, outer); I64(8, len);
+  F64(9, eps);
+  CHECK(wdh_rmsnorm(X, R, G, S, Y, Q, QS, outer, (int)len, (float)eps));
+  return make_undefined(env);
+}
+
+FN(js_quantize_fp8) { /* (X, Q, QScale, rows, cols, blockRows) */
+  ARGS("wdh_quantize_fp8", 6);
+  I64(0, X); I64(1, Q); I64(2, QS); I64(3, rows); I64(4, cols); I64(5, block_rows);
+  CHECK(wdh_quantize_fp8(X, Q, QS, rows, (int)cols, (int)block_rows));
+  return make_undefined(env);
+}
+
+FN(js_gemm_fp8) { /* (A, AScale, W, WScale, Bias, Y, m, n, k, epilogue, R) */
+  ARGS("wdh_gemm_fp8", 11);
+  I64(0, A); I64(1, SA); I64(2, W); I64(3, SW); I64(4, B); I64(5, Y); I64(6, m); I64(7, n); I64(8, k); I64(9, epilogue);
+  I64(10, R);
+  CHECK(wdh_gemm_fp8(A, SA, W, SW, B, Y, m, (int)n, (int)k, (int)epilogue, R));
+  return make_undefined(env);
+}
+
+FN(js_cache_append) { /* (K, kOffset, kStride, V, vOffset, vStride, KPages, KScales, VPages, VScales, Table, Lens, Starts, ...) */
+  ARGS("wdh_cache_append", 19);
+  int64_t a[19];
+  for (int i = 0; i < 19; i++)
+    if (!to_i64(env, argv[i], &a[i])) return throw_arg(env, FNAME, "integer argument expected");
+  CHECK(wdh_cache_append(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], (int)a[13], (int)a[14],
+                         (int)a[15], (int)a[16], (int)a[17], (int)a[18]));
+  return make_undefined(env);
+}
+
+FN(js_cache_attention) { /* (Q, qOffset, qStride, KPages, KScales, VPages, VScales, Table, Lens, Starts, Y, ..., alpha) */
+  ARGS("wdh_cache_attention", 19);
+  int64_t a[18];
+  for (int i = 0; i < 18; i++)
+    if (!to_i64(env, argv[i], &a[i])) return throw_arg(env, FNAME, "integer argument expected");
+  F64(18, alpha);
+  CHECK(wdh_cache_attention(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], (int)a[11], (int)a[12], (int)a[13],
+                            (int)a[14], (int)a[15], (int)a[16], (int)a[17], (float)alpha));
+  return make_undefined(env);
+}
+
 FN(js_reduce_mean) {
   ARGS("wdh_reduce_mean", 4);
   I64(0, X); I64(1, Y); I64(2, outer); I64(3, len);
@@ -515,6 +559,8 @@ static napi_value init_module(napi_env env, napi_value exports) {
       {"trim", js_trim}, {"eventRecord", js_event_record}, {"eventElapsedMs", js_event_elapsed_ms},
       {"gemm", js_gemm}, {"gemmEx", js_gemm_ex}, {"linearGroup", js_linear_group}, {"conv2d", js_conv2d}, {"conv2dEx", js_conv2d_ex}, {"binary", js_binary}, {"unary", js_unary},
       {"softmax", js_softmax}, {"attention", js_attention}, {"layernorm", js_layernorm}, {"layernormAdd", js_layernorm_add}, {"reduceMean", js_reduce_mean}, {"reduceAxis", js_reduce_axis},
+      {"rmsnorm", js_rmsnorm}, {"quantizeFp8", js_quantize_fp8}, {"gemmFp8", js_gemm_fp8}, {"cacheAppend", js_cache_append},
+      {"cacheAttention", js_cache_attention},
       {"maxpool2d", js_maxpool2d}, {"globalAvgpool", js_global_avgpool},
       {"transpose", js_transpose}, {"gather", js_gather}, {"cast", js_cast},
       {"stridedCopy", js_strided_copy}, {"graphBegin", js_graph_begin}, {"graphEnd", js_graph_end},
