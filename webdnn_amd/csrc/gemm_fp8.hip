@@ -49,10 +49,17 @@ __device__ __forceinline__ i32x8 load32(const unsigned char *row, int k, int len
   return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-__device__ __forceinline__ float finish(const ProductParams &p, long long i, int j, float v) {
-  if (p.bias) v = v + p.bias[j];
-  if (p.R) v = v + p.R[i * p.n + j];
-  return p.relu && !(v > 0.0f) && v == v ? 0.0f : v;
+// Columns j .. j+3 of row i: bias, residual, Relu, and out.
+__device__ __forceinline__ void finish4(const ProductParams &p, long long i, int j, f32x4 v) {
+  const int left = p.n - j;
+  if (left <= 0) return;
+  float *y = p.Y + i * p.n;
+  if (p.bias) v = v + load4(p.bias, j, p.n);
+  if (p.R) v = v + load4(p.R + i * p.n, j, p.n);
+  if (p.relu)
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = !(v[e] > 0.0f) && v[e] == v[e] ? 0.0f : v[e];
+  store4(y, j, p.n, v);
 }
 
 // Few rows of A: a workgroup has 16 rows of W and 16 MT of A, its wavefronts take K blocks in turn and add up through LDS.
@@ -90,12 +97,7 @@ __global__ __launch_bounds__(256) void product_few(ProductParams p) {
       const int t = cell >> 6, l = cell & 63;
       const f32x4 v = (part[0][t][l] + part[1][t][l]) + (part[2][t][l] + part[3][t][l]);
       const long long i = m0 + 16 * t + (l & 15);
-      if (i < p.m)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int j = n0 + 4 * (l >> 4) + e;
-          if (j < p.n) p.Y[i * p.n + j] = finish(p, i, j, v[e]);
-        }
+      if (i < p.m) finish4(p, i, n0 + 4 * (l >> 4), v);
     }
     __syncthreads();
   }
@@ -107,6 +109,132 @@ void launch_few(const ProductParams &p, bool aligned) {
   const dim3 grid((unsigned)((p.n + 15) / 16), (unsigned)(rows < 65535 ? rows : 65535));
   if (aligned) hipLaunchKernelGGL((product_few<MT, true>), grid, dim3(256), 0, wdh::stream(), p);
   else hipLaunchKernelGGL((product_few<MT, false>), grid, dim3(256), 0, wdh::stream(), p);
+}
+
+// Tiles of NW TN x 32 columns of Y (rows of W) and MW TM x 32 rows: NW x MW wavefronts with TN x TM blocks of 32 x 32 each.
+// A slab is a block of K: 128 bytes of every row of the tile, which pass through registers into LDS while the slab before is
+// multiplied.  In LDS a row's eight 16-byte pieces are exchanged by its number (piece ^ row % 8), so that the 32 rows that a
+// fragment read takes a piece of lie on different banks.  A fragment's 16 bytes serve two instructions (their k are the first and the
+// last eight of them, on both sides alike).
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int NW, int MW, int TN, int TM, bool ALIGNED>
+__global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p) {
+  constexpr int THREADS = 64 * NW * MW, BN = 32 * NW * TN, BM = 32 * MW * TM, ROWS = BN + BM;
+  constexpr int LOADS = ROWS * 8 / THREADS;
+  static_assert(ROWS * 8 % THREADS == 0 && BM <= THREADS && BLOCK % (32 * TN) == 0, "tile");
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2][ROWS * BLOCK];
+  __shared__ float scales[2][BM];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
+  const int wn = wave % NW, wm = wave / NW;
+  const int tiles_n = (p.n + BN - 1) / BN;
+  const long long m0 = (long long)(blockIdx.x / tiles_n) * BM;
+  const int n0 = (int)(blockIdx.x % tiles_n) * BN;
+
+  const unsigned char *row[LOADS];
+  int to[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; i++) {
+    const int at = tid + THREADS * i, r = at >> 3;
+    if (r < BN) row[i] = p.W + (long long)(n0 + r < p.n ? n0 + r : p.n - 1) * p.k;
+    else row[i] = p.A + (m0 + r - BN < p.m ? m0 + r - BN : p.m - 1) * p.k;
+    to[i] = r * BLOCK + 16 * ((at & 7) ^ (r & 7));
+  }
+  const int piece = 16 * (tid & 7);
+  const float *my_scale = p.SA + (m0 + tid % BM < p.m ? m0 + tid % BM : p.m - 1) * p.blocks;
+  const int wide = (n0 + 32 * TN * wn) / BLOCK;  // (columns beyond n: any scale will do)
+  const float *sw = p.SW + (long long)(wide * BLOCK < p.n ? wide : 0) * p.blocks;
+
+  i32x4 next[LOADS];
+  float next_scale = 0.0f;
+  auto fetch = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) next[i] = load16<ALIGNED>(row[i], b * BLOCK + piece, p.k);
+    if (tid < BM) next_scale = my_scale[b];
+  };
+  auto keep = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) *reinterpret_cast<i32x4 *>(&lds[buf][to[i]]) = next[i];
+    if (tid < BM) scales[buf][tid] = next_scale;
+  };
+  // a 32-row block's fragments: 16 bytes for each quarter of the slab
+  auto fragment = [&](int buf, int r0, bf16x8 (&f)[8]) {
+    const int r = r0 + li;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const i32x4 x = *reinterpret_cast<const i32x4 *>(&lds[buf][r * BLOCK + 16 * ((2 * q + half) ^ (r & 7))]);
+      f[2 * q] = widen(x[0], x[1]);
+      f[2 * q + 1] = widen(x[2], x[3]);
+    }
+  };
+
+  f32x16 acc[TN][TM];
+#pragma unroll
+  for (int i = 0; i < TN; i++)
+#pragma unroll
+    for (int j = 0; j < TM; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
+  if (p.blocks > 0) {
+    fetch(0);
+    keep(0);
+  }
+  __syncthreads();
+  for (int b = 0; b < p.blocks; b++) {
+    const int buf = b & 1;
+    if (b + 1 < p.blocks) fetch(b + 1);
+    const float s = sw[b];
+    bf16x8 a[TM][8];
+    float c[TM];
+#pragma unroll
+    for (int j = 0; j < TM; j++) {
+      fragment(buf, BN + 32 * (TM * wm + j), a[j]);
+      c[j] = scales[buf][32 * (TM * wm + j) + li] * s;
+    }
+#pragma unroll
+    for (int i = 0; i < TN; i++) {
+      bf16x8 w[8];
+      fragment(buf, 32 * (TN * wn + i), w);
+      f32x16 x[TM];
+#pragma unroll
+      for (int j = 0; j < TM; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[j][e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+#pragma unroll
+        for (int j = 0; j < TM; j++) x[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[k], a[j][k], x[j], 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < TM; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[i][j][e] = __builtin_fmaf(x[j][e], c[j], acc[i][j][e]);
+    }
+    if (b + 1 < p.blocks) keep(buf ^ 1);
+    __syncthreads();
+  }
+  // lane: row li of a block; registers 4 q .. + 3 are columns 8 q + 4 half .. + 3
+#pragma unroll
+  for (int j = 0; j < TM; j++) {
+    const long long i = m0 + 32 * (TM * wm + j) + li;
+    if (i >= p.m) continue;
+#pragma unroll
+    for (int t = 0; t < TN; t++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int col = n0 + 32 * (TN * wn + t) + 8 * q + 4 * half;
+        f32x4 v = {acc[t][j][4 * q], acc[t][j][4 * q + 1], acc[t][j][4 * q + 2], acc[t][j][4 * q + 3]};
+        finish4(p, i, col, v);
+      }
+  }
+}
+
+template <int NW, int MW, int TN, int TM>
+void launch_tiles(const ProductParams &p, bool aligned) {
+  constexpr int BN = 32 * NW * TN, BM = 32 * MW * TM;
+  const long long tiles = (p.n + BN - 1) / BN * ((p.m + BM - 1) / BM);
+  const dim3 grid((unsigned)tiles), wg(64 * NW * MW);
+  if (aligned) hipLaunchKernelGGL((product_tiles<NW, MW, TN, TM, true>), grid, wg, 0, wdh::stream(), p);
+  else hipLaunchKernelGGL((product_tiles<NW, MW, TN, TM, false>), grid, wg, 0, wdh::stream(), p);
 }
 
 }  // namespace
@@ -139,7 +267,9 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
   p.m = m; p.n = n; p.k = k; p.blocks = (int)blocks; p.relu = epilogue == WDH_EPI_RELU;
   const bool aligned = k % 16 == 0;  // (buffers are)
   if (m <= 16) launch_few<1>(p, aligned);
-  else launch_few<4>(p, aligned);
+  else if (m <= 64) launch_few<4>(p, aligned);
+  else if ((n + 127) / 128 * ((m + 127) / 128) < 2LL * wdh::compute_units()) launch_tiles<2, 2, 1, 1>(p, aligned);
+  else launch_tiles<4, 2, 2, 2>(p, aligned);
   WDH_LAUNCH_CHECK();
   return WDH_OK;
 }
