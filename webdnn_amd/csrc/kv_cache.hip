@@ -10,6 +10,7 @@
 #include <stdio.h>
 
 #include "common.h"
+#include "fastdiv.h"
 #include "fp8.h"
 
 namespace {
@@ -32,47 +33,52 @@ struct Place {
   int seq, row0, n, len, index;  // rows row0 .. row0+n-1 of the call are the last n of the sequence's len tokens
 };
 
-// A sequence's rows; n = 0 for one that has none, or whose numbers do not fit the call or the table.
+// A sequence's rows; n = 0 for one that has none, whose numbers do not fit the call or the table, or that is not there.
 __device__ __forceinline__ Place sequence(const Sequences &q, int s) {
-  Place p;
-  p.seq = s;
+  Place p = {s, 0, 0, 0, 0};
+  if (s >= q.seqs) return p;
   p.row0 = q.starts[s];
   p.len = q.lens[s];
   const long long n = (long long)q.starts[s + 1] - p.row0;
   const bool fits = p.row0 >= 0 && n > 0 && p.row0 + n <= q.tokens && n <= p.len && p.len <= (long long)q.max_pages * PAGE;
   p.n = fits ? (int)n : 0;
-  p.index = 0;
   return p;
 }
 
+// A number the compiler knows nothing about: what is computed from it stays where it is used and holds no registers in between.
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// Sums over the lanes up to and with each: shifts within rows of 16, then the last lanes of rows 0 and 2, and of row 1, into
+// those behind them.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<wdh::rowmath::DPP_BCAST15, 0xa>(v);
+  return dpp_add<wdh::rowmath::DPP_BCAST31, 0xc>(v);
+}
 // The sequence that holds work item `item` when each has count(place) of them in turn, and which of its items that is; n = 0
-// behind the last.  Whole wavefronts call this: 64 sequences are looked at side by side.
+// behind the last.  Whole wavefronts call this: they look at 64 sequences side by side.
 template <class Count>
-__device__ __forceinline__ Place locate(const Sequences &q, long long item, Count count) {
-  const int lane = threadIdx.x & 63;
-  for (int s0 = 0; s0 < q.seqs; s0 += 64) {
-    Place p = {0, 0, 0, 0, 0};
-    if (s0 + lane < q.seqs) p = sequence(q, s0 + lane);
-    const int mine = p.n ? count(p) : 0;
-    long long upto = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const long long below = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += below;
-    }
+__device__ __forceinline__ Place locate(const Sequences &q, int item, Count count) {
+  for (int i = 0; i < (q.seqs + 63) / 64; i++) {
+    const Place mine = sequence(q, 64 * i + (int)(threadIdx.x & 63));
+    const int items = mine.n ? count(mine) : 0, upto = wave_scan(items);
     const unsigned long long has = __ballot(item < upto);
     if (has) {
       const int at = __ffsll(has) - 1;
-      const long long before = __shfl(upto - mine, at, 64);
-      Place r;
-      r.seq = __builtin_amdgcn_readlane(p.seq, at);
-      r.row0 = __builtin_amdgcn_readlane(p.row0, at);
-      r.n = __builtin_amdgcn_readlane(p.n, at);
-      r.len = __builtin_amdgcn_readlane(p.len, at);
-      r.index = __builtin_amdgcn_readfirstlane((int)(item - before));
-      return r;
+      return Place{__builtin_amdgcn_readlane(mine.seq, at), __builtin_amdgcn_readlane(mine.row0, at), __builtin_amdgcn_readlane(mine.n, at),
+                   __builtin_amdgcn_readlane(mine.len, at), item - __builtin_amdgcn_readlane(upto - items, at)};
     }
-    item -= __shfl(upto, 63, 64);
+    item -= __builtin_amdgcn_readlane(upto, 63);
   }
   return Place{0, 0, 0, 0, 0};
 }
@@ -185,19 +191,84 @@ struct AttendParams {
   const unsigned char *KP, *VP;
   const float *KS, *VS;
   float *Y;
-  int heads, kv_heads, group;
-  float scale;       // alpha * log2(e): powers are taken of two
-  int splits;
-  float *partial;    // splits > 1: [item][kv head][split][16][D + 2]
+  int heads, kv_heads;
+  wdh::FastDiv group;  // queries that share a head of the cache
+  float scale;     // alpha * log2(e): powers are taken of two
+  int wgs;         // workgroups for each head of the cache
+  float *partial;  // results [workgroup][2][kv head][16][D] of items that more than one workgroup works on (null: there are none),
+  float *stats;    // and their tops and sums [workgroup][2][kv head][16][2]
 };
 
-__device__ __forceinline__ float wave_pairs_max(float v) {  // over the four lanes that share lane % 16
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+// Work of attention: items of 16 rows (a row is a token and one of the queries that share a head of the cache), each as many units
+// of four pages (one for each wavefront of a workgroup) as its sequence has.  The units of all items stand in a row, and every
+// workgroup takes `share` neighbouring ones: all end at the same time, whatever the sequences' lengths.
+// (us, shares / a fixed number of parts for every item: see DECODE below.)
+struct Work {
+  Place s;
+  int item, unit, units;  // the item, the unit of it that was asked for, and how many it has
+  int before;             // units in front of the item
+  int share, total;
+};
+__device__ __forceinline__ int items_of(const Place &s, int group) { return s.n ? (int)(((long long)s.n * group + 15) / 16) : 0; }
+__device__ __forceinline__ int units_of(const Place &s) { return (s.len + 4 * PAGE - 1) / (4 * PAGE); }
+__device__ __forceinline__ int total_units(const AttendParams &p) {
+  int total = 0;
+  for (int i = 0; i < (p.q.seqs + 63) / 64; i++) {
+    const Place mine = sequence(p.q, 64 * i + fresh(threadIdx.x & 63));
+    total += __builtin_amdgcn_readlane(wave_scan(items_of(mine, p.group.d) * units_of(mine)), 63);
+  }
+  return total;
+}
+// The item that holds unit number `index` of all (or, by_item, item number `index`); s.n = 0 behind the last.
+__device__ __forceinline__ Work locate_work(const AttendParams &p, int index, bool by_item) {
+  Work w;
+  int before = 0, before_items = 0;
+  for (int i = 0; i < (p.q.seqs + 63) / 64; i++) {
+    const Place mine = sequence(p.q, 64 * i + fresh(threadIdx.x & 63));
+    const int items = items_of(mine, p.group.d), units = units_of(mine);
+    const int upto = before + wave_scan(items * units), upto_items = by_item ? before_items + wave_scan(items) : 0;
+    const unsigned long long has = __ballot(index < (by_item ? upto_items : upto));
+    if (has) {
+      const int at = __ffsll(has) - 1;
+      w.s.seq = __builtin_amdgcn_readlane(mine.seq, at);
+      w.s.row0 = __builtin_amdgcn_readlane(mine.row0, at);
+      w.s.n = __builtin_amdgcn_readlane(mine.n, at);
+      w.s.len = __builtin_amdgcn_readlane(mine.len, at);
+      w.units = __builtin_amdgcn_readlane(units, at);
+      const int first = __builtin_amdgcn_readlane(upto - items * units, at);
+      w.item = by_item ? index - __builtin_amdgcn_readlane(upto_items - items, at) : (index - first) / w.units;
+      w.before = first + w.item * w.units;
+      w.unit = by_item ? 0 : index - w.before;
+      return w;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+    before_items = __builtin_amdgcn_readlane(upto_items, 63);
+  }
+  w.s = Place{0, 0, 0, 0, 0};
+  return w;
+}
+
+// Element `at`, the same for the whole wavefront, of something no kernel writes meanwhile: through the scalar cache, past the
+// queue of vector loads (which come back in order: behind a page's worth of them this one number would wait for all).
+template <class T>
+__device__ __forceinline__ T scalar(const T *from, long long at) {
+  typedef const __attribute__((address_space(4))) T *constant;
+  return *(constant)(uintptr_t)(from + at);
+}
+
+// Over the four lanes that share lane % 16: a swap of a register with itself leaves both halves' values side by side.
+template <class Op>
+__device__ __forceinline__ float across_groups(float v, Op op) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float wave_pairs_max(float v) {
+  return across_groups(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float wave_pairs_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  return across_groups(v, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -220,8 +291,8 @@ __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&part)[3]) {
   for (int k = 0; k < 3; k++) part[k] = r[k].v;
 }
 
-// 16 rows (a row is a token and one of the `group` queries that share a head of the cache) against the pages of their sequence;
-// the wavefronts of a workgroup, and the workgroups of a split, take pages in turn.  Everything is computed transposed:
+// Rows of an item against a part of their sequence's pages; the wavefronts of a workgroup take pages in turn.  Everything is
+// computed transposed:
 //   S^T [key][row] = K Q^T    (v_mfma_f32_16x16x32_bf16, K widened from e4m3, Q in three bfloat16 parts)
 //   O^T [d][row]  += V^T P^T  (V^T is how pages hold values, P in three parts)
 // so that a lane holds scores of one row, P is an operand of the second product as it stands, and both K and V pass from memory
@@ -231,208 +302,300 @@ template <int D>
 __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
   constexpr int STEPS = D / 32, CH = D >= 64 ? D / 64 : 1, DT = D / 16;
   constexpr int OP = D + 4;
-  __shared__ __attribute__((aligned(16))) float outs[4][16 * OP];
+  // the queries' parts, one fragment to a lane, later the wavefronts' results
+  __shared__ __attribute__((aligned(16))) union { bf16x8 q[STEPS][3][64]; float outs[4][16 * OP]; } lds;
   __shared__ float tops[4][16], sums[4][16];
-  const int group = p.group;
-  const Place s = locate(p.q, blockIdx.x, [group](const Place &s) { return (int)(((long long)s.n * group + 15) / 16); });
-  if (s.n == 0) return;
+  const int group = p.group.d;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, g = lane >> 4;
+  const unsigned k_lane = (16 * (i16 >> 2) + (i16 & 3)) * D + (D >= 64 ? 16 : 8) * g, v_lane = i16 * PAGE + 16 * g;  // (of a page)
   const int head = blockIdx.y;
+  const int total = total_units(p), share = (total + p.wgs - 1) / p.wgs;
+  int unit = blockIdx.x * share;
+  const int units_end = total - unit < share ? total : unit + share;
+  Work w;
+  w.s.n = 0;
+  for (bool first_segment = true; unit < units_end; first_segment = false) {
+  // the item of the last segment has another behind it, or the next sequence's first one follows
+  if (!first_segment && (w.item + 1) * 16LL < (long long)w.s.n * group) {
+    w.item++;
+    w.before = unit;
+    w.unit = 0;
+  } else {
+    w = locate_work(p, unit, false);
+    if (w.s.n == 0) return;  // (numbers that contradict each other)
+  }
+  const Place s = w.s;
   // this lane's row
-  const long long flat = (long long)s.index * 16 + i16;
-  const int token = (int)(flat / group), sub = (int)(flat - (long long)token * group);
+  const int flat = w.item * 16 + fresh(i16), token = wdh::fdiv(flat, p.group), sub = flat - token * group;
   const bool live = token < s.n;
   const int limit = live ? s.len - s.n + token : -1;  // its last key
-  const float *qrow = p.Q + (long long)(s.row0 + (live ? token : 0)) * p.q_stride + (long long)(head * group + sub) * D;
-  bf16x8 q[STEPS][3];
+  const int last_token = wdh::fdiv(w.item * 16 + 15, p.group), first_limit = s.len - s.n + wdh::fdiv(w.item * 16, p.group);
+  const int last_key = s.len - s.n + (last_token < s.n ? last_token : s.n - 1);
+  const int seg_end = w.units - w.unit < units_end - unit ? w.units : w.unit + (units_end - unit);  // in units of the item
+  const int begin = 4 * w.unit, seen = last_key / PAGE + 1, end = seen < 4 * seg_end ? seen : 4 * seg_end;
+  const bool alone = w.unit == 0 && seg_end == w.units;  // the whole item is this workgroup's
+  const int *table = p.q.table + (long long)s.seq * p.q.max_pages;
+
+  // A page's keys and values are asked for while the page before is worked on: keys once its scores are there, values once its
+  // output is.  The number of the page after that comes a turn earlier still.
+  struct Page { long long at; float ks, vs; };
+  auto find = [&](int pg) {
+    const int id = scalar(table, pg < end ? pg : end - 1);
+    const bool known = id >= 0 && id < p.q.pages;  // (a page that is not there makes its rows NaN)
+    const long long at = (long long)(known ? id : 0) * p.kv_heads + head;
+    float ks = scalar(p.KS, at), vs = scalar(p.VS, at);
+    // (a scale that is no number shows through the scores, which are masked, not through 0 * NaN)
+    if (!known || !(fabsf(vs) <= FLT_MAX)) ks = NAN, vs = 0.0f;
+    return Page{at, ks, vs};
+  };
+  i32x4 k[4][CH], v[DT];
+  auto fetch_k = [&](long long at) {
+    const unsigned char *kp = p.KP + at * (PAGE * D);
 #pragma unroll
-  for (int st = 0; st < STEPS; st++) {
-    const int d0 = D >= 64 ? 64 * (st / 2) + 16 * g + 8 * (st & 1) : 8 * g;
+    for (int t = 0; t < 4; t++) {
+      if constexpr (D >= 64) {
+#pragma unroll
+        for (int c = 0; c < CH; c++) k[t][c] = *reinterpret_cast<const i32x4 *>(kp + (k_lane + 4 * t * D + 64 * c));
+      } else {
+        const i32x2 h = *reinterpret_cast<const i32x2 *>(kp + (k_lane + 4 * t * D));
+        k[t][0] = i32x4{h[0], h[1], 0, 0};
+      }
+    }
+  };
+  auto fetch_v = [&](long long at) {
+    const unsigned char *vp = p.VP + at * (PAGE * D);
+#pragma unroll
+    for (int i = 0; i < DT; i++) v[i] = *reinterpret_cast<const i32x4 *>(vp + (v_lane + 16 * i * PAGE));
+  };
+
+  int pg = begin + wave;
+  Page now = find(pg), then = find(pg + 4);
+  if (pg < end) {
+    fetch_k(now.at);
+    fetch_v(now.at);
+  }
+  if (wave < STEPS) {
+    const float *qrow = p.Q + (long long)(s.row0 + (live ? token : 0)) * p.q_stride + (long long)(head * group + sub) * D;
+    const int d0 = D >= 64 ? 64 * (wave / 2) + 16 * g + 8 * (wave & 1) : 8 * g;
     const f32x4 a = *reinterpret_cast<const f32x4 *>(qrow + d0), b = *reinterpret_cast<const f32x4 *>(qrow + d0 + 4);
     const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    split3(x, q[st]);
+    bf16x8 parts[3];
+    split3(x, parts);
+#pragma unroll
+    for (int i = 0; i < 3; i++) lds.q[wave][i][lane] = parts[i];
   }
-  const int last_token = (int)(((long long)s.index * 16 + 15) / group);
-  const int last_key = s.len - s.n + (last_token < s.n ? last_token : s.n - 1);
-  const int count = last_key / PAGE + 1, step = 4 * p.splits;
-  const int *table = p.q.table + (long long)s.seq * p.q.max_pages;
+  __syncthreads();
 
   f32x4 o[DT];
 #pragma unroll
   for (int i = 0; i < DT; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float top = -INFINITY, sum = 0.0f;
-  for (int pg = blockIdx.z * 4 + wave; pg < count; pg += step) {
-    int id = table[pg];
-    const bool known = id >= 0 && id < p.q.pages;  // (a page that is not there makes its rows NaN)
-    if (!known) id = 0;
-    const long long at = (long long)id * p.kv_heads + head;
-    const unsigned char *kp = p.KP + at * (PAGE * D), *vp = p.VP + at * (PAGE * D);
-    // (a scale that is no number shows through the scores, which are masked, not through 0 * NaN)
-    float ks = p.KS[at], vs = p.VS[at];
-    if (!known || !(fabsf(vs) <= FLT_MAX)) ks = NAN, vs = 0.0f;
-    i32x4 k[4][CH], v[DT];
+  for (; pg < end; pg += 4) {
+    const bool more = pg + 4 < end, whole = pg * PAGE + PAGE - 1 <= first_limit;  // whole: every row sees every key
+    f32x4 sc[4];
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      const unsigned char *row = kp + (16 * (i16 >> 2) + 4 * t + (i16 & 3)) * D;
-      if constexpr (D >= 64) {
+    for (int t = 0; t < 4; t++) sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < CH; c++) k[t][c] = *reinterpret_cast<const i32x4 *>(row + 64 * c + 16 * g);
-      } else {
-        const i32x2 h = *reinterpret_cast<const i32x2 *>(row + 8 * g);
-        k[t][0] = i32x4{h[0], h[1], 0, 0};
-      }
-    }
+    for (int st = 0; st < STEPS; st++) {
+      bf16x8 q[3];
 #pragma unroll
-    for (int i = 0; i < DT; i++) v[i] = *reinterpret_cast<const i32x4 *>(vp + (16 * i + i16) * PAGE + 16 * g);
-    float x[16];
+      for (int i = 0; i < 3; i++) q[i] = lds.q[st][i][lane];
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int st = 0; st < STEPS; st++) {
+      for (int t = 0; t < 4; t++) {
         const bf16x8 kw = widen(k[t][st / 2][2 * (st & 1)], k[t][st / 2][2 * (st & 1) + 1]);
 #pragma unroll
-        for (int part = 2; part >= 0; part--) a = mfma(kw, q[st][part], a);
+        for (int i = 2; i >= 0; i--) sc[t] = mfma(kw, q[i], sc[t]);
       }
-#pragma unroll
-      for (int r = 0; r < 4; r++) x[4 * t + r] = a[r];
     }
+    if (more) fetch_k(then.at);
     // softmax: keys beyond the row's last, and whatever the page holds behind the sequence, count for nothing
-    const float c = p.scale * ks;
-    float most = -INFINITY;
+    const float c = p.scale * now.ks;
+    float x[16], most = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-      const bool in = pg * PAGE + 16 * g + e <= limit;
-      most = fmaxf(most, in ? x[e] * c : -INFINITY);
+    for (int e = 0; e < 16; e++) x[e] = sc[e >> 2][e & 3];
+    if (!whole) {
+      const int ahead = limit - pg * PAGE - 16 * g;
+#pragma unroll
+      for (int e = 0; e < 16; e++) most = fmaxf(most, e <= ahead ? x[e] * c : -INFINITY);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++) most = fmaxf(most, x[e] * c);
     }
     most = wave_pairs_max(fmaxf(most, top));
-    const float ref = most == -INFINITY ? 0.0f : most, back = __builtin_amdgcn_exp2f(top - ref);
+    const float ref = most == -INFINITY ? 0.0f : most;
+    if (__any(most > top)) {  // (false for most pages of a long sequence)
+      const float back = __builtin_amdgcn_exp2f(top - ref);
+      sum *= back;
+#pragma unroll
+      for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[i][e] *= back;
+    }
     top = most;
-    sum *= back;
 #pragma unroll
-    for (int i = 0; i < DT; i++)
+    for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -ref));
+    if (!whole) {
+      const int ahead = fresh(limit) - pg * PAGE - 16 * g;
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[i][e] *= back;
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-      const bool in = pg * PAGE + 16 * g + e <= limit;
-      x[e] = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -ref)) : 0.0f;
-      sum += x[e];
+      for (int e = 0; e < 16; e++) x[e] = e <= ahead ? x[e] : 0.0f;
     }
-    bf16x8 pr[2][3];
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = x[8 * u + e] * vs;
-      split3(y, pr[u]);
-    }
+    for (int e = 0; e < 16; e++) sum += x[e];
     // Values of keys that some row of the 16 does not see: those behind the sequence are put to 0 (0 * NaN is NaN), and a NaN among the
     // others is kept from the rows before it by hand.
-    const int first_limit = s.len - s.n + (int)((long long)s.index * 16 / group);
     bool poison = false;
-    if (pg * PAGE + PAGE - 1 > first_limit) {
-      const int behind = s.len - pg * PAGE - 16 * g;  // how many of the lane's 16 keys are the sequence's
+    if (!whole) {
+      const int behind = s.len - pg * PAGE - 16 * fresh(g);  // how many of the lane's 16 keys are the sequence's
       int bad = 0;
 #pragma unroll
       for (int i = 0; i < DT; i++)
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-          const int n = behind - 4 * w;
-          unsigned b = (unsigned)v[i][w] & (n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
+        for (int word = 0; word < 4; word++) {
+          const int n = behind - 4 * word;
+          unsigned b = (unsigned)v[i][word] & (n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
           const unsigned nan = ((b & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
           bad |= (int)nan;
-          v[i][w] = (int)(b & ~((nan >> 7) * 0xffu));
+          v[i][word] = (int)(b & ~((nan >> 7) * 0xffu));
         }
       poison = __any(bad != 0);
     }
 #pragma unroll
-    for (int i = 0; i < DT; i++)
+    for (int u = 0; u < 2; u++) {
+      float y[8];
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
+      for (int e = 0; e < 8; e++) y[e] = x[8 * u + e] * now.vs;
+      bf16x8 pr[3];
+      split3(y, pr);
+#pragma unroll
+      for (int i = 0; i < DT; i++) {
         const bf16x8 vw = widen(v[i][2 * u], v[i][2 * u + 1]);
 #pragma unroll
-        for (int part = 2; part >= 0; part--) o[i] = mfma(vw, pr[u][part], o[i]);
+        for (int part = 2; part >= 0; part--) o[i] = mfma(vw, pr[part], o[i]);
       }
-    if (poison) {
-      for (int j = 0; j < PAGE && pg * PAGE + j <= limit; j++)
-#pragma unroll
-        for (int i = 0; i < DT; i++)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if ((vp[(16 * i + 4 * g + e) * PAGE + j] & 0x7f) == 0x7f) o[i][e] = NAN;
     }
+    if (poison) {  // (loops kept as loops: registers of this rare path must not weigh on the others)
+      const unsigned char *vp = p.VP + now.at * (PAGE * D) + 4 * g * PAGE;
+      unsigned nan = 0;
+#pragma unroll 1
+      for (int i = 0; i < 4 * DT; i++)
+#pragma unroll 1
+        for (int j = 0; j < PAGE && pg * PAGE + j <= limit; j++)
+          if ((vp[(16 * (i >> 2) + (i & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << i;
+#pragma unroll
+      for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[i][e] = (nan >> (4 * i + e)) & 1 ? NAN : o[i][e];
+    }
+    if (more) fetch_v(then.at);
+    now = then;
+    then = find(pg + 8);
   }
   sum = wave_pairs_sum(sum);
+  __syncthreads();  // the queries' place is free
 
   // the wavefronts' shares together
 #pragma unroll
-  for (int i = 0; i < DT; i++) *reinterpret_cast<f32x4 *>(&outs[wave][i16 * OP + 16 * i + 4 * g]) = o[i];
+  for (int i = 0; i < DT; i++) *reinterpret_cast<f32x4 *>(&lds.outs[wave][fresh(i16) * OP + 16 * i + 4 * g]) = o[i];
   if (g == 0) {
     tops[wave][i16] = top;
     sums[wave][i16] = sum;
   }
   __syncthreads();
-  for (int cell = threadIdx.x; cell < 16 * D; cell += 256) {
-    const int row = cell / D, d = cell - row * D;
-    float most = fmaxf(fmaxf(tops[0][row], tops[1][row]), fmaxf(tops[2][row], tops[3][row]));
-    const float ref = most == -INFINITY ? 0.0f : most;
-    float total = 0.0f, y = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      const float f = __builtin_amdgcn_exp2f(tops[w][row] - ref);
-      total += f * sums[w][row];
-      y += f * outs[w][row * OP + d];
-    }
-    const long long flat_row = (long long)s.index * 16 + row;
-    const int tk = (int)(flat_row / group);
+  for (int cell = fresh(threadIdx.x); cell < 16 * (D / 4); cell += 256) {
+    const int row = cell / (D / 4), d = cell % (D / 4) * 4;
+    const int flat_row = w.item * 16 + row, tk = wdh::fdiv(flat_row, p.group);
     if (tk >= s.n) continue;
-    if (p.splits == 1) {
-      p.Y[((long long)(s.row0 + tk) * p.heads + head * group + (flat_row - (long long)tk * group)) * D + d] = total == 0.0f ? 0.0f : y / total;
-    } else {
-      float *to = p.partial + ((((long long)blockIdx.x * p.kv_heads + head) * p.splits + blockIdx.z) * 16 + row) * (D + 2);
-      to[d] = y;
+    const float most = fmaxf(fmaxf(tops[0][row], tops[1][row]), fmaxf(tops[2][row], tops[3][row]));
+    const float ref = most == -INFINITY ? 0.0f : most;
+    float total_p = 0.0f;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float f = __builtin_amdgcn_exp2f(tops[i][row] - ref);
+      const f32x4 x = *reinterpret_cast<const f32x4 *>(&lds.outs[i][row * OP + d]);
+      total_p = __builtin_fmaf(f, sums[i][row], total_p);
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(f, x[e], y[e]);
+    }
+    if (alone) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = total_p == 0.0f ? 0.0f : y[e] / total_p;
+      *reinterpret_cast<f32x4 *>(p.Y + ((long long)(s.row0 + tk) * p.heads + head * group + (flat_row - tk * group)) * D + d) = y;
+    } else if (p.partial) {
+      // (an item that more than one workgroup works on is the first or the last of each)
+      const long long at = ((2LL * blockIdx.x + (first_segment ? 0 : 1)) * p.kv_heads + head) * 16 + row;
+      *reinterpret_cast<f32x4 *>(p.partial + at * D + d) = y;
       if (d == 0) {
-        to[D] = most;
-        to[D + 1] = total;
+        p.stats[2 * at] = most;
+        p.stats[2 * at + 1] = total_p;
       }
     }
   }
+  unit += seg_end - w.unit;
+  __syncthreads();  // the next segment's queries go where the results were
+  }
 }
 
-// The shares of the splits together: a workgroup to the 16 rows of an item.
+// What several workgroups have of an item together: a workgroup to a row (and every gridDim.z-th after it), four elements and
+// every (256 / (D/4))th of the shares to a lane.
 template <int D>
 __global__ __launch_bounds__(256) void attend_join(AttendParams p) {
-  const int group = p.group, head = blockIdx.y;
-  const Place s = locate(p.q, blockIdx.x, [group](const Place &s) { return (int)(((long long)s.n * group + 15) / 16); });
-  if (s.n == 0) return;
-  for (int cell = threadIdx.x; cell < 16 * D; cell += 256) {
-    const int row = cell / D, d = cell - row * D;
-    const long long flat_row = (long long)s.index * 16 + row;
-    const int tk = (int)(flat_row / group);
-    if (tk >= s.n) continue;
-    const float *from = p.partial + ((((long long)blockIdx.x * p.kv_heads + head) * p.splits) * 16 + row) * (D + 2);
-    const long long pitch = 16 * (D + 2);
-    float most = -INFINITY;
-    for (int i = 0; i < p.splits; i++) most = fmaxf(most, from[i * pitch + D]);
-    const float ref = most == -INFINITY ? 0.0f : most;
-    float total = 0.0f, y = 0.0f;
-    for (int i = 0; i < p.splits; i++) {
-      const float f = __builtin_amdgcn_exp2f(from[i * pitch + D] - ref);
-      total += f * from[i * pitch + D + 1];
-      y += f * from[i * pitch + d];
+  constexpr int LANES = D / 4, SIDE = 256 / LANES;
+  __shared__ __attribute__((aligned(16))) f32x4 results[SIDE][LANES];
+  __shared__ float totals[SIDE];
+  const int head = blockIdx.y, total_u = total_units(p), share = (total_u + p.wgs - 1) / p.wgs;
+  const Work w = locate_work(p, blockIdx.x, true);
+  if (w.s.n == 0 || share == 0) return;
+  const int from_wg = w.before / share, to_wg = (w.before + w.units - 1) / share;
+  if (from_wg == to_wg) return;
+  const int lane = threadIdx.x % LANES, side = threadIdx.x / LANES;
+  for (int row = blockIdx.z; row < 16; row += gridDim.z) {
+    const int flat = w.item * 16 + row, token = wdh::fdiv(flat, p.group);
+    if (token >= w.s.n) return;
+    // the first workgroup has the item at its end, unless its share begins with it; the others begin with it
+    auto slot = [&](int wg) {
+      return ((2LL * wg + (wg == from_wg && w.before != from_wg * share ? 1 : 0)) * p.kv_heads + head) * 16 + row;
+    };
+    float top = -INFINITY;
+    for (int i = from_wg + (threadIdx.x & 63); i <= to_wg; i += 64) top = fmaxf(top, p.stats[2 * slot(i)]);
+    top = wdh::rowmath::wave_max(top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.0f;
+#pragma unroll 4
+    for (int i = from_wg + side; i <= to_wg; i += SIDE) {
+      const long long at = slot(i);
+      const float f = __builtin_amdgcn_exp2f(p.stats[2 * at] - ref);
+      const f32x4 x = *reinterpret_cast<const f32x4 *>(p.partial + at * D + 4 * lane);
+      total = __builtin_fmaf(f, p.stats[2 * at + 1], total);
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(f, x[e], y[e]);
     }
-    p.Y[((long long)(s.row0 + tk) * p.heads + head * group + (flat_row - (long long)tk * group)) * D + d] = total == 0.0f ? 0.0f : y / total;
+    results[side][lane] = y;
+    if (lane == 0) totals[side] = total;
+    __syncthreads();
+    if (side == 0) {
+#pragma unroll
+      for (int i = 1; i < SIDE; i++) {
+        total += totals[i];
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] += results[i][lane][e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = total == 0.0f ? 0.0f : y[e] / total;
+      *reinterpret_cast<f32x4 *>(p.Y + ((long long)(w.s.row0 + token) * p.heads + head * p.group.d + (flat - token * p.group.d)) * D + 4 * lane) = y;
+    }
+    __syncthreads();
   }
 }
 
 template <int D>
 int launch_attend(const AttendParams &p, long long items) {
   hipStream_t st = wdh::stream();
-  hipLaunchKernelGGL((attend_rows<D>), dim3((unsigned)items, (unsigned)p.kv_heads, (unsigned)p.splits), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((attend_rows<D>), dim3((unsigned)p.wgs, (unsigned)p.kv_heads), dim3(256), 0, st, p);
   WDH_LAUNCH_CHECK();
-  if (p.splits > 1) {
-    hipLaunchKernelGGL((attend_join<D>), dim3((unsigned)items, (unsigned)p.kv_heads), dim3(256), 0, st, p);
+  if (p.partial) {
+    hipLaunchKernelGGL((attend_join<D>), dim3((unsigned)items, (unsigned)p.kv_heads, (unsigned)(p.group.d < 16 ? p.group.d : 16)), dim3(256), 0, st, p);
     WDH_LAUNCH_CHECK();
   }
   return WDH_OK;
@@ -543,22 +706,25 @@ extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_strid
   p.q_stride = q_stride;
   p.KP = (const unsigned char *)kp; p.KS = (const float *)ks; p.VP = (const unsigned char *)vp; p.VS = (const float *)vs;
   p.Y = (float *)py;
-  p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads;
+  p.heads = heads; p.kv_heads = kv_heads; p.group = wdh::make_fastdiv(heads / kv_heads);
   p.scale = alpha * 1.44269504088896341f;
   // items of 16 rows: a sequence of n tokens has ceil(n group / 16)
-  const long long loose = (long long)tokens * p.group / 16 + seqs, tight = (long long)tokens * ((p.group + 15) / 16);
+  const long long loose = (long long)tokens * p.group.d / 16 + seqs, tight = (long long)tokens * ((p.group.d + 15) / 16);
   const long long items = loose < tight ? loose : tight;
-  if (items > 0xffffffffLL / 256) return fail(WDH_EINVAL, "%s: too many rows", who);
-  const long long wanted = 2LL * wdh::compute_units(), have = items * kv_heads, most = ((long long)max_pages + 7) / 8;
-  long long splits = (wanted + have - 1) / have;
-  p.splits = (int)(splits < most ? splits : most);
-  p.partial = nullptr;
+  if (items > 0xffffffLL / 2) return fail(WDH_EINVAL, "%s: too many rows", who);
+  // As many workgroups as the chip holds at a time, or as there can be units.
+  const long long units = items * ((max_pages + 3) / 4), resident = 2LL * wdh::compute_units() / kv_heads;
+  if (units > (1LL << 30)) return fail(WDH_EINVAL, "%s: too many rows of tables so wide", who);
+  p.wgs = (int)(units < resident ? units : resident > 0 ? resident : 1);
+  p.partial = p.stats = nullptr;
   wdh_buf work = 0;
-  if (p.splits > 1) {
-    work = wdh_alloc((size_t)have * p.splits * 16 * (d + 2) * 4);
+  if (max_pages > 4 && p.wgs > 1) {  // (items of one unit are never cut)
+    const size_t rows = (size_t)p.wgs * 2 * kv_heads * 16;
+    work = wdh_alloc(rows * (d + 2) * 4);
     if (!work) return WDH_ENOMEM;
     size_t have_bytes;
     p.partial = (float *)wdh::resolve(work, &have_bytes);
+    p.stats = p.partial + rows * d;
   }
   const int rc = d == 32 ? launch_attend<32>(p, items) : d == 64 ? launch_attend<64>(p, items) : launch_attend<128>(p, items);
   if (work) (void)wdh_free(work);
