@@ -345,7 +345,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     const long long at = (long long)(known ? id : 0) * p.kv_heads + head;
     float ks = scalar(p.KS, at), vs = scalar(p.VS, at);
     // (a scale that is no number shows through the scores, which are masked, not through 0 * NaN)
-    if (!known || !(fabsf(vs) <= FLT_MAX)) ks = NAN, vs = 0.0f;
+    if (!known || !(ks > 0.0f) || !(vs > 0.0f && vs <= FLT_MAX)) ks = NAN, vs = 0.0f;
     return Page{at, ks, vs};
   };
   i32x4 k[4][CH], v[DT];
@@ -589,6 +589,277 @@ __global__ __launch_bounds__(256) void attend_join(AttendParams p) {
   }
 }
 
+// ---- attention of many rows ------------------------------------------------------------------
+// Prompts: items of 128 rows, 32 to a wavefront, that share the pages of their sequence through LDS (v_mfma_f32_32x32x16_bf16, the
+// same transposed products).  A page's 64 keys are two blocks of 32, in an order that leaves lanes of the lower half of a
+// wavefront keys 0..15 and of the upper half keys 16..31 of a block in one run, as the second product wants them.  In LDS, rows
+// (128 bytes of a key, 64 of a value's d) have their 16-byte pieces exchanged so that the rows a read takes lie on different banks.
+constexpr int MANY = 128;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float halves_max(float v) {
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
+  constexpr int QN = D / 32, DT = D / 32;           // runs of 32 elements of d in a key; blocks of 32 rows of O^T
+  constexpr int KPIECES = PAGE * D / 16 / 256 > 0 ? PAGE * D / 16 / 256 : 1;  // 16-byte pieces a thread brings of a page's keys, and of its values
+  constexpr int KP_ROW = D / 16;                    // pieces of a key
+  __shared__ __attribute__((aligned(16))) unsigned char keys[2][PAGE * D], values[2][PAGE * D];
+  __shared__ int bad[3];                            // NaN among values that some row does not see
+  const int group = p.group.d;
+  // The items at the end of a sequence are the longest: they start first, for all heads.
+  const int at_item = blockIdx.x / p.kv_heads, head = blockIdx.x - at_item * p.kv_heads, item = gridDim.x / p.kv_heads - 1 - at_item;
+  const Place s = locate(p.q, item, [group](const Place &s) { return (int)(((long long)s.n * group + MANY - 1) / MANY); });
+  if (s.n == 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
+  const int past = s.len - s.n;
+  const int row0 = s.index * MANY, flat = row0 + 32 * wave + li, token = wdh::fdiv(flat, p.group), sub = flat - token * group;
+  const bool live = token < s.n;
+  const int limit = live ? past + token : -1;
+  const int first_limit = past + wdh::fdiv(row0, p.group);  // of the item's first row
+  const int last_token = wdh::fdiv(row0 + MANY - 1, p.group), last_key = past + (last_token < s.n ? last_token : s.n - 1);
+  const int seen = last_key / PAGE + 1, begin = (int)((long long)seen * blockIdx.y / gridDim.y), end = (int)((long long)seen * (blockIdx.y + 1) / gridDim.y);
+  // this wavefront's own pages end earlier
+  const int wave_last = wdh::fdiv(row0 + 32 * wave + 31, p.group), wave_end = wdh::fdiv(row0 + 32 * wave, p.group) < s.n ? (past + (wave_last < s.n ? wave_last : s.n - 1)) / PAGE + 1 : 0;
+  const int wave_first = past + wdh::fdiv(row0 + 32 * wave, p.group);
+  const int *table = p.q.table + (long long)s.seq * p.q.max_pages;
+
+  struct Page { long long at; float ks, vs; };
+  auto find = [&](int pg) {
+    const int id = scalar(table, pg < seen ? pg : seen - 1);
+    const bool known = id >= 0 && id < p.q.pages;
+    const long long at = (long long)(known ? id : 0) * p.kv_heads + head;
+    float ks = scalar(p.KS, at), vs = scalar(p.VS, at);
+    if (!known || !(ks > 0.0f) || !(vs > 0.0f && vs <= FLT_MAX)) ks = NAN, vs = 0.0f;
+    return Page{at, ks, vs};
+  };
+  i32x4 kr[KPIECES], vr[KPIECES];
+  const bool brings = PAGE * D / 16 >= 256 || tid < PAGE * D / 16;
+  auto fetch = [&](long long at) {
+    const unsigned char *kp = p.KP + at * (PAGE * D), *vp = p.VP + at * (PAGE * D);
+    if (brings)
+#pragma unroll
+      for (int i = 0; i < KPIECES; i++) {
+        kr[i] = *reinterpret_cast<const i32x4 *>(kp + 16 * (tid + 256 * i));
+        vr[i] = *reinterpret_cast<const i32x4 *>(vp + 16 * (tid + 256 * i));
+      }
+  };
+  auto key_place = [](int row, int piece) { return row * D + 16 * (D == 128 ? piece ^ (row & 7) : D == 64 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1)); };
+  auto value_place = [](int row, int piece) { return row * PAGE + 16 * (piece ^ ((row >> 1) & 3)); };
+  auto keep = [&](int buf, int pg) {
+    if (!brings) return;
+#pragma unroll
+    for (int i = 0; i < KPIECES; i++) {
+      const int at = tid + 256 * i;
+      *reinterpret_cast<i32x4 *>(&keys[buf][key_place(at / KP_ROW, at % KP_ROW)]) = kr[i];
+      i32x4 v = vr[i];
+      if (pg * PAGE + PAGE - 1 > first_limit) {  // some row does not see all of the page: see attend_rows
+        const int behind = s.len - pg * PAGE - 16 * (at & 3);
+        int nans = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const int n = behind - 4 * w;
+          const unsigned b = (unsigned)v[w] & (n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
+          const unsigned nan = ((b & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+          nans |= (int)nan;
+          v[w] = (int)(b & ~((nan >> 7) * 0xffu));
+        }
+        if (nans) bad[pg % 3] = 1;
+      }
+      *reinterpret_cast<i32x4 *>(&values[buf][value_place(at >> 2, at & 3)]) = v;
+    }
+  };
+
+  // queries, scaled, in three parts: lane's row, 8 elements for each instruction
+  bf16x8 q[2 * QN][3];
+  {
+    const float *qrow = p.Q + (long long)(s.row0 + (live ? token : 0)) * p.q_stride + (long long)(head * group + sub) * D;
+#pragma unroll
+    for (int i = 0; i < 2 * QN; i++) {
+      const int d0 = 32 * (i / 2) + 16 * half + 8 * (i & 1);
+      const f32x4 a = *reinterpret_cast<const f32x4 *>(qrow + d0), b = *reinterpret_cast<const f32x4 *>(qrow + d0 + 4);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = a[e] * p.scale, x[4 + e] = b[e] * p.scale;
+      split3(x, q[i]);
+    }
+  }
+  f32x16 o[DT];
+#pragma unroll
+  for (int i = 0; i < DT; i++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
+  float top = -INFINITY, sum = 0.0f;
+  if (tid < 3) bad[tid] = 0;
+  Page now = find(begin), then = now;
+  __syncthreads();
+  if (begin < end) {
+    fetch(now.at);
+    keep(0, begin);
+  }
+  __syncthreads();
+  for (int pg = begin; pg < end; pg++) {
+    const int buf = (pg - begin) & 1;
+    if (tid == 0) bad[(pg + 2) % 3] = 0;  // (read in the last turn, written in the next)
+    if (pg + 1 < end) {
+      then = find(pg + 1);
+      fetch(then.at);
+    }
+    if (pg < wave_end) {
+      const bool whole = pg * PAGE + PAGE - 1 <= wave_first;
+      const float c = now.ks;
+#pragma unroll
+      for (int t = 0; t < 2; t++) {  // 32 keys at a time: registers hold no more beside the queries
+        f32x16 sc;
+#pragma unroll
+        for (int e = 0; e < 16; e++) sc[e] = 0.0f;
+        const int row = 32 * t + 16 * ((li >> 2) & 1) + 4 * (li >> 3) + (li & 3);
+#pragma unroll
+        for (int i = 0; i < QN; i++) {
+          const i32x4 x = *reinterpret_cast<const i32x4 *>(&keys[buf][key_place(row, 2 * i + half)]);
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const bf16x8 kw = widen(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+            for (int part = 2; part >= 0; part--) sc = mfma32(kw, q[2 * i + j][part], sc);
+          }
+        }
+        // lane: keys 32 t + 16 half + r of the page
+        const int ahead = limit - pg * PAGE - 32 * t - 16 * half;
+        if (!whole)
+#pragma unroll
+          for (int r = 0; r < 16; r++) sc[r] = r <= ahead ? sc[r] : -INFINITY;
+        float most = sc[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) most = fmaxf(most, sc[r]);
+        most = fmaxf(halves_max(most) * c, top);  // (c is positive, or NaN: then top stays)
+        const float ref = most == -INFINITY ? 0.0f : most;
+        if (__any(most > top)) {
+          const float back = __builtin_amdgcn_exp2f(top - ref);
+          sum *= back;
+#pragma unroll
+          for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[i][e] *= back;
+        }
+        top = most;
+#pragma unroll
+        for (int r = 0; r < 16; r++) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c, -ref));
+        if (!whole && !(c == c))  // a page that is not there: NaN for the keys that the row sees, nothing for the others
+#pragma unroll
+          for (int r = 0; r < 16; r++) sc[r] = r <= ahead ? sc[r] : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r++) sum += sc[r];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) y[e] = sc[8 * u + e] * now.vs;
+          bf16x8 pr[3];
+          split3(y, pr);
+#pragma unroll
+          for (int i = 0; i < DT; i++) {
+            const i32x2 v = *reinterpret_cast<const i32x2 *>(&values[buf][value_place(32 * i + li, 2 * t + half) + 8 * u]);
+            const bf16x8 vw = widen(v[0], v[1]);
+#pragma unroll
+            for (int part = 2; part >= 0; part--) o[i] = mfma32(vw, pr[part], o[i]);
+          }
+        }
+      }
+      if (bad[pg % 3]) {
+        const unsigned char *vp = p.VP + now.at * (PAGE * D);
+#pragma unroll
+        for (int i = 0; i < DT; i++) {
+          unsigned nan = 0;
+#pragma unroll 1
+          for (int e = 0; e < 16; e++)
+#pragma unroll 1
+            for (int j = 0; j < PAGE && pg * PAGE + j <= limit; j++)
+              if ((vp[(32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << e;
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[i][e] = (nan >> e) & 1 ? NAN : o[i][e];
+        }
+      }
+    }
+    if (pg + 1 < end) keep(buf ^ 1, pg + 1);
+    now = then;
+    __syncthreads();
+  }
+  {
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+    sum = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  }
+  if (!live) return;
+  // lane: row li of the wavefront's 32; registers 4 a .. + 3 of block i are elements 32 i + 8 a + 4 half .. + 3
+  if (gridDim.y == 1) {
+    float *y = p.Y + ((long long)(s.row0 + token) * p.heads + head * group + sub) * D;
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+      for (int a = 0; a < 4; a++) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = sum == 0.0f ? 0.0f : o[i][4 * a + e] / sum;
+        *reinterpret_cast<f32x4 *>(y + 32 * i + 8 * a + 4 * half) = v;
+      }
+  } else {
+    const long long at = (((long long)item * p.kv_heads + head) * gridDim.y + blockIdx.y) * MANY + 32 * wave + li;
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+      for (int a = 0; a < 4; a++)
+        *reinterpret_cast<f32x4 *>(p.partial + at * D + 32 * i + 8 * a + 4 * half) =
+            f32x4{o[i][4 * a], o[i][4 * a + 1], o[i][4 * a + 2], o[i][4 * a + 3]};
+    if (half == 0) {
+      p.stats[2 * at] = top;
+      p.stats[2 * at + 1] = sum;
+    }
+  }
+}
+
+// The parts of an item's pages together: a lane to four elements of a row, few parts.
+template <int D>
+__global__ __launch_bounds__(256) void attend_many_join(AttendParams p, int parts) {
+  constexpr int LANES = D / 4, ROWS = 256 / LANES;
+  const int group = p.group.d, head = blockIdx.y;
+  const Place s = locate(p.q, blockIdx.x, [group](const Place &s) { return (int)(((long long)s.n * group + MANY - 1) / MANY); });
+  const int row = blockIdx.z * ROWS + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const int flat = s.index * MANY + row, token = wdh::fdiv(flat, p.group);
+  if (token >= s.n) return;
+  const long long at = ((long long)blockIdx.x * p.kv_heads + head) * parts * MANY + row;
+  float top = -INFINITY;
+  for (int i = 0; i < parts; i++) top = fmaxf(top, p.stats[2 * (at + (long long)i * MANY)]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  float total = 0.0f;
+  for (int i = 0; i < parts; i++) {
+    const long long one = at + (long long)i * MANY;
+    const float f = __builtin_amdgcn_exp2f(p.stats[2 * one] - ref);
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(p.partial + one * D + 4 * lane);
+    total = __builtin_fmaf(f, p.stats[2 * one + 1], total);
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(f, x[e], y[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) y[e] = total == 0.0f ? 0.0f : y[e] / total;
+  *reinterpret_cast<f32x4 *>(p.Y + ((long long)(s.row0 + token) * p.heads + head * group + (flat - token * group)) * D + 4 * lane) = y;
+}
+
+template <int D>
+int launch_many(const AttendParams &p, long long items, int parts) {
+  hipStream_t st = wdh::stream();
+  hipLaunchKernelGGL((attend_many<D>), dim3((unsigned)(items * p.kv_heads), (unsigned)parts), dim3(256), 0, st, p);
+  WDH_LAUNCH_CHECK();
+  if (parts > 1) {
+    hipLaunchKernelGGL((attend_many_join<D>), dim3((unsigned)items, (unsigned)p.kv_heads, MANY * D / 1024), dim3(256), 0, st, p, parts);
+    WDH_LAUNCH_CHECK();
+  }
+  return WDH_OK;
+}
+
 template <int D>
 int launch_attend(const AttendParams &p, long long items) {
   hipStream_t st = wdh::stream();
@@ -708,25 +979,41 @@ extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_strid
   p.Y = (float *)py;
   p.heads = heads; p.kv_heads = kv_heads; p.group = wdh::make_fastdiv(heads / kv_heads);
   p.scale = alpha * 1.44269504088896341f;
-  // items of 16 rows: a sequence of n tokens has ceil(n group / 16)
-  const long long loose = (long long)tokens * p.group.d / 16 + seqs, tight = (long long)tokens * ((p.group.d + 15) / 16);
-  const long long items = loose < tight ? loose : tight;
+  // items of 16 or 128 rows: a sequence of n tokens has ceil(n group / rows); whichever bound of their number is lower
+  auto items_of_rows = [&](int rows) {
+    const long long loose = (long long)tokens * p.group.d / rows + seqs, tight = (long long)tokens * ((p.group.d + rows - 1) / rows);
+    return loose < tight ? loose : tight;
+  };
+  const bool many = (long long)tokens * p.group.d >= 64LL * seqs;  // (on average: more than half of an item of 128)
+  const long long items = items_of_rows(many ? MANY : 16);
   if (items > 0xffffffLL / 2) return fail(WDH_EINVAL, "%s: too many rows", who);
-  // As many workgroups as the chip holds at a time, or as there can be units.
-  const long long units = items * ((max_pages + 3) / 4), resident = 2LL * wdh::compute_units() / kv_heads;
-  if (units > (1LL << 30)) return fail(WDH_EINVAL, "%s: too many rows of tables so wide", who);
-  p.wgs = (int)(units < resident ? units : resident > 0 ? resident : 1);
   p.partial = p.stats = nullptr;
   wdh_buf work = 0;
-  if (max_pages > 4 && p.wgs > 1) {  // (items of one unit are never cut)
-    const size_t rows = (size_t)p.wgs * 2 * kv_heads * 16;
+  auto workspace = [&](size_t rows) {
     work = wdh_alloc(rows * (d + 2) * 4);
-    if (!work) return WDH_ENOMEM;
+    if (!work) return false;
     size_t have_bytes;
     p.partial = (float *)wdh::resolve(work, &have_bytes);
     p.stats = p.partial + rows * d;
+    return true;
+  };
+  int rc;
+  if (many) {
+    // pages are cut into parts where there are fewer items than the chip holds at a time
+    if (items * kv_heads > 0xffffffLL / 2) return fail(WDH_EINVAL, "%s: too many rows", who);
+    const long long have = items * kv_heads, wanted = 2LL * wdh::compute_units();
+    long long parts = have >= wanted ? 1 : wanted / have;
+    if (parts > (max_pages + 3) / 4) parts = (max_pages + 3) / 4;
+    if (parts > 1 && !workspace((size_t)have * parts * MANY)) return WDH_ENOMEM;
+    rc = d == 32 ? launch_many<32>(p, items, (int)parts) : d == 64 ? launch_many<64>(p, items, (int)parts) : launch_many<128>(p, items, (int)parts);
+  } else {
+    // as many workgroups as the chip holds at a time, or as there can be units
+    const long long units = items * ((max_pages + 3) / 4), resident = 2LL * wdh::compute_units() / kv_heads;
+    if (units > (1LL << 30)) return fail(WDH_EINVAL, "%s: too many rows of tables so wide", who);
+    p.wgs = (int)(units < resident ? units : resident > 0 ? resident : 1);
+    if (max_pages > 4 && p.wgs > 1 && !workspace((size_t)p.wgs * 2 * kv_heads * 16)) return WDH_ENOMEM;  // (items of one unit are never cut)
+    rc = d == 32 ? launch_attend<32>(p, items) : d == 64 ? launch_attend<64>(p, items) : launch_attend<128>(p, items);
   }
-  const int rc = d == 32 ? launch_attend<32>(p, items) : d == 64 ? launch_attend<64>(p, items) : launch_attend<128>(p, items);
   if (work) (void)wdh_free(work);
   return rc;
 }
