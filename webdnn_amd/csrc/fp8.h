@@ -21,6 +21,8 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef int i32_any __attribute__((aligned(1)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // |x| if x is finite, else 0: a block's scale follows its finite elements.
 __device__ __forceinline__ float finite_abs(float x) {
@@ -86,6 +88,15 @@ __device__ __forceinline__ bf16x8 widen(int lo, int hi) {
   u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, 1.0f, true);
   u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, 1.0f, false);
   u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, 1.0f, true);
+  return u.v;
+}
+// ... and as float16 (exact as well: 2^-9 to 448).
+__device__ __forceinline__ f16x8 widen_f16(int lo, int hi) {
+  union { f16x2 h[4]; f16x8 v; } u;
+  u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)lo, 1.0f, false);
+  u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)lo, 1.0f, true);
+  u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)hi, 1.0f, false);
+  u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)hi, 1.0f, true);
   return u.v;
 }
 

@@ -291,6 +291,31 @@ __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&part)[3]) {
   for (int k = 0; k < 3; k++) part[k] = r[k].v;
 }
 
+// The same for values below 2^127, rounded to nearest part by part: two subtractions of a bfloat16 from an fp32 number are one
+// instruction each (a dot product with -1 and 0, exact here), 7 instructions a pair where split3 takes 11.
+struct Minus { bf16x2 low, high; };
+__device__ __forceinline__ Minus minus_one() {
+  unsigned l = 0x0000bf80u, h = 0xbf800000u;
+  asm volatile("" : "+s"(l), "+s"(h));  // (as literals they would be taken for the inline constants of another type)
+  return Minus{__builtin_bit_cast(bf16x2, l), __builtin_bit_cast(bf16x2, h)};
+}
+__device__ __forceinline__ void split3_nearest(const float (&x)[8], Minus m, bf16x8 (&part)[3]) {
+  union { bf16x2 h[4]; bf16x8 v; } r[3];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      r[k].h[i] = __builtin_convertvector(f32x2{a, b}, bf16x2);
+      if (k == 2) break;
+      a = __builtin_amdgcn_fdot2_f32_bf16(r[k].h[i], m.low, a, false);
+      b = __builtin_amdgcn_fdot2_f32_bf16(r[k].h[i], m.high, b, false);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 3; k++) part[k] = r[k].v;
+}
+
 // Rows of an item against a part of their sequence's pages; the wavefronts of a workgroup take pages in turn.  Everything is
 // computed transposed:
 //   S^T [key][row] = K Q^T    (v_mfma_f32_16x16x32_bf16, K widened from e4m3, Q in three bfloat16 parts)
@@ -310,6 +335,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
   const unsigned k_lane = (16 * (i16 >> 2) + (i16 & 3)) * D + (D >= 64 ? 16 : 8) * g, v_lane = i16 * PAGE + 16 * g;  // (of a page)
   const int head = blockIdx.y;
   const int total = total_units(p), share = (total + p.wgs - 1) / p.wgs;
+  const Minus minus = minus_one();
   int unit = blockIdx.x * share;
   const int units_end = total - unit < share ? total : unit + share;
   Work w;
@@ -465,7 +491,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
 #pragma unroll
       for (int e = 0; e < 8; e++) y[e] = x[8 * u + e] * now.vs;
       bf16x8 pr[3];
-      split3(y, pr);
+      split3_nearest(y, minus, pr);
 #pragma unroll
       for (int i = 0; i < DT; i++) {
         const bf16x8 vw = widen(v[i][2 * u], v[i][2 * u + 1]);
@@ -673,19 +699,35 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
     }
   };
 
-  // queries, scaled, in three parts: lane's row, 8 elements for each instruction
-  bf16x8 q[2 * QN][3];
+  // Queries in two float16 parts, 8 elements of the lane's row for each instruction.  A row is brought to [2^14, 2^15) by a power of two:
+  // what two parts leave out is at most 2^-24 of its largest element, the size of an fp32 rounding in the sum that this element dominates.
+  const Minus minus = minus_one();
+  f16x8 q[2 * QN][2];
+  float row_scale;
   {
     const float *qrow = p.Q + (long long)(s.row0 + (live ? token : 0)) * p.q_stride + (long long)(head * group + sub) * D;
+    float x[2 * QN][8], most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2 * QN; i++) {
       const int d0 = 32 * (i / 2) + 16 * half + 8 * (i & 1);
       const f32x4 a = *reinterpret_cast<const f32x4 *>(qrow + d0), b = *reinterpret_cast<const f32x4 *>(qrow + d0 + 4);
-      float x[8];
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = a[e] * p.scale, x[4 + e] = b[e] * p.scale;
-      split3(x, q[i]);
+      for (int e = 0; e < 4; e++) x[i][e] = a[e] * p.scale, x[i][4 + e] = b[e] * p.scale;
+#pragma unroll
+      for (int e = 0; e < 8; e++) most = fmaxf(most, finite_abs(x[i][e]));
     }
+    const int exponent = (int)(__float_as_uint(halves_max(most)) >> 23);  // (of zeros and of subnormal rows: 0)
+    const int up = 141 - exponent < 126 ? 141 - exponent : 126;           // bias 127: the row times 2^up has exponent 14
+    const float to = __uint_as_float((unsigned)(127 + up) << 23);
+    row_scale = __uint_as_float((unsigned)(127 - up) << 23);
+#pragma unroll
+    for (int i = 0; i < 2 * QN; i++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float y = x[i][e] * to;
+        q[i][0][e] = (_Float16)y;
+        q[i][1][e] = (_Float16)(y - (float)q[i][0][e]);
+      }
   }
   f32x16 o[DT];
 #pragma unroll
@@ -710,7 +752,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
     }
     if (pg < wave_end) {
       const bool whole = pg * PAGE + PAGE - 1 <= wave_first;
-      const float c = now.ks;
+      const float c = now.ks * row_scale;
 #pragma unroll
       for (int t = 0; t < 2; t++) {  // 32 keys at a time: registers hold no more beside the queries
         f32x16 sc;
@@ -722,9 +764,9 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
           const i32x4 x = *reinterpret_cast<const i32x4 *>(&keys[buf][key_place(row, 2 * i + half)]);
 #pragma unroll
           for (int j = 0; j < 2; j++) {
-            const bf16x8 kw = widen(x[2 * j], x[2 * j + 1]);
+            const f16x8 kw = widen_f16(x[2 * j], x[2 * j + 1]);
 #pragma unroll
-            for (int part = 2; part >= 0; part--) sc = mfma32(kw, q[2 * i + j][part], sc);
+            for (int part = 1; part >= 0; part--) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kw, q[2 * i + j][part], sc, 0, 0, 0);
           }
         }
         // lane: keys 32 t + 16 half + r of the page
@@ -748,7 +790,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
         top = most;
 #pragma unroll
         for (int r = 0; r < 16; r++) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c, -ref));
-        if (!whole && !(c == c))  // a page that is not there: NaN for the keys that the row sees, nothing for the others
+        if (!whole && !(now.ks == now.ks))  // a page that is not there: NaN for the keys that the row sees, nothing for the others
 #pragma unroll
           for (int r = 0; r < 16; r++) sc[r] = r <= ahead ? sc[r] : 0.0f;
 #pragma unroll
@@ -759,7 +801,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 #pragma unroll
           for (int e = 0; e < 8; e++) y[e] = sc[8 * u + e] * now.vs;
           bf16x8 pr[3];
-          split3(y, pr);
+          split3_nearest(y, minus, pr);
 #pragma unroll
           for (int i = 0; i < DT; i++) {
             const i32x2 v = *reinterpret_cast<const i32x2 *>(&values[buf][value_place(32 * i + li, 2 * t + half) + 8 * u]);
