@@ -316,6 +316,20 @@ __device__ __forceinline__ void split3_nearest(const float (&x)[8], Minus m, bf1
   for (int k = 0; k < 3; k++) part[k] = r[k].v;
 }
 
+// Eight values of at most 2^15 as the sums of two float16 ones: off by at most 2^-23 of each and, where they are below 2^-1, half a
+// step of float16's least numbers (2^-25).
+__device__ __forceinline__ void split2_f16(const float (&x)[8], f16x8 (&part)[2]) {
+  union { f16x2 h[4]; f16x8 v; } r[2];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const f16x2 h = __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, f16x2);
+    r[0].h[i] = h;
+    r[1].h[i] = __builtin_convertvector(f32x2{__builtin_fmaf(-1.0f, (float)h[0], x[2 * i]), __builtin_fmaf(-1.0f, (float)h[1], x[2 * i + 1])}, f16x2);
+  }
+  part[0] = r[0].v;
+  part[1] = r[1].v;
+}
+
 // Rows of an item against a part of their sequence's pages; the wavefronts of a workgroup take pages in turn.  Everything is
 // computed transposed:
 //   S^T [key][row] = K Q^T    (v_mfma_f32_16x16x32_bf16, K widened from e4m3, Q in three bfloat16 parts)
@@ -616,13 +630,13 @@ __global__ __launch_bounds__(256) void attend_join(AttendParams p) {
 }
 
 // ---- attention of many rows ------------------------------------------------------------------
-// Prompts: items of 128 rows, 32 to a wavefront, that share the pages of their sequence through LDS (v_mfma_f32_32x32x16_bf16, the
+// Prompts: items of 128 rows, 32 to a wavefront, that share the pages of their sequence through LDS (v_mfma_f32_32x32x16_f16, the
 // same transposed products).  A page's 64 keys are two blocks of 32, in an order that leaves lanes of the lower half of a
 // wavefront keys 0..15 and of the upper half keys 16..31 of a block in one run, as the second product wants them.  In LDS, rows
 // (128 bytes of a key, 64 of a value's d) have their 16-byte pieces exchanged so that the rows a read takes lie on different banks.
 constexpr int MANY = 128;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float halves_max(float v) {
   auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
@@ -633,8 +647,8 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   constexpr int QN = D / 32, DT = D / 32;           // runs of 32 elements of d in a key; blocks of 32 rows of O^T
   constexpr int KPIECES = PAGE * D / 16 / 256 > 0 ? PAGE * D / 16 / 256 : 1;  // 16-byte pieces a thread brings of a page's keys, and of its values
   constexpr int KP_ROW = D / 16;                    // pieces of a key
-  __shared__ __attribute__((aligned(16))) unsigned char keys[2][PAGE * D], values[2][PAGE * D];
-  __shared__ int bad[3];                            // NaN among values that some row does not see
+  __shared__ __attribute__((aligned(16))) unsigned char keys[3][PAGE * D], values[3][PAGE * D];
+  __shared__ int bad[4];                            // NaN among values that some row does not see
   const int group = p.group.d;
   // The items at the end of a sequence are the longest: they start first, for all heads.
   const int at_item = blockIdx.x / p.kv_heads, head = blockIdx.x - at_item * p.kv_heads, item = gridDim.x / p.kv_heads - 1 - at_item;
@@ -653,14 +667,16 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   const int wave_first = past + wdh::fdiv(row0 + 32 * wave, p.group);
   const int *table = p.q.table + (long long)s.seq * p.q.max_pages;
 
-  struct Page { long long at; float ks, vs; };
+  struct Page { long long at; float ks, vs; bool known; };
   auto find = [&](int pg) {
     const int id = scalar(table, pg < seen ? pg : seen - 1);
-    const bool known = id >= 0 && id < p.q.pages;
+    bool known = id >= 0 && id < p.q.pages;
     const long long at = (long long)(known ? id : 0) * p.kv_heads + head;
     float ks = scalar(p.KS, at), vs = scalar(p.VS, at);
-    if (!known || !(ks > 0.0f) || !(vs > 0.0f && vs <= FLT_MAX)) ks = NAN, vs = 0.0f;
-    return Page{at, ks, vs};
+    // (a page that is not there, or has no scale, makes its rows NaN, at the end of its turn)
+    known = known && ks > 0.0f && ks <= FLT_MAX && vs > 0.0f && vs <= FLT_MAX;
+    if (!known) ks = FLT_MIN, vs = 0.0f;
+    return Page{at, ks, vs, known};
   };
   i32x4 kr[KPIECES], vr[KPIECES];
   const bool brings = PAGE * D / 16 >= 256 || tid < PAGE * D / 16;
@@ -693,7 +709,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
           nans |= (int)nan;
           v[w] = (int)(b & ~((nan >> 7) * 0xffu));
         }
-        if (nans) bad[pg % 3] = 1;
+        if (nans) bad[pg & 3] = 1;
       }
       *reinterpret_cast<i32x4 *>(&values[buf][value_place(at >> 2, at & 3)]) = v;
     }
@@ -701,7 +717,6 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 
   // Queries in two float16 parts, 8 elements of the lane's row for each instruction.  A row is brought to [2^14, 2^15) by a power of two:
   // what two parts leave out is at most 2^-24 of its largest element, the size of an fp32 rounding in the sum that this element dominates.
-  const Minus minus = minus_one();
   f16x8 q[2 * QN][2];
   float row_scale;
   {
@@ -735,51 +750,76 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 #pragma unroll
     for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
   float top = -INFINITY, sum = 0.0f;
-  if (tid < 3) bad[tid] = 0;
-  Page now = find(begin), then = now;
+  // Weights go in two float16 parts as well, times 2^15 and their page's scale over the largest scale so far, in whose units (times
+  // 2^-15) the output is held: what is left out of a key's share is at most 2^-23 of it and 2^-40 of the largest value.
+  float unit = 0.0f;
+
+  // Half a page of scores: 32 keys, of which a lane has keys 16 half + r of block t.
+  auto scores = [&](int buf, int t) {
+    f32x16 sc;
+#pragma unroll
+    for (int e = 0; e < 16; e++) sc[e] = 0.0f;
+    const int row = 32 * t + 16 * ((li >> 2) & 1) + 4 * (li >> 3) + (li & 3);
+#pragma unroll
+    for (int i = 0; i < QN; i++) {
+      const i32x4 x = *reinterpret_cast<const i32x4 *>(&keys[buf][key_place(row, 2 * i + half)]);
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const f16x8 kw = widen_f16(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+        for (int part = 1; part >= 0; part--) sc = mfma32(kw, q[2 * i + j][part], sc);
+      }
+    }
+    return sc;
+  };
+  // What a row does not see counts for nothing; the largest of the rest.
+  auto mask = [&](f32x16 &sc, int pg, int t) {
+    if (pg * PAGE + PAGE - 1 <= wave_first) return;
+    const int ahead = limit - pg * PAGE - 32 * t - 16 * half;
+#pragma unroll
+    for (int r = 0; r < 16; r++) sc[r] = r <= ahead ? sc[r] : -INFINITY;
+  };
+  auto largest = [&](const f32x16 &sc) {
+    float most = sc[0];
+#pragma unroll
+    for (int r = 1; r < 16; r++) most = fmaxf(most, sc[r]);
+    return halves_max(most);
+  };
+
+  if (tid < 4) bad[tid] = 0;
+  Page now = find(begin), then = find(begin + 1), after = find(begin + 2), later = after;
   __syncthreads();
   if (begin < end) {
     fetch(now.at);
     keep(0, begin);
+    if (begin + 1 < end) fetch(then.at);
   }
   __syncthreads();
+  // The scores of the next half page are multiplied while the present one's weights are worked out, in one stretch of
+  // instructions without branches: a wavefront then keeps the matrix cores busy by itself.  So keys have to be in LDS half a
+  // page early, and a page's place is free again a page and a half later: three places, one barrier a page.
+  f32x16 sc = scores(0, 0);
+  mask(sc, begin, 0);
+  float most = largest(sc);
+  int buf = 0;
   for (int pg = begin; pg < end; pg++) {
-    const int buf = (pg - begin) & 1;
-    if (tid == 0) bad[(pg + 2) % 3] = 0;  // (read in the last turn, written in the next)
-    if (pg + 1 < end) {
-      then = find(pg + 1);
-      fetch(then.at);
+    const int next_buf = buf == 2 ? 0 : buf + 1;
+    const bool active = pg < wave_end;
+    if (active && now.vs > unit) {
+      const float back = unit / now.vs;
+#pragma unroll
+      for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[i][e] *= back;
+      unit = now.vs;
     }
-    if (pg < wave_end) {
-      const bool whole = pg * PAGE + PAGE - 1 <= wave_first;
-      const float c = now.ks * row_scale;
+    const float weight = unit > 0.0f ? 32768.0f * (now.vs / unit) : 0.0f;
 #pragma unroll
-      for (int t = 0; t < 2; t++) {  // 32 keys at a time: registers hold no more beside the queries
-        f32x16 sc;
-#pragma unroll
-        for (int e = 0; e < 16; e++) sc[e] = 0.0f;
-        const int row = 32 * t + 16 * ((li >> 2) & 1) + 4 * (li >> 3) + (li & 3);
-#pragma unroll
-        for (int i = 0; i < QN; i++) {
-          const i32x4 x = *reinterpret_cast<const i32x4 *>(&keys[buf][key_place(row, 2 * i + half)]);
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            const f16x8 kw = widen_f16(x[2 * j], x[2 * j + 1]);
-#pragma unroll
-            for (int part = 1; part >= 0; part--) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kw, q[2 * i + j][part], sc, 0, 0, 0);
-          }
-        }
-        // lane: keys 32 t + 16 half + r of the page
-        const int ahead = limit - pg * PAGE - 32 * t - 16 * half;
-        if (!whole)
-#pragma unroll
-          for (int r = 0; r < 16; r++) sc[r] = r <= ahead ? sc[r] : -INFINITY;
-        float most = sc[0];
-#pragma unroll
-        for (int r = 1; r < 16; r++) most = fmaxf(most, sc[r]);
-        most = fmaxf(halves_max(most) * c, top);  // (c is positive, or NaN: then top stays)
-        const float ref = most == -INFINITY ? 0.0f : most;
-        if (__any(most > top)) {
+    for (int t = 0; t < 2; t++) {
+      if (active) {
+        const float c = now.ks * row_scale;  // (positive)
+        const float up = fmaxf(most * c, top), ref = up == -INFINITY ? 0.0f : up;
+        if (__any(up > top)) {
           const float back = __builtin_amdgcn_exp2f(top - ref);
           sum *= back;
 #pragma unroll
@@ -787,53 +827,66 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 #pragma unroll
             for (int e = 0; e < 16; e++) o[i][e] *= back;
         }
-        top = most;
+        top = up;
+        const f32x16 next = scores(t == 0 ? buf : next_buf, 1 - t);
 #pragma unroll
         for (int r = 0; r < 16; r++) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c, -ref));
-        if (!whole && !(now.ks == now.ks))  // a page that is not there: NaN for the keys that the row sees, nothing for the others
-#pragma unroll
-          for (int r = 0; r < 16; r++) sc[r] = r <= ahead ? sc[r] : 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; r++) sum += sc[r];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
           float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; e++) y[e] = sc[8 * u + e] * now.vs;
-          bf16x8 pr[3];
-          split3_nearest(y, minus, pr);
+          for (int e = 0; e < 8; e++) y[e] = sc[8 * u + e] * weight;
+          f16x8 pr[2];
+          split2_f16(y, pr);
 #pragma unroll
           for (int i = 0; i < DT; i++) {
             const i32x2 v = *reinterpret_cast<const i32x2 *>(&values[buf][value_place(32 * i + li, 2 * t + half) + 8 * u]);
-            const bf16x8 vw = widen(v[0], v[1]);
+            const f16x8 vw = widen_f16(v[0], v[1]);
 #pragma unroll
-            for (int part = 2; part >= 0; part--) o[i] = mfma32(vw, pr[part], o[i]);
+            for (int part = 1; part >= 0; part--) o[i] = mfma32(vw, pr[part], o[i]);
           }
         }
+        sc = next;
       }
-      if (bad[pg % 3]) {
-        const unsigned char *vp = p.VP + now.at * (PAGE * D);
+      if (t == 0) {
+        if (pg + 1 < end) keep(next_buf, pg + 1);
+        __syncthreads();
+        if (tid == 0) bad[(pg + 3) & 3] = 0;  // (of the page before, which nobody reads any more; written again three pages on)
+        if (pg + 2 < end) fetch(after.at);
+        later = find(pg + 3);
+        mask(sc, pg, 1);
+      } else {
+        mask(sc, pg + 1, 0);
+      }
+      if (active) most = largest(sc);
+    }
+    if (active && bad[pg & 3]) {
+      const unsigned char *vp = p.VP + now.at * (PAGE * D);
 #pragma unroll
-        for (int i = 0; i < DT; i++) {
-          unsigned nan = 0;
+      for (int i = 0; i < DT; i++) {
+        unsigned nan = 0;
 #pragma unroll 1
-          for (int e = 0; e < 16; e++)
+        for (int e = 0; e < 16; e++)
 #pragma unroll 1
-            for (int j = 0; j < PAGE && pg * PAGE + j <= limit; j++)
-              if ((vp[(32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << e;
+          for (int j = 0; j < PAGE && pg * PAGE + j <= limit; j++)
+            if ((vp[(32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << e;
 #pragma unroll
-          for (int e = 0; e < 16; e++) o[i][e] = (nan >> e) & 1 ? NAN : o[i][e];
-        }
+        for (int e = 0; e < 16; e++) o[i][e] = (nan >> e) & 1 ? NAN : o[i][e];
       }
     }
-    if (pg + 1 < end) keep(buf ^ 1, pg + 1);
+    if (active && !now.known && limit >= pg * PAGE) sum = NAN;
     now = then;
-    __syncthreads();
+    then = after;
+    after = later;
+    buf = next_buf;
   }
   {
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     sum = __uint_as_float(b[0]) + __uint_as_float(b[1]);
   }
+  unit *= 1.0f / 32768.0f;
   if (!live) return;
   // lane: row li of the wavefront's 32; registers 4 a .. + 3 of block i are elements 32 i + 8 a + 4 half .. + 3
   if (gridDim.y == 1) {
@@ -844,7 +897,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
       for (int a = 0; a < 4; a++) {
         f32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = sum == 0.0f ? 0.0f : o[i][4 * a + e] / sum;
+        for (int e = 0; e < 4; e++) v[e] = sum == 0.0f ? 0.0f : o[i][4 * a + e] * unit / sum;
         *reinterpret_cast<f32x4 *>(y + 32 * i + 8 * a + 4 * half) = v;
       }
   } else {
@@ -854,7 +907,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 #pragma unroll
       for (int a = 0; a < 4; a++)
         *reinterpret_cast<f32x4 *>(p.partial + at * D + 32 * i + 8 * a + 4 * half) =
-            f32x4{o[i][4 * a], o[i][4 * a + 1], o[i][4 * a + 2], o[i][4 * a + 3]};
+            f32x4{o[i][4 * a] * unit, o[i][4 * a + 1] * unit, o[i][4 * a + 2] * unit, o[i][4 * a + 3] * unit};
     if (half == 0) {
       p.stats[2 * at] = top;
       p.stats[2 * at + 1] = sum;
