@@ -13,7 +13,6 @@ namespace {
 using namespace wdh::fp8;
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 struct ProductParams {
@@ -22,6 +21,7 @@ struct ProductParams {
   float *Y;
   long long m;
   int n, k, blocks, relu;
+  long long pitch;  // bytes between rows of A, and of W
 };
 
 // 32 bytes a lane of each operand: the lanes that share a row hold its 128 elements, in the same order on both sides.
@@ -33,21 +33,66 @@ __device__ __forceinline__ f32x4 block_product(i32x8 a, i32x8 b) {
   return c;
 }
 
-// Bytes k .. k+15 of a row of length `len`, 0 beyond its end.
+// Bytes k .. k+15 of a row of length `len`, 0 beyond its end.  Rows of whole 16-byte pieces are loaded as they lie; others dword by
+// dword (the hardware takes loads off dword boundaries, but slowly) and put together where they are used, so that nothing
+// waits for them before.  Every dword read holds a byte of the row.
 template <bool ALIGNED>
-__device__ __forceinline__ i32x4 load16(const unsigned char *row, int k, int len) {
-  if (k + 16 <= len)
-    return ALIGNED ? *reinterpret_cast<const i32x4 *>(row + k) : (i32x4)*reinterpret_cast<const i32x4_any *>(row + k);
-  i32x4 v = {0, 0, 0, 0};
-  if (!ALIGNED)  // (rows of whole pieces end where a piece does)
-    for (int e = 0; e < 15 && k + e < len; e++) v[e >> 2] |= (int)row[k + e] << (8 * (e & 3));
-  return v;
-}
+struct Piece {
+  i32x4 d;
+  __device__ __forceinline__ void load(const unsigned char *row, int k, int len) {
+    if (k < len) d = *reinterpret_cast<const i32x4 *>(row + k);
+    else d = i32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ i32x4 get(const unsigned char *, int, int) const { return d; }
+};
+template <>
+struct Piece<false> {
+  i32x4 d;
+  int e;
+  __device__ __forceinline__ void load(const unsigned char *row, int k, int len) {
+    const int left = len - k, from = left > 0 ? k : len - 1;  // (behind the end: the last byte's dword, of which nothing is kept)
+    const uintptr_t at = (uintptr_t)(row + from);
+    const int *base = reinterpret_cast<const int *>(at & ~(uintptr_t)3);
+    const unsigned shift = (unsigned)at & 3u;
+    if (left >= 16) {
+      typedef int i32x4_dwords __attribute__((ext_vector_type(4), aligned(4)));
+      d = *reinterpret_cast<const i32x4_dwords *>(base);
+      e = base[(shift + 15) >> 2];
+    } else {
+      const int last = (int)(shift + (left > 0 ? left : 1) - 1) >> 2;
+#pragma unroll
+      for (int i = 0; i < 4; i++) d[i] = base[i < last ? i : last];
+      e = base[last];
+    }
+  }
+  __device__ __forceinline__ i32x4 get(const unsigned char *row, int k, int len) const {
+    const unsigned shift = (unsigned)((uintptr_t)row + k) & 3u;
+    i32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = (int)__builtin_amdgcn_alignbyte((unsigned)(i < 3 ? d[i + 1] : e), (unsigned)d[i], shift);
+    const int left = len - k;
+    if (left < 16)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int n = left - 4 * i;
+        v[i] &= n >= 4 ? -1 : n <= 0 ? 0 : (int)((1u << (8 * n)) - 1u);
+      }
+    return v;
+  }
+};
+// 32 bytes: a lane's share of a block.
 template <bool ALIGNED>
-__device__ __forceinline__ i32x8 load32(const unsigned char *row, int k, int len) {
-  const i32x4 a = load16<ALIGNED>(row, k, len), b = load16<ALIGNED>(row, k + 16, len);
-  return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
+struct Pieces {
+  Piece<ALIGNED> a, b;
+  __device__ __forceinline__ void load(const unsigned char *row, int k, int len) {
+    a.load(row, k, len);
+    b.load(row, k + 16, len);
+  }
+  __device__ __forceinline__ i32x8 get(const unsigned char *row, int k, int len) const {
+    const i32x4 x = a.get(row, k, len), y = b.get(row, k + 16, len);
+    return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  }
+};
 
 // Columns j .. j+3 of row i: bias, residual, Relu, and out.
 __device__ __forceinline__ void finish4(const ProductParams &p, long long i, int j, f32x4 v) {
@@ -62,53 +107,91 @@ __device__ __forceinline__ void finish4(const ProductParams &p, long long i, int
   store4(y, j, p.n, v);
 }
 
-// Few rows of A: a workgroup has 16 rows of W and 16 MT of A, its wavefronts take K blocks in turn and add up through LDS.
-template <int MT, bool ALIGNED>
-__global__ __launch_bounds__(256) void product_few(ProductParams p) {
-  __shared__ __attribute__((aligned(16))) f32x4 part[4][MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const unsigned char *w = p.W + (long long)(n0 + i16 < p.n ? n0 + i16 : p.n - 1) * p.k;
-  const float *sw = p.SW + (long long)(n0 / BLOCK) * p.blocks;
+// Few rows of A, or few results: a workgroup has 16 NT rows of W and 16 MT of A, its wavefronts take K blocks in turn, U at a time,
+// straight from memory into operand registers, and add up through LDS.  Bound: memory (W is read once for 16 MT rows), or latency: so
+// a wavefront asks for all of its U blocks at once.
+template <int NT, int MT, int WAVES, int U, bool ALIGNED>
+__global__ __launch_bounds__(64 * WAVES) void product_few(ProductParams p) {
+  __shared__ __attribute__((aligned(16))) f32x4 part[WAVES][NT * MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * (16 * NT);
+  const unsigned char *w[NT];
+  const float *sw[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int j = n0 + 16 * t + i16, tile = n0 + 16 * t;
+    w[t] = p.W + (long long)(j < p.n ? j : p.n - 1) * p.pitch;
+    sw[t] = p.SW + (long long)((tile < p.n ? tile : p.n - 1) / BLOCK) * p.blocks;
+  }
   for (long long m0 = (long long)blockIdx.y * (16 * MT); m0 < p.m; m0 += (long long)gridDim.y * (16 * MT)) {
-    long long row[MT];
-    f32x4 acc[MT];
+    const unsigned char *a[MT];
+    const float *sa[MT];
+    f32x4 acc[NT][MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) {
-      const long long r = m0 + 16 * t + i16;
-      row[t] = r < p.m ? r : p.m - 1;
-      acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const long long r = m0 + 16 * t + i16 < p.m ? m0 + 16 * t + i16 : p.m - 1;
+      a[t] = p.A + r * p.pitch;
+      sa[t] = p.SA + r * p.blocks;
+#pragma unroll
+      for (int q = 0; q < NT; q++) acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int b = wave; b < p.blocks; b += 4) {
-      const i32x8 a = load32<ALIGNED>(w, b * BLOCK + 32 * g, p.k);
-      const float s = sw[b];
+    for (int b0 = wave; b0 < p.blocks; b0 += WAVES * U) {
+      Pieces<ALIGNED> wv[U][NT], av[U][MT];
+      float sav[U][MT], swv[U][NT];
 #pragma unroll
-      for (int t = 0; t < MT; t++) {
-        const f32x4 x = block_product(a, load32<ALIGNED>(p.A + row[t] * p.k, b * BLOCK + 32 * g, p.k));
-        const float c = p.SA[row[t] * p.blocks + b] * s;
+      for (int u = 0; u < U; u++) {
+        const int b = b0 + WAVES * u;
+        if (b >= p.blocks) break;
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[t][e] = __builtin_fmaf(x[e], c, acc[t][e]);
+        for (int t = 0; t < NT; t++) wv[u][t].load(w[t], b * BLOCK + 32 * g, p.k), swv[u][t] = sw[t][b];
+#pragma unroll
+        for (int t = 0; t < MT; t++) av[u][t].load(a[t], b * BLOCK + 32 * g, p.k), sav[u][t] = sa[t][b];
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int b = b0 + WAVES * u;
+        if (b >= p.blocks) break;
+        i32x8 x8[NT];
+#pragma unroll
+        for (int q = 0; q < NT; q++) x8[q] = wv[u][q].get(w[q], b * BLOCK + 32 * g, p.k);
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+          const i32x8 y8 = av[u][t].get(a[t], b * BLOCK + 32 * g, p.k);
+#pragma unroll
+          for (int q = 0; q < NT; q++) {
+            const f32x4 x = block_product(x8[q], y8);
+            const float c = sav[u][t] * swv[u][q];
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[q][t][e] = __builtin_fmaf(x[e], c, acc[q][t][e]);
+          }
+        }
       }
     }
 #pragma unroll
-    for (int t = 0; t < MT; t++) part[wave][t][lane] = acc[t];
+    for (int q = 0; q < NT; q++)
+#pragma unroll
+      for (int t = 0; t < MT; t++) part[wave][q * MT + t][lane] = acc[q][t];
     __syncthreads();
-    for (int cell = threadIdx.x; cell < 64 * MT; cell += 256) {
-      const int t = cell >> 6, l = cell & 63;
-      const f32x4 v = (part[0][t][l] + part[1][t][l]) + (part[2][t][l] + part[3][t][l]);
-      const long long i = m0 + 16 * t + (l & 15);
-      if (i < p.m) finish4(p, i, n0 + 4 * (l >> 4), v);
+    for (int cell = threadIdx.x; cell < 64 * NT * MT; cell += 64 * WAVES) {
+      const int tile = cell >> 6, l = cell & 63;
+      f32x4 v = part[0][tile][l];
+#pragma unroll
+      for (int i = 1; i < WAVES; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += part[i][tile][l][e];
+      const long long i = m0 + 16 * (tile % MT) + (l & 15);
+      if (i < p.m) finish4(p, i, n0 + 16 * (tile / MT) + 4 * (l >> 4), v);
     }
     __syncthreads();
   }
 }
 
-template <int MT>
+template <int NT, int MT, int WAVES, int U>
 void launch_few(const ProductParams &p, bool aligned) {
   const long long rows = (p.m + 16 * MT - 1) / (16 * MT);
-  const dim3 grid((unsigned)((p.n + 15) / 16), (unsigned)(rows < 65535 ? rows : 65535));
-  if (aligned) hipLaunchKernelGGL((product_few<MT, true>), grid, dim3(256), 0, wdh::stream(), p);
-  else hipLaunchKernelGGL((product_few<MT, false>), grid, dim3(256), 0, wdh::stream(), p);
+  const dim3 grid((unsigned)((p.n + 16 * NT - 1) / (16 * NT)), (unsigned)(rows < 65535 ? rows : 65535)), wg(64 * WAVES);
+  if (aligned) hipLaunchKernelGGL((product_few<NT, MT, WAVES, U, true>), grid, wg, 0, wdh::stream(), p);
+  else hipLaunchKernelGGL((product_few<NT, MT, WAVES, U, false>), grid, wg, 0, wdh::stream(), p);
 }
 
 // Tiles of NW TN x 32 columns of Y (rows of W) and MW TM x 32 rows: NW x MW wavefronts with TN x TM blocks of 32 x 32 each.
@@ -118,7 +201,7 @@ void launch_few(const ProductParams &p, bool aligned) {
 // last eight of them, on both sides alike).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <int NW, int MW, int TN, int TM, bool ALIGNED>
+template <int NW, int MW, int TN, int TM, int DEPTH>
 __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p) {
   constexpr int THREADS = 64 * NW * MW, BN = 32 * NW * TN, BM = 32 * MW * TM, ROWS = BN + BM;
   constexpr int LOADS = ROWS * 8 / THREADS;
@@ -127,17 +210,18 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
   __shared__ float scales[2][BM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int wn = wave % NW, wm = wave / NW;
+  // (Workgroups go to the eight XCDs in turn: those that run at a time on one of them are a block of several columns by several rows of
+  // tiles.  A strip of neighbouring columns for each XCD, which reads W once, is slower: 8192^3 1139 / 1363 us.)
   const int tiles_n = (p.n + BN - 1) / BN;
   const long long m0 = (long long)(blockIdx.x / tiles_n) * BM;
   const int n0 = (int)(blockIdx.x % tiles_n) * BN;
-
   const unsigned char *row[LOADS];
   int to[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; i++) {
     const int at = tid + THREADS * i, r = at >> 3;
-    if (r < BN) row[i] = p.W + (long long)(n0 + r < p.n ? n0 + r : p.n - 1) * p.k;
-    else row[i] = p.A + (m0 + r - BN < p.m ? m0 + r - BN : p.m - 1) * p.k;
+    if (r < BN) row[i] = p.W + (long long)(n0 + r < p.n ? n0 + r : p.n - 1) * p.pitch;
+    else row[i] = p.A + (m0 + r - BN < p.m ? m0 + r - BN : p.m - 1) * p.pitch;
     to[i] = r * BLOCK + 16 * ((at & 7) ^ (r & 7));
   }
   const int piece = 16 * (tid & 7);
@@ -145,17 +229,19 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
   const int wide = (n0 + 32 * TN * wn) / BLOCK;  // (columns beyond n: any scale will do)
   const float *sw = p.SW + (long long)(wide * BLOCK < p.n ? wide : 0) * p.blocks;
 
-  i32x4 next[LOADS];
-  float next_scale = 0.0f;
-  auto fetch = [&](int b) {
+  Piece<true> next[DEPTH][LOADS];
+  float next_scale[DEPTH];
+  auto fetch = [&](int slot, int b) {
+    if (b >= p.blocks) return;
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) next[i] = load16<ALIGNED>(row[i], b * BLOCK + piece, p.k);
-    if (tid < BM) next_scale = my_scale[b];
+    for (int i = 0; i < LOADS; i++) next[slot][i].load(row[i], b * BLOCK + piece, p.k);
+    if (tid < BM) next_scale[slot] = my_scale[b];
   };
-  auto keep = [&](int buf) {
+  auto keep = [&](int slot, int b) {
+    if (b >= p.blocks) return;
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) *reinterpret_cast<i32x4 *>(&lds[buf][to[i]]) = next[i];
-    if (tid < BM) scales[buf][tid] = next_scale;
+    for (int i = 0; i < LOADS; i++) *reinterpret_cast<i32x4 *>(&lds[b & 1][to[i]]) = next[slot][i].get(row[i], b * BLOCK + piece, p.k);
+    if (tid < BM) scales[b & 1][tid] = next_scale[slot];
   };
   // a 32-row block's fragments: 16 bytes for each quarter of the slab
   auto fragment = [&](int buf, int r0, bf16x8 (&f)[8]) {
@@ -175,42 +261,47 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
     for (int j = 0; j < TM; j++)
 #pragma unroll
       for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
-  if (p.blocks > 0) {
-    fetch(0);
-    keep(0);
-  }
+  // slab b goes to LDS through registers slot b % DEPTH, which then ask for slab b + DEPTH
+#pragma unroll
+  for (int d = 0; d < DEPTH; d++) fetch(d, d);
+  keep(0, 0);
+  fetch(0, DEPTH);
   __syncthreads();
-  for (int b = 0; b < p.blocks; b++) {
-    const int buf = b & 1;
-    if (b + 1 < p.blocks) fetch(b + 1);
-    const float s = sw[b];
-    bf16x8 a[TM][8];
-    float c[TM];
+  for (int b0 = 0; b0 < p.blocks; b0 += DEPTH) {
 #pragma unroll
-    for (int j = 0; j < TM; j++) {
-      fragment(buf, BN + 32 * (TM * wm + j), a[j]);
-      c[j] = scales[buf][32 * (TM * wm + j) + li] * s;
+    for (int d = 0; d < DEPTH; d++) {
+      const int b = b0 + d, buf = b & 1;
+      if (b >= p.blocks) break;
+      keep((d + 1) % DEPTH, b + 1);
+      fetch((d + 1) % DEPTH, b + 1 + DEPTH);
+      const float s = sw[b];
+      bf16x8 a[TM][8];
+      float c[TM];
+#pragma unroll
+      for (int j = 0; j < TM; j++) {
+        fragment(buf, BN + 32 * (TM * wm + j), a[j]);
+        c[j] = scales[buf][32 * (TM * wm + j) + li] * s;
+      }
+#pragma unroll
+      for (int i = 0; i < TN; i++) {
+        bf16x8 w[8];
+        fragment(buf, 32 * (TN * wn + i), w);
+        f32x16 x[TM];
+#pragma unroll
+        for (int j = 0; j < TM; j++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) x[j][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+#pragma unroll
+          for (int j = 0; j < TM; j++) x[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[k], a[j][k], x[j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < TM; j++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) acc[i][j][e] = __builtin_fmaf(x[j][e], c[j], acc[i][j][e]);
+      }
+      __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < TN; i++) {
-      bf16x8 w[8];
-      fragment(buf, 32 * (TN * wn + i), w);
-      f32x16 x[TM];
-#pragma unroll
-      for (int j = 0; j < TM; j++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[j][e] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 8; k++)
-#pragma unroll
-        for (int j = 0; j < TM; j++) x[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[k], a[j][k], x[j], 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < TM; j++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) acc[i][j][e] = __builtin_fmaf(x[j][e], c[j], acc[i][j][e]);
-    }
-    if (b + 1 < p.blocks) keep(buf ^ 1);
-    __syncthreads();
   }
   // lane: row li of a block; registers 4 q .. + 3 are columns 8 q + 4 half .. + 3
 #pragma unroll
@@ -228,13 +319,28 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
   }
 }
 
-template <int NW, int MW, int TN, int TM>
-void launch_tiles(const ProductParams &p, bool aligned) {
+template <int NW, int MW, int TN, int TM, int DEPTH>
+void launch_tiles(const ProductParams &p) {
   constexpr int BN = 32 * NW * TN, BM = 32 * MW * TM;
   const long long tiles = (p.n + BN - 1) / BN * ((p.m + BM - 1) / BM);
-  const dim3 grid((unsigned)tiles), wg(64 * NW * MW);
-  if (aligned) hipLaunchKernelGGL((product_tiles<NW, MW, TN, TM, true>), grid, wg, 0, wdh::stream(), p);
-  else hipLaunchKernelGGL((product_tiles<NW, MW, TN, TM, false>), grid, wg, 0, wdh::stream(), p);
+  hipLaunchKernelGGL((product_tiles<NW, MW, TN, TM, DEPTH>), dim3((unsigned)tiles), dim3(64 * NW * MW), 0, wdh::stream(), p);
+}
+
+// Rows of a length that is no multiple of 16, copied to rows that are (zeros behind their end): A's, then W's.
+__global__ __launch_bounds__(256) void pack_rows(const unsigned char *A, const unsigned char *W, unsigned char *to, long long m, long long rows, int k,
+                                                 long long pitch) {
+  for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += 4LL * gridDim.x) {
+    const unsigned char *row = r < m ? A + r * k : W + (r - m) * k;
+    for (int at = 16 * (threadIdx.x & 63); at < k; at += 4096) {
+      Piece<false> x[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (at + 1024 * i < k) x[i].load(row, at + 1024 * i, k);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (at + 1024 * i < k) *reinterpret_cast<i32x4 *>(to + r * pitch + at + 1024 * i) = x[i].get(row, at + 1024 * i, k);
+    }
+  }
 }
 
 }  // namespace
@@ -265,11 +371,41 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
   p.SA = (const float *)psa; p.SW = (const float *)psw; p.bias = (const float *)pb; p.R = (const float *)pr;
   p.Y = (float *)py;
   p.m = m; p.n = n; p.k = k; p.blocks = (int)blocks; p.relu = epilogue == WDH_EPI_RELU;
-  const bool aligned = k % 16 == 0;  // (buffers are)
-  if (m <= 16) launch_few<1>(p, aligned);
-  else if (m <= 64) launch_few<4>(p, aligned);
-  else if ((n + 127) / 128 * ((m + 127) / 128) < 2LL * wdh::compute_units()) launch_tiles<2, 2, 1, 1>(p, aligned);
-  else launch_tiles<4, 2, 2, 2>(p, aligned);
+  p.pitch = k;
+  // The smallest tile (columns x rows of Y) that leaves no more workgroups than the chip has CUs.
+  const long long cus = wdh::compute_units();
+  auto fits = [&](int cols, int rows) { return ((long long)n + cols - 1) / cols * ((m + rows - 1) / rows) <= cus; };
+  const bool few = m <= 16 || fits(64, 64);
+  // Tiles of many rows take rows of whole 16-byte pieces: others are copied first.
+  wdh_buf packed = 0;
+  bool aligned = k % 16 == 0;  // (buffers start on 512-byte boundaries)
+  if (!aligned && !few) {
+    const long long pitch = ((long long)k + 15) / 16 * 16, rows = m + n;
+    packed = wdh_alloc((size_t)(rows * pitch));
+    size_t have;
+    unsigned char *to = packed ? (unsigned char *)wdh::resolve(packed, &have) : nullptr;
+    if (to) {
+      hipLaunchKernelGGL(pack_rows, dim3((unsigned)(rows < (1 << 18) ? (rows + 3) / 4 : 1 << 16)), dim3(256), 0, wdh::stream(), p.A, p.W, to,
+                         (long long)m, rows, k, pitch);
+      p.A = to;
+      p.W = to + m * pitch;
+      p.pitch = pitch;
+      aligned = true;
+    }
+  }
+  if (few || !aligned) {  // (no room for the copy: the direct form takes any rows)
+    if (m <= 16) {
+      if (fits(16, 16)) launch_few<1, 1, 8, 4>(p, aligned);
+      else if (fits(32, 16)) launch_few<2, 1, 8, 4>(p, aligned);
+      else launch_few<4, 1, 8, 2>(p, aligned);
+    } else if (fits(16, 16)) launch_few<1, 1, 8, 4>(p, aligned);
+    else if (fits(32, 32)) launch_few<2, 2, 8, 2>(p, aligned);
+    else if (fits(64, 32)) launch_few<4, 2, 8, 1>(p, aligned);
+    else launch_few<4, 4, 8, 1>(p, aligned);
+  } else if (fits(128, 64)) launch_tiles<4, 2, 1, 1, 3>(p);
+  else if (fits(128, 128) || ((long long)n + 255) / 256 * ((m + 127) / 128) < 4 * cus) launch_tiles<4, 2, 1, 2, 2>(p);
+  else launch_tiles<4, 2, 2, 2, 1>(p);
+  if (packed) (void)wdh_free(packed);
   WDH_LAUNCH_CHECK();
   return WDH_OK;
 }
