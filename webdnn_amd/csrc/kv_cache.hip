@@ -130,26 +130,36 @@ __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
   const Place s = locate(p.q, blockIdx.x, [](const Place &s) { return (s.len - 1) / PAGE - (s.len - s.n) / PAGE + 1; });
   if (s.n == 0) return;
   const int before = s.len - s.n, pi = before / PAGE + s.index, id = p.q.table[(long long)s.seq * p.q.max_pages + pi];
-  if (id < 0 || id >= p.q.pages) return;
   const bool values = blockIdx.z;
   const int head = blockIdx.y, t = threadIdx.x;
   const int first = before > pi * PAGE ? before - pi * PAGE : 0, last = s.len - pi * PAGE < PAGE ? s.len - pi * PAGE : PAGE;
   const long long stride = values ? p.v_stride : p.k_stride;
-  // (token `slot` of the page is row row0 + pi*64 + slot - before of the call)
+  // (token `slot` of the page is row row0 + slot of the call)
   const float *x = (values ? p.V : p.K) + head * D;
   const long long row0 = (long long)s.row0 + (long long)pi * PAGE - before;
-  const long long at = (long long)id * p.heads + head;
-  unsigned char *page = (values ? p.VP : p.KP) + at * (PAGE * D);
-  float *scale = (values ? p.VS : p.KS) + at;
   f32x4 v[NP];
-  float amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < NP; i++) {
     const int slot = (t + 256 * i) / PPT, d0 = (t + 256 * i) % PPT * 4;
     v[i] = slot >= first && slot < last ? *reinterpret_cast<const f32x4 *>(x + (row0 + slot) * stride + d0) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (id < 0 || id >= p.q.pages) return;
+  const long long at = (long long)id * p.heads + head;
+  unsigned char *page = (values ? p.VP : p.KP) + at * (PAGE * D);
+  float *scale = (values ? p.VS : p.KS) + at;
+  // values: words of four tokens that the new ones share with others
+  int shared[NP];
+  if (values)
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int s0 = (t + 256 * i) % (PAGE / 4) * 4;
+      shared[i] = s0 < last && s0 + 4 > first && !(s0 >= first && s0 + 4 <= last) ? reinterpret_cast<const int *>(page)[t + 256 * i] : 0;
+    }
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NP; i++)
 #pragma unroll
     for (int e = 0; e < 4; e++) amax = fmaxf(amax, finite_abs(v[i][e]));
-  }
   const float old = first > 0 ? *scale : 0.0f;
   amax = wdh::rowmath::wave_max(amax);
   if ((t & 63) == 0) part[t >> 6] = amax;
@@ -177,7 +187,8 @@ __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
 #pragma unroll
       for (int e = 0; e < 4; e++) fresh |= (int)(((unsigned)turn[(s0 + e) * (PPT + 1) + d / 4] >> (8 * (d & 3))) & 0xffu) << (8 * e);
       int *to = reinterpret_cast<int *>(page) + t + 256 * i;
-      *to = s0 >= first && s0 + 4 <= last ? fresh : merge4(*to, fresh, first - s0, last - s0, grown, factor);
+      if (s0 >= first && s0 + 4 <= last) *to = fresh;
+      else *to = merge4(s0 + 4 <= first ? *to : shared[i], fresh, first - s0, last - s0, grown, factor);
     }
   }
   if (t == 0) *scale = c;
@@ -211,33 +222,43 @@ struct Work {
 };
 __device__ __forceinline__ int items_of(const Place &s, int group) { return s.n ? (int)(((long long)s.n * group + 15) / 16) : 0; }
 __device__ __forceinline__ int units_of(const Place &s) { return (s.len + 4 * PAGE - 1) / (4 * PAGE); }
-__device__ __forceinline__ int total_units(const AttendParams &p) {
-  int total = 0;
-  for (int i = 0; i < (p.q.seqs + 63) / 64; i++) {
-    const Place mine = sequence(p.q, 64 * i + fresh(threadIdx.x & 63));
-    total += __builtin_amdgcn_readlane(wave_scan(items_of(mine, p.group.d) * units_of(mine)), 63);
-  }
+// 64 sequences side by side, a lane to each; upto: units of these up to and with the lane's.
+struct Look {
+  Place mine;
+  int items, units, upto;
+};
+__device__ __forceinline__ Look look(const AttendParams &p, int round) {
+  Look l;
+  l.mine = sequence(p.q, 64 * round + fresh(threadIdx.x & 63));
+  l.items = items_of(l.mine, p.group.d);
+  l.units = units_of(l.mine);
+  l.upto = wave_scan(l.items * l.units);
+  return l;
+}
+__device__ __forceinline__ int total_units(const AttendParams &p, const Look &first) {
+  int total = __builtin_amdgcn_readlane(first.upto, 63);
+  for (int i = 1; i < (p.q.seqs + 63) / 64; i++) total += __builtin_amdgcn_readlane(look(p, i).upto, 63);
   return total;
 }
 // The item that holds unit number `index` of all (or, by_item, item number `index`); s.n = 0 behind the last.
-__device__ __forceinline__ Work locate_work(const AttendParams &p, int index, bool by_item) {
+__device__ __forceinline__ Work locate_work(const AttendParams &p, const Look &first, int index, bool by_item) {
   Work w;
   int before = 0, before_items = 0;
+  Look l = first;
   for (int i = 0; i < (p.q.seqs + 63) / 64; i++) {
-    const Place mine = sequence(p.q, 64 * i + fresh(threadIdx.x & 63));
-    const int items = items_of(mine, p.group.d), units = units_of(mine);
-    const int upto = before + wave_scan(items * units), upto_items = by_item ? before_items + wave_scan(items) : 0;
+    if (i) l = look(p, i);
+    const int upto = before + l.upto, upto_items = by_item ? before_items + wave_scan(l.items) : 0;
     const unsigned long long has = __ballot(index < (by_item ? upto_items : upto));
     if (has) {
       const int at = __ffsll(has) - 1;
-      w.s.seq = __builtin_amdgcn_readlane(mine.seq, at);
-      w.s.row0 = __builtin_amdgcn_readlane(mine.row0, at);
-      w.s.n = __builtin_amdgcn_readlane(mine.n, at);
-      w.s.len = __builtin_amdgcn_readlane(mine.len, at);
-      w.units = __builtin_amdgcn_readlane(units, at);
-      const int first = __builtin_amdgcn_readlane(upto - items * units, at);
-      w.item = by_item ? index - __builtin_amdgcn_readlane(upto_items - items, at) : (index - first) / w.units;
-      w.before = first + w.item * w.units;
+      w.s.seq = __builtin_amdgcn_readlane(l.mine.seq, at);
+      w.s.row0 = __builtin_amdgcn_readlane(l.mine.row0, at);
+      w.s.n = __builtin_amdgcn_readlane(l.mine.n, at);
+      w.s.len = __builtin_amdgcn_readlane(l.mine.len, at);
+      w.units = __builtin_amdgcn_readlane(l.units, at);
+      const int begin = __builtin_amdgcn_readlane(upto - l.items * l.units, at);
+      w.item = by_item ? index - __builtin_amdgcn_readlane(upto_items - l.items, at) : (index - begin) / w.units;
+      w.before = begin + w.item * w.units;
       w.unit = by_item ? 0 : index - w.before;
       return w;
     }
@@ -348,7 +369,8 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, g = lane >> 4;
   const unsigned k_lane = (16 * (i16 >> 2) + (i16 & 3)) * D + (D >= 64 ? 16 : 8) * g, v_lane = i16 * PAGE + 16 * g;  // (of a page)
   const int head = blockIdx.y;
-  const int total = total_units(p), share = (total + p.wgs - 1) / p.wgs;
+  const Look first = look(p, 0);
+  const int total = total_units(p, first), share = (total + p.wgs - 1) / p.wgs;
   const Minus minus = minus_one();
   int unit = blockIdx.x * share;
   const int units_end = total - unit < share ? total : unit + share;
@@ -361,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     w.before = unit;
     w.unit = 0;
   } else {
-    w = locate_work(p, unit, false);
+    w = locate_work(p, first_segment ? first : look(p, 0), unit, false);
     if (w.s.n == 0) return;  // (numbers that contradict each other)
   }
   const Place s = w.s;
@@ -577,14 +599,15 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
 }
 
 // What several workgroups have of an item together: a workgroup to a row (and every gridDim.z-th after it), four elements and
-// every (256 / (D/4))th of the shares to a lane.
-template <int D>
-__global__ __launch_bounds__(256) void attend_join(AttendParams p) {
-  constexpr int LANES = D / 4, SIDE = 256 / LANES;
+// every (threads / (D/4))th of the shares to a lane.
+template <int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void attend_join(AttendParams p) {
+  constexpr int LANES = D / 4, SIDE = THREADS / LANES;
   __shared__ __attribute__((aligned(16))) f32x4 results[SIDE][LANES];
   __shared__ float totals[SIDE];
-  const int head = blockIdx.y, total_u = total_units(p), share = (total_u + p.wgs - 1) / p.wgs;
-  const Work w = locate_work(p, blockIdx.x, true);
+  const Look first = look(p, 0);
+  const int head = blockIdx.y, total_u = total_units(p, first), share = (total_u + p.wgs - 1) / p.wgs;
+  const Work w = locate_work(p, first, blockIdx.x, true);
   if (w.s.n == 0 || share == 0) return;
   const int from_wg = w.before / share, to_wg = (w.before + w.units - 1) / share;
   if (from_wg == to_wg) return;
@@ -597,6 +620,7 @@ __global__ __launch_bounds__(256) void attend_join(AttendParams p) {
       return ((2LL * wg + (wg == from_wg && w.before != from_wg * share ? 1 : 0)) * p.kv_heads + head) * 16 + row;
     };
     float top = -INFINITY;
+#pragma unroll 4
     for (int i = from_wg + (threadIdx.x & 63); i <= to_wg; i += 64) top = fmaxf(top, p.stats[2 * slot(i)]);
     top = wdh::rowmath::wave_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
@@ -613,14 +637,17 @@ __global__ __launch_bounds__(256) void attend_join(AttendParams p) {
     }
     results[side][lane] = y;
     if (lane == 0) totals[side] = total;
-    __syncthreads();
+    for (int half = SIDE / 2; half; half >>= 1) {
+      __syncthreads();
+      if (side >= half) continue;
+      total += totals[side + half];
+      const f32x4 x = results[side + half][lane];
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] += x[e];
+      results[side][lane] = y;
+      if (lane == 0) totals[side] = total;
+    }
     if (side == 0) {
-#pragma unroll
-      for (int i = 1; i < SIDE; i++) {
-        total += totals[i];
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] += results[i][lane][e];
-      }
 #pragma unroll
       for (int e = 0; e < 4; e++) y[e] = total == 0.0f ? 0.0f : y[e] / total;
       *reinterpret_cast<f32x4 *>(p.Y + ((long long)(w.s.row0 + token) * p.heads + head * p.group.d + (flat - token * p.group.d)) * D + 4 * lane) = y;
@@ -961,7 +988,10 @@ int launch_attend(const AttendParams &p, long long items) {
   hipLaunchKernelGGL((attend_rows<D>), dim3((unsigned)p.wgs, (unsigned)p.kv_heads), dim3(256), 0, st, p);
   WDH_LAUNCH_CHECK();
   if (p.partial) {
-    hipLaunchKernelGGL((attend_join<D>), dim3((unsigned)items, (unsigned)p.kv_heads, (unsigned)(p.group.d < 16 ? p.group.d : 16)), dim3(256), 0, st, p);
+    // (an item of hundreds of shares is a wide workgroup's work, one of a few shares a small one's)
+    const dim3 grid((unsigned)items, (unsigned)p.kv_heads, (unsigned)(p.group.d < 16 ? p.group.d : 16));
+    if (p.wgs >= 32 * items) hipLaunchKernelGGL((attend_join<D, 1024>), grid, dim3(1024), 0, st, p);
+    else hipLaunchKernelGGL((attend_join<D, 256>), grid, dim3(256), 0, st, p);
     WDH_LAUNCH_CHECK();
   }
   return WDH_OK;

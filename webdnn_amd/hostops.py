@@ -95,12 +95,12 @@ class HipTensor:
         self._shared = shared
         shared["refs"] += 1
         self._disposed = False
+        self.handle = shared["handle"]  # (a plain attribute: every operator call reads several)
 
-    @property
-    def handle(self):
-        if self._disposed:
+    def __getattr__(self, name):
+        if name == "handle":            # dispose() took it away
             raise OperatorError("HipTensor used after dispose()")
-        return self._shared["handle"]
+        raise AttributeError(name)
 
     def alias(self, dims):
         """A tensor with other dims over the same buffer (zero-copy reshape)."""
@@ -134,6 +134,7 @@ class HipTensor:
         if self._disposed:
             return
         self._disposed = True
+        del self.handle
         self._shared["refs"] -= 1
         if self._shared["refs"] == 0:
             call("wdh_free", self._shared["handle"])
@@ -831,7 +832,6 @@ def _fp8_blocks(n):
 
 def _result(ctx, given, dims, data_type="float32"):
     """The buffer a result goes to: the caller's, if it has one of that shape and type."""
-    dims = [int(d) for d in dims]
     if given is None:
         return ctx.empty_tensor(dims, data_type)
     if given.dims != dims or given.data_type != data_type:
@@ -840,8 +840,8 @@ def _result(ctx, given, dims, data_type="float32"):
 
 
 def _require(what, tensor, dims, data_type="float32"):
-    if tensor.data_type != data_type or tensor.dims != list(dims):
-        raise OperatorError("%s: %s of shape %s expected, got %s of %s" % (what, data_type, list(dims), tensor.data_type, tensor.dims))
+    if tensor.data_type != data_type or tensor.dims != dims:
+        raise OperatorError("%s: %s of shape %s expected, got %s of %s" % (what, data_type, dims, tensor.data_type, tensor.dims))
 
 
 def _handle(tensor):
