@@ -53,6 +53,22 @@ function layernormRows(X, G, B, Y, outer, len, eps) {
   }
 }
 
+// e4m3: 1 sign, 4 exponent (bias 7), 3 fraction bits; steps of 2^-9 below 2^-6; 0x7f / 0xff are NaN
+const E4M3 = Array.from({ length: 256 }, (_, b) => {
+  const e = (b >> 3) & 15, f = b & 7, v = (b & 127) === 127 ? NaN : e ? (8 + f) * 2 ** (e - 10) : f * 2 ** -9;
+  return b & 128 ? -v : v;
+});
+function toE4m3(v) {
+  if (!isFinite(v)) return 0x7f;
+  const a = Math.min(Math.abs(v), 448);
+  let best = 0;
+  for (let b = 1; b < 127; b++) {
+    const d = Math.abs(E4M3[b] - a) - Math.abs(E4M3[best] - a);
+    if (d < 0 || (d === 0 && b % 2 === 0)) best = b;
+  }
+  return best | (v < 0 || Object.is(v, -0) ? 128 : 0);
+}
+
 const native = {
   init(device) {
     count("init");
@@ -269,6 +285,52 @@ const native = {
     for (let i = 0; i < outer * len; i++) y2[i] = y[i] + p[i];
   },
 
+  rmsnorm(X, Skip, Gamma, Sum, Y, Q, QScale, outer, len, eps) {
+    count("rmsnorm");
+    if (Q || QScale || !Y) throw new Error("fake rmsnorm: fp32 results only");
+    need(X, outer * len * 4, "wdh_rmsnorm: X"); need(Y, outer * len * 4, "wdh_rmsnorm: Y");
+    const x = f32(X), r = Skip ? f32(Skip) : null, g = Gamma ? f32(Gamma) : null, s = new Float32Array(len), y = f32(Y), t = new Float32Array(2);
+    for (let o = 0; o < outer; o++) {
+      let q = 0;
+      for (let i = 0; i < len; i++) { s[i] = x[o * len + i] + (r ? r[o * len + i] : 0); q += s[i] * s[i]; }
+      t[0] = 1 / Math.sqrt(q / len + Math.fround(eps));
+      if (Sum) f32(Sum).set(s, o * len);
+      for (let i = 0; i < len; i++) { t[1] = s[i] * t[0]; y[o * len + i] = g ? t[1] * g[i] : t[1]; }
+    }
+  },
+
+  quantizeFp8(X, Q, QScale, rows, cols, blockRows) {
+    count("quantizeFp8");
+    if (blockRows !== 1) throw new Error("fake quantizeFp8: rows only");
+    need(X, rows * cols * 4, "wdh_quantize_fp8: X"); need(Q, rows * cols, "wdh_quantize_fp8: Q");
+    const x = f32(X), q = buf(Q), c = f32(QScale), nb = Math.ceil(cols / 128);
+    for (let r = 0; r < rows; r++) for (let b = 0; b < nb; b++) {
+      let amax = 0;
+      const end = Math.min(cols, 128 * b + 128);
+      for (let i = 128 * b; i < end; i++) if (isFinite(x[r * cols + i])) amax = Math.max(amax, Math.abs(x[r * cols + i]));
+      const scale = Math.fround(Math.max(Math.fround(amax / 448), 2 ** -100));
+      c[r * nb + b] = scale;
+      for (let i = 128 * b; i < end; i++) q[r * cols + i] = toE4m3(x[r * cols + i] / scale);
+    }
+  },
+
+  gemmFp8(A, AScale, W, WScale, Bias, Y, m, n, k, epilogue, R) {
+    count("gemmFp8");
+    need(A, m * k, "wdh_gemm_fp8: A"); need(W, n * k, "wdh_gemm_fp8: W"); need(Y, m * n * 4, "wdh_gemm_fp8: Y");
+    const a = buf(A), w = buf(W), sa = f32(AScale), sw = f32(WScale), b = Bias ? f32(Bias) : null, r = R ? f32(R) : null, y = f32(Y);
+    const nb = Math.ceil(k / 128);
+    for (let i = 0; i < m; i++) for (let j = 0; j < n; j++) {
+      let s = 0;
+      for (let p = 0; p < k; p++) {
+        const block = p >> 7;
+        s += E4M3[a[i * k + p]] * E4M3[w[j * k + p]] * sa[i * nb + block] * sw[(j >> 7) * nb + block];
+      }
+      if (b) s += b[j];
+      if (r) s += r[i * n + j];
+      y[i * n + j] = epilogue === 1 ? Math.max(s, 0) : s;
+    }
+  },
+
   reduceAxis(X, Y, outer, red, inner, divisor) {
     count("reduceAxis");
     const x = f32(X), y = f32(Y);
@@ -377,7 +439,7 @@ const native = {
 // Like the library: between graphBegin and graphEnd compute calls are recorded, not executed;
 // alloc/free work, but a buffer freed meanwhile keeps its storage for the graph's lifetime;
 // calls that need device data on the host throw and spoil the capture.
-const RECORDED = ["copy", "gemm", "gemmEx", "linearGroup", "conv2d", "conv2dEx", "binary", "unary", "softmax", "attention", "layernorm", "layernormAdd", "reduceMean", "reduceAxis", "maxpool2d",
+const RECORDED = ["copy", "gemm", "gemmEx", "linearGroup", "conv2d", "conv2dEx", "binary", "unary", "softmax", "attention", "layernorm", "layernormAdd", "rmsnorm", "quantizeFp8", "gemmFp8", "reduceMean", "reduceAxis", "maxpool2d",
   "globalAvgpool", "transpose", "gather", "cast", "stridedCopy"];
 const REFUSED = ["write", "read", "sync", "trim", "eventRecord", "eventElapsedMs"];
 const graphs = new Map();

@@ -6,6 +6,8 @@
 const { TensorImpl } = require("../../core/tensorImpl");
 const { DataArrayConstructor } = require("../../interface/constants");
 
+const ELEMENT_BYTES = { float32: 4, int32: 4, float8e4m3fn: 1 };
+
 class HipSharedBuffer {
   constructor(native, byteLength) {
     this.native = native;
@@ -31,7 +33,7 @@ class HipSharedBuffer {
 class HipTensorImpl extends TensorImpl {
   constructor(context, dims, dataType, sharedBuffer) {
     super(dims, dataType || "float32", "hip");
-    if (this.dataType !== "float32" && this.dataType !== "int32") {
+    if (!(this.dataType in ELEMENT_BYTES)) {
       throw new Error(`HipTensor: dataType ${this.dataType} is not supported`);
     }
     this.context = context;
@@ -39,7 +41,7 @@ class HipTensorImpl extends TensorImpl {
       sharedBuffer.incrementRef();
       this.sharedBuffer = sharedBuffer;
     } else {
-      this.sharedBuffer = new HipSharedBuffer(context.native, this.length * 4);
+      this.sharedBuffer = new HipSharedBuffer(context.native, this.length * ELEMENT_BYTES[this.dataType]);
     }
     this.disposedFlag = false;
   }

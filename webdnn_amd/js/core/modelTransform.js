@@ -268,7 +268,7 @@ function fuseForHip(model) {
     graph.node = nodes.filter((n, idx) => !removed.has(idx));
     logger.info(`hip fusion: ${fusedCount} chains fused, ${removed.size} nodes removed`);
   }
-  return fusedCount + fuseAttention(graph) + fuseLayerNormAdd(graph) + groupLinears(graph);
+  return fusedCount + fuseAttention(graph) + fuseLayerNormAdd(graph) + fuseAddRMSNorm(graph) + groupLinears(graph);
 }
 
 // Neighbouring linear layers that do not read each other  ->  one WebDNNHipLinearGroup node.
@@ -376,6 +376,43 @@ function fuseLayerNormAdd(graph) {
   return count;
 }
 
+// Add -> RMSNormalization  ->  WebDNNHipAddRMSNorm with two outputs (the sum, which the graph usually reads again, and the
+// normalised sum), in the Add's place.  The scale has to be there by then: an initializer, a graph input or an earlier
+// node's output.  Of several RMSNormalizations of one sum the first qualifies.
+function fuseAddRMSNorm(graph) {
+  const nodes = graph.node;
+  const known = new Set(graph.initializer.map((t) => t.name));
+  for (const input of graph.input) known.add(input.name);
+  const removed = new Set();
+  let count = 0;
+  nodes.forEach((add, ai) => {
+    if (add.opType === "Add" && add.input.length === 2 && add.output.length === 1) {
+      const sum = add.output[0];
+      const ni = nodes.findIndex((n, idx) => idx > ai && !removed.has(idx) && n.opType === "RMSNormalization" && n.input.length === 2 &&
+        n.output.length === 1 && n.input[0] === sum && known.has(n.input[1]));
+      if (ni >= 0) {
+        const norm = nodes[ni];
+        nodes[ai] = {
+          input: [add.input[0], add.input[1], norm.input[1]],
+          output: [sum, norm.output[0]],
+          name: norm.name,
+          opType: "WebDNNHipAddRMSNorm",
+          attribute: norm.attribute,
+          domain: "webdnn.hip",
+        };
+        removed.add(ni);
+        count++;
+      }
+    }
+    for (const name of nodes[ai].output) known.add(name);
+  });
+  if (count > 0) {
+    graph.node = nodes.filter((n, idx) => !removed.has(idx));
+    logger.info(`hip fusion: ${count} Add + RMSNormalization pairs fused`);
+  }
+  return count;
+}
+
 // (Fused)MatMul -> Softmax -> (Fused)MatMul  ->  WebDNNHipAttention
 // where the first product carries nothing but operand permutations and a scale, the Softmax
 // normalises the last axis of its rank-3 result, and the second product takes the
@@ -469,4 +506,4 @@ function findTensorReleaseTiming(model, initializerTensorNames) {
   return timing;
 }
 
-module.exports = { modelTransform, findTensorReleaseTiming, fuseForHip, fuseAttention, fuseLayerNormAdd, groupLinears, hoistSideBranches };
+module.exports = { modelTransform, findTensorReleaseTiming, fuseForHip, fuseAttention, fuseLayerNormAdd, fuseAddRMSNorm, groupLinears, hoistSideBranches };

@@ -12,7 +12,7 @@
 // they are tensor data or exceed 2^53 (the reference clips them the same way:
 // src/descriptor_runner/util.ts:73-92).
 
-const DataType = { FLOAT: 1, UINT8: 2, INT8: 3, INT32: 6, INT64: 7, BOOL: 9 };
+const DataType = { FLOAT: 1, UINT8: 2, INT8: 3, INT32: 6, INT64: 7, BOOL: 9, FLOAT8E4M3FN: 17 };
 const AttributeType = { FLOAT: 1, INT: 2, STRING: 3, TENSOR: 4, FLOATS: 6, INTS: 7, STRINGS: 8 };
 
 // ---- schema ------------------------------------------------------------------

@@ -113,12 +113,12 @@ class RunnerImpl {
     this.loaded = true;
   }
 
-  // FLOAT / INT64 (clipped to int32) / INT32 initializers become CPU tensors; anything
-  // else throws (runnerImpl.ts:136-233).
+  // FLOAT / INT64 (clipped to int32) / INT32 initializers become CPU tensors, and FLOAT8E4M3FN ones (8-bit weights) as
+  // bytes; anything else throws (runnerImpl.ts:136-233).
   extractInitializerTensor() {
     const tensors = new Map();
     for (const initializer of this.model.graph.initializer) {
-      if (![DataType.FLOAT, DataType.INT64, DataType.INT32].includes(initializer.dataType)) {
+      if (![DataType.FLOAT, DataType.INT64, DataType.INT32, DataType.FLOAT8E4M3FN].includes(initializer.dataType)) {
         throw new Error(`Unsupported initializer dataType ${initializer.dataType}`);
       }
       const { dims, dataType, data } = tensorProtoToArray(initializer);

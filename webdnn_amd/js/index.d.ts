@@ -55,5 +55,5 @@ export interface Runner {
 }
 
 export function load(directory: string, options?: InitOption): Promise<Runner>;
-export const CPUTensor: new (dims: ReadonlyArray<number>, dataType?: "float32" | "int32" | "bool",
+export const CPUTensor: new (dims: ReadonlyArray<number>, dataType?: "float32" | "int32" | "bool" | "float8e4m3fn",
                              data?: Float32Array | Int32Array | Uint8Array) => Tensor;

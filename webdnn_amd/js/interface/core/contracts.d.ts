@@ -7,8 +7,8 @@
 /** Every backend but the host: tensors of these live in device memory. */
 export type BackendWithoutCPU = "hip";
 export type Backend = "cpu" | BackendWithoutCPU;
-/** Element types; "bool" is one byte per element. */
-export type DataType = "float32" | "int32" | "bool";
+/** Element types; "bool" and "float8e4m3fn" (8-bit weights on hip, as bytes) are one byte per element. */
+export type DataType = "float32" | "int32" | "bool" | "float8e4m3fn";
 /** What getData() hands back and setData() takes, by DataType. */
 export type DataArrayTypes = Float32Array | Int32Array | Uint8Array;
 /** Run-time values of ../constants.js. */
@@ -18,6 +18,7 @@ export const DataArrayConstructor: {
   float32: Float32ArrayConstructor;
   int32: Int32ArrayConstructor;
   bool: Uint8ArrayConstructor;
+  float8e4m3fn: Uint8ArrayConstructor;
 };
 
 // ---- a tensor on any backend (tensor.ts:3-14) ---------------------------------------------------------------

@@ -1,6 +1,7 @@
 "use strict";
 // auto-generated by webdnn_amd/make_operator_entries.py
 
+const { getOpEntries: getOpEntriesoperatorsstandardattention } = require("./operators/standard/attention");
 const { getOpEntries: getOpEntriesoperatorsstandardbinary7 } = require("./operators/standard/binary7");
 const { getOpEntries: getOpEntriesoperatorsstandardcast } = require("./operators/standard/cast");
 const { getOpEntries: getOpEntriesoperatorsstandardconcat } = require("./operators/standard/concat");
@@ -11,12 +12,13 @@ const { getOpEntries: getOpEntriesoperatorsstandardgemm } = require("./operators
 const { getOpEntries: getOpEntriesoperatorsstandardglobalaveragepool } = require("./operators/standard/globalaveragepool");
 const { getOpEntries: getOpEntriesoperatorsstandardlayernormalization } = require("./operators/standard/layernormalization");
 const { getOpEntries: getOpEntriesoperatorsstandardmatmul } = require("./operators/standard/matmul");
+const { getOpEntries: getOpEntriesoperatorsstandardmatmulfp8 } = require("./operators/standard/matmulfp8");
 const { getOpEntries: getOpEntriesoperatorsstandardmaxpool } = require("./operators/standard/maxpool");
 const { getOpEntries: getOpEntriesoperatorsstandardreducemean } = require("./operators/standard/reducemean");
 const { getOpEntries: getOpEntriesoperatorsstandardreshape5 } = require("./operators/standard/reshape5");
+const { getOpEntries: getOpEntriesoperatorsstandardrmsnormalization } = require("./operators/standard/rmsnormalization");
 const { getOpEntries: getOpEntriesoperatorsstandardslice } = require("./operators/standard/slice");
 const { getOpEntries: getOpEntriesoperatorsstandardsoftmax } = require("./operators/standard/softmax");
-const { getOpEntries: getOpEntriesoperatorsstandardattention } = require("./operators/standard/attention");
 const { getOpEntries: getOpEntriesoperatorsstandardsplit } = require("./operators/standard/split");
 const { getOpEntries: getOpEntriesoperatorsstandardsqueeze } = require("./operators/standard/squeeze");
 const { getOpEntries: getOpEntriesoperatorsstandardtranspose } = require("./operators/standard/transpose");
@@ -25,6 +27,7 @@ const { getOpEntries: getOpEntriesoperatorsstandardunsqueeze } = require("./oper
 
 function getOpEntries() {
   const entries = [];
+  entries.push(...getOpEntriesoperatorsstandardattention());
   entries.push(...getOpEntriesoperatorsstandardbinary7());
   entries.push(...getOpEntriesoperatorsstandardcast());
   entries.push(...getOpEntriesoperatorsstandardconcat());
@@ -35,12 +38,13 @@ function getOpEntries() {
   entries.push(...getOpEntriesoperatorsstandardglobalaveragepool());
   entries.push(...getOpEntriesoperatorsstandardlayernormalization());
   entries.push(...getOpEntriesoperatorsstandardmatmul());
+  entries.push(...getOpEntriesoperatorsstandardmatmulfp8());
   entries.push(...getOpEntriesoperatorsstandardmaxpool());
   entries.push(...getOpEntriesoperatorsstandardreducemean());
   entries.push(...getOpEntriesoperatorsstandardreshape5());
+  entries.push(...getOpEntriesoperatorsstandardrmsnormalization());
   entries.push(...getOpEntriesoperatorsstandardslice());
   entries.push(...getOpEntriesoperatorsstandardsoftmax());
-  entries.push(...getOpEntriesoperatorsstandardattention());
   entries.push(...getOpEntriesoperatorsstandardsplit());
   entries.push(...getOpEntriesoperatorsstandardsqueeze());
   entries.push(...getOpEntriesoperatorsstandardtranspose());

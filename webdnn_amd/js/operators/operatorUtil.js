@@ -78,6 +78,11 @@ function tensorProtoToArray(t) {
       }
       return { dims, dataType: "int32", data: new Int32Array(t.int32Data || []) };
     }
+    case DataType.FLOAT8E4M3FN: {
+      // (without raw data ONNX keeps the bytes in int32_data)
+      if (raw && raw.byteLength) return { dims, dataType: "float8e4m3fn", data: Uint8Array.from(raw) };
+      return { dims, dataType: "float8e4m3fn", data: Uint8Array.from(t.int32Data || []) };
+    }
     default:
       throw new Error(`Unsupported TensorProto dataType ${t.dataType}`);
   }

@@ -18,7 +18,7 @@ import struct
 
 import numpy as np
 
-FLOAT, INT32, INT64 = 1, 6, 7
+FLOAT, INT32, INT64, FLOAT8E4M3FN = 1, 6, 7, 17
 ATTR_FLOAT, ATTR_INT, ATTR_STRING, ATTR_TENSOR, ATTR_FLOATS, ATTR_INTS = 1, 2, 3, 4, 6, 7
 
 
@@ -62,6 +62,8 @@ def tensor_proto(name, array):
         dt = INT64
     elif array.dtype == np.int32:
         dt = INT32
+    elif array.dtype == np.uint8:      # e4m3 values, as their bytes
+        dt = FLOAT8E4M3FN
     else:
         raise TypeError("unsupported initializer dtype %s" % array.dtype)
     return (_packed_ints(1, array.shape) + _int(2, dt) + _str(8, name)
@@ -172,7 +174,7 @@ def parse_model(data):
                 name = bytes(v).decode()
             elif f == 9:
                 raw = bytes(v)
-        np_dt = {FLOAT: np.float32, INT64: np.int64, INT32: np.int32}[dt]
+        np_dt = {FLOAT: np.float32, INT64: np.int64, INT32: np.int32, FLOAT8E4M3FN: np.uint8}[dt]
         return name, np.frombuffer(raw, dtype=np_dt).reshape(dims).copy()
 
     def parse_attr(buf):
