@@ -501,7 +501,9 @@ int wdh_rmsnorm(wdh_buf X, wdh_buf Skip, wdh_buf Gamma, wdh_buf Sum, wdh_buf Y, 
 int wdh_quantize_fp8(wdh_buf X, wdh_buf Q, wdh_buf QScale, int64_t rows, int cols, int block_rows);
 /* Y[i, j] = sum_b AScale[i, b] WScale[j / 128, b] sum_{x in block b} A[i, x] W[j, x]  (+ Bias[j]) (+ R[i, j]), then the
  * epilogue.  A [m, k] and W [n, k] are e4m3, both with k contiguous; scales [m, ceil(k/128)] and [ceil(n/128), ceil(k/128)]
- * are any fp32 numbers.  Bias and R may be 0; R may be Y.  Sums are held in fp32.  k = 0 leaves Bias and R. */
+ * are any fp32 numbers.  Bias and R may be 0; R may be Y.  Sums are held in fp32.  k = 0 leaves Bias and R.  Where the result
+ * is large and k is no multiple of 16, the operands are first copied to 16-byte rows in a workspace from the pool (without
+ * room for it the product is computed in place, slower). */
 int wdh_gemm_fp8(wdh_buf A, wdh_buf AScale, wdh_buf W, wdh_buf WScale, wdh_buf Bias, wdh_buf Y, int64_t m, int n, int k,
                  int epilogue, wdh_buf R);
 
@@ -526,9 +528,9 @@ int wdh_cache_append(wdh_buf K, int64_t k_offset, int64_t k_stride, wdh_buf V, i
  *   Y[row, h] = sum_j softmax_j(alpha q.k_j) v_j  over the tokens j of its sequence up to and with the row's own,
  * which wdh_cache_append has to have written before.  Prompts, parts of prompts and single tokens may be mixed in a call.
  * Y [tokens, heads * d] is dense; rows that belong to no sequence are left as they are.  A token on a page whose number is
- * outside the cache makes the rows that see it NaN; slots behind a sequence's tokens and tokens behind a row do not touch
- * it, whatever they hold.  Where one call's rows do not fill the chip the tokens are cut into parts whose results are
- * joined by a second launch, in a workspace from the pool. */
+ * outside the cache, or whose scales are not positive and finite, makes the rows that see it NaN; slots behind a sequence's
+ * tokens and tokens behind a row do not touch it, whatever they hold.  Where one call's rows do not fill the chip the tokens
+ * are cut into parts whose results are joined by a second launch, in a workspace from the pool (WDH_ENOMEM without room). */
 int wdh_cache_attention(wdh_buf Q, int64_t q_offset, int64_t q_stride, wdh_buf KPages, wdh_buf KScales, wdh_buf VPages,
                         wdh_buf VScales, wdh_buf Table, wdh_buf Lens, wdh_buf Starts, wdh_buf Y, int seqs, int tokens,
                         int heads, int kv_heads, int d, int pages, int max_pages, float alpha);

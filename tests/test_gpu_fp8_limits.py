@@ -1,0 +1,190 @@
+"""The 8-bit serving operators where their forms change and where they end: every tile of the products, many sequences, caches
+beyond 4 GiB, scales that are none, sequences that contradict each other, no room for a workspace, several recorded runs."""
+import numpy as np
+import pytest
+
+import fp8_ref as F
+import test_gpu_fp8_serving as S
+from webdnn_amd import capi
+from webdnn_amd import hostops as H
+
+pytestmark = pytest.mark.gpu
+
+
+# few rows by 16, 32 and 64 columns; 64 x 64; 128 x 128 with rows that are copied first, and more of them than the chip takes at
+# once; 256 x 128
+@pytest.mark.parametrize("m,n,k", [(16, 5000, 272), (3, 20000, 260), (11, 9000, 1030), (600, 1500, 400), (1500, 2000, 130), (3000, 2900, 144), (8192, 4096, 200)])
+def test_every_tile_of_the_products(ctx, m, n, k):
+    S.check_product(ctx, np.random.default_rng(m + n + k), m, n, k, bias=True, residual=m < 2000)
+
+
+@pytest.mark.parametrize("new,heads,kv,d", [([1, 0, 2] * 45, 4, 2, 32), ([20] * 70, 8, 2, 64), ([1] * 200, 3, 3, 64)])
+def test_attention_of_more_sequences_than_lanes(ctx, new, heads, kv, d):
+    rng = np.random.default_rng(len(new))
+    past = rng.integers(0, 400, len(new))
+    past[5], past[66] = 1500, 0
+    c, table, lens, starts = S.filled(rng, new, past, kv, d)
+    q = rng.standard_normal((int(starts[-1]), heads, d)).astype(np.float32)
+    want, bound = c.attention(q, table, lens, starts, d ** -0.5)
+    assert np.all(np.abs(S.attend(ctx, c, q, table, lens, starts, np.float32(d ** -0.5)) - want) <= bound)
+
+
+def test_a_cache_beyond_4_gib(ctx):
+    """Keys alone take 4.3 GiB: pages on both sides of 2 and 4 GiB, tokens one by one and in a prompt."""
+    rng = np.random.default_rng(31)
+    heads, kv, d, pages = 16, 8, 128, 70000
+    far = np.array([[69999, 32768, 65535], [65536, -1, -1], [32767, 1, -1]], np.int32)
+    near = np.array([[0, 1, 2], [3, -1, -1], [4, 5, -1]], np.int32)
+    lens, starts = np.array([150, 1, 70], np.int32), np.array([0, 150, 151, 221], np.int32)
+    k, v = (rng.standard_normal((221, kv, d)).astype(np.float32) for _ in range(2))
+    c = F.Cache(6, kv, d)
+    c.append(k, v, near, lens, starts)
+    cache = H.KvCache.empty(ctx, pages, kv, d)
+    up = ctx.move_tensor
+    H.cache_append(ctx, cache, up(k.reshape(221, -1)), up(v.reshape(221, -1)), up(far), up(lens), up(starts))
+    for scales, want in ((cache.k_scales, c.ks), (cache.v_scales, c.vs)):
+        assert np.array_equal(scales.get_data()[far[far >= 0]], want[near[near >= 0]])
+    for begin in (starts, np.array([0, 1, 2, 3], np.int32)):                    # the prompts; their last tokens alone
+        q = rng.standard_normal((int(begin[-1]), heads, d)).astype(np.float32)
+        want, bound = c.attention(q, near, lens, begin, 0.1)
+        got = H.cache_attention(ctx, cache, up(q.reshape(len(q), -1)), heads, 0.1, up(far), up(lens), up(begin)).get_data().reshape(q.shape)
+        assert np.all(np.abs(got - want) <= bound)
+    for t in (cache.k, cache.v, cache.k_scales, cache.v_scales):
+        t.dispose()
+    ctx.sync()
+    capi.call("wdh_trim", 0)
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("new", [1, 90])
+@pytest.mark.parametrize("values", [False, True])
+def test_a_scale_that_is_none_makes_its_rows_nan(ctx, scale, new, values):
+    rng = np.random.default_rng(14)
+    c, table, lens, starts = S.filled(rng, [new], [100], 2, 64)
+    q = rng.standard_normal((new, 4, 64)).astype(np.float32)
+    want, bound = c.attention(q, table, lens, starts, 0.125)
+    (c.vs if values else c.ks)[table[0, 1], 1] = scale                          # tokens 64 .. 127 of one head: rows from 64 on see them
+    got = S.attend(ctx, c, q, table, lens, starts, 0.125)
+    assert np.all(np.abs(got - want)[:, :2] <= bound[:, :2]) and np.isnan(got[:, 2:]).all()
+
+
+def test_sequences_that_contradict_each_other(ctx):
+    """Every other sequence claims all rows of the call: 2^31 units of work, which no call with sequences behind each other has.  Rows that
+    more than one sequence claims may hold anything; the call ends, and the next one is right."""
+    seqs, tokens, heads, pages = 1024, 60 * 1024, 1, 4096
+    starts = np.zeros(seqs + 1, np.int32)
+    starts[1::2] = tokens
+    lens = np.full(seqs, 64 * pages, np.int32)
+    up = ctx.move_tensor
+    cache = H.KvCache.empty(ctx, 1, 1, 32)
+    q = ctx.empty_tensor([tokens, 32])
+    y = H.cache_attention(ctx, cache, q, heads, 1.0, up(np.full((seqs, pages), -1, np.int32)), up(lens), up(starts))
+    ctx.sync()
+    y.dispose()
+    rng = np.random.default_rng(3)
+    c, table, lens, starts = S.filled(rng, [1, 2], [300, 7], 1, 32)
+    q = rng.standard_normal((3, 2, 32)).astype(np.float32)
+    want, bound = c.attention(q, table, lens, starts, 0.2)
+    assert np.all(np.abs(S.attend(ctx, c, q, table, lens, starts, 0.2) - want) <= bound)
+
+
+def test_no_room_for_a_workspace(ctx):
+    """Attention that needs one fails and leaves no trace; a product that would copy its operands goes without."""
+    rng = np.random.default_rng(6)
+    c, table, lens, starts = S.filled(rng, [1], [2000], 4, 128)
+    q = rng.standard_normal((1, 8, 128)).astype(np.float32)
+    want, bound = c.attention(q, table, lens, starts, 0.1)
+    up = ctx.move_tensor
+    cache, ints, rows = S.on_device(ctx, c), [up(t) for t in (table, lens, starts)], up(q.reshape(1, -1))
+    y = ctx.empty_tensor([1, 1024])
+    m, n, k = 1500, 2000, 130
+    a, w = S.bytes_of(rng, (m, k)), S.bytes_of(rng, (n, k))
+    sa, sw = np.full((m, 2), 0.5, np.float32), np.full((16, 2), 0.25, np.float32)
+    ops, product = [up(t) for t in (a, sa, w, sw)], ctx.empty_tensor([m, n])
+    ctx.sync()
+    capi.call("wdh_trim", 0)
+    ctx.set_option("memory_limit_mib", 1)
+    try:
+        with pytest.raises(capi.HipError) as err:
+            H.cache_attention(ctx, cache, rows, 8, 0.1, *ints, out=y)
+        assert err.value.code == -3
+        H.matmul_fp8(ctx, *ops, out=product)
+    finally:
+        ctx.set_option("memory_limit_mib", 0)
+    sums, size = F.product(a, sa, w, sw)
+    assert np.all(np.abs(product.get_data() - sums) <= (128 + 2 + 2) * 2 * S.E * size)
+    got = H.cache_attention(ctx, cache, rows, 8, 0.1, *ints, out=y).get_data().reshape(q.shape)
+    assert np.all(np.abs(got - want) <= bound)
+
+
+def test_recorded_runs_do_not_share_workspaces(ctx):
+    """Three recorded calls with workspaces (shares of single tokens, parts of a prompt, copied operands), replayed in turn with eager
+    work of the same kinds and other allocations between them: every replay against the first results."""
+    rng = np.random.default_rng(17)
+    up = ctx.move_tensor
+    calls = []
+    for new, past in (([1, 1], [3000, 40]), ([100], [900])):
+        c, table, lens, starts = S.filled(rng, new, past, 2, 64)
+        operands = (S.on_device(ctx, c), up(rng.standard_normal((sum(new), 512)).astype(np.float32)), up(table), up(lens), up(starts))
+        calls.append(lambda o=operands, out=None: H.cache_attention(ctx, o[0], o[1], 8, 0.125, *o[2:], out=out))
+    a, w = up(S.bytes_of(rng, (1500, 130))), up(S.bytes_of(rng, (2000, 130)))
+    sa, sw = ctx.move_tensor(np.full((1500, 2), 0.5, np.float32)), up(np.full((16, 2), 0.25, np.float32))
+    calls.append(lambda out=None: H.matmul_fp8(ctx, a, sa, w, sw, out=out))
+    want = [call().get_data() for call in calls]
+    graphs, outs = [], []
+    try:
+        for call in calls:
+            ctx.graph_begin()
+            outs.append(call())
+            graphs.append(ctx.graph_end())
+        for turn in range(3):
+            noise = up(np.full(1 << 20, np.nan, np.float32))
+            for g in graphs[::1 if turn % 2 else -1]:
+                ctx.graph_launch(g)
+            eager = [call() for call in calls]
+            for out, again, first in zip(outs, eager, want):
+                assert np.array_equal(out.get_data(), first) and np.array_equal(again.get_data(), first)
+                again.dispose()
+            assert np.isnan(noise.get_data()).all()
+            noise.dispose()
+    finally:
+        for g in graphs:
+            ctx.graph_destroy(g)
+
+
+def test_a_side_lane_takes_recorded_attention_only(ctx):
+    rng = np.random.default_rng(18)
+    c, table, lens, starts = S.filled(rng, [1, 3], [900, 20], 2, 64)
+    up = ctx.move_tensor
+    cache, q, ints = S.on_device(ctx, c), up(rng.standard_normal((4, 256)).astype(np.float32)), [up(t) for t in (table, lens, starts)]
+    run = lambda: H.cache_attention(ctx, cache, q, 4, 0.125, *ints)
+    want = run().get_data()
+    ctx.set_lane(1)
+    try:
+        with pytest.raises(capi.HipError) as err:
+            run()
+        assert "recorded work only" in str(err.value)
+        ctx.graph_begin()
+        out = run()
+        graph = ctx.graph_end()
+        for _ in range(3):
+            ctx.graph_launch(graph)
+            assert np.array_equal(out.get_data(), want)
+    finally:
+        ctx.set_lane(0)
+    ctx.graph_launch(graph)
+    assert np.array_equal(out.get_data(), want)
+    ctx.graph_destroy(graph)
+
+
+def test_what_is_too_large_or_empty_is_refused(ctx):
+    f, i, e = lambda *s: ctx.empty_tensor(s), lambda *s: ctx.empty_tensor(s, "int32"), lambda *s: ctx.empty_tensor(s, "float8e4m3fn")
+    cache = H.KvCache(ctx, e(0, 1, 64, 32), f(0, 1), e(0, 1, 32, 64), f(0, 1))
+    with pytest.raises(capi.HipError) as err:                                  # rows that see no page of it
+        H.cache_attention(ctx, cache, f(1, 32), 1, 1.0, i(1, 1), i(1), i(2))
+    assert err.value.code == -2 and "without pages" in str(err.value)
+    H.cache_append(ctx, cache, f(1, 32), f(1, 32), i(1, 1), i(1), i(2))        # nothing to write to
+    for m, n, k in ((1, (1 << 28) + 1, 1), (1 << 31, 1, 1), (1, 1, (1 << 30) + 1)):
+        with pytest.raises(capi.HipError) as err:
+            H.call("wdh_gemm_fp8", 1, 1, 1, 1, 0, 1, m, n, k, 0, 0)
+        assert err.value.code == -2 and "too many" in str(err.value)

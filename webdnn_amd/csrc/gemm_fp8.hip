@@ -354,7 +354,7 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
   if (m < 0 || n < 0 || k < 0) return fail(WDH_EINVAL, "wdh_gemm_fp8: negative extent");
   if (epilogue != WDH_EPI_NONE && epilogue != WDH_EPI_RELU) return fail(WDH_EINVAL, "wdh_gemm_fp8: unknown epilogue %d", epilogue);
   if (m == 0 || n == 0) return WDH_OK;
-  if (n > (1 << 30) || k > (1 << 30) || m > (1LL << 46) / n || (k && m > (1LL << 46) / k)) return fail(WDH_EINVAL, "wdh_gemm_fp8: too many elements");
+  if (n > (1 << 28) || k > (1 << 30) || ((m + 127) / 128) * (((long long)n + 127) / 128) > 0x7fffff || m > (1LL << 46) / n || (k && m > (1LL << 46) / k)) return fail(WDH_EINVAL, "wdh_gemm_fp8: too many elements");
   const size_t blocks = ((size_t)k + BLOCK - 1) / BLOCK, wide = ((size_t)n + BLOCK - 1) / BLOCK, results = (size_t)m * n * 4;
   void *pa, *psa, *pw, *psw, *pb = nullptr, *py, *pr = nullptr;
   if (!wdh::operand(hA, (size_t)m * k, "wdh_gemm_fp8: A", &pa)) return WDH_EINVAL;

@@ -52,10 +52,11 @@ __device__ __forceinline__ int fresh(int v) {
 }
 
 // Sums over the lanes up to and with each: shifts within rows of 16, then the last lanes of rows 0 and 2, and of row 1, into
-// those behind them.
+// those behind them.  They end at the largest int (sequences that contradict each other can claim more rows than the call has).
+__device__ __forceinline__ int add_sat(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
 template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ int dpp_add(int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
+  return add_sat(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false));
 }
 __device__ __forceinline__ int wave_scan(int v) {
   v = dpp_add<0x111, 0xf>(v);
@@ -213,7 +214,7 @@ struct AttendParams {
 // Work of attention: items of 16 rows (a row is a token and one of the queries that share a head of the cache), each as many units
 // of four pages (one for each wavefront of a workgroup) as its sequence has.  The units of all items stand in a row, and every
 // workgroup takes `share` neighbouring ones: all end at the same time, whatever the sequences' lengths.
-// (us, shares / a fixed number of parts for every item: see DECODE below.)
+constexpr int MOST_UNITS = 1 << 30;
 struct Work {
   Place s;
   int item, unit, units;  // the item, the unit of it that was asked for, and how many it has
@@ -237,8 +238,8 @@ __device__ __forceinline__ Look look(const AttendParams &p, int round) {
 }
 __device__ __forceinline__ int total_units(const AttendParams &p, const Look &first) {
   int total = __builtin_amdgcn_readlane(first.upto, 63);
-  for (int i = 1; i < (p.q.seqs + 63) / 64; i++) total += __builtin_amdgcn_readlane(look(p, i).upto, 63);
-  return total;
+  for (int i = 1; i < (p.q.seqs + 63) / 64; i++) total = add_sat(total, __builtin_amdgcn_readlane(look(p, i).upto, 63));
+  return total <= MOST_UNITS ? total : 0;  // (more than the host allows: numbers that contradict each other)
 }
 // The item that holds unit number `index` of all (or, by_item, item number `index`); s.n = 0 behind the last.
 __device__ __forceinline__ Work locate_work(const AttendParams &p, const Look &first, int index, bool by_item) {
@@ -247,7 +248,7 @@ __device__ __forceinline__ Work locate_work(const AttendParams &p, const Look &f
   Look l = first;
   for (int i = 0; i < (p.q.seqs + 63) / 64; i++) {
     if (i) l = look(p, i);
-    const int upto = before + l.upto, upto_items = by_item ? before_items + wave_scan(l.items) : 0;
+    const int upto = add_sat(before, l.upto), upto_items = by_item ? add_sat(before_items, wave_scan(l.items)) : 0;
     const unsigned long long has = __ballot(index < (by_item ? upto_items : upto));
     if (has) {
       const int at = __ffsll(has) - 1;
@@ -1089,7 +1090,8 @@ extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_strid
   if (heads <= 0 || heads % kv_heads || heads > 65536) return fail(WDH_EINVAL, "%s: %d heads on %d of the cache", who, heads, kv_heads);
   const int64_t width = (int64_t)heads * d;
   if (int rc = check_rows(who, "Q", q_offset, q_stride, width)) return rc;
-  if (seqs == 0 || tokens == 0 || pages == 0 || max_pages == 0) return WDH_OK;
+  if (seqs == 0 || tokens == 0 || max_pages == 0) return WDH_OK;
+  if (pages == 0) return fail(WDH_EINVAL, "%s: a cache without pages", who);
   AttendParams p;
   void *pq, *py, *kp, *ks, *vp, *vs;
   if (!wdh::operand(hQ, (size_t)(q_offset + (tokens - 1) * q_stride + width) * 4, "wdh_cache_attention: Q", &pq)) return WDH_EINVAL;
@@ -1134,7 +1136,7 @@ extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_strid
   } else {
     // as many workgroups as the chip holds at a time, or as there can be units
     const long long units = items * ((max_pages + 3) / 4), resident = 2LL * wdh::compute_units() / kv_heads;
-    if (units > (1LL << 30)) return fail(WDH_EINVAL, "%s: too many rows of tables so wide", who);
+    if (units > MOST_UNITS) return fail(WDH_EINVAL, "%s: too many rows of tables so wide", who);
     p.wgs = (int)(units < resident ? units : resident > 0 ? resident : 1);
     if (max_pages > 4 && p.wgs > 1 && !workspace((size_t)p.wgs * 2 * kv_heads * 16)) return WDH_ENOMEM;  // (items of one unit are never cut)
     rc = d == 32 ? launch_attend<32>(p, items) : d == 64 ? launch_attend<64>(p, items) : launch_attend<128>(p, items);
