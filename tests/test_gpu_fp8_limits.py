@@ -18,6 +18,14 @@ def test_every_tile_of_the_products(ctx, m, n, k):
     S.check_product(ctx, np.random.default_rng(m + n + k), m, n, k, bias=True, residual=m < 2000)
 
 
+@pytest.mark.parametrize("cols", [3, 5, 20, 33, 64, 65, 100, 132, 137, 156, 190, 193])
+def test_narrow_last_blocks(ctx, cols):
+    rng = np.random.default_rng(cols)
+    x = (rng.standard_normal((1300, cols)) * 2.0 ** rng.integers(-20, 20, (1300, 1))).astype(np.float32)
+    q, c = (t.get_data() for t in H.quantize_fp8(ctx, ctx.move_tensor(x), 128))
+    F.check_quantized(q, c, x.astype(np.float64), 128, 0.0)
+
+
 @pytest.mark.parametrize("new,heads,kv,d", [([1, 0, 2] * 45, 4, 2, 32), ([20] * 70, 8, 2, 64), ([1] * 200, 3, 3, 64)])
 def test_attention_of_more_sequences_than_lanes(ctx, new, heads, kv, d):
     rng = np.random.default_rng(len(new))
