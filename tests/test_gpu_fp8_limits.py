@@ -12,8 +12,8 @@ pytestmark = pytest.mark.gpu
 
 
 # few rows by 16, 32 and 64 columns; 64 x 64; 128 x 128 with rows that are copied first, and more of them than the chip takes at
-# once; 256 x 128
-@pytest.mark.parametrize("m,n,k", [(16, 5000, 272), (3, 20000, 260), (11, 9000, 1030), (600, 1500, 400), (1500, 2000, 130), (3000, 2900, 144), (8192, 4096, 200)])
+# once; 256 x 128; and cut along K, the last part being shorter, with and without whole 16-byte rows
+@pytest.mark.parametrize("m,n,k", [(20, 1000, 12000), (100, 900, 9001), (300, 700, 14336), (500, 2000, 5000), (260, 1024, 16384), (2, 130, 20001), (16, 5000, 272), (3, 20000, 260), (11, 9000, 1030), (600, 1500, 400), (1500, 2000, 130), (3000, 2900, 144), (8192, 4096, 200)])
 def test_every_tile_of_the_products(ctx, m, n, k):
     S.check_product(ctx, np.random.default_rng(m + n + k), m, n, k, bias=True, residual=m < 2000)
 

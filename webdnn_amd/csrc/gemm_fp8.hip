@@ -22,6 +22,7 @@ struct ProductParams {
   long long m;
   int n, k, blocks, relu;
   long long pitch;  // bytes between rows of A, and of W
+  int part;         // blocks of K that a part of the product takes: its results go to Y [part][m][n]
 };
 
 // 32 bytes a lane of each operand: the lanes that share a row hold its 128 elements, in the same order on both sides.
@@ -95,16 +96,15 @@ struct Pieces {
 };
 
 // Columns j .. j+3 of row i: bias, residual, Relu, and out.
-__device__ __forceinline__ void finish4(const ProductParams &p, long long i, int j, f32x4 v) {
+__device__ __forceinline__ void finish4(const ProductParams &p, float *Y, long long i, int j, f32x4 v) {
   const int left = p.n - j;
   if (left <= 0) return;
-  float *y = p.Y + i * p.n;
   if (p.bias) v = v + load4(p.bias, j, p.n);
   if (p.R) v = v + load4(p.R + i * p.n, j, p.n);
   if (p.relu)
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] = !(v[e] > 0.0f) && v[e] == v[e] ? 0.0f : v[e];
-  store4(y, j, p.n, v);
+  store4(Y + i * p.n, j, p.n, v);
 }
 
 // Few rows of A, or few results: a workgroup has 16 NT rows of W and 16 MT of A, its wavefronts take K blocks in turn, U at a time,
@@ -114,7 +114,7 @@ template <int NT, int MT, int WAVES, int U, bool ALIGNED>
 __global__ __launch_bounds__(64 * WAVES) void product_few(ProductParams p) {
   __shared__ __attribute__((aligned(16))) f32x4 part[WAVES][NT * MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * (16 * NT);
+  const int n0 = blockIdx.x * (16 * NT), begin = blockIdx.z * p.part, end = begin + p.part < p.blocks ? begin + p.part : p.blocks;
   const unsigned char *w[NT];
   const float *sw[NT];
 #pragma unroll
@@ -135,13 +135,13 @@ __global__ __launch_bounds__(64 * WAVES) void product_few(ProductParams p) {
 #pragma unroll
       for (int q = 0; q < NT; q++) acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int b0 = wave; b0 < p.blocks; b0 += WAVES * U) {
+    for (int b0 = begin + wave; b0 < end; b0 += WAVES * U) {
       Pieces<ALIGNED> wv[U][NT], av[U][MT];
       float sav[U][MT], swv[U][NT];
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const int b = b0 + WAVES * u;
-        if (b >= p.blocks) break;
+        if (b >= end) break;
 #pragma unroll
         for (int t = 0; t < NT; t++) wv[u][t].load(w[t], b * BLOCK + 32 * g, p.k), swv[u][t] = sw[t][b];
 #pragma unroll
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_few(ProductParams p) {
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const int b = b0 + WAVES * u;
-        if (b >= p.blocks) break;
+        if (b >= end) break;
         i32x8 x8[NT];
 #pragma unroll
         for (int q = 0; q < NT; q++) x8[q] = wv[u][q].get(w[q], b * BLOCK + 32 * g, p.k);
@@ -180,16 +180,18 @@ __global__ __launch_bounds__(64 * WAVES) void product_few(ProductParams p) {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] += part[i][tile][l][e];
       const long long i = m0 + 16 * (tile % MT) + (l & 15);
-      if (i < p.m) finish4(p, i, n0 + 16 * (tile / MT) + 4 * (l >> 4), v);
+      if (i < p.m) finish4(p, p.Y + blockIdx.z * p.m * p.n, i, n0 + 16 * (tile / MT) + 4 * (l >> 4), v);
     }
     __syncthreads();
   }
 }
 
+unsigned parts_of(const ProductParams &p) { return p.part < p.blocks ? (unsigned)((p.blocks + p.part - 1) / p.part) : 1u; }
+
 template <int NT, int MT, int WAVES, int U>
 void launch_few(const ProductParams &p, bool aligned) {
   const long long rows = (p.m + 16 * MT - 1) / (16 * MT);
-  const dim3 grid((unsigned)((p.n + 16 * NT - 1) / (16 * NT)), (unsigned)(rows < 65535 ? rows : 65535)), wg(64 * WAVES);
+  const dim3 grid((unsigned)((p.n + 16 * NT - 1) / (16 * NT)), (unsigned)(rows < 65535 ? rows : 65535), parts_of(p)), wg(64 * WAVES);
   if (aligned) hipLaunchKernelGGL((product_few<NT, MT, WAVES, U, true>), grid, wg, 0, wdh::stream(), p);
   else hipLaunchKernelGGL((product_few<NT, MT, WAVES, U, false>), grid, wg, 0, wdh::stream(), p);
 }
@@ -231,14 +233,15 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
 
   Piece<true> next[DEPTH][LOADS];
   float next_scale[DEPTH];
+  const int begin = blockIdx.y * p.part, end = begin + p.part < p.blocks ? begin + p.part : p.blocks;
   auto fetch = [&](int slot, int b) {
-    if (b >= p.blocks) return;
+    if (b >= end) return;
 #pragma unroll
     for (int i = 0; i < LOADS; i++) next[slot][i].load(row[i], b * BLOCK + piece, p.k);
     if (tid < BM) next_scale[slot] = my_scale[b];
   };
   auto keep = [&](int slot, int b) {
-    if (b >= p.blocks) return;
+    if (b >= end) return;
 #pragma unroll
     for (int i = 0; i < LOADS; i++) *reinterpret_cast<i32x4 *>(&lds[b & 1][to[i]]) = next[slot][i].get(row[i], b * BLOCK + piece, p.k);
     if (tid < BM) scales[b & 1][tid] = next_scale[slot];
@@ -261,17 +264,17 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
     for (int j = 0; j < TM; j++)
 #pragma unroll
       for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
-  // slab b goes to LDS through registers slot b % DEPTH, which then ask for slab b + DEPTH
+  // slab begin + b goes to LDS through registers slot b % DEPTH, which then ask for the slab DEPTH behind it
 #pragma unroll
-  for (int d = 0; d < DEPTH; d++) fetch(d, d);
-  keep(0, 0);
-  fetch(0, DEPTH);
+  for (int d = 0; d < DEPTH; d++) fetch(d, begin + d);
+  keep(0, begin);
+  fetch(0, begin + DEPTH);
   __syncthreads();
-  for (int b0 = 0; b0 < p.blocks; b0 += DEPTH) {
+  for (int b0 = begin; b0 < end; b0 += DEPTH) {
 #pragma unroll
     for (int d = 0; d < DEPTH; d++) {
       const int b = b0 + d, buf = b & 1;
-      if (b >= p.blocks) break;
+      if (b >= end) break;
       keep((d + 1) % DEPTH, b + 1);
       fetch((d + 1) % DEPTH, b + 1 + DEPTH);
       const float s = sw[b];
@@ -303,6 +306,7 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
       __syncthreads();
     }
   }
+  float *Y = p.Y + blockIdx.y * p.m * p.n;
   // lane: row li of a block; registers 4 q .. + 3 are columns 8 q + 4 half .. + 3
 #pragma unroll
   for (int j = 0; j < TM; j++) {
@@ -314,7 +318,7 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
       for (int q = 0; q < 4; q++) {
         const int col = n0 + 32 * (TN * wn + t) + 8 * q + 4 * half;
         f32x4 v = {acc[t][j][4 * q], acc[t][j][4 * q + 1], acc[t][j][4 * q + 2], acc[t][j][4 * q + 3]};
-        finish4(p, i, col, v);
+        finish4(p, Y, i, col, v);
       }
   }
 }
@@ -323,7 +327,21 @@ template <int NW, int MW, int TN, int TM, int DEPTH>
 void launch_tiles(const ProductParams &p) {
   constexpr int BN = 32 * NW * TN, BM = 32 * MW * TM;
   const long long tiles = (p.n + BN - 1) / BN * ((p.m + BM - 1) / BM);
-  hipLaunchKernelGGL((product_tiles<NW, MW, TN, TM, DEPTH>), dim3((unsigned)tiles), dim3(64 * NW * MW), 0, wdh::stream(), p);
+  hipLaunchKernelGGL((product_tiles<NW, MW, TN, TM, DEPTH>), dim3((unsigned)tiles, parts_of(p)), dim3(64 * NW * MW), 0, wdh::stream(), p);
+}
+
+// The parts of a product together, in order: four results to a lane.
+__global__ __launch_bounds__(256) void product_join(ProductParams p, const float *partial, int parts) {
+  const int pieces = (p.n + 3) / 4;
+  for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < p.m * pieces; at += 256LL * gridDim.x) {
+    const long long i = at / pieces;
+    const int j = (int)(at - i * pieces) * 4;
+    const float *from = partial + i * p.n;
+    f32x4 v = load4(from, j, p.n);
+#pragma unroll 4
+    for (int part = 1; part < parts; part++) v = v + load4(from + part * p.m * p.n, j, p.n);
+    finish4(p, p.Y, i, j, v);
+  }
 }
 
 // Rows of a length that is no multiple of 16, copied to rows that are (zeros behind their end): A's, then W's.
@@ -341,6 +359,49 @@ __global__ __launch_bounds__(256) void pack_rows(const unsigned char *A, const u
         if (at + 1024 * i < k) *reinterpret_cast<i32x4 *>(to + r * pitch + at + 1024 * i) = x[i].get(row, at + 1024 * i, k);
     }
   }
+}
+
+// Which form a product takes, and in how many parts along K.  A workgroup of a form takes `start` + `block` per block of K us (measured
+// with every CU busy: K of 2048 to 14336, 16 to 8192 rows; wavefronts of the direct forms take blocks eight at a time; fewer rows
+// than 16 cost the smallest form, which is bound by its loads, less).  Tiles that leave
+// CUs idle are cut along K into as many parts as there are CUs for; the parts' join is a launch of 4 us and its bytes.  The cheapest
+// of all wins (us, so / the smallest tile that fits the chip, uncut: 4096 columns, K = 14336: 32 rows 20 / 36, 64 rows 24 / 36, 256 rows
+// 46 / 70; 8192 x 8192: 128 rows 33 / 44, 1024 rows 153 / 161).
+struct Form {
+  int cols, rows;
+  float start, block;
+};
+constexpr int FIRST_TILES = 6, FORMS = 9;
+constexpr Form forms[FORMS] = {{16, 16, 3.0f, 0.16f}, {32, 16, 1.5f, 0.27f}, {64, 16, 1.5f, 0.47f},   {32, 32, 3.0f, 0.31f},  {64, 32, 2.0f, 0.48f},
+                               {64, 64, 4.0f, 0.62f}, {128, 64, 5.0f, 0.87f}, {128, 128, 8.0f, 1.15f}, {256, 128, 9.0f, 2.25f}};
+struct Plan {
+  int form, parts;
+};
+Plan cheapest_plan(const ProductParams &p, bool aligned) {
+  const long long cus = wdh::compute_units();
+  Plan best = {0, 1};
+  double least = -1.0;
+  for (int f = 0; f < FORMS; f++) {
+    const long long tiles = ((p.n + forms[f].cols - 1LL) / forms[f].cols) * ((p.m + forms[f].rows - 1) / forms[f].rows);
+    const bool direct = f < FIRST_TILES;
+    const double block = f == 0 && p.m < 16 ? forms[f].block - 0.005 * (double)(16 - p.m) : forms[f].block;
+    for (int cut = 0; cut < 2; cut++) {
+      long long parts = cut ? cus / tiles : 1;
+      if (parts > p.blocks) parts = p.blocks;
+      if (cut && parts < 2) continue;
+      const long long part = parts > 1 ? (p.blocks + parts - 1) / parts : p.blocks;
+      if (parts > 1) parts = (p.blocks + part - 1) / part;
+      const double rounds = (double)((tiles * parts + cus - 1) / cus);
+      double us = rounds * (forms[f].start + block * (double)(direct ? (part + 7) / 8 * 8 : part));
+      if (parts > 1) us += 4.0 + (double)parts * (double)p.m * p.n * 8e-7;
+      if (!direct && !aligned) us += 4.0 + (double)(p.m + p.n) * p.k * 5e-7;  // (the copy)
+      if (least < 0.0 || us < least) {
+        least = us;
+        best = Plan{f, (int)parts};
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -372,14 +433,12 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
   p.Y = (float *)py;
   p.m = m; p.n = n; p.k = k; p.blocks = (int)blocks; p.relu = epilogue == WDH_EPI_RELU;
   p.pitch = k;
-  // The smallest tile (columns x rows of Y) that leaves no more workgroups than the chip has CUs.
-  const long long cus = wdh::compute_units();
-  auto fits = [&](int cols, int rows) { return ((long long)n + cols - 1) / cols * ((m + rows - 1) / rows) <= cus; };
-  const bool few = m <= 16 || fits(64, 64);
+  p.part = p.blocks;
+  bool aligned = k % 16 == 0;  // (buffers start on 512-byte boundaries)
+  Plan plan = cheapest_plan(p, aligned);
   // Tiles of many rows take rows of whole 16-byte pieces: others are copied first.
   wdh_buf packed = 0;
-  bool aligned = k % 16 == 0;  // (buffers start on 512-byte boundaries)
-  if (!aligned && !few) {
+  if (!aligned && plan.form >= FIRST_TILES) {
     const long long pitch = ((long long)k + 15) / 16 * 16, rows = m + n;
     packed = wdh_alloc((size_t)(rows * pitch));
     size_t have;
@@ -391,20 +450,36 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
       p.W = to + m * pitch;
       p.pitch = pitch;
       aligned = true;
-    }
+    } else plan = Plan{FIRST_TILES - 1, 1};  // (no room for the copy: the direct form takes any rows)
   }
-  if (few || !aligned) {  // (no room for the copy: the direct form takes any rows)
-    if (m <= 16) {
-      if (fits(16, 16)) launch_few<1, 1, 8, 4>(p, aligned);
-      else if (fits(32, 16)) launch_few<2, 1, 8, 4>(p, aligned);
-      else launch_few<4, 1, 8, 2>(p, aligned);
-    } else if (fits(16, 16)) launch_few<1, 1, 8, 4>(p, aligned);
-    else if (fits(32, 32)) launch_few<2, 2, 8, 2>(p, aligned);
-    else if (fits(64, 32)) launch_few<4, 2, 8, 1>(p, aligned);
-    else launch_few<4, 4, 8, 1>(p, aligned);
-  } else if (fits(128, 64)) launch_tiles<4, 2, 1, 1, 3>(p);
-  else if (fits(128, 128) || ((long long)n + 255) / 256 * ((m + 127) / 128) < 4 * cus) launch_tiles<4, 2, 1, 2, 2>(p);
-  else launch_tiles<4, 2, 2, 2, 1>(p);
+  // Parts go to a workspace and are joined; without room for it there is one part.
+  wdh_buf work = 0;
+  ProductParams parts = p;
+  float *partial = nullptr;
+  if (plan.parts > 1 && (work = wdh_alloc((size_t)plan.parts * results))) {
+    size_t have;
+    parts.Y = partial = (float *)wdh::resolve(work, &have);
+    parts.part = (p.blocks + plan.parts - 1) / plan.parts;
+    parts.bias = parts.R = nullptr;
+    parts.relu = 0;
+  }
+  switch (plan.form) {
+    case 0: launch_few<1, 1, 8, 4>(parts, aligned); break;
+    case 1: launch_few<2, 1, 8, 4>(parts, aligned); break;
+    case 2: launch_few<4, 1, 8, 2>(parts, aligned); break;
+    case 3: launch_few<2, 2, 8, 2>(parts, aligned); break;
+    case 4: launch_few<4, 2, 8, 1>(parts, aligned); break;
+    case 5: launch_few<4, 4, 8, 1>(parts, aligned); break;
+    case 6: launch_tiles<4, 2, 1, 1, 3>(parts); break;
+    case 7: launch_tiles<4, 2, 1, 2, 2>(parts); break;
+    default: launch_tiles<4, 2, 2, 2, 1>(parts); break;
+  }
+  if (work) {
+    const long long pieces = m * (((long long)n + 3) / 4);
+    hipLaunchKernelGGL(product_join, dim3((unsigned)(pieces < (1LL << 30) ? (pieces + 255) / 256 : 1 << 22)), dim3(256), 0, wdh::stream(), p, partial,
+                       plan.parts);
+    (void)wdh_free(work);
+  }
   if (packed) (void)wdh_free(packed);
   WDH_LAUNCH_CHECK();
   return WDH_OK;
