@@ -200,10 +200,13 @@ void launch_few(const ProductParams &p, bool aligned) {
 // A slab is a block of K: 128 bytes of every row of the tile, which pass through registers into LDS while the slab before is
 // multiplied.  In LDS a row's eight 16-byte pieces are exchanged by its number (piece ^ row % 8), so that the 32 rows that a
 // fragment read takes a piece of lie on different banks.  A fragment's 16 bytes serve two instructions (their k are the first and the
-// last eight of them, on both sides alike).
+// last eight of them, on both sides alike).  A slab is multiplied by quarters, the next one's fragments on their way from LDS
+// meanwhile (8192^3: 1035 to 1055 us, 1042 to 1062 TFLOP/s; fragments of the whole slab at a time 1146).
+// Bound: the matrix cores, the conversions and the way through LDS alternate more than they overlap (without the loads of slabs that
+// product takes 890 us, without their way into LDS either 800; library products of bfloat16 operands of that size take 954).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <int NW, int MW, int TN, int TM, int DEPTH>
+template <int NW, int MW, int TN, int TM>
 __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p) {
   constexpr int THREADS = 64 * NW * MW, BN = 32 * NW * TN, BM = 32 * MW * TM, ROWS = BN + BM;
   constexpr int LOADS = ROWS * 8 / THREADS;
@@ -213,7 +216,7 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int wn = wave % NW, wm = wave / NW;
   // (Workgroups go to the eight XCDs in turn: those that run at a time on one of them are a block of several columns by several rows of
-  // tiles.  A strip of neighbouring columns for each XCD, which reads W once, is slower: 8192^3 1139 / 1363 us.)
+  // tiles.  A strip of neighbouring columns for each XCD, which reads W once, is slower: 8192^3, an earlier form of this kernel: 1139 / 1363 us.)
   const int tiles_n = (p.n + BN - 1) / BN;
   const long long m0 = (long long)(blockIdx.x / tiles_n) * BM;
   const int n0 = (int)(blockIdx.x % tiles_n) * BN;
@@ -231,30 +234,29 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
   const int wide = (n0 + 32 * TN * wn) / BLOCK;  // (columns beyond n: any scale will do)
   const float *sw = p.SW + (long long)(wide * BLOCK < p.n ? wide : 0) * p.blocks;
 
-  Piece<true> next[DEPTH][LOADS];
-  float next_scale[DEPTH];
   const int begin = blockIdx.y * p.part, end = begin + p.part < p.blocks ? begin + p.part : p.blocks;
-  auto fetch = [&](int slot, int b) {
+  Piece<true> next[LOADS];
+  float next_scale;
+  auto fetch = [&](int b) {
     if (b >= end) return;
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) next[slot][i].load(row[i], b * BLOCK + piece, p.k);
-    if (tid < BM) next_scale[slot] = my_scale[b];
+    for (int i = 0; i < LOADS; i++) next[i].load(row[i], b * BLOCK + piece, p.k);
+    if (tid < BM) next_scale = my_scale[b];
   };
-  auto keep = [&](int slot, int b) {
+  auto keep = [&](int b) {
     if (b >= end) return;
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) *reinterpret_cast<i32x4 *>(&lds[b & 1][to[i]]) = next[slot][i].get(row[i], b * BLOCK + piece, p.k);
-    if (tid < BM) scales[b & 1][tid] = next_scale[slot];
+    for (int i = 0; i < LOADS; i++) *reinterpret_cast<i32x4 *>(&lds[b & 1][to[i]]) = next[i].d;
+    if (tid < BM) scales[b & 1][tid] = next_scale;
   };
-  // a 32-row block's fragments: 16 bytes for each quarter of the slab
-  auto fragment = [&](int buf, int r0, bf16x8 (&f)[8]) {
-    const int r = r0 + li;
+  // 16 bytes of each row of the wavefront's blocks: its share of a quarter of the slab
+  i32x4 rw[TN], ra[TM];
+  auto quarter = [&](int buf, int q) {
+    const int at = 16 * ((2 * q + half) ^ (li & 7));
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-      const i32x4 x = *reinterpret_cast<const i32x4 *>(&lds[buf][r * BLOCK + 16 * ((2 * q + half) ^ (r & 7))]);
-      f[2 * q] = widen(x[0], x[1]);
-      f[2 * q + 1] = widen(x[2], x[3]);
-    }
+    for (int i = 0; i < TN; i++) rw[i] = *reinterpret_cast<const i32x4 *>(&lds[buf][(32 * (TN * wn + i) + li) * BLOCK + at]);
+#pragma unroll
+    for (int j = 0; j < TM; j++) ra[j] = *reinterpret_cast<const i32x4 *>(&lds[buf][(BN + 32 * (TM * wm + j) + li) * BLOCK + at]);
   };
 
   f32x16 acc[TN][TM];
@@ -264,47 +266,53 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
     for (int j = 0; j < TM; j++)
 #pragma unroll
       for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
-  // slab begin + b goes to LDS through registers slot b % DEPTH, which then ask for the slab DEPTH behind it
-#pragma unroll
-  for (int d = 0; d < DEPTH; d++) fetch(d, begin + d);
-  keep(0, begin);
-  fetch(0, begin + DEPTH);
+  fetch(begin);
+  keep(begin);
+  fetch(begin + 1);
   __syncthreads();
-  for (int b0 = begin; b0 < end; b0 += DEPTH) {
+  quarter(begin & 1, 0);
+  for (int b = begin; b < end; b++) {
+    const int buf = b & 1;
+    const float s = sw[b];
+    float c[TM];
 #pragma unroll
-    for (int d = 0; d < DEPTH; d++) {
-      const int b = b0 + d, buf = b & 1;
-      if (b >= end) break;
-      keep((d + 1) % DEPTH, b + 1);
-      fetch((d + 1) % DEPTH, b + 1 + DEPTH);
-      const float s = sw[b];
-      bf16x8 a[TM][8];
-      float c[TM];
+    for (int j = 0; j < TM; j++) c[j] = scales[buf][32 * (TM * wm + j) + li] * s;
+    f32x16 x[TN][TM];
 #pragma unroll
-      for (int j = 0; j < TM; j++) {
-        fragment(buf, BN + 32 * (TM * wm + j), a[j]);
-        c[j] = scales[buf][32 * (TM * wm + j) + li] * s;
+    for (int i = 0; i < TN; i++)
+#pragma unroll
+      for (int j = 0; j < TM; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[i][j][e] = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      bf16x8 fw[TN][2], fa[TM][2];
+#pragma unroll
+      for (int i = 0; i < TN; i++) fw[i][0] = widen(rw[i][0], rw[i][1]), fw[i][1] = widen(rw[i][2], rw[i][3]);
+#pragma unroll
+      for (int j = 0; j < TM; j++) fa[j][0] = widen(ra[j][0], ra[j][1]), fa[j][1] = widen(ra[j][2], ra[j][3]);
+      if (q == 2) {
+        keep(b + 1);
+        fetch(b + 2);
+      }
+      if (q < 3) quarter(buf, q + 1);
+      else {
+        __syncthreads();  // (the slab has been read, the next one is there)
+        quarter(buf ^ 1, 0);
       }
 #pragma unroll
-      for (int i = 0; i < TN; i++) {
-        bf16x8 w[8];
-        fragment(buf, 32 * (TN * wn + i), w);
-        f32x16 x[TM];
+      for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int j = 0; j < TM; j++)
+        for (int i = 0; i < TN; i++)
 #pragma unroll
-          for (int e = 0; e < 16; e++) x[j][e] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-#pragma unroll
-          for (int j = 0; j < TM; j++) x[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[k], a[j][k], x[j], 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < TM; j++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) acc[i][j][e] = __builtin_fmaf(x[j][e], c[j], acc[i][j][e]);
-      }
-      __syncthreads();
+          for (int j = 0; j < TM; j++) x[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fw[i][h], fa[j][h], x[i][j], 0, 0, 0);
     }
+#pragma unroll
+    for (int i = 0; i < TN; i++)
+#pragma unroll
+      for (int j = 0; j < TM; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[i][j][e] = __builtin_fmaf(x[i][j][e], c[j], acc[i][j][e]);
   }
   float *Y = p.Y + blockIdx.y * p.m * p.n;
   // lane: row li of a block; registers 4 q .. + 3 are columns 8 q + 4 half .. + 3
@@ -323,11 +331,11 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
   }
 }
 
-template <int NW, int MW, int TN, int TM, int DEPTH>
+template <int NW, int MW, int TN, int TM>
 void launch_tiles(const ProductParams &p) {
   constexpr int BN = 32 * NW * TN, BM = 32 * MW * TM;
   const long long tiles = (p.n + BN - 1) / BN * ((p.m + BM - 1) / BM);
-  hipLaunchKernelGGL((product_tiles<NW, MW, TN, TM, DEPTH>), dim3((unsigned)tiles, parts_of(p)), dim3(64 * NW * MW), 0, wdh::stream(), p);
+  hipLaunchKernelGGL((product_tiles<NW, MW, TN, TM>), dim3((unsigned)tiles, parts_of(p)), dim3(64 * NW * MW), 0, wdh::stream(), p);
 }
 
 // The parts of a product together, in order: four results to a lane.
@@ -366,14 +374,14 @@ __global__ __launch_bounds__(256) void pack_rows(const unsigned char *A, const u
 // than 16 cost the smallest form, which is bound by its loads, less).  Tiles that leave
 // CUs idle are cut along K into as many parts as there are CUs for; the parts' join is a launch of 4 us and its bytes.  The cheapest
 // of all wins (us, so / the smallest tile that fits the chip, uncut: 4096 columns, K = 14336: 32 rows 20 / 36, 64 rows 24 / 36, 256 rows
-// 46 / 70; 8192 x 8192: 128 rows 33 / 44, 1024 rows 153 / 161).
+// 46 / 70; 8192 x 8192: 128 rows 33 / 44, 1024 rows 138 / 161).
 struct Form {
   int cols, rows;
   float start, block;
 };
 constexpr int FIRST_TILES = 6, FORMS = 9;
 constexpr Form forms[FORMS] = {{16, 16, 3.0f, 0.16f}, {32, 16, 1.5f, 0.27f}, {64, 16, 1.5f, 0.47f},   {32, 32, 3.0f, 0.31f},  {64, 32, 2.0f, 0.48f},
-                               {64, 64, 4.0f, 0.62f}, {128, 64, 5.0f, 0.87f}, {128, 128, 8.0f, 1.15f}, {256, 128, 9.0f, 2.25f}};
+                               {64, 64, 4.0f, 0.62f}, {128, 64, 5.0f, 0.87f}, {128, 128, 8.0f, 1.2f}, {256, 128, 9.0f, 2.0f}};
 struct Plan {
   int form, parts;
 };
@@ -470,9 +478,9 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
     case 3: launch_few<2, 2, 8, 2>(parts, aligned); break;
     case 4: launch_few<4, 2, 8, 1>(parts, aligned); break;
     case 5: launch_few<4, 4, 8, 1>(parts, aligned); break;
-    case 6: launch_tiles<4, 2, 1, 1, 3>(parts); break;
-    case 7: launch_tiles<4, 2, 1, 2, 2>(parts); break;
-    default: launch_tiles<4, 2, 2, 2, 1>(parts); break;
+    case 6: launch_tiles<4, 2, 1, 1>(parts); break;
+    case 7: launch_tiles<4, 2, 1, 2>(parts); break;
+    default: launch_tiles<4, 2, 2, 2>(parts); break;
   }
   if (work) {
     const long long pieces = m * (((long long)n + 3) / 4);
