@@ -677,6 +677,38 @@ __device__ __forceinline__ float halves_max(float v) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// Item number `rank` of `items`, the longest (in pages) first, so that what is left at the end are short ones (three prompts of 1200 to
+// 4000 tokens, 976 items for the 512 places of the chip: 257 us, sequence by sequence 279).  Of the items of a sequence, those that see
+// at least T pages are the last ones, so their number is one division, the number of all of them one sum over the lanes, and T a search
+// over the pages of the longest sequence.  That takes 1 us: items of one sequence need no search, and beyond 64 sequences, which a
+// wavefront looks at side by side, they come sequence by sequence.
+__device__ __forceinline__ Place many_item(const AttendParams &p, int rank, int items) {
+  const int group = p.group.d;
+  auto count = [group](const Place &s) { return (int)(((long long)s.n * group + MANY - 1) / MANY); };
+  if (p.q.seqs == 1 || p.q.seqs > 64) return locate(p.q, items - 1 - rank, count);
+  const Place mine = sequence(p.q, threadIdx.x & 63);
+  const int all = mine.n ? count(mine) : 0, past = mine.len - mine.n;
+  // the first of the lane's items that sees `pages` pages: its last token is not before 64 (pages - 1), and tokens' rows are `group` each
+  auto first = [&](int pages) {
+    const long long token = (long long)PAGE * (pages - 1) - past;
+    return token <= 0 ? 0 : token >= mine.n ? all : (int)(token * group / MANY);
+  };
+  auto total = [](int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); };
+  if (rank >= total(all)) return Place{0, 0, 0, 0, 0};
+  int least = 1, most = __builtin_amdgcn_readfirstlane((int)wdh::rowmath::wave_max(all ? (float)((mine.len - 1) / PAGE + 1) : 0.0f));
+  while (least < most) {
+    const int middle = (least + most + 1) / 2;
+    if (total(all - first(middle)) > rank) least = middle;
+    else most = middle - 1;
+  }
+  const int from = first(least), to = first(least + 1), upto = wave_scan(to - from), left = rank - total(all - to);
+  const unsigned long long has = __ballot(left < upto);
+  if (!has) return Place{0, 0, 0, 0, 0};  // (numbers that contradict each other)
+  const int at = __ffsll(has) - 1;
+  return Place{__builtin_amdgcn_readlane(mine.seq, at), __builtin_amdgcn_readlane(mine.row0, at), __builtin_amdgcn_readlane(mine.n, at),
+               __builtin_amdgcn_readlane(mine.len, at), __builtin_amdgcn_readlane(from + left - (upto - (to - from)), at)};
+}
+
 template <int D>
 __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   constexpr int QN = D / 32, DT = D / 32;           // runs of 32 elements of d in a key; blocks of 32 rows of O^T
@@ -685,9 +717,8 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   __shared__ __attribute__((aligned(16))) unsigned char keys[3][PAGE * D], values[3][PAGE * D];
   __shared__ int bad[4];                            // NaN among values that some row does not see
   const int group = p.group.d;
-  // The items at the end of a sequence are the longest: they start first, for all heads.
-  const int at_item = blockIdx.x / p.kv_heads, head = blockIdx.x - at_item * p.kv_heads, item = gridDim.x / p.kv_heads - 1 - at_item;
-  const Place s = locate(p.q, item, [group](const Place &s) { return (int)(((long long)s.n * group + MANY - 1) / MANY); });
+  const int item = blockIdx.x / p.kv_heads, head = blockIdx.x - item * p.kv_heads;
+  const Place s = many_item(p, item, gridDim.x / p.kv_heads);
   if (s.n == 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int past = s.len - s.n;
@@ -955,7 +986,7 @@ template <int D>
 __global__ __launch_bounds__(256) void attend_many_join(AttendParams p, int parts) {
   constexpr int LANES = D / 4, ROWS = 256 / LANES;
   const int group = p.group.d, head = blockIdx.y;
-  const Place s = locate(p.q, blockIdx.x, [group](const Place &s) { return (int)(((long long)s.n * group + MANY - 1) / MANY); });
+  const Place s = many_item(p, blockIdx.x, gridDim.x);
   const int row = blockIdx.z * ROWS + threadIdx.x / LANES, lane = threadIdx.x % LANES;
   const int flat = s.index * MANY + row, token = wdh::fdiv(flat, p.group);
   if (token >= s.n) return;
