@@ -37,19 +37,78 @@ def test_attention_of_more_sequences_than_lanes(ctx, new, heads, kv, d):
     assert np.all(np.abs(S.attend(ctx, c, q, table, lens, starts, np.float32(d ** -0.5)) - want) <= bound)
 
 
+# Items of 128 rows (calls of 16384 rows of queries and more): one long sequence cut into parts, several with short and empty ones between
+# them, a head of the cache for each query, one for 64, more sequences than lanes
+MANY = [([300], [700], 64, 2, 32), ([260, 100, 1, 0, 40], [0, 65, 500, 0, 0], 48, 3, 64), ([1030], [0], 16, 4, 128), ([200, 150], [30, 1], 64, 64, 32),
+        ([257], [3000], 64, 1, 128), ([20] * 70, list(range(0, 210, 3)), 16, 2, 64), ([900, 300, 50], [10, 0, 700], 24, 8, 128)]
+
+
+@pytest.mark.parametrize("new,past,heads,kv,d", MANY)
+def test_attention_of_many_rows(ctx, new, past, heads, kv, d):
+    assert sum(new) * heads >= 16384 and sum(new) * heads // kv >= 64 * len(new)
+    rng = np.random.default_rng(sum(new))
+    c, table, lens, starts = S.filled(rng, new, past, kv, d)
+    q = rng.standard_normal((int(starts[-1]), heads, d)).astype(np.float32)
+    want, bound = c.attention(q, table, lens, starts, d ** -0.5)
+    got = S.attend(ctx, c, q, table, lens, starts, np.float32(d ** -0.5), wide=4 * (len(new) % 2))
+    assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) - bound))
+
+
+def test_many_rows_with_sharp_scores(ctx):
+    rng = np.random.default_rng(8)
+    c, table, lens, starts = S.filled(rng, [300, 2], [40, 400], 2, 64)
+    q = rng.standard_normal((302, 64, 64)).astype(np.float32) * np.float32(50)
+    q[3] = 0
+    want, bound = c.attention(q, table, lens, starts, -1.0)
+    assert np.all(np.abs(S.attend(ctx, c, q, table, lens, starts, -1.0) - want) <= bound)
+
+
+def test_nan_behind_a_row_of_many_does_not_reach_it(ctx):
+    rng = np.random.default_rng(9)
+    c, table, lens, starts = S.filled(rng, [300], [30], 2, 64)
+    q = rng.standard_normal((300, 64, 64)).astype(np.float32)
+    want, bound = c.attention(q, table, lens, starts, 0.125)
+    for hit, where in ((110, 5), (317, 40)):                             # a page in the middle and the last one
+        page, slot = table[0, hit // 64], hit % 64
+        c.v[page, 0, where, slot] = 0x7f
+        c.k[page, 1, slot, 9] = 0xff
+    got = S.attend(ctx, c, q, table, lens, starts, 0.125)
+    rows = np.arange(300)[:, None, None] + 30
+    nan = np.zeros(got.shape, bool)
+    nan[:, :32, 5], nan[:, :32, 40], nan[:, 32:] = rows[..., 0] >= 110, rows[..., 0] >= 317, rows >= 110
+    assert np.isnan(got[nan]).all() and np.all((np.abs(got - want) <= bound)[~nan])
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, np.inf, np.nan])
+@pytest.mark.parametrize("values", [False, True])
+def test_many_rows_and_a_page_without_a_scale_or_a_place(ctx, scale, values):
+    rng = np.random.default_rng(14)
+    c, table, lens, starts = S.filled(rng, [400, 1], [100, 70], 2, 64)
+    q = rng.standard_normal((401, 64, 64)).astype(np.float32)
+    want, bound = c.attention(q, table, lens, starts, 0.125)
+    (c.vs if values else c.ks)[table[0, 3], 1] = scale                    # tokens 192 .. 255 of one head
+    table[0, 6] = -5                                                      # tokens 384 .. 447 of both
+    got = S.attend(ctx, c, q, table, lens, starts, 0.125)
+    rows = np.arange(401)[:, None, None] + 100
+    nan = np.broadcast_to((rows >= 384) & (rows < 500), got.shape).copy()
+    nan[:, 32:] |= ((rows >= 192) & (rows < 500))
+    assert np.isnan(got[nan]).all() and np.all((np.abs(got - want) <= bound)[~nan])
+
+
 def test_a_cache_beyond_4_gib(ctx):
     """Keys alone take 4.3 GiB: pages on both sides of 2 and 4 GiB, tokens one by one and in a prompt."""
     rng = np.random.default_rng(31)
     heads, kv, d, pages = 16, 8, 128, 70000
-    far = np.array([[69999, 32768, 65535], [65536, -1, -1], [32767, 1, -1]], np.int32)
-    near = np.array([[0, 1, 2], [3, -1, -1], [4, 5, -1]], np.int32)
-    lens, starts = np.array([150, 1, 70], np.int32), np.array([0, 150, 151, 221], np.int32)
-    k, v = (rng.standard_normal((221, kv, d)).astype(np.float32) for _ in range(2))
-    c = F.Cache(6, kv, d)
+    far = np.full((3, 18), -1, np.int32)
+    far[0, :3], far[1, 0], far[2] = [69999, 32768, 65535], 65536, np.append([32767, 1], 66000 + np.arange(16))
+    near = np.where(far < 0, -1, np.cumsum(far >= 0).reshape(far.shape) - 1).astype(np.int32)
+    lens, starts = np.array([150, 1, 1100], np.int32), np.array([0, 150, 151, 1251], np.int32)
+    k, v = (rng.standard_normal((1251, kv, d)).astype(np.float32) for _ in range(2))
+    c = F.Cache(22, kv, d)
     c.append(k, v, near, lens, starts)
     cache = H.KvCache.empty(ctx, pages, kv, d)
     up = ctx.move_tensor
-    H.cache_append(ctx, cache, up(k.reshape(221, -1)), up(v.reshape(221, -1)), up(far), up(lens), up(starts))
+    H.cache_append(ctx, cache, up(k.reshape(1251, -1)), up(v.reshape(1251, -1)), up(far), up(lens), up(starts))
     for scales, want in ((cache.k_scales, c.ks), (cache.v_scales, c.vs)):
         assert np.array_equal(scales.get_data()[far[far >= 0]], want[near[near >= 0]])
     for begin in (starts, np.array([0, 1, 2, 3], np.int32)):                    # the prompts; their last tokens alone
@@ -126,12 +185,12 @@ def test_no_room_for_a_workspace(ctx):
 
 
 def test_recorded_runs_do_not_share_workspaces(ctx):
-    """Three recorded calls with workspaces (shares of single tokens, parts of a prompt, copied operands), replayed in turn with eager
+    """Recorded calls with workspaces (shares of single tokens, parts of prompts, copied operands), replayed in turn with eager
     work of the same kinds and other allocations between them: every replay against the first results."""
     rng = np.random.default_rng(17)
     up = ctx.move_tensor
     calls = []
-    for new, past in (([1, 1], [3000, 40]), ([100], [900])):
+    for new, past in (([1, 1], [3000, 40]), ([100], [900]), ([1100, 1000], [60, 0])):
         c, table, lens, starts = S.filled(rng, new, past, 2, 64)
         operands = (S.on_device(ctx, c), up(rng.standard_normal((sum(new), 512)).astype(np.float32)), up(table), up(lens), up(starts))
         calls.append(lambda o=operands, out=None: H.cache_attention(ctx, o[0], o[1], 8, 0.125, *o[2:], out=out))

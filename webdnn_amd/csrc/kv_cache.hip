@@ -1028,7 +1028,8 @@ int launch_attend(const AttendParams &p, long long items) {
   WDH_LAUNCH_CHECK();
   if (p.partial) {
     // (an item of hundreds of shares is a wide workgroup's work, one of a few shares a small one's)
-    const dim3 grid((unsigned)items, (unsigned)p.kv_heads, (unsigned)(p.group.d < 16 ? p.group.d : 16));
+    const long long rows = ((long long)p.q.tokens * p.group.d + p.q.seqs - 1) / p.q.seqs;  // (of a sequence, on average)
+    const dim3 grid((unsigned)items, (unsigned)p.kv_heads, (unsigned)(rows < 16 ? rows : 16));
     if (p.wgs >= 32 * items) hipLaunchKernelGGL((attend_join<D, 1024>), grid, dim3(1024), 0, st, p);
     else hipLaunchKernelGGL((attend_join<D, 256>), grid, dim3(256), 0, st, p);
     WDH_LAUNCH_CHECK();
@@ -1149,7 +1150,11 @@ extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_strid
     const long long loose = (long long)tokens * p.group.d / rows + seqs, tight = (long long)tokens * ((p.group.d + rows - 1) / rows);
     return loose < tight ? loose : tight;
   };
-  const bool many = (long long)tokens * p.group.d >= 64LL * seqs;  // (on average: more than half of an item of 128)
+  // Items of 128 rows read a page once for eight times the rows, but need more of them to fill the chip: they are taken where sequences
+  // fill half an item on average, and the call has 64 rows for each CU (us, 16 / 128 rows an item, 32 heads on 8 behind 2000 tokens: 16 x
+  // 64 tokens 167 / 100, 4 x 128 78 / 73, 1 x 256 42 / 50, 16 x 16 51 / 77; 16 heads on 4: 4 x 512 329 / 171, 4 x 64 and below 0.85 of
+  // the other's time).
+  const bool many = (long long)tokens * p.group.d >= 64LL * seqs && (long long)tokens * heads >= 64LL * wdh::compute_units();
   const long long items = items_of_rows(many ? MANY : 16);
   if (items > 0xffffffLL / 2) return fail(WDH_EINVAL, "%s: too many rows", who);
   p.partial = p.stats = nullptr;
