@@ -27,10 +27,11 @@ def test_narrow_last_blocks(ctx, cols):
 
 
 @pytest.mark.parametrize("new,heads,kv,d", [([1, 0, 2] * 45, 4, 2, 32), ([20] * 70, 8, 2, 64), ([1] * 200, 3, 3, 64)])
-def test_attention_of_more_sequences_than_lanes(ctx, new, heads, kv, d):
+@pytest.mark.parametrize("longest", [350, 900, 1500])          # (a workgroup to an item; the same for many items; shares of all pages)
+def test_attention_of_more_sequences_than_lanes(ctx, new, heads, kv, d, longest):
     rng = np.random.default_rng(len(new))
-    past = rng.integers(0, 400, len(new))
-    past[5], past[66] = 1500, 0
+    past = rng.integers(0, 350, len(new))
+    past[5], past[66] = longest, 0
     c, table, lens, starts = S.filled(rng, new, past, kv, d)
     q = rng.standard_normal((int(starts[-1]), heads, d)).astype(np.float32)
     want, bound = c.attention(q, table, lens, starts, d ** -0.5)

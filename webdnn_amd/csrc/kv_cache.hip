@@ -206,7 +206,7 @@ struct AttendParams {
   int heads, kv_heads;
   wdh::FastDiv group;  // queries that share a head of the cache
   float scale;     // alpha * log2(e): powers are taken of two
-  int wgs;         // workgroups for each head of the cache
+  int wgs;         // workgroups for each head of the cache (0: one for each item, which works on the whole of it)
   float *partial;  // results [workgroup][2][kv head][16][D] of items that more than one workgroup works on (null: there are none),
   float *stats;    // and their tops and sums [workgroup][2][kv head][16][2]
 };
@@ -371,19 +371,25 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
   const unsigned k_lane = (16 * (i16 >> 2) + (i16 & 3)) * D + (D >= 64 ? 16 : 8) * g, v_lane = i16 * PAGE + 16 * g;  // (of a page)
   const int head = blockIdx.y;
   const Look first = look(p, 0);
-  const int total = total_units(p, first), share = (total + p.wgs - 1) / p.wgs;
   const Minus minus = minus_one();
-  int unit = blockIdx.x * share;
-  const int units_end = total - unit < share ? total : unit + share;
   Work w;
-  w.s.n = 0;
+  int unit, units_end;
+  if (p.wgs) {
+    const int total = total_units(p, first), share = (total + p.wgs - 1) / p.wgs;
+    unit = blockIdx.x * share;
+    units_end = total - unit < share ? total : unit + share;
+  } else {
+    w = locate_work(p, first, blockIdx.x, true);
+    unit = w.before;
+    units_end = w.s.n ? w.before + w.units : unit;
+  }
   for (bool first_segment = true; unit < units_end; first_segment = false) {
   // the item of the last segment has another behind it, or the next sequence's first one follows
   if (!first_segment && (w.item + 1) * 16LL < (long long)w.s.n * group) {
     w.item++;
     w.before = unit;
     w.unit = 0;
-  } else {
+  } else if (p.wgs) {
     w = locate_work(p, first_segment ? first : look(p, 0), unit, false);
     if (w.s.n == 0) return;  // (numbers that contradict each other)
   }
@@ -1024,7 +1030,7 @@ int launch_many(const AttendParams &p, long long items, int parts) {
 template <int D>
 int launch_attend(const AttendParams &p, long long items) {
   hipStream_t st = wdh::stream();
-  hipLaunchKernelGGL((attend_rows<D>), dim3((unsigned)p.wgs, (unsigned)p.kv_heads), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((attend_rows<D>), dim3((unsigned)(p.wgs ? p.wgs : items), (unsigned)p.kv_heads), dim3(256), 0, st, p);
   WDH_LAUNCH_CHECK();
   if (p.partial) {
     // (an item of hundreds of shares is a wide workgroup's work, one of a few shares a small one's)
@@ -1181,7 +1187,11 @@ extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_strid
     const long long units = items * ((max_pages + 3) / 4), resident = 2LL * wdh::compute_units() / kv_heads;
     if (units > MOST_UNITS) return fail(WDH_EINVAL, "%s: too many rows of tables so wide", who);
     p.wgs = (int)(units < resident ? units : resident > 0 ? resident : 1);
-    if (max_pages > 4 && p.wgs > 1 && !workspace((size_t)p.wgs * 2 * kv_heads * 16)) return WDH_ENOMEM;  // (items of one unit are never cut)
+    // Where tables hold few pages, sharing them out costs more (the join's launch) than it evens out: a workgroup to an item then (us, shared /
+    // so, 32 heads on 8: 4 x 60 tokens behind 300 23.0 / 14.6, 64 single ones behind 100 to 1000 32.6 / 21.8, 8 behind 500 12.3 / 10.6,
+    // behind 1000 12.5 / 14.8).
+    if (max_pages <= (items * kv_heads >= wdh::compute_units() ? 16 : 8)) p.wgs = 0;
+    if (p.wgs > 1 && !workspace((size_t)p.wgs * 2 * kv_heads * 16)) return WDH_ENOMEM;  // (items of one unit are never cut)
     rc = d == 32 ? launch_attend<32>(p, items) : d == 64 ? launch_attend<64>(p, items) : launch_attend<128>(p, items);
   }
   if (work) (void)wdh_free(work);
