@@ -18,6 +18,12 @@ def test_every_tile_of_the_products(ctx, m, n, k):
     S.check_product(ctx, np.random.default_rng(m + n + k), m, n, k, bias=True, residual=m < 2000)
 
 
+@pytest.mark.parametrize("rows,length", [(9, 700), (6, 768), (1030, 769), (11, 1400), (3, 1536), (70, 1537), (2, 5000), (3, 6144), (40, 6145), (600, 8500), (5, 12000),
+                                         (2, 16384), (513, 9001), (3, 16385)])
+def test_every_form_of_the_norm(ctx, rows, length):
+    S.test_norm(ctx, rows, length, True, True)
+
+
 @pytest.mark.parametrize("cols", [3, 5, 20, 33, 64, 65, 100, 132, 137, 156, 190, 193])
 def test_narrow_last_blocks(ctx, cols):
     rng = np.random.default_rng(cols)

@@ -52,9 +52,9 @@ __device__ __forceinline__ void finish_piece(const NormParams &p, long long row,
 
 // WAVES wavefronts to a row, NP pieces of four elements to a lane: a row of up to 256 * WAVES * NP elements in registers.
 template <int WAVES, int NP>
-__global__ __launch_bounds__(256) void rmsnorm_rows(NormParams p) {
-  constexpr int ROWS = 4 / WAVES;
-  __shared__ double part[4];
+__global__ __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) void rmsnorm_rows(NormParams p) {
+  constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
+  __shared__ double part[ROWS * WAVES];
   const int wave = threadIdx.x >> 6, t = threadIdx.x % (64 * WAVES);
   for (long long row0 = (long long)blockIdx.x * ROWS; row0 < p.outer; row0 += (long long)gridDim.x * ROWS) {
     const bool live = row0 + wave / WAVES < p.outer;
@@ -84,7 +84,10 @@ __global__ __launch_bounds__(256) void rmsnorm_rows(NormParams p) {
     if constexpr (WAVES > 1) {
       if ((threadIdx.x & 63) == 0) part[wave] = sum;
       __syncthreads();
-      sum = ((part[0] + part[1]) + part[2]) + part[3];
+      const double *mine = part + wave / WAVES * WAVES;
+      sum = mine[0];
+#pragma unroll
+      for (int i = 1; i < WAVES; i++) sum += mine[i];
       __syncthreads();  // (the next row's sums go to the same places)
     }
     const float inv = (float)(1.0 / sqrt(sum / (double)p.len + (double)p.eps));
@@ -204,6 +207,13 @@ __global__ __launch_bounds__(256) void quantize_tiles(const float *__restrict__ 
   if (threadIdx.x == 0) QS[unit] = c;
 }
 
+constexpr long long MOST_WGS = 1 << 20;  // (more rows than these hold are taken in turns)
+template <int WAVES, int NP>
+void launch_rows(const NormParams &p) {
+  const long long wgs = WAVES < 4 ? (p.outer + 4 / WAVES - 1) / (4 / WAVES) : p.outer;
+  hipLaunchKernelGGL((rmsnorm_rows<WAVES, NP>), dim3((unsigned)(wgs < MOST_WGS ? wgs : MOST_WGS)), dim3(WAVES < 4 ? 256 : 64 * WAVES), 0, wdh::stream(), p);
+}
+
 }  // namespace
 
 using wdh::fail;
@@ -238,17 +248,21 @@ extern "C" int wdh_rmsnorm(wdh_buf hX, wdh_buf hSkip, wdh_buf hGamma, wdh_buf hS
   p.X = (const float *)px; p.R = (const float *)pr; p.G = (const float *)pg; p.S = (float *)ps; p.Y = (float *)py;
   p.Q = (unsigned char *)pq; p.QS = (float *)pqs;
   p.outer = outer; p.len = len; p.blocks = (int)blocks; p.eps = eps;
-  hipStream_t st = wdh::stream();
-  const long long most = 1 << 20;  // (workgroups; more rows than that are taken in turns)
-  const long long quarters = (outer + 3) / 4;
-  const dim3 four((unsigned)(quarters < most ? quarters : most)), one((unsigned)(outer < most ? outer : most)), wg(256);
-  if (len <= 256) hipLaunchKernelGGL((rmsnorm_rows<1, 1>), four, wg, 0, st, p);
-  else if (len <= 512) hipLaunchKernelGGL((rmsnorm_rows<1, 2>), four, wg, 0, st, p);
-  else if (len <= 1024) hipLaunchKernelGGL((rmsnorm_rows<4, 1>), one, wg, 0, st, p);
-  else if (len <= 2048) hipLaunchKernelGGL((rmsnorm_rows<4, 2>), one, wg, 0, st, p);
-  else if (len <= 4096) hipLaunchKernelGGL((rmsnorm_rows<4, 4>), one, wg, 0, st, p);
-  else if (len <= 8192) hipLaunchKernelGGL((rmsnorm_rows<4, 8>), one, wg, 0, st, p);
-  else hipLaunchKernelGGL(rmsnorm_stream, one, wg, 0, st, p);
+  // As few wavefronts to a row as leave a lane four pieces, and as few pieces as hold it, but for one thing: long rows take more wavefronts,
+  // a lane's eight pieces of X and Skip being too many registers.  (us, 100 MB of rows of 782 elements: 1 wavefront of 4 pieces 78.7, 4 of
+  // 1 85.6; of 570: 1 of 3 77.5, 4 of 1 107.0; of 6000: 8 of 3 74.7, 4 of 8 94.4; of 8192: 8 of 4 71.2, 4 of 8 79.2.)  Rows beyond 8192
+  // elements stay in registers where there are few of them (100 of 12000: 8.2 us, read twice 15.8; 2000: 92.7 and 85.8).
+  if (len <= 256) launch_rows<1, 1>(p);
+  else if (len <= 512) launch_rows<1, 2>(p);
+  else if (len <= 768) launch_rows<1, 3>(p);
+  else if (len <= 1024) launch_rows<1, 4>(p);
+  else if (len <= 1536) launch_rows<2, 3>(p);
+  else if (len <= 2048) launch_rows<4, 2>(p);
+  else if (len <= 4096) launch_rows<4, 4>(p);
+  else if (len <= 6144) launch_rows<8, 3>(p);
+  else if (len <= 8192) launch_rows<8, 4>(p);
+  else if (len <= 16384 && outer <= 2 * wdh::compute_units()) launch_rows<16, 4>(p);
+  else hipLaunchKernelGGL(rmsnorm_stream, dim3((unsigned)(outer < MOST_WGS ? outer : MOST_WGS)), dim3(256), 0, wdh::stream(), p);
   WDH_LAUNCH_CHECK();
   return WDH_OK;
 }
