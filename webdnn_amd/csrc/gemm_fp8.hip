@@ -52,9 +52,8 @@ struct Piece<false> {
   int e;
   __device__ __forceinline__ void load(const unsigned char *row, int k, int len) {
     const int left = len - k, from = left > 0 ? k : len - 1;  // (behind the end: the last byte's dword, of which nothing is kept)
-    const uintptr_t at = (uintptr_t)(row + from);
-    const int *base = reinterpret_cast<const int *>(at & ~(uintptr_t)3);
-    const unsigned shift = (unsigned)at & 3u;
+    const unsigned shift = (unsigned)((uintptr_t)row + from) & 3u;
+    const int *base = reinterpret_cast<const int *>(row + from - shift);  // (a number made a pointer again would be loaded from as of any kind)
     if (left >= 16) {
       typedef int i32x4_dwords __attribute__((ext_vector_type(4), aligned(4)));
       d = *reinterpret_cast<const i32x4_dwords *>(base);
