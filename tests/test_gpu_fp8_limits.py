@@ -44,15 +44,15 @@ def test_attention_of_more_sequences_than_lanes(ctx, new, heads, kv, d, longest)
     assert np.all(np.abs(S.attend(ctx, c, q, table, lens, starts, np.float32(d ** -0.5)) - want) <= bound)
 
 
-# Items of 128 rows (calls of 16384 rows of queries and more): one long sequence cut into parts, several with short and empty ones between
-# them, a head of the cache for each query, one for 64, more sequences than lanes
-MANY = [([300], [700], 64, 2, 32), ([260, 100, 1, 0, 40], [0, 65, 500, 0, 0], 48, 3, 64), ([1030], [0], 16, 4, 128), ([200, 150], [30, 1], 64, 64, 32),
-        ([257], [3000], 64, 1, 128), ([20] * 70, list(range(0, 210, 3)), 16, 2, 64), ([900, 300, 50], [10, 0, 700], 24, 8, 128)]
+# Items of 128 rows (calls of 80 * 256 rows of queries of 128 elements and more): one long sequence cut into parts, several with short and
+# empty ones between them, a head of the cache for each query, one for 64, more sequences than lanes
+MANY = [([1300], [700], 64, 2, 32), ([600, 251, 1, 0, 40], [0, 65, 500, 0, 0], 48, 3, 64), ([1300], [0], 16, 4, 128), ([700, 600], [30, 1], 64, 64, 32),
+        ([330], [3000], 64, 1, 128), ([20] * 70, list(range(0, 210, 3)), 30, 2, 64), ([900, 300, 50], [10, 0, 700], 24, 8, 128)]
 
 
 @pytest.mark.parametrize("new,past,heads,kv,d", MANY)
 def test_attention_of_many_rows(ctx, new, past, heads, kv, d):
-    assert sum(new) * heads >= 16384 and sum(new) * heads // kv >= 64 * len(new)
+    assert sum(new) * heads * d >= 80 * 128 * 256 and sum(new) * heads // kv >= 64 * len(new)
     rng = np.random.default_rng(sum(new))
     c, table, lens, starts = S.filled(rng, new, past, kv, d)
     q = rng.standard_normal((int(starts[-1]), heads, d)).astype(np.float32)
@@ -63,8 +63,8 @@ def test_attention_of_many_rows(ctx, new, past, heads, kv, d):
 
 def test_many_rows_with_sharp_scores(ctx):
     rng = np.random.default_rng(8)
-    c, table, lens, starts = S.filled(rng, [300, 2], [40, 400], 2, 64)
-    q = rng.standard_normal((302, 64, 64)).astype(np.float32) * np.float32(50)
+    c, table, lens, starts = S.filled(rng, [650, 2], [40, 400], 2, 64)
+    q = rng.standard_normal((652, 64, 64)).astype(np.float32) * np.float32(50)
     q[3] = 0
     want, bound = c.attention(q, table, lens, starts, -1.0)
     assert np.all(np.abs(S.attend(ctx, c, q, table, lens, starts, -1.0) - want) <= bound)
@@ -72,17 +72,17 @@ def test_many_rows_with_sharp_scores(ctx):
 
 def test_nan_behind_a_row_of_many_does_not_reach_it(ctx):
     rng = np.random.default_rng(9)
-    c, table, lens, starts = S.filled(rng, [300], [30], 2, 64)
-    q = rng.standard_normal((300, 64, 64)).astype(np.float32)
+    c, table, lens, starts = S.filled(rng, [650], [30], 2, 64)
+    q = rng.standard_normal((650, 64, 64)).astype(np.float32)
     want, bound = c.attention(q, table, lens, starts, 0.125)
-    for hit, where in ((110, 5), (317, 40)):                             # a page in the middle and the last one
+    for hit, where in ((110, 5), (667, 40)):                             # a page in the middle and the last one
         page, slot = table[0, hit // 64], hit % 64
         c.v[page, 0, where, slot] = 0x7f
         c.k[page, 1, slot, 9] = 0xff
     got = S.attend(ctx, c, q, table, lens, starts, 0.125)
-    rows = np.arange(300)[:, None, None] + 30
+    rows = np.arange(650)[:, None, None] + 30
     nan = np.zeros(got.shape, bool)
-    nan[:, :32, 5], nan[:, :32, 40], nan[:, 32:] = rows[..., 0] >= 110, rows[..., 0] >= 317, rows >= 110
+    nan[:, :32, 5], nan[:, :32, 40], nan[:, 32:] = rows[..., 0] >= 110, rows[..., 0] >= 667, rows >= 110
     assert np.isnan(got[nan]).all() and np.all((np.abs(got - want) <= bound)[~nan])
 
 
@@ -90,15 +90,15 @@ def test_nan_behind_a_row_of_many_does_not_reach_it(ctx):
 @pytest.mark.parametrize("values", [False, True])
 def test_many_rows_and_a_page_without_a_scale_or_a_place(ctx, scale, values):
     rng = np.random.default_rng(14)
-    c, table, lens, starts = S.filled(rng, [400, 1], [100, 70], 2, 64)
-    q = rng.standard_normal((401, 64, 64)).astype(np.float32)
+    c, table, lens, starts = S.filled(rng, [650, 1], [100, 70], 2, 64)
+    q = rng.standard_normal((651, 64, 64)).astype(np.float32)
     want, bound = c.attention(q, table, lens, starts, 0.125)
     (c.vs if values else c.ks)[table[0, 3], 1] = scale                    # tokens 192 .. 255 of one head
     table[0, 6] = -5                                                      # tokens 384 .. 447 of both
     got = S.attend(ctx, c, q, table, lens, starts, 0.125)
-    rows = np.arange(401)[:, None, None] + 100
-    nan = np.broadcast_to((rows >= 384) & (rows < 500), got.shape).copy()
-    nan[:, 32:] |= ((rows >= 192) & (rows < 500))
+    rows = np.arange(651)[:, None, None] + 100
+    nan = np.broadcast_to((rows >= 384) & (rows < 750), got.shape).copy()
+    nan[:, 32:] |= ((rows >= 192) & (rows < 750))
     assert np.isnan(got[nan]).all() and np.all((np.abs(got - want) <= bound)[~nan])
 
 
@@ -109,13 +109,13 @@ def test_a_cache_beyond_4_gib(ctx):
     far = np.full((3, 18), -1, np.int32)
     far[0, :3], far[1, 0], far[2] = [69999, 32768, 65535], 65536, np.append([32767, 1], 66000 + np.arange(16))
     near = np.where(far < 0, -1, np.cumsum(far >= 0).reshape(far.shape) - 1).astype(np.int32)
-    lens, starts = np.array([150, 1, 1100], np.int32), np.array([0, 150, 151, 1251], np.int32)
-    k, v = (rng.standard_normal((1251, kv, d)).astype(np.float32) for _ in range(2))
+    lens, starts = np.array([150, 1, 1140], np.int32), np.array([0, 150, 151, 1291], np.int32)
+    k, v = (rng.standard_normal((1291, kv, d)).astype(np.float32) for _ in range(2))
     c = F.Cache(22, kv, d)
     c.append(k, v, near, lens, starts)
     cache = H.KvCache.empty(ctx, pages, kv, d)
     up = ctx.move_tensor
-    H.cache_append(ctx, cache, up(k.reshape(1251, -1)), up(v.reshape(1251, -1)), up(far), up(lens), up(starts))
+    H.cache_append(ctx, cache, up(k.reshape(1291, -1)), up(v.reshape(1291, -1)), up(far), up(lens), up(starts))
     for scales, want in ((cache.k_scales, c.ks), (cache.v_scales, c.vs)):
         assert np.array_equal(scales.get_data()[far[far >= 0]], want[near[near >= 0]])
     for begin in (starts, np.array([0, 1, 2, 3], np.int32)):                    # the prompts; their last tokens alone
@@ -197,10 +197,10 @@ def test_recorded_runs_do_not_share_workspaces(ctx):
     rng = np.random.default_rng(17)
     up = ctx.move_tensor
     calls = []
-    for new, past in (([1, 1], [3000, 40]), ([100], [900]), ([1100, 1000], [60, 0])):
+    for new, past in (([1, 1], [3000, 40]), ([100], [900]), ([1000, 300], [60, 0])):
         c, table, lens, starts = S.filled(rng, new, past, 2, 64)
-        operands = (S.on_device(ctx, c), up(rng.standard_normal((sum(new), 512)).astype(np.float32)), up(table), up(lens), up(starts))
-        calls.append(lambda o=operands, out=None: H.cache_attention(ctx, o[0], o[1], 8, 0.125, *o[2:], out=out))
+        operands = (S.on_device(ctx, c), up(rng.standard_normal((sum(new), 2048)).astype(np.float32)), up(table), up(lens), up(starts))
+        calls.append(lambda o=operands, out=None: H.cache_attention(ctx, o[0], o[1], 32, 0.125, *o[2:], out=out))
     a, w = up(S.bytes_of(rng, (1500, 130))), up(S.bytes_of(rng, (2000, 130)))
     sa, sw = ctx.move_tensor(np.full((1500, 2), 0.5, np.float32)), up(np.full((16, 2), 0.25, np.float32))
     calls.append(lambda out=None: H.matmul_fp8(ctx, a, sa, w, sw, out=out))

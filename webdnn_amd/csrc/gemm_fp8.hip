@@ -370,7 +370,7 @@ __global__ __launch_bounds__(256) void pack_rows(const unsigned char *A, const u
 
 // Which form a product takes, and in how many parts along K.  A workgroup of a form takes `start` + `block` per block of K us (measured
 // with every CU busy: K of 2048 to 14336, 16 to 8192 rows; wavefronts of the direct forms take blocks eight at a time; fewer rows
-// than 16 cost the smallest form, which is bound by its loads, less).  Tiles that leave
+// than 16 cost the smallest form, which is bound by its loads, less; odd rows cost the direct forms 1.15 times as much and the others the copy).  Tiles that leave
 // CUs idle are cut along K into as many parts as there are CUs for; the parts' join is a launch of 4 us and its bytes.  The cheapest
 // of all wins (us, so / the smallest tile that fits the chip, uncut: 4096 columns, K = 14336: 32 rows 20 / 36, 64 rows 24 / 36, 256 rows
 // 46 / 70; 8192 x 8192: 128 rows 33 / 44, 1024 rows 138 / 161).
@@ -391,7 +391,8 @@ Plan cheapest_plan(const ProductParams &p, bool aligned) {
   for (int f = 0; f < FORMS; f++) {
     const long long tiles = ((p.n + forms[f].cols - 1LL) / forms[f].cols) * ((p.m + forms[f].rows - 1) / forms[f].rows);
     const bool direct = f < FIRST_TILES;
-    const double block = f == 0 && p.m < 16 ? forms[f].block - 0.005 * (double)(16 - p.m) : forms[f].block;
+    double block = f == 0 && p.m < 16 ? forms[f].block - 0.005 * (double)(16 - p.m) : forms[f].block;
+    if (direct && !aligned) block *= 1.15;
     for (int cut = 0; cut < 2; cut++) {
       long long parts = cut ? cus / tiles : 1;
       if (parts > p.blocks) parts = p.blocks;
@@ -401,7 +402,7 @@ Plan cheapest_plan(const ProductParams &p, bool aligned) {
       const double rounds = (double)((tiles * parts + cus - 1) / cus);
       double us = rounds * (forms[f].start + block * (double)(direct ? (part + 7) / 8 * 8 : part));
       if (parts > 1) us += 4.0 + (double)parts * (double)p.m * p.n * 8e-7;
-      if (!direct && !aligned) us += 4.0 + (double)(p.m + p.n) * p.k * 5e-7;  // (the copy)
+      if (!direct && !aligned) us += 3.0 + (double)(p.m + p.n) * p.k * 4e-7;  // (the copy)
       if (least < 0.0 || us < least) {
         least = us;
         best = Plan{f, (int)parts};

@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     unit = blockIdx.x * share;
     units_end = total - unit < share ? total : unit + share;
   } else {
-    w = locate_work(p, first, blockIdx.x, true);
+    w = locate_work(p, first, gridDim.x - 1 - blockIdx.x, true);  // (a prompt's last items are its longest)
     unit = w.before;
     units_end = w.s.n ? w.before + w.units : unit;
   }
@@ -1157,10 +1157,10 @@ extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_strid
     return loose < tight ? loose : tight;
   };
   // Items of 128 rows read a page once for eight times the rows, but need more of them to fill the chip: they are taken where sequences
-  // fill half an item on average, and the call has 64 rows for each CU (us, 16 / 128 rows an item, 32 heads on 8 behind 2000 tokens: 16 x
-  // 64 tokens 167 / 100, 4 x 128 78 / 73, 1 x 256 42 / 50, 16 x 16 51 / 77; 16 heads on 4: 4 x 512 329 / 171, 4 x 64 and below 0.85 of
-  // the other's time).
-  const bool many = (long long)tokens * p.group.d >= 64LL * seqs && (long long)tokens * heads >= 64LL * wdh::compute_units();
+  // fill half an item on average, and the call has 80 rows of 128 elements for each CU (us, 16 / 128 rows an item; 32 heads of 128 on 8,
+  // behind nothing: 3 x 256 tokens 29 / 22, 1 x 2000 140 / 94, 1 x 512 26 / 31; 16 heads of 64 on 4: 3 x 1000 42 / 38, 1 x 2000 42 / 59).
+  const long long rows = (long long)tokens * p.group.d;
+  const bool many = rows >= 64LL * seqs && (long long)tokens * width >= 80LL * 128 * wdh::compute_units();
   const long long items = items_of_rows(many ? MANY : 16);
   if (items > 0xffffffLL / 2) return fail(WDH_EINVAL, "%s: too many rows", who);
   p.partial = p.stats = nullptr;
@@ -1187,10 +1187,13 @@ extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_strid
     const long long units = items * ((max_pages + 3) / 4), resident = 2LL * wdh::compute_units() / kv_heads;
     if (units > MOST_UNITS) return fail(WDH_EINVAL, "%s: too many rows of tables so wide", who);
     p.wgs = (int)(units < resident ? units : resident > 0 ? resident : 1);
-    // Where tables hold few pages, sharing them out costs more (the join's launch) than it evens out: a workgroup to an item then (us, shared /
-    // so, 32 heads on 8: 4 x 60 tokens behind 300 23.0 / 14.6, 64 single ones behind 100 to 1000 32.6 / 21.8, 8 behind 500 12.3 / 10.6,
-    // behind 1000 12.5 / 14.8).
-    if (max_pages <= (items * kv_heads >= wdh::compute_units() ? 16 : 8)) p.wgs = 0;
+    // Shares end together whatever the sequences' lengths, but cost their join, and the first rows of a prompt, which see few pages, leave theirs
+    // half empty.  A workgroup to an item, the last ones first, is faster where there are many items for the pages that one can have: for
+    // prompts 14 to a unit, for single tokens, whose lengths nothing is known about, 64 (us, shared / so: one prompt of 1024, 32 heads
+    // of 128 on 8, behind nothing 97 / 57, 256 behind 2000 47 / 38, 128 behind 8000 71 / 99; single tokens of 128 sequences of 100 to 4000 137
+    // / 117, of 64 of which one has 8000 and the others 500 31 / 92).
+    const long long most_units = (max_pages + 3) / 4;
+    if (most_units <= 2 || most_units * (rows >= 16LL * seqs ? 14 : 64) <= items * kv_heads) p.wgs = 0;
     if (p.wgs > 1 && !workspace((size_t)p.wgs * 2 * kv_heads * 16)) return WDH_ENOMEM;  // (items of one unit are never cut)
     rc = d == 32 ? launch_attend<32>(p, items) : d == 64 ? launch_attend<64>(p, items) : launch_attend<128>(p, items);
   }
