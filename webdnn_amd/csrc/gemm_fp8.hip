@@ -200,7 +200,7 @@ void launch_few(const ProductParams &p, bool aligned) {
 // multiplied.  In LDS a row's eight 16-byte pieces are exchanged by its number (piece ^ row % 8), so that the 32 rows that a
 // fragment read takes a piece of lie on different banks.  A fragment's 16 bytes serve two instructions (their k are the first and the
 // last eight of them, on both sides alike).  A slab is multiplied by quarters, the next one's fragments on their way from LDS
-// meanwhile (8192^3: 1035 to 1055 us, 1042 to 1062 TFLOP/s; fragments of the whole slab at a time 1146).
+// meanwhile (8192^3: 1032 to 1080 us from run to run, 1018 to 1065 TFLOP/s; fragments of the whole slab at a time 1146).
 // Bound: the matrix cores, the conversions and the way through LDS alternate more than they overlap (without the loads of slabs that
 // product takes 890 us, without their way into LDS either 800; library products of bfloat16 operands of that size take 954).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -314,19 +314,29 @@ __global__ __launch_bounds__(64 * NW * MW, 2) void product_tiles(ProductParams p
         for (int e = 0; e < 16; e++) acc[i][j][e] = __builtin_fmaf(x[i][j][e], c[j], acc[i][j][e]);
   }
   float *Y = p.Y + blockIdx.y * p.m * p.n;
-  // lane: row li of a block; registers 4 q .. + 3 are columns 8 q + 4 half .. + 3
+  // Lane: row li of a block; registers 4 q .. + 3 are columns 8 q + 4 half .. + 3.  A wavefront turns 32 rows of them at a time in a part of LDS
+  // of its own (nobody reads slabs any more), so that it stores runs of 32 TN columns (8192 x 4096, K = 512: 58 us, straight from the
+  // registers 81).
+  constexpr int PITCH = 32 * TN + 4, LANES = 8 * TN;
+  static_assert(NW * MW * 32 * PITCH * 4 <= (int)sizeof(lds), "room for the results");
+  float *turn = reinterpret_cast<float *>(&lds[0][0]) + wave * (32 * PITCH);
 #pragma unroll
   for (int j = 0; j < TM; j++) {
-    const long long i = m0 + 32 * (TM * wm + j) + li;
-    if (i >= p.m) continue;
 #pragma unroll
     for (int t = 0; t < TN; t++)
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const int col = n0 + 32 * (TN * wn + t) + 8 * q + 4 * half;
-        f32x4 v = {acc[t][j][4 * q], acc[t][j][4 * q + 1], acc[t][j][4 * q + 2], acc[t][j][4 * q + 3]};
-        finish4(p, Y, i, col, v);
-      }
+      for (int q = 0; q < 4; q++)
+        *reinterpret_cast<f32x4 *>(&turn[li * PITCH + 32 * t + 8 * q + 4 * half]) =
+            f32x4{acc[t][j][4 * q], acc[t][j][4 * q + 1], acc[t][j][4 * q + 2], acc[t][j][4 * q + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int r = 0; r < 32; r += 64 / LANES) {
+      const int row = r + lane / LANES, col = 4 * (lane % LANES);
+      const long long i = m0 + 32 * (TM * wm + j) + row;
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(&turn[row * PITCH + col]);
+      if (i < p.m) finish4(p, Y, i, n0 + 32 * TN * wn + col, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -369,11 +379,11 @@ __global__ __launch_bounds__(256) void pack_rows(const unsigned char *A, const u
 }
 
 // Which form a product takes, and in how many parts along K.  A workgroup of a form takes `start` + `block` per block of K us (measured
-// with every CU busy: K of 2048 to 14336, 16 to 8192 rows; wavefronts of the direct forms take blocks eight at a time; fewer rows
-// than 16 cost the smallest form, which is bound by its loads, less; odd rows cost the direct forms 1.15 times as much and the others the copy).  Tiles that leave
-// CUs idle are cut along K into as many parts as there are CUs for; the parts' join is a launch of 4 us and its bytes.  The cheapest
-// of all wins (us, so / the smallest tile that fits the chip, uncut: 4096 columns, K = 14336: 32 rows 20 / 36, 64 rows 24 / 36, 256 rows
-// 46 / 70; 8192 x 8192: 128 rows 33 / 44, 1024 rows 138 / 161).
+// with every CU busy: K of 2048 to 14336, 16 to 8192 rows).  Wavefronts of the direct forms take blocks eight at a time; fewer rows than 16
+// cost the smallest form, which is bound by its loads, less; odd rows cost the direct forms 1.15 times as much, the others the copy.
+// Tiles that leave CUs idle are cut along K into as many parts as there are CUs for; the parts' join is a launch of 4 us and its bytes.
+// The cheapest of all wins (us, so / the smallest tile that fits the chip, uncut: 4096 columns, K = 14336: 32 rows 20 / 36, 64 rows 24 / 36,
+// 256 rows 51 / 70; 8192 x 8192: 128 rows 36 / 44, 1024 rows 139 / 161).
 struct Form {
   int cols, rows;
   float start, block;
@@ -423,7 +433,8 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
   if (m < 0 || n < 0 || k < 0) return fail(WDH_EINVAL, "wdh_gemm_fp8: negative extent");
   if (epilogue != WDH_EPI_NONE && epilogue != WDH_EPI_RELU) return fail(WDH_EINVAL, "wdh_gemm_fp8: unknown epilogue %d", epilogue);
   if (m == 0 || n == 0) return WDH_OK;
-  if (n > (1 << 28) || k > (1 << 30) || ((m + 127) / 128) * (((long long)n + 127) / 128) > 0x7fffff || m > (1LL << 46) / n || (k && m > (1LL << 46) / k)) return fail(WDH_EINVAL, "wdh_gemm_fp8: too many elements");
+  if (n > (1 << 28) || k > (1 << 30) || m > (1LL << 46) / n || (k && m > (1LL << 46) / k) || (m + 127) / 128 * (((long long)n + 127) / 128) > 0x7fffff)
+    return fail(WDH_EINVAL, "wdh_gemm_fp8: too many elements");
   const size_t blocks = ((size_t)k + BLOCK - 1) / BLOCK, wide = ((size_t)n + BLOCK - 1) / BLOCK, results = (size_t)m * n * 4;
   void *pa, *psa, *pw, *psw, *pb = nullptr, *py, *pr = nullptr;
   if (!wdh::operand(hA, (size_t)m * k, "wdh_gemm_fp8: A", &pa)) return WDH_EINVAL;

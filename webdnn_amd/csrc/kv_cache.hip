@@ -735,8 +735,8 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   const int last_token = wdh::fdiv(row0 + MANY - 1, p.group), last_key = past + (last_token < s.n ? last_token : s.n - 1);
   const int seen = last_key / PAGE + 1, begin = (int)((long long)seen * blockIdx.y / gridDim.y), end = (int)((long long)seen * (blockIdx.y + 1) / gridDim.y);
   // this wavefront's own pages end earlier
-  const int wave_last = wdh::fdiv(row0 + 32 * wave + 31, p.group), wave_end = wdh::fdiv(row0 + 32 * wave, p.group) < s.n ? (past + (wave_last < s.n ? wave_last : s.n - 1)) / PAGE + 1 : 0;
-  const int wave_first = past + wdh::fdiv(row0 + 32 * wave, p.group);
+  const int wave_token = wdh::fdiv(row0 + 32 * wave, p.group), wave_last = wdh::fdiv(row0 + 32 * wave + 31, p.group), wave_first = past + wave_token;
+  const int wave_end = wave_token < s.n ? (past + (wave_last < s.n ? wave_last : s.n - 1)) / PAGE + 1 : 0;
   const int *table = p.q.table + (long long)s.seq * p.q.max_pages;
 
   struct Page { long long at; float ks, vs; bool known; };
