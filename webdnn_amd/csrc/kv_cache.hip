@@ -121,7 +121,8 @@ __device__ __forceinline__ int merge4(int old, int fresh, int first, int last, b
 
 // A workgroup owns a touched page of one head, keys (blockIdx.z 0) or values: nobody else reads or writes it, and its scale
 // needs the largest of the new elements before any of them is stored.  They stay in registers in between.
-// Bound: memory for prompts, latency for single tokens.
+// Bound: memory for prompts (6 of 100 to 2900 tokens, 8 heads of 128: 18.3 us, 5.0 TB/s), latency for single tokens (48: 6.6 us, a
+// call's own time 5.3).
 template <int D>
 __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
   constexpr int NP = PAGE * D / 4 / 256;       // pieces of four elements a thread holds
@@ -359,6 +360,9 @@ __device__ __forceinline__ void split2_f16(const float (&x)[8], f16x8 (&part)[2]
 // so that a lane holds scores of one row, P is an operand of the second product as it stands, and both K and V pass from memory
 // into operand registers with 16-byte loads.  That takes an order of keys in which the four that a lane gets from score tile t are
 // keys 16 g + 4 t .. + 3 of the page (g = lane / 16), and an order of d in which a lane's 16 bytes serve two products.
+// Bound: memory where rows are few (32 tokens behind 500 to 8500, 32 heads of 128 on 8: 56 us, 5.3 TB/s; a copy of this kernel that only
+// loads takes 55), so three exact parts cost nothing that two would not; with all rows in use, instructions (1.3 us for a page of each
+// wavefront, two workgroups to a CU).
 template <int D>
 __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
   constexpr int STEPS = D / 32, CH = D >= 64 ? D / 64 : 1, DT = D / 16;
@@ -715,6 +719,9 @@ __device__ __forceinline__ Place many_item(const AttendParams &p, int rank, int 
                __builtin_amdgcn_readlane(mine.len, at), __builtin_amdgcn_readlane(from + left - (upto - (to - from)), at)};
 }
 
+// Bound: instructions.  A page takes 64 matrix ones of 32 cycles a wavefront and about as long of others (conversions of keys and values,
+// powers, splitting weights), which alternate more than they overlap: matrix cores busy 41 % of the time (three prompts of 1200 to 4000
+// tokens, 16 heads of 128 on 4: 250 us, 457 TFLOP/s counted once).
 template <int D>
 __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   constexpr int QN = D / 32, DT = D / 32;           // runs of 32 elements of d in a key; blocks of 32 rows of O^T
@@ -987,7 +994,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   }
 }
 
-// The parts of an item's pages together: a lane to four elements of a row, few parts.
+// The parts of an item's pages together: a lane to four elements of a row, few parts.  Bound: memory.
 template <int D>
 __global__ __launch_bounds__(256) void attend_many_join(AttendParams p, int parts) {
   constexpr int LANES = D / 4, ROWS = 256 / LANES;
