@@ -519,8 +519,8 @@ int wdh_gemm_fp8(wdh_buf A, wdh_buf AScale, wdh_buf W, wdh_buf WScale, wdh_buf B
  * Appending: new tokens go behind the earlier ones, keys and values each with the least power of two c >= 2^-100 as scale
  * that holds the page's largest finite element (<= 448 c); where a page held earlier tokens, their scale only grows, and they
  * are rounded again to the new one (exact but for values that become subnormal).  Slots behind the last token and pages that
- * no new token lies on are left as they are; a page number outside the cache is skipped.  Two sequences of a call must
- * not append to the same page (they may share full pages of a common prefix). */
+ * no new token lies on are left as they are; a page number outside the cache is skipped.  A call must not
+ * append to one page from two places, of two sequences or of one (sequences may share full pages of a common prefix). */
 int wdh_cache_append(wdh_buf K, int64_t k_offset, int64_t k_stride, wdh_buf V, int64_t v_offset, int64_t v_stride,
                      wdh_buf KPages, wdh_buf KScales, wdh_buf VPages, wdh_buf VScales, wdh_buf Table, wdh_buf Lens,
                      wdh_buf Starts, int seqs, int tokens, int kv_heads, int d, int pages, int max_pages);

@@ -70,6 +70,27 @@ def test_many_rows_with_sharp_scores(ctx):
     assert np.all(np.abs(S.attend(ctx, c, q, table, lens, starts, -1.0) - want) <= bound)
 
 
+@pytest.mark.parametrize("new", [90, 650])
+@pytest.mark.parametrize("size", [2.0 ** -70, 2.0 ** -95, 2.0 ** 100])
+def test_tiny_and_huge_keys_and_queries(ctx, new, size):
+    """Scores that are nothing next to each other, queries of zeros, and a page that only the last rows see and that is not there."""
+    rng = np.random.default_rng(24)
+    kv, d, heads = 2, 64, 64
+    table, lens, starts, pages = S.layout(rng, [new], [30])
+    c = F.Cache(pages, kv, d)
+    k, v = (rng.standard_normal((int(lens[0]), kv, d)).astype(np.float32) for _ in range(2))
+    c.append(k * np.float32(size), v, table, lens, [0, int(lens[0])])
+    q = (rng.standard_normal((new, heads, d)) * min(1.0, 2.0 ** 20 / size)).astype(np.float32)
+    q[5] = 0
+    q[6:9] *= np.float32(2.0 ** -60)
+    want, bound = c.attention(q, table, lens, starts, 0.125)
+    last = (int(lens[0]) - 1) // 64
+    table[0, last] = -1
+    got = S.attend(ctx, c, q, table, lens, starts, 0.125)
+    seen = 64 * last - 30
+    assert np.all(np.abs(got - want)[:seen] <= bound[:seen]) and np.isnan(got[seen:]).all()
+
+
 def test_nan_behind_a_row_of_many_does_not_reach_it(ctx):
     rng = np.random.default_rng(9)
     c, table, lens, starts = S.filled(rng, [650], [30], 2, 64)

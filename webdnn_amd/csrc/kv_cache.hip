@@ -896,7 +896,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
       if (active) {
-        const float c = now.ks * row_scale;  // (positive)
+        const float c = fmaxf(now.ks * row_scale, FLT_MIN);  // (never 0: -inf * 0 is NaN; scores that need less are all 0 to the softmax)
         const float up = fmaxf(most * c, top), ref = up == -INFINITY ? 0.0f : up;
         if (__any(up > top)) {
           const float back = __builtin_amdgcn_exp2f(top - ref);
