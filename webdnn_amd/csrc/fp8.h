@@ -24,6 +24,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+// A number the compiler knows nothing about: what is computed from it stays where it is used and holds no registers in between.
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // |x| if x is finite, else 0: a block's scale follows its finite elements.
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);

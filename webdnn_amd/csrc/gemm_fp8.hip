@@ -25,7 +25,7 @@ struct ProductParams {
   int part;         // blocks of K that a part of the product takes: its results go to Y [part][m][n]
 };
 
-// 32 bytes a lane of each operand: the lanes that share a row hold its 128 elements, in the same order on both sides.
+// 32 bytes a lane of each operand.
 __device__ __forceinline__ f32x4 block_product(i32x8 a, i32x8 b) {
   f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -36,7 +36,8 @@ __device__ __forceinline__ f32x4 block_product(i32x8 a, i32x8 b) {
 
 // Bytes k .. k+15 of a row of length `len`, 0 beyond its end.  Rows of whole 16-byte pieces are loaded as they lie; others dword by
 // dword (the hardware takes loads off dword boundaries, but slowly) and put together where they are used, so that nothing
-// waits for them before.  Every dword read holds a byte of the row.
+// waits for them before.  A piece that ends behind the row is cut out of the row's last 16 bytes: every dword read holds a byte of
+// the row, and loads are behind no branch that lanes take differently.
 template <bool ALIGNED>
 struct Piece {
   i32x4 d;
@@ -50,50 +51,42 @@ template <>
 struct Piece<false> {
   i32x4 d;
   int e;
+  static __device__ __forceinline__ int begin(int k, int len) { return k + 16 <= len ? k : len > 16 ? len - 16 : 0; }
   __device__ __forceinline__ void load(const unsigned char *row, int k, int len) {
-    const int left = len - k, from = left > 0 ? k : len - 1;  // (behind the end: the last byte's dword, of which nothing is kept)
+    const int from = begin(k, len);
     const unsigned shift = (unsigned)((uintptr_t)row + from) & 3u;
     const int *base = reinterpret_cast<const int *>(row + from - shift);  // (a number made a pointer again would be loaded from as of any kind)
-    if (left >= 16) {
+    if (len >= 16) {
       typedef int i32x4_dwords __attribute__((ext_vector_type(4), aligned(4)));
       d = *reinterpret_cast<const i32x4_dwords *>(base);
       e = base[(shift + 15) >> 2];
     } else {
-      const int last = (int)(shift + (left > 0 ? left : 1) - 1) >> 2;
+      const int last = (int)(shift + len - 1) >> 2;
 #pragma unroll
       for (int i = 0; i < 4; i++) d[i] = base[i < last ? i : last];
       e = base[last];
     }
   }
   __device__ __forceinline__ i32x4 get(const unsigned char *row, int k, int len) const {
-    const unsigned shift = (unsigned)((uintptr_t)row + k) & 3u;
+    const int from = begin(k, len);
+    const unsigned shift = (unsigned)((uintptr_t)row + from) & 3u;
     i32x4 v;
 #pragma unroll
     for (int i = 0; i < 4; i++) v[i] = (int)__builtin_amdgcn_alignbyte((unsigned)(i < 3 ? d[i + 1] : e), (unsigned)d[i], shift);
-    const int left = len - k;
-    if (left < 16)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int n = left - 4 * i;
-        v[i] &= n >= 4 ? -1 : n <= 0 ? 0 : (int)((1u << (8 * n)) - 1u);
-      }
+    if (k + 16 > len) {
+      const int left = len - k, skip = k - from;  // bytes of v that are kept, and those in front of them
+      unsigned long long lo = (unsigned)v[0] | (unsigned long long)(unsigned)v[1] << 32, hi = (unsigned)v[2] | (unsigned long long)(unsigned)v[3] << 32;
+      const int bits = 8 * (skip & 7);
+      if (skip >= 8) lo = hi, hi = 0;
+      lo = bits ? lo >> bits | hi << (64 - bits) : lo;
+      hi >>= bits;
+      lo = left >= 8 ? lo : left > 0 ? lo & ((1ull << (8 * left)) - 1) : 0;
+      hi = left >= 16 ? hi : left > 8 ? hi & ((1ull << (8 * (left - 8))) - 1) : 0;
+      v = i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+    }
     return v;
   }
 };
-// 32 bytes: a lane's share of a block.
-template <bool ALIGNED>
-struct Pieces {
-  Piece<ALIGNED> a, b;
-  __device__ __forceinline__ void load(const unsigned char *row, int k, int len) {
-    a.load(row, k, len);
-    b.load(row, k + 16, len);
-  }
-  __device__ __forceinline__ i32x8 get(const unsigned char *row, int k, int len) const {
-    const i32x4 x = a.get(row, k, len), y = b.get(row, k + 16, len);
-    return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-  }
-};
-
 // Columns j .. j+3 of row i: bias, residual, Relu, and out.
 __device__ __forceinline__ void finish4(const ProductParams &p, float *Y, long long i, int j, f32x4 v) {
   const int left = p.n - j;
@@ -106,78 +99,111 @@ __device__ __forceinline__ void finish4(const ProductParams &p, float *Y, long l
   store4(Y + i * p.n, j, p.n, v);
 }
 
-// Few rows of A, or few results: a workgroup has 16 NT rows of W and 16 MT of A, its wavefronts take K blocks in turn, U at a time,
-// straight from memory into operand registers, and add up through LDS.  Bound: memory (W is read once for 16 MT rows), or latency: so
-// a wavefront asks for all of its U blocks at once.
-template <int NT, int MT, int WAVES, int U, bool ALIGNED>
+// Few rows of A, or few results: a workgroup has 16 NT rows of W and 16 MT of A, its wavefronts take K blocks in turn and add up through
+// LDS.  A wavefront brings its blocks itself, eight lanes to a row, the next one while it works on this one, and turns them in a part of LDS
+// of its own, where a row's pieces are exchanged by its number (as below), into what the matrix instructions take: a row to each of
+// 16 neighbouring lanes, which straight from memory is 16 lines for 16 lanes (us, so / straight from memory: 64 rows, 4096 x 4096, 8.4 /
+// 12.9, 333 x 1000 x 2048 7.4 / 9.8, x 2050 10.3 / 12.8; a single row, 8192 x 4096, 9.2 / 8.8).  More than one block on its way is slower
+// (64 rows 9.4).  Bound: memory (W is read once for 16 MT rows), or latency.
+template <int NT, int MT, int WAVES, bool ALIGNED>
 __global__ __launch_bounds__(64 * WAVES) void product_few(ProductParams p) {
-  __shared__ __attribute__((aligned(16))) f32x4 part[WAVES][NT * MT][64];
+  constexpr int ROWS = 16 * (NT + MT), LOADS = ROWS / 8;
+  __shared__ __attribute__((aligned(16))) union { unsigned char rows[WAVES][ROWS * BLOCK]; f32x4 part[WAVES][NT * MT][64]; } lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * (16 * NT), begin = blockIdx.z * p.part, end = begin + p.part < p.blocks ? begin + p.part : p.blocks;
-  const unsigned char *w[NT];
+  const int piece = 16 * (lane & 7);
+  unsigned char *mine = lds.rows[wave];
   const float *sw[NT];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    const int j = n0 + 16 * t + i16, tile = n0 + 16 * t;
-    w[t] = p.W + (long long)(j < p.n ? j : p.n - 1) * p.pitch;
+    const int tile = n0 + 16 * t;
     sw[t] = p.SW + (long long)((tile < p.n ? tile : p.n - 1) / BLOCK) * p.blocks;
   }
   for (long long m0 = (long long)blockIdx.y * (16 * MT); m0 < p.m; m0 += (long long)gridDim.y * (16 * MT)) {
-    const unsigned char *a[MT];
+    const unsigned char *w0 = p.W + n0 * p.pitch, *a0 = p.A + m0 * p.pitch;
+    const int w_last = p.n - 1 - n0, a_last = p.m - 1 - m0 < 16 * MT ? (int)(p.m - 1 - m0) : 16 * MT;
+    auto row = [&](int i) {  // (rows behind the last are the last one again; addresses are worked out where they are used)
+      const int r = 8 * i + fresh(lane >> 3) - (8 * i < 16 * NT ? 0 : 16 * NT), last = 8 * i < 16 * NT ? w_last : a_last;
+      return (8 * i < 16 * NT ? w0 : a0) + (unsigned long long)(unsigned)(r < last ? r : last) * (unsigned)p.pitch;
+    };
     const float *sa[MT];
     f32x4 acc[NT][MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) {
-      const long long r = m0 + 16 * t + i16 < p.m ? m0 + 16 * t + i16 : p.m - 1;
-      a[t] = p.A + r * p.pitch;
-      sa[t] = p.SA + r * p.blocks;
+      sa[t] = p.SA + (m0 + 16 * t + i16 < p.m ? m0 + 16 * t + i16 : p.m - 1) * p.blocks;
 #pragma unroll
       for (int q = 0; q < NT; q++) acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int b0 = begin + wave; b0 < end; b0 += WAVES * U) {
-      Pieces<ALIGNED> wv[U][NT], av[U][MT];
-      float sav[U][MT], swv[U][NT];
+    Piece<ALIGNED> next[LOADS];
+    float next_sa[MT], next_sw[NT];
+    auto fetch = [&](int b) {
+      if (b >= end) return;
+      if constexpr (ALIGNED) {
+        const int k = b * BLOCK + piece;
+        if (k < p.k)
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int b = b0 + WAVES * u;
-        if (b >= end) break;
+          for (int i = 0; i < LOADS; i++) next[i].d = *reinterpret_cast<const i32x4 *>(row(i) + k);
+        else
 #pragma unroll
-        for (int t = 0; t < NT; t++) wv[u][t].load(w[t], b * BLOCK + 32 * g, p.k), swv[u][t] = sw[t][b];
+          for (int i = 0; i < LOADS; i++) next[i].d = i32x4{0, 0, 0, 0};
+      } else {
 #pragma unroll
-        for (int t = 0; t < MT; t++) av[u][t].load(a[t], b * BLOCK + 32 * g, p.k), sav[u][t] = sa[t][b];
+        for (int i = 0; i < LOADS; i++) next[i].load(row(i), b * BLOCK + piece, p.k);
       }
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int b = b0 + WAVES * u;
-        if (b >= end) break;
-        i32x8 x8[NT];
+      for (int t = 0; t < MT; t++) next_sa[t] = sa[t][b];
 #pragma unroll
-        for (int q = 0; q < NT; q++) x8[q] = wv[u][q].get(w[q], b * BLOCK + 32 * g, p.k);
+      for (int q = 0; q < NT; q++) next_sw[q] = sw[q][b];
+    };
+    // 32 bytes of row r: the lanes that share a row hold its 128 elements, in the same order on both sides
+    auto fragment = [&](int r) {
+      const i32x4 x = *reinterpret_cast<const i32x4 *>(mine + r * BLOCK + 16 * ((2 * g) ^ (r & 7)));
+      const i32x4 y = *reinterpret_cast<const i32x4 *>(mine + r * BLOCK + 16 * ((2 * g + 1) ^ (r & 7)));
+      return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    };
+    fetch(begin + wave);
+    for (int b = begin + wave; b < end; b += WAVES) {
 #pragma unroll
-        for (int t = 0; t < MT; t++) {
-          const i32x8 y8 = av[u][t].get(a[t], b * BLOCK + 32 * g, p.k);
+      for (int i = 0; i < LOADS; i++) {
+        const int r = 8 * i + (lane >> 3);
+        *reinterpret_cast<i32x4 *>(mine + r * BLOCK + 16 * ((lane & 7) ^ (r & 7))) = next[i].get(row(i), b * BLOCK + piece, p.k);
+      }
+      float ca[MT], cw[NT];
 #pragma unroll
-          for (int q = 0; q < NT; q++) {
-            const f32x4 x = block_product(x8[q], y8);
-            const float c = sav[u][t] * swv[u][q];
+      for (int t = 0; t < MT; t++) ca[t] = next_sa[t];
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[q][t][e] = __builtin_fmaf(x[e], c, acc[q][t][e]);
-          }
+      for (int q = 0; q < NT; q++) cw[q] = next_sw[q];
+      fetch(b + WAVES);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      i32x8 w8[NT];
+#pragma unroll
+      for (int q = 0; q < NT; q++) w8[q] = fragment(16 * q + i16);
+#pragma unroll
+      for (int t = 0; t < MT; t++) {
+        const i32x8 a8 = fragment(16 * (NT + t) + i16);
+#pragma unroll
+        for (int q = 0; q < NT; q++) {
+          const f32x4 x = block_product(w8[q], a8);
+          const float c = ca[t] * cw[q];
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[q][t][e] = __builtin_fmaf(x[e], c, acc[q][t][e]);
         }
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
+    __syncthreads();
 #pragma unroll
     for (int q = 0; q < NT; q++)
 #pragma unroll
-      for (int t = 0; t < MT; t++) part[wave][q * MT + t][lane] = acc[q][t];
+      for (int t = 0; t < MT; t++) lds.part[wave][q * MT + t][lane] = acc[q][t];
     __syncthreads();
     for (int cell = threadIdx.x; cell < 64 * NT * MT; cell += 64 * WAVES) {
       const int tile = cell >> 6, l = cell & 63;
-      f32x4 v = part[0][tile][l];
+      f32x4 v = lds.part[0][tile][l];
 #pragma unroll
       for (int i = 1; i < WAVES; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] += part[i][tile][l][e];
+        for (int e = 0; e < 4; e++) v[e] += lds.part[i][tile][l][e];
       const long long i = m0 + 16 * (tile % MT) + (l & 15);
       if (i < p.m) finish4(p, p.Y + blockIdx.z * p.m * p.n, i, n0 + 16 * (tile / MT) + 4 * (l >> 4), v);
     }
@@ -187,12 +213,12 @@ __global__ __launch_bounds__(64 * WAVES) void product_few(ProductParams p) {
 
 unsigned parts_of(const ProductParams &p) { return p.part < p.blocks ? (unsigned)((p.blocks + p.part - 1) / p.part) : 1u; }
 
-template <int NT, int MT, int WAVES, int U>
+template <int NT, int MT, int WAVES>
 void launch_few(const ProductParams &p, bool aligned) {
   const long long rows = (p.m + 16 * MT - 1) / (16 * MT);
   const dim3 grid((unsigned)((p.n + 16 * NT - 1) / (16 * NT)), (unsigned)(rows < 65535 ? rows : 65535), parts_of(p)), wg(64 * WAVES);
-  if (aligned) hipLaunchKernelGGL((product_few<NT, MT, WAVES, U, true>), grid, wg, 0, wdh::stream(), p);
-  else hipLaunchKernelGGL((product_few<NT, MT, WAVES, U, false>), grid, wg, 0, wdh::stream(), p);
+  if (aligned) hipLaunchKernelGGL((product_few<NT, MT, WAVES, true>), grid, wg, 0, wdh::stream(), p);
+  else hipLaunchKernelGGL((product_few<NT, MT, WAVES, false>), grid, wg, 0, wdh::stream(), p);
 }
 
 // Tiles of NW TN x 32 columns of Y (rows of W) and MW TM x 32 rows: NW x MW wavefronts with TN x TM blocks of 32 x 32 each.
@@ -379,18 +405,18 @@ __global__ __launch_bounds__(256) void pack_rows(const unsigned char *A, const u
 }
 
 // Which form a product takes, and in how many parts along K.  A workgroup of a form takes `start` + `block` per block of K us (measured
-// with every CU busy: K of 2048 to 14336, 16 to 8192 rows).  Wavefronts of the direct forms take blocks eight at a time; fewer rows than 16
-// cost the smallest form, which is bound by its loads, less; odd rows cost the direct forms 1.15 times as much, the others the copy.
-// Tiles that leave CUs idle are cut along K into as many parts as there are CUs for; the parts' join is a launch of 4 us and its bytes.
-// The cheapest of all wins (us, so / the smallest tile that fits the chip, uncut: 4096 columns, K = 14336: 32 rows 20 / 36, 64 rows 24 / 36,
-// 256 rows 51 / 70; 8192 x 8192: 128 rows 36 / 44, 1024 rows 139 / 161).
+// with every CU busy: K of 2048 to 14336, 1 to 8192 rows).  Wavefronts of the first forms take blocks eight (64 x 64: four) at a time; odd
+// rows cost these 1.4 times as much, the others the copy.  Tiles that leave CUs idle are cut along K into as many parts as there are CUs
+// for; the parts' join is a launch of 4 us and its bytes.  The cheapest of all wins (us, so / the smallest tile that fits the chip, uncut:
+// 4096 columns, K = 14336: 17 rows 16.4 / 19.9, 64 rows 23 / 25, 256 rows 47 / 53; 8192 x 8192: 128 rows 33 / 34, 256 rows 51 / 57, 1024
+// rows 139 / 161).
 struct Form {
   int cols, rows;
   float start, block;
 };
 constexpr int FIRST_TILES = 6, FORMS = 9;
-constexpr Form forms[FORMS] = {{16, 16, 3.0f, 0.16f}, {32, 16, 1.5f, 0.27f}, {64, 16, 1.5f, 0.47f},   {32, 32, 3.0f, 0.31f},  {64, 32, 2.0f, 0.48f},
-                               {64, 64, 4.0f, 0.62f}, {128, 64, 5.0f, 0.87f}, {128, 128, 8.0f, 1.2f}, {256, 128, 9.0f, 2.0f}};
+constexpr Form forms[FORMS] = {{16, 16, 3.0f, 0.116f}, {32, 16, 1.9f, 0.16f}, {64, 16, 2.2f, 0.21f},   {32, 32, 1.5f, 0.21f},  {64, 32, 2.0f, 0.28f},
+                               {64, 64, 5.0f, 0.43f},  {128, 64, 4.0f, 0.85f}, {128, 128, 8.0f, 1.2f}, {256, 128, 9.0f, 2.0f}};
 struct Plan {
   int form, parts;
 };
@@ -401,8 +427,8 @@ Plan cheapest_plan(const ProductParams &p, bool aligned) {
   for (int f = 0; f < FORMS; f++) {
     const long long tiles = ((p.n + forms[f].cols - 1LL) / forms[f].cols) * ((p.m + forms[f].rows - 1) / forms[f].rows);
     const bool direct = f < FIRST_TILES;
-    double block = f == 0 && p.m < 16 ? forms[f].block - 0.005 * (double)(16 - p.m) : forms[f].block;
-    if (direct && !aligned) block *= 1.15;
+    const double block = forms[f].block * (direct && !aligned ? 1.4 : 1.0);
+    const long long turns = f == FIRST_TILES - 1 ? 4 : 8;  // (wavefronts)
     for (int cut = 0; cut < 2; cut++) {
       long long parts = cut ? cus / tiles : 1;
       if (parts > p.blocks) parts = p.blocks;
@@ -410,7 +436,7 @@ Plan cheapest_plan(const ProductParams &p, bool aligned) {
       const long long part = parts > 1 ? (p.blocks + parts - 1) / parts : p.blocks;
       if (parts > 1) parts = (p.blocks + part - 1) / part;
       const double rounds = (double)((tiles * parts + cus - 1) / cus);
-      double us = rounds * (forms[f].start + block * (double)(direct ? (part + 7) / 8 * 8 : part));
+      double us = rounds * (forms[f].start + block * (double)(direct ? (part + turns - 1) / turns * turns : part));
       if (parts > 1) us += 4.0 + (double)parts * (double)p.m * p.n * 8e-7;
       if (!direct && !aligned) us += 3.0 + (double)(p.m + p.n) * p.k * 4e-7;  // (the copy)
       if (least < 0.0 || us < least) {
@@ -483,12 +509,12 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
     parts.relu = 0;
   }
   switch (plan.form) {
-    case 0: launch_few<1, 1, 8, 4>(parts, aligned); break;
-    case 1: launch_few<2, 1, 8, 4>(parts, aligned); break;
-    case 2: launch_few<4, 1, 8, 2>(parts, aligned); break;
-    case 3: launch_few<2, 2, 8, 2>(parts, aligned); break;
-    case 4: launch_few<4, 2, 8, 1>(parts, aligned); break;
-    case 5: launch_few<4, 4, 8, 1>(parts, aligned); break;
+    case 0: launch_few<1, 1, 8>(parts, aligned); break;
+    case 1: launch_few<2, 1, 8>(parts, aligned); break;
+    case 2: launch_few<4, 1, 8>(parts, aligned); break;
+    case 3: launch_few<2, 2, 8>(parts, aligned); break;
+    case 4: launch_few<4, 2, 8>(parts, aligned); break;
+    case 5: launch_few<4, 4, 4>(parts, aligned); break;
     case 6: launch_tiles<4, 2, 1, 1>(parts); break;
     case 7: launch_tiles<4, 2, 1, 2>(parts); break;
     default: launch_tiles<4, 2, 2, 2>(parts); break;

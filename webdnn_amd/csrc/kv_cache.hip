@@ -45,12 +45,6 @@ __device__ __forceinline__ Place sequence(const Sequences &q, int s) {
   return p;
 }
 
-// A number the compiler knows nothing about: what is computed from it stays where it is used and holds no registers in between.
-__device__ __forceinline__ int fresh(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-
 // Sums over the lanes up to and with each: shifts within rows of 16, then the last lanes of rows 0 and 2, and of row 1, into
 // those behind them.  They end at the largest int (sequences that contradict each other can claim more rows than the call has).
 __device__ __forceinline__ int add_sat(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
