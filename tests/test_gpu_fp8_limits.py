@@ -18,6 +18,18 @@ def test_every_tile_of_the_products(ctx, m, n, k):
     S.check_product(ctx, np.random.default_rng(m + n + k), m, n, k, bias=True, residual=m < 2000)
 
 
+@pytest.mark.parametrize("n,k", [(1, 1), (3, 15), (130, 1023), (9001, 4100), (300, 14336), (257, 5000), (128, 1024), (5, 4097)])
+def test_products_of_one_row(ctx, n, k):
+    rng = np.random.default_rng(n + k)
+    S.check_product(ctx, rng, 1, n, k, bias=True, residual=True, relu=True)
+    a, w = S.bytes_of(rng, (1, k)), S.bytes_of(rng, (n, k))
+    sa, sw = np.ones((1, -(-k // 128)), np.float32), np.ones((-(-n // 128), -(-k // 128)), np.float32)
+    w[n // 2, k - 1] = 0xff
+    up = ctx.move_tensor
+    y = H.matmul_fp8(ctx, up(a), up(sa), up(w), up(sw)).get_data()
+    assert np.array_equal(np.isnan(y[0]), np.arange(n) == n // 2)
+
+
 @pytest.mark.parametrize("rows,length", [(9, 700), (6, 768), (1030, 769), (11, 1400), (3, 1536), (70, 1537), (2, 5000), (3, 6144), (40, 6145), (600, 8500), (5, 12000),
                                          (2, 16384), (513, 9001), (3, 16385)])
 def test_every_form_of_the_norm(ctx, rows, length):

@@ -12,6 +12,7 @@ namespace {
 
 using namespace wdh::fp8;
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -99,11 +100,69 @@ __device__ __forceinline__ void finish4(const ProductParams &p, float *Y, long l
   store4(Y + i * p.n, j, p.n, v);
 }
 
+// One row of A: a workgroup has four rows of W, its wavefronts a quarter of K each, a KB of a row at a time; products and sums in fp32 on
+// the vector units, which keep up with memory where the matrix ones would work for 1 row of 16.  Bound: memory (us, so / in tiles of
+// 16 rows: 8192 x 8192 13.3 / 16.9, 5.1 TB/s; 4096 columns, K = 14336, 12.3 / 15.9; 14336 columns, K = 4096, 11.9 / 15.0; 211 columns, K =
+// 3705, 5.2 / 15.2).
+template <bool ALIGNED>
+__global__ __launch_bounds__(256) void product_row(ProductParams p) {
+  constexpr int R = 4;
+  __shared__ float part[4][R];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int j0 = blockIdx.x * R; j0 < p.n; j0 += gridDim.x * R) {
+    const float *sw = p.SW + (long long)(j0 / BLOCK) * p.blocks;
+    float acc[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) acc[r] = 0.0f;
+#pragma unroll 2
+    for (int k = 1024 * wave + 16 * lane; k < p.k; k += 4096) {
+      Piece<ALIGNED> a, w[R];
+      a.load(p.A, k, p.k);
+#pragma unroll
+      for (int r = 0; r < R; r++) w[r].load(p.W + (long long)(j0 + r < p.n ? j0 + r : p.n - 1) * p.pitch, k, p.k);
+      const float c = p.SA[k / BLOCK] * sw[k / BLOCK];
+      const i32x4 a16 = a.get(p.A, k, p.k);
+      f32x2 x[8];
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[2 * i] = __builtin_amdgcn_cvt_pk_f32_fp8(a16[i], false), x[2 * i + 1] = __builtin_amdgcn_cvt_pk_f32_fp8(a16[i], true);
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const i32x4 w16 = w[r].get(p.W + (long long)(j0 + r < p.n ? j0 + r : p.n - 1) * p.pitch, k, p.k);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w16[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w16[i], true);
+          sum = __builtin_fmaf(x[2 * i][0], lo[0], sum);
+          sum = __builtin_fmaf(x[2 * i][1], lo[1], sum);
+          sum = __builtin_fmaf(x[2 * i + 1][0], hi[0], sum);
+          sum = __builtin_fmaf(x[2 * i + 1][1], hi[1], sum);
+        }
+        acc[r] = __builtin_fmaf(sum, c, acc[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const float sum = wdh::rowmath::wave_sum(acc[r]);
+      if (lane == 0) part[wave][r] = sum;
+    }
+    __syncthreads();
+    const int j = j0 + (int)threadIdx.x;
+    if (threadIdx.x < R && j < p.n) {
+      const int r = threadIdx.x;
+      float v = ((part[0][r] + part[1][r]) + part[2][r]) + part[3][r];
+      if (p.bias) v = v + p.bias[j];
+      if (p.R) v = v + p.R[j];
+      p.Y[j] = p.relu && !(v > 0.0f) && v == v ? 0.0f : v;
+    }
+    __syncthreads();  // (the next rows' sums go to the same places)
+  }
+}
+
 // Few rows of A, or few results: a workgroup has 16 NT rows of W and 16 MT of A, its wavefronts take K blocks in turn and add up through
 // LDS.  A wavefront brings its blocks itself, eight lanes to a row, the next one while it works on this one, and turns them in a part of LDS
 // of its own, where a row's pieces are exchanged by its number (as below), into what the matrix instructions take: a row to each of
 // 16 neighbouring lanes, which straight from memory is 16 lines for 16 lanes (us, so / straight from memory: 64 rows, 4096 x 4096, 8.4 /
-// 12.9, 333 x 1000 x 2048 7.4 / 9.8, x 2050 10.3 / 12.8; a single row, 8192 x 4096, 9.2 / 8.8).  More than one block on its way is slower
+// 12.9, 333 x 1000 x 2048 7.4 / 9.8, x 2050 10.3 / 12.8).  More than one block on its way is slower
 // (64 rows 9.4).  Bound: memory (W is read once for 16 MT rows), or latency.
 template <int NT, int MT, int WAVES, bool ALIGNED>
 __global__ __launch_bounds__(64 * WAVES) void product_few(ProductParams p) {
@@ -480,6 +539,13 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
   p.pitch = k;
   p.part = p.blocks;
   bool aligned = k % 16 == 0;  // (buffers start on 512-byte boundaries)
+  if (m == 1) {  // (see product_row)
+    const dim3 grid((unsigned)((n + 3) / 4 < 1 << 20 ? (n + 3) / 4 : 1 << 20));
+    if (aligned) hipLaunchKernelGGL((product_row<true>), grid, dim3(256), 0, wdh::stream(), p);
+    else hipLaunchKernelGGL((product_row<false>), grid, dim3(256), 0, wdh::stream(), p);
+    WDH_LAUNCH_CHECK();
+    return WDH_OK;
+  }
   Plan plan = cheapest_plan(p, aligned);
   // Tiles of many rows take rows of whole 16-byte pieces: others are copied first.
   wdh_buf packed = 0;
