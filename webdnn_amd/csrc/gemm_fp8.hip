@@ -100,62 +100,81 @@ __device__ __forceinline__ void finish4(const ProductParams &p, float *Y, long l
   store4(Y + i * p.n, j, p.n, v);
 }
 
-// One row of A: a workgroup has four rows of W, its wavefronts a quarter of K each, a KB of a row at a time; products and sums in fp32 on
-// the vector units, which keep up with memory where the matrix ones would work for 1 row of 16.  Bound: memory (us, so / in tiles of
-// 16 rows: 8192 x 8192 13.3 / 16.9, 5.1 TB/s; 4096 columns, K = 14336, 12.3 / 15.9; 14336 columns, K = 4096, 11.9 / 15.0; 211 columns, K =
-// 3705, 5.2 / 15.2).
-template <bool ALIGNED>
-__global__ __launch_bounds__(256) void product_row(ProductParams p) {
+// One or two rows of A: a workgroup has four rows of W, its wavefronts a quarter of K each, a KB of a row at a time; products and sums in
+// fp32 on the vector units, which keep up with memory where the matrix ones would work for one row of 16.  Bound: memory (us, so / in
+// tiles of 16 rows; one row: 8192 x 8192 13.3 / 16.9, 5.1 TB/s, 4096 columns, K = 14336, 12.3 / 15.9, 14336 columns, K = 4096, 11.9 / 15.0;
+// two rows: 14.6 / 17.0, 13.8 / 16.1, 14.0 / 15.0; three would be 17.2 / 17.1, 14.8 / 16.2, 15.8 / 15.0).
+template <int M, bool ALIGNED>
+__global__ __launch_bounds__(256) void product_rows(ProductParams p) {
   constexpr int R = 4;
-  __shared__ float part[4][R];
+  __shared__ float part[4][R * M];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int j0 = blockIdx.x * R; j0 < p.n; j0 += gridDim.x * R) {
     const float *sw = p.SW + (long long)(j0 / BLOCK) * p.blocks;
-    float acc[R];
+    auto row = [&](int r) { return p.W + (long long)(j0 + r < p.n ? j0 + r : p.n - 1) * p.pitch; };
+    float acc[R][M];
 #pragma unroll
-    for (int r = 0; r < R; r++) acc[r] = 0.0f;
-#pragma unroll 2
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int m = 0; m < M; m++) acc[r][m] = 0.0f;
+#pragma unroll(M == 1 ? 2 : 1)
     for (int k = 1024 * wave + 16 * lane; k < p.k; k += 4096) {
-      Piece<ALIGNED> a, w[R];
-      a.load(p.A, k, p.k);
+      Piece<ALIGNED> a[M], w[R];
+      float c[M];
 #pragma unroll
-      for (int r = 0; r < R; r++) w[r].load(p.W + (long long)(j0 + r < p.n ? j0 + r : p.n - 1) * p.pitch, k, p.k);
-      const float c = p.SA[k / BLOCK] * sw[k / BLOCK];
-      const i32x4 a16 = a.get(p.A, k, p.k);
-      f32x2 x[8];
+      for (int r = 0; r < R; r++) w[r].load(row(r), k, p.k);
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[2 * i] = __builtin_amdgcn_cvt_pk_f32_fp8(a16[i], false), x[2 * i + 1] = __builtin_amdgcn_cvt_pk_f32_fp8(a16[i], true);
+      for (int m = 0; m < M; m++) a[m].load(p.A + m * p.pitch, k, p.k);
+      const float s = sw[k / BLOCK];
+#pragma unroll
+      for (int m = 0; m < M; m++) c[m] = p.SA[(long long)m * p.blocks + k / BLOCK] * s;
+      f32x2 x[M][8];
+#pragma unroll
+      for (int m = 0; m < M; m++) {
+        const i32x4 v = a[m].get(p.A + m * p.pitch, k, p.k);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[m][2 * i] = __builtin_amdgcn_cvt_pk_f32_fp8(v[i], false), x[m][2 * i + 1] = __builtin_amdgcn_cvt_pk_f32_fp8(v[i], true);
+      }
 #pragma unroll
       for (int r = 0; r < R; r++) {
-        const i32x4 w16 = w[r].get(p.W + (long long)(j0 + r < p.n ? j0 + r : p.n - 1) * p.pitch, k, p.k);
-        float sum = 0.0f;
+        const i32x4 v = w[r].get(row(r), k, p.k);
+        float sum[M];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w16[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w16[i], true);
-          sum = __builtin_fmaf(x[2 * i][0], lo[0], sum);
-          sum = __builtin_fmaf(x[2 * i][1], lo[1], sum);
-          sum = __builtin_fmaf(x[2 * i + 1][0], hi[0], sum);
-          sum = __builtin_fmaf(x[2 * i + 1][1], hi[1], sum);
+        for (int m = 0; m < M; m++) sum[m] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const f32x2 y = i & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(v[i / 2], true) : __builtin_amdgcn_cvt_pk_f32_fp8(v[i / 2], false);
+#pragma unroll
+          for (int m = 0; m < M; m++) sum[m] = __builtin_fmaf(x[m][i][1], y[1], __builtin_fmaf(x[m][i][0], y[0], sum[m]));
         }
-        acc[r] = __builtin_fmaf(sum, c, acc[r]);
+#pragma unroll
+        for (int m = 0; m < M; m++) acc[r][m] = __builtin_fmaf(sum[m], c[m], acc[r][m]);
       }
     }
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-      const float sum = wdh::rowmath::wave_sum(acc[r]);
-      if (lane == 0) part[wave][r] = sum;
-    }
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int m = 0; m < M; m++) {
+        const float sum = wdh::rowmath::wave_sum(acc[r][m]);
+        if (lane == 0) part[wave][m * R + r] = sum;
+      }
     __syncthreads();
-    const int j = j0 + (int)threadIdx.x;
-    if (threadIdx.x < R && j < p.n) {
-      const int r = threadIdx.x;
-      float v = ((part[0][r] + part[1][r]) + part[2][r]) + part[3][r];
+    const int t = threadIdx.x, j = j0 + t % R, m = t / R;
+    if (t < R * M && j < p.n) {
+      float v = ((part[0][t] + part[1][t]) + part[2][t]) + part[3][t];
       if (p.bias) v = v + p.bias[j];
-      if (p.R) v = v + p.R[j];
-      p.Y[j] = p.relu && !(v > 0.0f) && v == v ? 0.0f : v;
+      if (p.R) v = v + p.R[(long long)m * p.n + j];
+      p.Y[(long long)m * p.n + j] = p.relu && !(v > 0.0f) && v == v ? 0.0f : v;
     }
     __syncthreads();  // (the next rows' sums go to the same places)
   }
+}
+
+template <int M>
+void launch_rows(const ProductParams &p, bool aligned) {
+  const dim3 grid((unsigned)((p.n + 3) / 4 < 1 << 20 ? (p.n + 3) / 4 : 1 << 20));
+  if (aligned) hipLaunchKernelGGL((product_rows<M, true>), grid, dim3(256), 0, wdh::stream(), p);
+  else hipLaunchKernelGGL((product_rows<M, false>), grid, dim3(256), 0, wdh::stream(), p);
 }
 
 // Few rows of A, or few results: a workgroup has 16 NT rows of W and 16 MT of A, its wavefronts take K blocks in turn and add up through
@@ -440,7 +459,7 @@ __global__ __launch_bounds__(256) void product_join(ProductParams p, const float
     const int j = (int)(at - i * pieces) * 4;
     const float *from = partial + i * p.n;
     f32x4 v = load4(from, j, p.n);
-#pragma unroll 4
+#pragma unroll 8
     for (int part = 1; part < parts; part++) v = v + load4(from + part * p.m * p.n, j, p.n);
     finish4(p, p.Y, i, j, v);
   }
@@ -466,7 +485,7 @@ __global__ __launch_bounds__(256) void pack_rows(const unsigned char *A, const u
 // Which form a product takes, and in how many parts along K.  A workgroup of a form takes `start` + `block` per block of K us (measured
 // with every CU busy: K of 2048 to 14336, 1 to 8192 rows).  Wavefronts of the first forms take blocks eight (64 x 64: four) at a time; odd
 // rows cost these 1.4 times as much, the others the copy.  Tiles that leave CUs idle are cut along K into as many parts as there are CUs
-// for; the parts' join is a launch of 4 us and its bytes.  The cheapest of all wins (us, so / the smallest tile that fits the chip, uncut:
+// for; the parts' join is a launch of 4 us, 0.15 for each part and its bytes.  The cheapest of all wins (us, so / the smallest tile that fits the chip, uncut:
 // 4096 columns, K = 14336: 17 rows 16.4 / 19.9, 64 rows 23 / 25, 256 rows 47 / 53; 8192 x 8192: 128 rows 33 / 34, 256 rows 51 / 57, 1024
 // rows 139 / 161).
 struct Form {
@@ -496,7 +515,7 @@ Plan cheapest_plan(const ProductParams &p, bool aligned) {
       if (parts > 1) parts = (p.blocks + part - 1) / part;
       const double rounds = (double)((tiles * parts + cus - 1) / cus);
       double us = rounds * (forms[f].start + block * (double)(direct ? (part + turns - 1) / turns * turns : part));
-      if (parts > 1) us += 4.0 + (double)parts * (double)p.m * p.n * 8e-7;
+      if (parts > 1) us += 4.0 + (double)parts * (0.15 + (double)p.m * p.n * 8e-7);
       if (!direct && !aligned) us += 3.0 + (double)(p.m + p.n) * p.k * 4e-7;  // (the copy)
       if (least < 0.0 || us < least) {
         least = us;
@@ -539,10 +558,9 @@ extern "C" int wdh_gemm_fp8(wdh_buf hA, wdh_buf hSA, wdh_buf hW, wdh_buf hSW, wd
   p.pitch = k;
   p.part = p.blocks;
   bool aligned = k % 16 == 0;  // (buffers start on 512-byte boundaries)
-  if (m == 1) {  // (see product_row)
-    const dim3 grid((unsigned)((n + 3) / 4 < 1 << 20 ? (n + 3) / 4 : 1 << 20));
-    if (aligned) hipLaunchKernelGGL((product_row<true>), grid, dim3(256), 0, wdh::stream(), p);
-    else hipLaunchKernelGGL((product_row<false>), grid, dim3(256), 0, wdh::stream(), p);
+  if (m <= 2) {  // (see product_rows)
+    if (m == 1) launch_rows<1>(p, aligned);
+    else launch_rows<2>(p, aligned);
     WDH_LAUNCH_CHECK();
     return WDH_OK;
   }
