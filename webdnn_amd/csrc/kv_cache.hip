@@ -355,7 +355,7 @@ __device__ __forceinline__ void split2_f16(const float (&x)[8], f16x8 (&part)[2]
 // into operand registers with 16-byte loads.  That takes an order of keys in which the four that a lane gets from score tile t are
 // keys 16 g + 4 t .. + 3 of the page (g = lane / 16), and an order of d in which a lane's 16 bytes serve two products.
 // Bound: memory where rows are few (32 tokens behind 500 to 8500, 32 heads of 128 on 8: 56 us, 5.3 TB/s; a copy of this kernel that only
-// loads takes 55), so three exact parts cost nothing that two would not; with all rows in use, instructions (1.3 us for a page of each
+// loads takes 55; pages brought line by line and turned in LDS: 61), so three exact parts cost nothing that two would not; with all rows in use, instructions (1.3 us for a page of each
 // wavefront, two workgroups to a CU).
 template <int D>
 __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
