@@ -480,8 +480,9 @@ int wdh_strided_copy(wdh_buf X, int64_t x_offset, wdh_buf Y, int64_t y_offset,
  * No counterpart in the reference, whose operators are fp32 only.  Activations, the residual stream and all results
  * are fp32; what large products and attention read is held in e4m3: 8-bit floating point with 4 exponent and 3 fraction
  * bits as the OCP specification and ONNX FLOAT8E4M3FN define it (largest value 448, no infinities, NaN = 0x7f or 0xff).
- * An element stands for its e4m3 value times the scale of its block.  Rounding is to nearest even; a block's scale
- * follows its finite elements, and what is not finite is held as NaN.  All of them can be recorded (wdh_graph_begin);
+ * An element stands for its e4m3 value times the scale of its block: the value is the fp32 quotient of both (rounded to
+ * nearest), rounded to the nearest e4m3 value, ties to even.  A block's scale follows its finite elements, and what is not
+ * finite is held as NaN.  All of them can be recorded (wdh_graph_begin);
  * Table, Lens and Starts are read on the device, so that a replay may find other sequences in them.
  * Results of a call do not depend on anything but its operands: no atomics, fixed orders of addition. */
 #define WDH_FP8_BLOCK 128   /* elements along a row that share a scale  */

@@ -1,0 +1,49 @@
+"""The 8-bit serving operators at operands where a definition and a shortcut part: quotients beside a tie."""
+import numpy as np
+import pytest
+import torch
+
+import fp8_ref as F
+from webdnn_amd import hostops as H
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- quantisation is a division ------------------------------------------------------------------
+def quotients(x, scales, block_rows):
+    """e4m3 bytes of the fp32 quotients of finite x and its blocks' scales (numpy divides fp32 numbers with one rounding)."""
+    c = np.repeat(np.repeat(scales, block_rows, 0), 128, 1)[:x.shape[0], :x.shape[1]]
+    y = np.clip(x / c, np.float32(-448), np.float32(448))
+    return torch.from_numpy(y).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+
+
+def beside_ties(rng, rows, cols, block_rows, sizes):
+    """Elements whose quotient by their block's scale is a middle between two e4m3 values, or a few fp32 steps from one."""
+    top = (rng.uniform(1, 2, (-(-rows // block_rows), -(-cols // 128))) * 448).astype(np.float32) * sizes
+    c = np.maximum(top / np.float32(448), np.float32(F.LEAST))
+    per = lambda t: np.repeat(np.repeat(t, block_rows, 0), 128, 1)[:rows, :cols]
+    ties = np.concatenate([(F.VALUES[:126] + F.VALUES[1:127]) / 2, F.VALUES[:127]])
+    x = (rng.choice(ties, (rows, cols)) * per(c).astype(np.float64)).astype(np.float32)
+    x = (x.view(np.int32) + np.where(x != 0, rng.integers(-2, 3, (rows, cols)), 0).astype(np.int32)).view(np.float32)
+    x = np.minimum(x, per(top)) * np.where(rng.random((rows, cols)) < 0.5, np.float32(-1), np.float32(1))
+    x[::block_rows, ::128] = top
+    return x
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -40, 2.0 ** -41, 2.0 ** -98, 2.0 ** -110, 2.0 ** 60, 2.0 ** 118])
+@pytest.mark.parametrize("rows,cols,block_rows", [(40, 1030, 1), (333, 128, 1), (300, 1028, 128), (512, 130, 128)])
+def test_quantised_values_are_those_of_the_quotients(ctx, rows, cols, block_rows, size):
+    rng = np.random.default_rng(rows + cols)
+    x = beside_ties(rng, rows, cols, block_rows, np.float32(size))
+    q, c = (t.get_data() for t in H.quantize_fp8(ctx, ctx.move_tensor(x), block_rows))
+    want = np.maximum(F.finite_amax(F.block_view(x, block_rows), (1, 3)) / np.float32(448), np.float32(F.LEAST))
+    assert np.array_equal(c, want) and F.same_bytes(q, quotients(x, c, block_rows))
+
+
+@pytest.mark.parametrize("rows,length", [(9, 128), (40, 1030), (7, 4096), (3, 20000)])
+def test_a_norms_8_bit_rows_are_the_quotients_of_its_fp32_ones(ctx, rows, length):
+    rng = np.random.default_rng(length)
+    x = (rng.standard_normal((rows, length)) * 2.0 ** rng.integers(-8, 8, (rows, length))).astype(np.float32)
+    y, q, c = ctx.empty_tensor(x.shape), ctx.empty_tensor(x.shape, "float8e4m3fn"), ctx.empty_tensor([rows, -(-length // 128)])
+    H.call("wdh_rmsnorm", ctx.move_tensor(x).handle, 0, 0, 0, y.handle, q.handle, c.handle, rows, length, 1e-5)
+    assert F.same_bytes(q.get_data(), quotients(y.get_data(), c.get_data(), 1))

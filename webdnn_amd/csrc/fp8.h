@@ -47,13 +47,46 @@ __device__ __forceinline__ float half_max(float v) {
 // The scale of a block whose largest finite magnitude is `amax`.
 __device__ __forceinline__ float block_scale(float amax) { return fmaxf(amax / E4M3_MAX, LEAST_SCALE); }
 
-// Four elements times `inv` (the reciprocal of their block's scale) to e4m3, rounded to nearest even, packed in order.  What is
-// not finite becomes NaN.  A quotient beyond 448 is at most 448 (1 + 2^-22) and rounds to 448.
+// Four elements, two to a conversion, packed in order: rounded to the nearest e4m3 value, ties to even.
+__device__ __forceinline__ int convert4(f32x4 v) {
+  int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], q, true);
+}
+// Four elements times `inv` to e4m3, for scales that are powers of two: nothing is rounded but the result.  What is not finite becomes NaN.
 __device__ __forceinline__ int pack4(f32x4 v, float inv) {
 #pragma unroll
   for (int e = 0; e < 4; e++) v[e] = fabsf(v[e]) <= FLT_MAX ? v[e] * inv : NAN;
-  int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-  return __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], q, true);
+  return convert4(v);
+}
+
+// A block's scale as a divisor.  Quotients have to be the fp32 ones: a product with the reciprocal is up to 1.5 steps of fp32 off, and where that
+// crosses the middle between two e4m3 values (1 of 10^4 to 10^5 elements) the result is a whole step of e4m3 off.
+// Two corrections q <- q + r (v - q c) with the rounded reciprocal r: the first leaves a quotient less than a step off, whose remainder
+// is exact, and the second is the quotient rounded to nearest (Markstein's theorem).  Remainders of blocks below 2^-40 could be among the
+// subnormal numbers: those are worked on 2^60 times as large.
+// Cost (us, so / with the reciprocal alone): quantisation of 5000 rows of 8192 38.4 / 37.9, of 30000 x 1030 in 128 x 128 35.7 / 35.4.
+struct Divisor {
+  float c, r, up;
+};
+__device__ __forceinline__ Divisor divisor(float c) {
+  Divisor d;
+  d.up = c < 0x1p-40f ? 0x1p60f : 1.0f;
+  d.c = c * d.up;
+  d.r = 1.0f / d.c;
+  return d;
+}
+// Four elements over their block's scale to e4m3.  What is not finite becomes NaN (the remainder of an infinity is none); a quotient beyond 448
+// is at most 448 (1 + 2^-22) and rounds to 448.  (Quotients that are subnormal numbers of fp32 may be off: they are 0 as e4m3.)
+__device__ __forceinline__ int divide4(f32x4 v, Divisor d) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float x = v[e] * d.up;
+    float q = x * d.r;
+    q = __builtin_fmaf(__builtin_fmaf(-q, d.c, x), d.r, q);
+    q = __builtin_fmaf(__builtin_fmaf(-q, d.c, x), d.r, q);
+    v[e] = copysignf(q, x);  // (the corrections make -0 a 0)
+  }
+  return convert4(v);
 }
 
 // Elements idx .. idx+3 of a row of `len` (0 beyond its end), and back.
