@@ -531,7 +531,9 @@ int wdh_cache_append(wdh_buf K, int64_t k_offset, int64_t k_stride, wdh_buf V, i
  * which wdh_cache_append has to have written before.  Prompts, parts of prompts and single tokens may be mixed in a call.
  * Y [tokens, heads * d] is dense; rows that belong to no sequence are left as they are.  A token on a page whose number is
  * outside the cache, or whose scales are not positive and finite, makes the rows that see it NaN; slots behind a sequence's
- * tokens and tokens behind a row do not touch it, whatever they hold.  Where one call's rows do not fill the chip the tokens
+ * tokens and tokens behind a row do not touch it, whatever they hold.  Results have the precision of fp32 relative to the
+ * largest shares (weight times value) of a row, pages' scales differing as they may; weights below 2^-112 of a row's largest may
+ * count for nothing.  Where one call's rows do not fill the chip the tokens
  * are cut into parts whose results are joined by a second launch, in a workspace from the pool (WDH_ENOMEM without room). */
 int wdh_cache_attention(wdh_buf Q, int64_t q_offset, int64_t q_stride, wdh_buf KPages, wdh_buf KScales, wdh_buf VPages,
                         wdh_buf VScales, wdh_buf Table, wdh_buf Lens, wdh_buf Starts, wdh_buf Y, int seqs, int tokens,

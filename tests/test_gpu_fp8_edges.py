@@ -1,9 +1,11 @@
-"""The 8-bit serving operators at operands where a definition and a shortcut part: quotients beside a tie."""
+"""The 8-bit serving operators at operands where a definition and a shortcut part: quotients beside a tie, pages of
+values that differ in size."""
 import numpy as np
 import pytest
 import torch
 
 import fp8_ref as F
+import test_gpu_fp8_serving as S
 from webdnn_amd import hostops as H
 
 pytestmark = pytest.mark.gpu
@@ -47,3 +49,56 @@ def test_a_norms_8_bit_rows_are_the_quotients_of_its_fp32_ones(ctx, rows, length
     y, q, c = ctx.empty_tensor(x.shape), ctx.empty_tensor(x.shape, "float8e4m3fn"), ctx.empty_tensor([rows, -(-length // 128)])
     H.call("wdh_rmsnorm", ctx.move_tensor(x).handle, 0, 0, 0, y.handle, q.handle, c.handle, rows, length, 1e-5)
     assert F.same_bytes(q.get_data(), quotients(y.get_data(), c.get_data(), 1))
+
+
+# ---- attention over pages whose values differ in size ----------------------------------------------
+def sized_pages(rng, new, past, heads, kv, d, large, octaves):
+    """Sequences of one call, some pages of which hold values 2^octaves as large as the others', behind keys that no query wants
+    (60 nats below the others, weights of 2^-86): (cache, table, lens, starts, q)."""
+    table, lens, starts, pages = S.layout(rng, [new], [past])
+    n = int(lens[0])
+    k, v = (rng.standard_normal((n, kv, d)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((new, heads, d)).astype(np.float32)
+    k[:, :, 0], q[:, :, 0] = 0, 16
+    for page in large:
+        at = slice(64 * page, 64 * page + 64)
+        k[at, :, 0] = -30 * 0.125 / d ** -0.5
+        v[at] *= np.float32(2.0 ** octaves)
+    c = F.Cache(pages, kv, d)
+    c.append(k, v, table, lens, np.array([0, n]))
+    return c, table, lens, starts, q
+
+
+def attention(c, q, table_row, length, alpha):
+    """The last len(q) tokens of one sequence in 64 bits."""
+    k, v = (torch.from_numpy(t) for t in c.tokens(table_row, length))
+    n, heads, d = q.shape
+    past, group = torch.arange(n)[:, None] + length - n, heads // len(k)
+    out = np.empty(q.shape)
+    for h in range(heads):
+        t = torch.from_numpy(q[:, h].astype(np.float64)) @ k[h // group].T * alpha
+        out[:, h] = (torch.softmax(t.masked_fill(torch.arange(length) > past, -np.inf), 1) @ v[h // group]).numpy()
+    return out
+
+
+def relative(got, want):
+    return np.linalg.norm(got.astype(np.float64) - want) / np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("octaves", [0, 16, 20, 30, 40, 60, 82])
+@pytest.mark.parametrize("new,heads,kv,d,large", [(1, 4, 2, 64, [0]), (90, 4, 2, 64, [2]), (650, 64, 2, 64, [0]), (650, 64, 2, 64, [3, 7]), (650, 64, 2, 64, [11]),
+                                                  (700, 32, 4, 128, [1]), (1300, 64, 2, 32, [0, 9])])
+def test_values_of_pages_that_differ_in_size(ctx, new, heads, kv, d, large, octaves):
+    """What a row attends to counts in full, however large the values are that it does not attend to.
+
+    2-norm over all results: a score's 3 d / 32 additions of its queries' parts and the roundings of its factor, argument and power
+    are some 2^-22.5 of a weight, different for each key (scores here are of size one); sums and second products add less.
+    2^-20 is four times that; weights or queries cut to 16 or fewer bits are 2^-17 and more.  (2^82 times as large, the values behind weights of
+    2^-86 show in the results.)"""
+    rng = np.random.default_rng(octaves)
+    past = 640
+    c, table, lens, starts, q = sized_pages(rng, new, past, heads, kv, d, large, octaves)
+    want = attention(c, q, table[0], int(lens[0]), d ** -0.5)
+    got = S.attend(ctx, c, q, table, lens, starts, np.float32(d ** -0.5))
+    assert relative(got, want) <= 2.0 ** -20, (relative(got, want) * 2 ** 20)
+    assert np.max(np.abs(want)) < 64                                         # (no row rests on a large page)

@@ -273,6 +273,9 @@ __device__ __forceinline__ T scalar(const T *from, long long at) {
   return *(constant)(uintptr_t)(from + at);
 }
 
+// A number that all lanes have alike, in a scalar register.
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+
 // Over the four lanes that share lane % 16: a swap of a register with itself leaves both halves' values side by side.
 template <class Op>
 __device__ __forceinline__ float across_groups(float v, Op op) {
@@ -789,7 +792,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   };
 
   // Queries in two float16 parts, 8 elements of the lane's row for each instruction.  A row is brought to [2^14, 2^15) by a power of two:
-  // what two parts leave out is at most 2^-24 of its largest element, the size of an fp32 rounding in the sum that this element dominates.
+  // what two parts leave out is at most 2^-23 of an element, or 2^-39 of the row's largest one (half a step of float16's least numbers).
   f16x8 q[2 * QN][2];
   float row_scale;
   {
@@ -822,10 +825,13 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   for (int i = 0; i < DT; i++)
 #pragma unroll
     for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
-  float top = -INFINITY, sum = 0.0f;
-  // Weights go in two float16 parts as well, times 2^15 and their page's scale over the largest scale so far, in whose units (times
-  // 2^-15) the output is held: what is left out of a key's share is at most 2^-23 of it and 2^-40 of the largest value.
-  float unit = 0.0f;
+  float top = -FLT_MAX, sum = 0.0f;
+  // Weights go in two float16 parts as well, times their page's scale and in such units that the row's largest product of both so far
+  // is in (2^13, 2^15]: what is left out of a key's share is at most 2^-23 of it and 2^-38 of the largest share, whatever the scales of pages
+  // that count for less.  `top` is the exponent that weights are relative to, the least whole number no score (as a power of two) is
+  // above, and the output is held in units of 2^(top + gap - 15): both change by whole powers of two, which round nothing.
+  // Keys of half a page none of whose weights reaches 2^-112 of the row's largest so far count for nothing.
+  float gap = -1e30f;
 
   // Half a page of scores: 32 keys, of which a lane has keys 16 half + r of block t.
   auto scores = [&](int buf, int t) {
@@ -878,32 +884,28 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   for (int pg = begin; pg < end; pg++) {
     const int next_buf = buf == 2 ? 0 : buf + 1;
     const bool active = pg < wave_end;
-    if (active && now.vs > unit) {
-      const float back = unit / now.vs;
-#pragma unroll
-      for (int i = 0; i < DT; i++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) o[i][e] *= back;
-      unit = now.vs;
-    }
-    const float weight = unit > 0.0f ? 32768.0f * (now.vs / unit) : 0.0f;
+    const float vs_exponent = uniform((float)__builtin_amdgcn_frexp_expf(now.vs)), vs_mantissa = uniform(__builtin_amdgcn_frexp_mantf(now.vs));  // (0 of 0)
 #pragma unroll
     for (int t = 0; t < 2; t++) {
       if (active) {
         const float c = fmaxf(now.ks * row_scale, FLT_MIN);  // (never 0: -inf * 0 is NaN; scores that need less are all 0 to the softmax)
-        const float up = fmaxf(most * c, top), ref = up == -INFINITY ? 0.0f : up;
-        if (__any(up > top)) {
-          const float back = __builtin_amdgcn_exp2f(top - ref);
-          sum *= back;
+        const float mine = ceilf(most * c), up = fmaxf(mine, top), below = mine - up;  // (none seen: mine = -inf)
+        const bool counts = below >= -112.0f;
+        const float had = gap + (top - up), has = counts ? fmaxf(had, below + vs_exponent) : had;
+        if (__any(has > had || up > top)) {  // (false for most pages of a long sequence)
+          sum *= __builtin_amdgcn_exp2f(top - up);
+          const float back = __builtin_amdgcn_exp2f(had - has);
 #pragma unroll
           for (int i = 0; i < DT; i++)
 #pragma unroll
             for (int e = 0; e < 16; e++) o[i][e] *= back;
         }
         top = up;
+        gap = has;
+        const float weight = counts ? vs_mantissa * __builtin_amdgcn_exp2f(vs_exponent - has + 15.0f) : 0.0f;
         const f32x16 next = scores(t == 0 ? buf : next_buf, 1 - t);
 #pragma unroll
-        for (int r = 0; r < 16; r++) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c, -ref));
+        for (int r = 0; r < 16; r++) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c, -up));
 #pragma unroll
         for (int r = 0; r < 16; r++) sum += sc[r];
 #pragma unroll
@@ -959,7 +961,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     sum = __uint_as_float(b[0]) + __uint_as_float(b[1]);
   }
-  unit *= 1.0f / 32768.0f;
+  const int exponent = (int)fmaxf(gap - 15.0f, -1000.0f);  // (a row that has seen nothing: 0 times whatever)
   if (!live) return;
   // lane: row li of the wavefront's 32; registers 4 a .. + 3 of block i are elements 32 i + 8 a + 4 half .. + 3
   if (gridDim.y == 1) {
@@ -970,7 +972,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
       for (int a = 0; a < 4; a++) {
         f32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = sum == 0.0f ? 0.0f : o[i][4 * a + e] * unit / sum;
+        for (int e = 0; e < 4; e++) v[e] = sum == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(o[i][4 * a + e] / sum, exponent);
         *reinterpret_cast<f32x4 *>(y + 32 * i + 8 * a + 4 * half) = v;
       }
   } else {
@@ -978,9 +980,12 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 #pragma unroll
     for (int i = 0; i < DT; i++)
 #pragma unroll
-      for (int a = 0; a < 4; a++)
-        *reinterpret_cast<f32x4 *>(p.partial + at * D + 32 * i + 8 * a + 4 * half) =
-            f32x4{o[i][4 * a] * unit, o[i][4 * a + 1] * unit, o[i][4 * a + 2] * unit, o[i][4 * a + 3] * unit};
+      for (int a = 0; a < 4; a++) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = __builtin_amdgcn_ldexpf(o[i][4 * a + e], exponent);
+        *reinterpret_cast<f32x4 *>(p.partial + at * D + 32 * i + 8 * a + 4 * half) = v;
+      }
     if (half == 0) {
       p.stats[2 * at] = top;
       p.stats[2 * at + 1] = sum;
