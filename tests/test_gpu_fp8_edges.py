@@ -1,5 +1,5 @@
 """The 8-bit serving operators at operands where a definition and a shortcut part: quotients beside a tie, pages of
-values that differ in size."""
+values that differ in size, scales that are no numbers."""
 import numpy as np
 import pytest
 import torch
@@ -102,3 +102,20 @@ def test_values_of_pages_that_differ_in_size(ctx, new, heads, kv, d, large, octa
     got = S.attend(ctx, c, q, table, lens, starts, np.float32(d ** -0.5))
     assert relative(got, want) <= 2.0 ** -20, (relative(got, want) * 2 ** 20)
     assert np.max(np.abs(want)) < 64                                         # (no row rests on a large page)
+
+
+# ---- scales that are no numbers ----------------------------------------------------------------------
+@pytest.mark.parametrize("past,new", [(64, 1), (0, 1), (63, 2), (128, 1), (640, 1)])
+def test_an_infinite_key_scale_shows_in_a_page_of_one_key(ctx, past, new):
+    """The page's only key lies against the query: its score would be -inf, whose weight is 0, if the scale were multiplied with."""
+    rng = np.random.default_rng(past)
+    c, table, lens, starts = S.filled(rng, [new], [past], 2, 64)
+    n = int(lens[0])
+    k, _ = c.tokens(table[0], n)
+    q = rng.standard_normal((new, 4, 64)).astype(np.float32)
+    q[-1] = -np.repeat(k[:, n - 1], 2, 0)
+    want, bound = c.attention(q, table, lens, starts, 0.125)
+    c.ks[table[0, (n - 1) // 64], 1] = np.inf
+    got = S.attend(ctx, c, q, table, lens, starts, 0.125)
+    assert np.isnan(got[-1, 2:]).all()
+    assert np.all((np.abs(got - want) <= bound)[:, :2]) and np.all((np.abs(got - want) <= bound)[:-1])

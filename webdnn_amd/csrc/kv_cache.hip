@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     const long long at = (long long)(known ? id : 0) * p.kv_heads + head;
     float ks = scalar(p.KS, at), vs = scalar(p.VS, at);
     // (a scale that is no number shows through the scores, which are masked, not through 0 * NaN)
-    if (!known || !(ks > 0.0f) || !(vs > 0.0f && vs <= FLT_MAX)) ks = NAN, vs = 0.0f;
+    if (!known || !(ks > 0.0f && ks <= FLT_MAX) || !(vs > 0.0f && vs <= FLT_MAX)) ks = NAN, vs = 0.0f;
     return Page{at, ks, vs};
   };
   i32x4 k[4][CH], v[DT];
