@@ -502,7 +502,9 @@ int wdh_rmsnorm(wdh_buf X, wdh_buf Skip, wdh_buf Gamma, wdh_buf Sum, wdh_buf Y, 
 int wdh_quantize_fp8(wdh_buf X, wdh_buf Q, wdh_buf QScale, int64_t rows, int cols, int block_rows);
 /* Y[i, j] = sum_b AScale[i, b] WScale[j / 128, b] sum_{x in block b} A[i, x] W[j, x]  (+ Bias[j]) (+ R[i, j]), then the
  * epilogue.  A [m, k] and W [n, k] are e4m3, both with k contiguous; scales [m, ceil(k/128)] and [ceil(n/128), ceil(k/128)]
- * are any fp32 numbers.  Bias and R may be 0; R may be Y.  Sums are held in fp32.  k = 0 leaves Bias and R.  Products
+ * are fp32 numbers, the two of a block multiplied first: their product has to be 0 or of 2^-126 to 2^128.  Smaller ones lose bits
+ * or count as 0 (with scales as above: where a block's largest |a| |w| is below 2^-108), larger ones make results infinite or no
+ * numbers, as scales that are neither finite do.  Bias and R may be 0; R may be Y.  Sums are held in fp32.  k = 0 leaves Bias and R.  Products
  * whose result is too small to fill the chip are cut along k, the parts' sums added in order by a second launch; rows of A and
  * W that are no whole 16-byte pieces may be copied first: both in workspaces from the pool, and without room for them the
  * product is computed without, slower. */

@@ -1,5 +1,5 @@
 """The 8-bit serving operators at operands where a definition and a shortcut part: quotients beside a tie, pages of
-values that differ in size, scales that are no numbers."""
+values that differ in size, scales that are no numbers, scales of every size."""
 import numpy as np
 import pytest
 import torch
@@ -9,6 +9,7 @@ import test_gpu_fp8_serving as S
 from webdnn_amd import hostops as H
 
 pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
 
 
 # ---- quantisation is a division ------------------------------------------------------------------
@@ -119,3 +120,54 @@ def test_an_infinite_key_scale_shows_in_a_page_of_one_key(ctx, past, new):
     got = S.attend(ctx, c, q, table, lens, starts, 0.125)
     assert np.isnan(got[-1, 2:]).all()
     assert np.all((np.abs(got - want) <= bound)[:, :2]) and np.all((np.abs(got - want) <= bound)[:-1])
+
+
+# ---- products of extreme scales ----------------------------------------------------------------------
+SHAPES = [(1, 40, 700), (2, 300, 1040), (3, 50, 260), (20, 200, 12000), (40, 300, 1024), (100, 900, 2050), (300, 700, 4096), (700, 2000, 130), (1500, 2000, 144),
+          (8192, 4096, 200)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("a_octave,w_octave", [(70, -90), (-70, 90), (-140, 110), (127, -149), (-100, -24), (-62, -62), (60, 60), (120, 0), (-100, -100)])
+def test_scales_of_any_size_with_a_normal_product(ctx, m, n, k, a_octave, w_octave):
+    """Every third block has extreme scales; their product is 2^-126 to 2^122, or 0 as for blocks of zeros, whose scales are 2^-100 both.
+    Half the rows have one element in each of these blocks and nothing else: small terms count for themselves.  One row is zeros."""
+    rng = np.random.default_rng(m + n)
+    kb, nb = -(-k // 128), -(-n // 128)
+    odd = np.arange(kb) % 3 == 0                                             # (the others have scales of size one)
+    a, w = S.bytes_of(rng, (m, k)), S.bytes_of(rng, (n, k))
+    sa, sw = (rng.uniform(1, 2, s).astype(np.float32) for s in ((m, kb), (nb, kb)))
+    sa[:, odd] *= np.float32(2.0 ** a_octave)
+    sw[:, odd] *= np.float32(2.0 ** w_octave)
+    if a_octave < -126 or w_octave < -126:                                   # (subnormal ones have few bits)
+        sa[:, odd], sw[:, odd] = np.float32(2.0 ** a_octave), np.float32(2.0 ** w_octave)
+    alone = rng.random(m) < 0.5
+    in_odd = np.repeat(odd, 128)[:k]
+    a[np.ix_(alone, ~in_odd)] = 0
+    a[np.ix_(alone, np.arange(k) % 128 != 5)] = 0
+    if a_octave + w_octave > 100:
+        a[:, in_odd] &= 0x83                                                 # subnormal values: at most 3 * 2^-9
+        w[:, in_odd] &= 0x83
+    if a_octave + w_octave == -200:
+        a[:, in_odd] &= 0x80
+        w[:, in_odd] &= 0x80
+    a[0] = 0x80
+    want, size = F.product(a, sa, w, sw)
+    y = H.matmul_fp8(ctx, *(ctx.move_tensor(t) for t in (a, sa, w, sw))).get_data().astype(np.float64)
+    assert np.array_equal(y[0], np.zeros(n))
+    # a block's sum (of one product: nothing), its scales' product, the product with it, the sum of blocks; at most 2^-23 of the sizes' sum each
+    bound = np.where(alone, 3 + kb, 128 + 3 + kb)[:, None] * 2 * E * size + kb * 2.0 ** -149
+    assert size.max() < 3e38 and np.all(np.abs(y - want) <= bound), float(np.max(np.abs(y - want) - bound))
+
+
+@pytest.mark.parametrize("m", [1, 3, 300])
+def test_scales_that_are_no_numbers_reach_their_rows_and_columns(ctx, m):
+    rng = np.random.default_rng(m)
+    n, k = 300, 260
+    a, w = S.bytes_of(rng, (m, k)), S.bytes_of(rng, (n, k))
+    sa, sw = np.ones((m, 3), np.float32), np.ones((3, 3), np.float32)
+    sa[m - 1, 1], sw[2, 0], sw[1, 2] = np.nan, np.inf, 0
+    y = H.matmul_fp8(ctx, *(ctx.move_tensor(t) for t in (a, sa, w, sw))).get_data()
+    bad = np.zeros((m, n), bool)
+    bad[m - 1], bad[:, 256:] = True, True
+    assert np.array_equal(~np.isfinite(y), bad) and np.isnan(y[m - 1]).all()

@@ -13,7 +13,7 @@ namespace fp8 {
 
 constexpr int BLOCK = 128;               // elements along a row that share a scale
 constexpr float E4M3_MAX = 448.0f;
-constexpr float LEAST_SCALE = 7.8886090522101181e-31f;  // 2^-100: products of two scales and their quotients stay normal numbers
+constexpr float LEAST_SCALE = 7.8886090522101181e-31f;  // 2^-100: its reciprocal and the elements' quotients are numbers of fp32
 
 // Rows need not start on 16-byte boundaries (odd lengths): global loads and stores of four elements take any address.
 typedef float f32x4 __attribute__((ext_vector_type(4)));

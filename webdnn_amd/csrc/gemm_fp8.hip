@@ -1,7 +1,9 @@
 // Y = A W^T of e4m3 operands with a scale for each block of 128 along K (and, of W, for 128 rows):
 //   Y[i, j] = sum_b SA[i, b] SW[j / 128, b] sum_{x in b} A[i, x] W[j, x]   (+ bias[j]) (+ R[i, j]), then Relu if asked for.
 // The inner sums run on the bfloat16 matrix instructions, operands widened from e4m3 in registers (exact products, sums in fp32);
-// their results are scaled and added up in fp32.
+// their results are scaled and added up in fp32.  The product of a block's two scales is taken first, and is a normal number (or 0) by
+// contract: splitting scales into a part whose products are always normal and a power of two that the widening instructions take
+// along was built and cost 1 to 8 % (us, so / split: 128 x 8192 x 8192 34.2 / 37.3, 333 x 1000 x 2050 9.8 / 10.2, 64 x 4096 x 4096 8.1 / 8.4).
 //
 // The product is computed transposed (W is the instruction's first operand): a lane then holds results of one row of A, so that
 // the scale of a block is one number to a lane, and four neighbouring results to store.
