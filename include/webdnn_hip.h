@@ -498,7 +498,8 @@ int wdh_strided_copy(wdh_buf X, int64_t x_offset, wdh_buf Y, int64_t y_offset,
 int wdh_rmsnorm(wdh_buf X, wdh_buf Skip, wdh_buf Gamma, wdh_buf Sum, wdh_buf Y, wdh_buf Q, wdh_buf QScale,
                 int64_t outer, int len, float eps);
 /* X [rows, cols] to e4m3: Q [rows, cols], QScale [ceil(rows / block_rows), ceil(cols / 128)] with scales as above for
- * blocks of block_rows x 128.  block_rows: 1 (activations, what wdh_gemm_fp8 takes as A) or 128 (weights, its W). */
+ * blocks of block_rows x 128.  block_rows: 1 (activations, what wdh_gemm_fp8 takes as A) or 128 (weights, its W).  At most
+ * 2^29 - 32 blocks of one row, or 2^24 - 8 of 128. */
 int wdh_quantize_fp8(wdh_buf X, wdh_buf Q, wdh_buf QScale, int64_t rows, int cols, int block_rows);
 /* Y[i, j] = sum_b AScale[i, b] WScale[j / 128, b] sum_{x in block b} A[i, x] W[j, x]  (+ Bias[j]) (+ R[i, j]), then the
  * epilogue.  A [m, k] and W [n, k] are e4m3, both with k contiguous; scales [m, ceil(k/128)] and [ceil(n/128), ceil(k/128)]

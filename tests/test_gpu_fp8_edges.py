@@ -1,11 +1,13 @@
 """The 8-bit serving operators at operands where a definition and a shortcut part: quotients beside a tie, pages of
-values that differ in size, scales that are no numbers, scales of every size."""
+values that differ in size, scales that are no numbers, scales of every size, more blocks than a launch has threads
+for."""
 import numpy as np
 import pytest
 import torch
 
 import fp8_ref as F
 import test_gpu_fp8_serving as S
+from webdnn_amd import capi
 from webdnn_amd import hostops as H
 
 pytestmark = pytest.mark.gpu
@@ -171,3 +173,31 @@ def test_scales_that_are_no_numbers_reach_their_rows_and_columns(ctx, m):
     bad = np.zeros((m, n), bool)
     bad[m - 1], bad[:, 256:] = True, True
     assert np.array_equal(~np.isfinite(y), bad) and np.isnan(y[m - 1]).all()
+
+
+# ---- limits --------------------------------------------------------------------------------------------
+def test_blocks_beyond_a_launch_are_refused(ctx):
+    """A launch has fewer than 2^32 threads; a block of 1 x 128 takes eight."""
+    for rows, cols in ((1 << 29, 1), (1 << 28, 129), ((1 << 29) - 31, 128)):
+        with pytest.raises(capi.HipError) as err:
+            H.call("wdh_quantize_fp8", 1, 1, 1, rows, cols, 1)
+        assert err.value.code == -2 and "too many blocks" in str(err.value)
+
+
+def test_as_many_blocks_as_a_launch_has(ctx):
+    rows, n = (1 << 29) - 32, 1000
+    x, q, c = ctx.empty_tensor([rows, 1]), ctx.empty_tensor([rows, 1], "float8e4m3fn"), ctx.empty_tensor([rows, 1])
+    some = np.random.default_rng(1).standard_normal((n, 1)).astype(np.float32)
+    ends = (0, rows - n)
+    for at in ends:
+        H.call("wdh_write", x.handle, 4 * at, some.ctypes.data, some.nbytes)
+    H.quantize_fp8(ctx, x, 1, out=(q, c))
+    for at in ends:
+        byte, scale = np.empty((n, 1), np.uint8), np.empty((n, 1), np.float32)
+        H.call("wdh_read", q.handle, at, byte.ctypes.data, n)
+        H.call("wdh_read", c.handle, 4 * at, scale.ctypes.data, 4 * n)
+        assert np.array_equal(scale, np.abs(some) / np.float32(448)) and F.same_bytes(byte, quotients(some, scale, 1))
+    for t in (x, q, c):
+        t.dispose()
+    ctx.sync()
+    capi.call("wdh_trim", 0)

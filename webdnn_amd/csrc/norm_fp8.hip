@@ -278,7 +278,8 @@ extern "C" int wdh_quantize_fp8(wdh_buf hX, wdh_buf hQ, wdh_buf hQScale, int64_t
   if (rows == 0 || cols == 0) return WDH_OK;
   if (cols > (1 << 30) || rows > (1LL << 46) / cols) return fail(WDH_EINVAL, "wdh_quantize_fp8: too many elements");
   const long long blocks = ((long long)cols + BLOCK - 1) / BLOCK, units = (rows + block_rows - 1) / block_rows * blocks;
-  if (units > (block_rows == 1 ? 0x7fffffffLL : 0xfffff8LL)) return fail(WDH_EINVAL, "wdh_quantize_fp8: too many blocks");
+  // (a launch has fewer than 2^32 threads: eight to a block of one row, 256 to one of 128)
+  if (units > (block_rows == 1 ? 0xffffffLL * 8 * UNROLL : 0xfffff8LL)) return fail(WDH_EINVAL, "wdh_quantize_fp8: too many blocks");
   void *px, *pq, *pqs;
   if (!wdh::operand(hX, (size_t)rows * cols * 4, "wdh_quantize_fp8: X", &px)) return WDH_EINVAL;
   if (!wdh::operand(hQ, (size_t)rows * cols, "wdh_quantize_fp8: Q", &pq)) return WDH_EINVAL;
