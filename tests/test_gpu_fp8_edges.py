@@ -1,6 +1,6 @@
 """The 8-bit serving operators at operands where a definition and a shortcut part: quotients beside a tie, pages of
 values that differ in size, scales that are no numbers, scales of every size, more blocks than a launch has threads
-for."""
+for, rows whose factor is no normal number."""
 import numpy as np
 import pytest
 import torch
@@ -201,3 +201,17 @@ def test_as_many_blocks_as_a_launch_has(ctx):
         t.dispose()
     ctx.sync()
     capi.call("wdh_trim", 0)
+
+
+# ---- rows whose factor is no normal number ---------------------------------------------------------------
+@pytest.mark.parametrize("length", [200, 700, 3000, 9000, 20000])
+@pytest.mark.parametrize("size", [1e-45, 1e-42, 1e-39, 1e-38, 1e-35, 1e30, 5e36, 5e37, 3e38])
+def test_norm_of_the_least_and_largest_rows(ctx, length, size):
+    """1 / sqrt(mean) of such rows is beyond fp32's numbers, or among its subnormal ones."""
+    rng = np.random.default_rng(length)
+    x = (rng.standard_normal((3, length)).clip(-1.1, 1.1) * size).astype(np.float32)
+    x[:, 0] = np.float32(size)
+    g = rng.uniform(0.5, 1.5, length).astype(np.float32)
+    want = F.rms(x.astype(np.float64), g.astype(np.float64), 0.0)
+    y = H.rms_normalization(ctx, ctx.move_tensor(x), ctx.move_tensor(g), epsilon=0.0).get_data()
+    assert np.all(np.abs(y - want) <= 3.01 * E * np.abs(want) + 2.0 ** -149)

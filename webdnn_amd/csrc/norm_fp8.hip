@@ -4,7 +4,8 @@
 // The reference has no such operators; in its terms the first is the chain Add, Mul, ReduceMean, Add, Sqrt, Div, Mul
 // (src/descriptor_runner/operators/cpu/operators/standard/binary7.ts:24-75, reduce.ts:369-405, unary.ts:10-32):
 //   s = x + r,  y = (s * t) * g  with  t = 1 / sqrt(mean(s^2) + eps).
-// Squares are summed in double (a row of values near 1e20 keeps a finite mean), t is rounded to fp32 once.
+// Squares are summed in double (a row of values near 1e20 keeps a finite mean), t is rounded to fp32 once; where it would leave fp32's
+// normal numbers (rows of subnormal numbers, or near the largest), a power of two goes into the row's elements first.
 // 8 bits: c = max(largest finite |y| of a block / 448, 2^-100), q = e4m3(y / c), the quotient rounded to fp32 first.
 //
 // Bound: memory.  Every element is read once and written once: a row stays in registers between its sum and its use (8192 rows of 4096
@@ -33,10 +34,21 @@ __device__ __forceinline__ double wave_sum_d(double v) {
   return v;
 }
 
+// A row's factor as two: t, rounded, and a power of two, 1 for all but extreme rows.
+struct RowFactor {
+  float power, t;
+};
+__device__ __forceinline__ RowFactor row_factor(double mean, float eps) {
+  const double t = 1.0 / sqrt(mean + (double)eps);
+  if (t > 0x1p100) return RowFactor{0x1p60f, (float)(t * 0x1p-60)};
+  if (t < 0x1p-100) return RowFactor{0x1p-40f, (float)(t * 0x1p40)};
+  return RowFactor{1.0f, (float)t};
+}
+
 // One piece (elements idx .. idx+3 of `row`) on its way out; the 32 lanes of a half wavefront hold the 128 elements of a block.
-__device__ __forceinline__ void finish_piece(const NormParams &p, long long row, int idx, bool live, float t, f32x4 v, f32x4 g) {
+__device__ __forceinline__ void finish_piece(const NormParams &p, long long row, int idx, bool live, RowFactor f, f32x4 v, f32x4 g) {
 #pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = v[e] * t;
+  for (int e = 0; e < 4; e++) v[e] = v[e] * f.power * f.t;
   if (p.G)
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] = v[e] * g[e];
@@ -91,12 +103,12 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) void rmsnorm_rows(Nor
       for (int i = 1; i < WAVES; i++) sum += mine[i];
       __syncthreads();  // (the next row's sums go to the same places)
     }
-    const float inv = (float)(1.0 / sqrt(sum / (double)p.len + (double)p.eps));
+    const RowFactor factor = row_factor(sum / (double)p.len, p.eps);
 #pragma unroll
     for (int i = 0; i < NP; i++) {
       const int idx = 4 * (t + 64 * WAVES * i);
       if (p.S && live) store4(p.S + row * p.len, idx, p.len, v[i]);
-      finish_piece(p, row, idx, live, inv, v[i], g[i]);
+      finish_piece(p, row, idx, live, factor, v[i], g[i]);
     }
   }
 }
@@ -128,7 +140,7 @@ __global__ __launch_bounds__(256) void rmsnorm_stream(NormParams p) {
     __syncthreads();
     sum = ((part[0] + part[1]) + part[2]) + part[3];
     __syncthreads();
-    const float inv = (float)(1.0 / sqrt(sum / (double)p.len + (double)p.eps));
+    const RowFactor factor = row_factor(sum / (double)p.len, p.eps);
     for (long long idx0 = 0; idx0 < p.len; idx0 += 1024) {  // (whole wavefronts take part in a block's maximum)
       const int idx = (int)(idx0 + 4 * t < p.len ? idx0 + 4 * t : (long long)p.len);
       f32x4 v = {0.f, 0.f, 0.f, 0.f}, g = {1.f, 1.f, 1.f, 1.f};
@@ -136,7 +148,7 @@ __global__ __launch_bounds__(256) void rmsnorm_stream(NormParams p) {
         v = p.S ? load4(p.S + row * p.len, idx, p.len) : piece(idx);
         if (p.G) g = load4(p.G, idx, p.len);
       }
-      finish_piece(p, row, idx, idx < p.len, inv, v, g);
+      finish_piece(p, row, idx, idx < p.len, factor, v, g);
     }
   }
 }
