@@ -41,7 +41,7 @@ class HipTensorImpl extends TensorImpl {
       sharedBuffer.incrementRef();
       this.sharedBuffer = sharedBuffer;
     } else {
-      this.sharedBuffer = new HipSharedBuffer(context.native, this.length * ELEMENT_BYTES[this.dataType]);
+      this.sharedBuffer = new HipSharedBuffer(context.native, this.byteLength);
     }
     this.disposedFlag = false;
   }
@@ -50,6 +50,10 @@ class HipTensorImpl extends TensorImpl {
   get handle() {
     if (this.disposedFlag) throw new Error("HipTensor is already disposed");
     return this.sharedBuffer.handle;
+  }
+
+  get byteLength() {
+    return this.length * ELEMENT_BYTES[this.dataType];
   }
 
   alias(dims) {

@@ -252,7 +252,7 @@ class RunnerImpl {
         if (t.backend === "hip") {
           const own = hip.emptyTensor(t.dims, t.dataType);
           graphInputs.push(own);
-          hip.native.copy(own.handle, 0, t.handle, 0, own.length * 4);
+          hip.native.copy(own.handle, 0, t.handle, 0, own.byteLength);
         } else {
           graphInputs.push(await hip.moveTensor(t, {}));
         }
@@ -300,7 +300,7 @@ class RunnerImpl {
     for (let i = 0; i < inputs.length; i++) {
       const src = inputs[i],
         dst = state.inputs[i];
-      if (src.backend === "hip") hip.native.copy(dst.handle, 0, src.handle, 0, dst.length * 4);
+      if (src.backend === "hip") hip.native.copy(dst.handle, 0, src.handle, 0, dst.byteLength);
       else await dst.setData(await src.getData());
     }
   }
