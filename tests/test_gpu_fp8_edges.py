@@ -1,6 +1,6 @@
 """The 8-bit serving operators at operands where a definition and a shortcut part: quotients beside a tie, pages of
 values that differ in size, scales that are no numbers, scales of every size, more blocks than a launch has threads
-for, rows whose factor is no normal number."""
+for, rows whose factor is no normal number, scores beyond 2^24."""
 import numpy as np
 import pytest
 import torch
@@ -215,3 +215,34 @@ def test_norm_of_the_least_and_largest_rows(ctx, length, size):
     want = F.rms(x.astype(np.float64), g.astype(np.float64), 0.0)
     y = H.rms_normalization(ctx, ctx.move_tensor(x), ctx.move_tensor(g), epsilon=0.0).get_data()
     assert np.all(np.abs(y - want) <= 3.01 * E * np.abs(want) + 2.0 ** -149)
+
+
+# ---- scores beyond 2^24 ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("size", [1e2, 3e3, 1e4, 1e5, 1e7, 1e9, 1e14])
+@pytest.mark.parametrize("new,past,heads,kv,d", [(1, 900, 8, 2, 64), (60, 100, 4, 2, 128), (1, 3000, 2, 1, 128), (650, 100, 64, 2, 64), (700, 0, 32, 4, 128)])
+@pytest.mark.parametrize("alpha", [1.0, -0.125])
+def test_scores_of_any_size(ctx, new, past, heads, kv, d, size, alpha):
+    """Where neighbouring fp32 numbers are further apart than the powers of two that weights are, rows rest on their largest score: the others
+    are left far behind (rows whose two largest scores are not further apart than their errors are left out)."""
+    rng = np.random.default_rng(new)
+    table, lens, starts, pages = S.layout(rng, [new], [past])
+    n = int(lens[0])
+    k, v = (rng.standard_normal((n, kv, d)).astype(np.float32) for _ in range(2))
+    c = F.Cache(pages, kv, d)
+    c.append(k * np.float32(size), v, table, lens, np.array([0, n]))
+    c.ks *= rng.uniform(0.5, 1, c.ks.shape).astype(np.float32)               # (append writes powers of two, but any number will do)
+    q = (rng.standard_normal((new, heads, d)) * size).astype(np.float32)
+    keys, values = c.tokens(table[0], n)
+    got = S.attend(ctx, c, q, table, lens, starts, alpha)
+    tried = 0
+    for h in range(heads):
+        t = q[:, h].astype(np.float64) @ keys[h // (heads // kv)].T * alpha
+        t[np.arange(n) > np.arange(new)[:, None] + past] = -np.inf
+        order = np.sort(t, 1)
+        far = np.ones(new, bool) if n == 1 else order[:, -1] - order[:, -2] > 2.0 ** -15 * np.abs(q[:, h]).sum(1) * size * abs(alpha) + 30
+        if past == 0:
+            far[0] = True
+        want = values[h // (heads // kv)][t.argmax(1)]
+        assert np.all(np.abs(got[:, h] - want)[far] <= 2.0 ** -20 * np.abs(values).max()), (h, got[:, h][far])
+        tried += far.sum()
+    assert tried > 0.7 * heads * new

@@ -210,6 +210,7 @@ struct AttendParams {
 // of four pages (one for each wavefront of a workgroup) as its sequence has.  The units of all items stand in a row, and every
 // workgroup takes `share` neighbouring ones: all end at the same time, whatever the sequences' lengths.
 constexpr int MOST_UNITS = 1 << 30;
+constexpr float LARGE_SCORE = 0x1p22f;  // from here on (as powers of two) half a step of fp32 is a quarter of an exponent and more
 struct Work {
   Place s;
   int item, unit, units;  // the item, the unit of it that was asked for, and how many it has
@@ -479,7 +480,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     }
     if (more) fetch_k(then.at);
     // softmax: keys beyond the row's last, and whatever the page holds behind the sequence, count for nothing
-    const float c = p.scale * now.ks;
+    float c = p.scale * now.ks;
     float x[16], most = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; e++) x[e] = sc[e >> 2][e & 3];
@@ -502,6 +503,12 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
         for (int e = 0; e < 4; e++) o[i][e] *= back;
     }
     top = most;
+    // The largest product was rounded before it became `ref`, these are not: half a step of numbers so large is a power's worth.
+    if (__any(fabsf(ref) >= LARGE_SCORE)) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) x[e] *= c;
+      c = 1.0f;
+    }
 #pragma unroll
     for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -ref));
     if (!whole) {
@@ -888,7 +895,7 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
       if (active) {
-        const float c = fmaxf(now.ks * row_scale, FLT_MIN);  // (never 0: -inf * 0 is NaN; scores that need less are all 0 to the softmax)
+        float c = fmaxf(now.ks * row_scale, FLT_MIN);  // (never 0: -inf * 0 is NaN; scores that need less are all 0 to the softmax)
         const float mine = ceilf(most * c), up = fmaxf(mine, top), below = mine - up;  // (none seen: mine = -inf)
         const bool counts = below >= -112.0f;
         const float had = gap + (top - up), has = counts ? fmaxf(had, below + vs_exponent) : had;
@@ -902,6 +909,11 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
         }
         top = up;
         gap = has;
+        if (__any(fabsf(up) >= LARGE_SCORE && up != -FLT_MAX)) {  // (see attend_rows)
+#pragma unroll
+          for (int r = 0; r < 16; r++) sc[r] *= c;
+          c = 1.0f;
+        }
         const float weight = counts ? vs_mantissa * __builtin_amdgcn_exp2f(vs_exponent - has + 15.0f) : 0.0f;
         const f32x16 next = scores(t == 0 ? buf : next_buf, 1 - t);
 #pragma unroll
