@@ -1,6 +1,6 @@
 """The 8-bit serving operators at operands where a definition and a shortcut part: quotients beside a tie, pages of
 values that differ in size, scales that are no numbers, scales of every size, more blocks than a launch has threads
-for, rows whose factor is no normal number, scores beyond 2^24."""
+for, rows whose factor is no normal number, scores beyond 2^24, more rows than a grid has workgroups for."""
 import numpy as np
 import pytest
 import torch
@@ -246,3 +246,40 @@ def test_scores_of_any_size(ctx, new, past, heads, kv, d, size, alpha):
         assert np.all(np.abs(got[:, h] - want)[far] <= 2.0 ** -20 * np.abs(values).max()), (h, got[:, h][far])
         tried += far.sum()
     assert tried > 0.7 * heads * new
+
+
+# ---- more rows than a grid has workgroups for --------------------------------------------------------------
+@pytest.mark.parametrize("rows,length", [(4200003, 5), (1050001, 300)])
+def test_norm_of_millions_of_rows(ctx, rows, length):
+    rng = np.random.default_rng(rows)
+    x = rng.standard_normal((1000, length)).astype(np.float32)
+    dx = ctx.empty_tensor([rows, length])
+    ends = (0, rows // 2, rows - 1000)
+    for at in ends:
+        H.call("wdh_write", dx.handle, 4 * at * length, x.ctypes.data, x.nbytes)
+    y = H.rms_normalization(ctx, dx)
+    want = F.rms(x.astype(np.float64), None, 1e-5)
+    got = np.empty_like(x)
+    for at in ends:
+        H.call("wdh_read", y.handle, 4 * at * length, got.ctypes.data, got.nbytes)
+        assert np.all(np.abs(got - want) <= 3.01 * E * np.abs(want))
+    for t in (dx, y):
+        t.dispose()
+    ctx.sync()
+    capi.call("wdh_trim", 0)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4194400, 17), (2, 4200001, 16), (2200001, 3, 17), (1100003, 9, 48), (1100001, 17, 40), (300001, 200, 130), (7, 5000001, 16)])
+def test_products_of_millions_of_rows(ctx, m, n, k):
+    rng = np.random.default_rng(m + n)
+    a, w = S.bytes_of(rng, (m, k)), S.bytes_of(rng, (n, k))
+    kb = -(-k // 128)
+    sa, sw = (rng.uniform(0.5, 1, s).astype(np.float32) for s in ((m, kb), (-(-n // 128), kb)))
+    y = H.matmul_fp8(ctx, *(ctx.move_tensor(t) for t in (a, sa, w, sw))).get_data()
+    for begin in range(0, max(m, n), 500000):                                # (the oracle's 64-bit copies a piece at a time)
+        i, j = (slice(begin, begin + 500000) if side > 1000 else slice(0, side) for side in (m, n))
+        columns = slice(j.start // 128, -(-min(j.stop, n) // 128))
+        lead = j.start % 128
+        w_piece, sw_piece = w[j.start - lead:j.stop], sw[columns]
+        want, size = (t[:, lead:] for t in F.product(a[i], sa[i], w_piece, sw_piece))
+        assert np.all(np.abs(y[i, j] - want) <= (128 + 2 + kb) * 2 * E * size)
