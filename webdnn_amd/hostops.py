@@ -844,6 +844,13 @@ def _require(what, tensor, dims, data_type="float32"):
         raise OperatorError("%s: %s of shape %s expected, got %s of %s" % (what, data_type, dims, tensor.data_type, tensor.dims))
 
 
+INT32_MAX = 0x7fffffff  # (extents the library takes as C ints: ctypes would pass their low bits)
+
+
+def _too_large(what, *extents):
+    raise OperatorError("%s: an extent of %d does not fit 32 bits" % (what, max(extents)))
+
+
 def _handle(tensor):
     return tensor.handle if tensor is not None else 0
 
@@ -857,6 +864,8 @@ def _rms_rows(x, scale, skip):
         raise OperatorError("RMSNormalization: scale must have the normalised length")
     if skip is not None and skip.dims != x.dims:
         raise OperatorError("RMSNormalization: skip must have the input's shape")
+    if length > INT32_MAX:
+        _too_large("RMSNormalization", length)
     return x.length // length if length else 0, length
 
 
@@ -893,6 +902,8 @@ def quantize_fp8(ctx, x, block_rows=1, out=None):
     if block_rows not in (1, FP8_BLOCK):
         raise OperatorError("quantize_fp8: blocks of 1 or %d rows" % FP8_BLOCK)
     rows, cols = x.dims
+    if cols > INT32_MAX:
+        _too_large("quantize_fp8", cols)
     q, scales = out if out is not None else (None, None)
     q = _result(ctx, q, x.dims, "float8e4m3fn")
     scales = _result(ctx, scales, [-(-rows // block_rows), _fp8_blocks(cols)])
@@ -906,6 +917,8 @@ def matmul_fp8(ctx, a, a_scales, w, w_scales, bias=None, residual=None, epilogue
     if a.ndim != 2 or w.ndim != 2 or a.dims[1] != w.dims[1]:
         raise OperatorError("matmul_fp8: shapes %s and %s" % (a.dims, w.dims))
     (m, k), n = a.dims, w.dims[0]
+    if n > INT32_MAX or k > INT32_MAX:
+        _too_large("matmul_fp8", n, k)
     _require("matmul_fp8: a", a, [m, k], "float8e4m3fn")
     _require("matmul_fp8: w", w, [n, k], "float8e4m3fn")
     _require("matmul_fp8: a_scales", a_scales, [m, _fp8_blocks(k)])
@@ -927,6 +940,8 @@ class KvCache:
         if k.ndim != 4:
             raise OperatorError("KvCache: k is [pages, heads, %d, d]" % CACHE_PAGE)
         self.pages, self.heads, _, self.d = k.dims
+        if max(k.dims) > INT32_MAX:
+            _too_large("KvCache", *k.dims)
         _require("KvCache: k", k, [self.pages, self.heads, CACHE_PAGE, self.d], "float8e4m3fn")
         _require("KvCache: v", v, [self.pages, self.heads, self.d, CACHE_PAGE], "float8e4m3fn")
         _require("KvCache: k_scales", k_scales, [self.pages, self.heads])
@@ -949,6 +964,8 @@ def _sequences(table, lens, starts):
     _require("cache: table", table, table.dims, "int32")
     _require("cache: lens", lens, [table.dims[0]], "int32")
     _require("cache: starts", starts, [table.dims[0] + 1], "int32")
+    if table.dims[0] > INT32_MAX or table.dims[1] > INT32_MAX:
+        _too_large("cache", *table.dims)
     return table.dims
 
 
@@ -957,6 +974,8 @@ def _rows_at(what, t, columns, width):
     _require_f32(t)
     if t.ndim != 2 or columns < 0 or columns + width > t.dims[1]:
         raise OperatorError("%s: rows %s do not hold %d elements from %d on" % (what, t.dims, width, columns))
+    if t.dims[0] > INT32_MAX:
+        _too_large(what, t.dims[0])
     return t.dims[1], t.dims[0]
 
 

@@ -113,6 +113,10 @@ static napi_value make_undefined(napi_env env) {
 #define I64(i, var)                                                          \
   int64_t var;                                                               \
   if (!to_i64(env, argv[i], &var)) return throw_arg(env, FNAME, "argument " #i " (" #var ") must be an integer")
+/* (for entries whose argument is an int: nothing is cut to its low bits) */
+#define I32(i, var)                                                          \
+  I64(i, var);                                                               \
+  if (var != (int32_t)var) return throw_arg(env, FNAME, "argument " #i " (" #var ") does not fit 32 bits")
 #define F64(i, var)                                                          \
   double var;                                                                \
   if (!to_f64(env, argv[i], &var)) return throw_arg(env, FNAME, "argument " #i " (" #var ") must be a number")
@@ -404,7 +408,7 @@ FN(js_layernorm) {
 
 FN(js_rmsnorm) { /* (X, Skip, Gamma, Sum, Y, Q, QScale, outer, len, eps); 0 = absent */
   ARGS("wdh_rmsnorm", 10);
-  I64(0, X); I64(1, R); I64(2, G); I64(3, S); I64(4, Y); I64(5, Q); I64(6, QS); I64(7, outer); I64(8, len);
+  I64(0, X); I64(1, R); I64(2, G); I64(3, S); I64(4, Y); I64(5, Q); I64(6, QS); I64(7, outer); I32(8, len);
   F64(9, eps);
   CHECK(wdh_rmsnorm(X, R, G, S, Y, Q, QS, outer, (int)len, (float)eps));
   return make_undefined(env);
@@ -412,14 +416,14 @@ FN(js_rmsnorm) { /* (X, Skip, Gamma, Sum, Y, Q, QScale, outer, len, eps); 0 = ab
 
 FN(js_quantize_fp8) { /* (X, Q, QScale, rows, cols, blockRows) */
   ARGS("wdh_quantize_fp8", 6);
-  I64(0, X); I64(1, Q); I64(2, QS); I64(3, rows); I64(4, cols); I64(5, block_rows);
+  I64(0, X); I64(1, Q); I64(2, QS); I64(3, rows); I32(4, cols); I32(5, block_rows);
   CHECK(wdh_quantize_fp8(X, Q, QS, rows, (int)cols, (int)block_rows));
   return make_undefined(env);
 }
 
 FN(js_gemm_fp8) { /* (A, AScale, W, WScale, Bias, Y, m, n, k, epilogue, R) */
   ARGS("wdh_gemm_fp8", 11);
-  I64(0, A); I64(1, SA); I64(2, W); I64(3, SW); I64(4, B); I64(5, Y); I64(6, m); I64(7, n); I64(8, k); I64(9, epilogue);
+  I64(0, A); I64(1, SA); I64(2, W); I64(3, SW); I64(4, B); I64(5, Y); I64(6, m); I32(7, n); I32(8, k); I32(9, epilogue);
   I64(10, R);
   CHECK(wdh_gemm_fp8(A, SA, W, SW, B, Y, m, (int)n, (int)k, (int)epilogue, R));
   return make_undefined(env);
@@ -428,8 +432,10 @@ FN(js_gemm_fp8) { /* (A, AScale, W, WScale, Bias, Y, m, n, k, epilogue, R) */
 FN(js_cache_append) { /* (K, kOffset, kStride, V, vOffset, vStride, KPages, KScales, VPages, VScales, Table, Lens, Starts, ...) */
   ARGS("wdh_cache_append", 19);
   int64_t a[19];
-  for (int i = 0; i < 19; i++)
+  for (int i = 0; i < 19; i++) {
     if (!to_i64(env, argv[i], &a[i])) return throw_arg(env, FNAME, "integer argument expected");
+    if (i >= 13 && a[i] != (int32_t)a[i]) return throw_arg(env, FNAME, "an extent does not fit 32 bits");
+  }
   CHECK(wdh_cache_append(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], (int)a[13], (int)a[14],
                          (int)a[15], (int)a[16], (int)a[17], (int)a[18]));
   return make_undefined(env);
@@ -438,8 +444,10 @@ FN(js_cache_append) { /* (K, kOffset, kStride, V, vOffset, vStride, KPages, KSca
 FN(js_cache_attention) { /* (Q, qOffset, qStride, KPages, KScales, VPages, VScales, Table, Lens, Starts, Y, ..., alpha) */
   ARGS("wdh_cache_attention", 19);
   int64_t a[18];
-  for (int i = 0; i < 18; i++)
+  for (int i = 0; i < 18; i++) {
     if (!to_i64(env, argv[i], &a[i])) return throw_arg(env, FNAME, "integer argument expected");
+    if (i >= 11 && a[i] != (int32_t)a[i]) return throw_arg(env, FNAME, "an extent does not fit 32 bits");
+  }
   F64(18, alpha);
   CHECK(wdh_cache_attention(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], (int)a[11], (int)a[12], (int)a[13],
                             (int)a[14], (int)a[15], (int)a[16], (int)a[17], (float)alpha));
