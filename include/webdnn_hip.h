@@ -202,8 +202,8 @@ int wdh_copy(wdh_buf dst, size_t dst_offset, wdh_buf src, size_t src_offset,
              size_t bytes);
 /* The device address of a buffer, for programs that read or fill it with other libraries of the same process (a
  * torch tensor over it, say).  The library's work runs on streams of its own: wdh_sync before others read what it
- * wrote, and other streams' writes have to be over before a call of this library uses them.  The address is valid
- * until wdh_free.  No counterpart in the reference. */
+ * wrote, and other streams' writes have to be over before a call of this library uses them.  Writes through the address
+ * break the promise of WDH_CONV_CONSTANT_WEIGHTS like any other.  The address is valid until wdh_free.  No counterpart in the reference. */
 int wdh_address(wdh_buf h, uint64_t *address);
 /* Waits for the work of the current lane (see wdh_set_lane). */
 int wdh_sync(void);
@@ -537,7 +537,8 @@ int wdh_cache_append(wdh_buf K, int64_t k_offset, int64_t k_stride, wdh_buf V, i
  * tokens and tokens behind a row do not touch it, whatever they hold.  Results have the precision of fp32 relative to the
  * largest shares (weight times value) of a row, pages' scales differing as they may; weights below 2^-112 of a row's largest may
  * count for nothing.  Where one call's rows do not fill the chip the tokens
- * are cut into parts whose results are joined by a second launch, in a workspace from the pool (WDH_ENOMEM without room). */
+ * are cut into parts whose results are joined by a second launch, in a workspace from the pool (WDH_ENOMEM without room).  The
+ * form goes by seqs, tokens and max_pages: a table no wider than the longest sequence needs is the faster one. */
 int wdh_cache_attention(wdh_buf Q, int64_t q_offset, int64_t q_stride, wdh_buf KPages, wdh_buf KScales, wdh_buf VPages,
                         wdh_buf VScales, wdh_buf Table, wdh_buf Lens, wdh_buf Starts, wdh_buf Y, int seqs, int tokens,
                         int heads, int kv_heads, int d, int pages, int max_pages, float alpha);

@@ -725,7 +725,7 @@ __device__ __forceinline__ Place many_item(const AttendParams &p, int rank, int 
 
 // Bound: instructions.  A page takes 64 matrix ones of 32 cycles a wavefront and about as long of others (conversions of keys and values,
 // powers, splitting weights), which alternate more than they overlap: matrix cores busy 41 % of the time (three prompts of 1200 to 4000
-// tokens, 16 heads of 128 on 4: 250 us, 457 TFLOP/s counted once).
+// tokens, 16 heads of 128 on 4: 243 us, 469 TFLOP/s counted once).
 template <int D>
 __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   constexpr int QN = D / 32, DT = D / 32;           // runs of 32 elements of d in a key; blocks of 32 rows of O^T

@@ -7,6 +7,8 @@ export interface HipTensor extends Tensor {
   readonly backend: "hip";
   /** Buffer handle of libwebdnn_hip.so (a wdh_buf, > 0).  Throws after dispose(). */
   readonly handle: number;
+  /** Bytes of its elements: four each, one of float8e4m3fn. */
+  readonly byteLength: number;
   /** Another view of the same device buffer with other dims (Reshape, Flatten, Squeeze, Unsqueeze);
    *  the buffer is freed when the last view is disposed. */
   alias(dims: ReadonlyArray<number>): HipTensor;
