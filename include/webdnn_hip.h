@@ -543,6 +543,65 @@ int wdh_cache_attention(wdh_buf Q, int64_t q_offset, int64_t q_stride, wdh_buf K
                         wdh_buf VScales, wdh_buf Table, wdh_buf Lens, wdh_buf Starts, wdh_buf Y, int seqs, int tokens,
                         int heads, int kv_heads, int d, int pages, int max_pages, float alpha);
 
+/* ---- positions and drafted tokens ------------------------------------------
+ * No counterpart in the reference.  What a serving step needs beside the operators above: positions of queries and keys, and
+ * a pass over several drafted tokens of each sequence at once, in place of one token.  Such a step appends the drafts to the cache
+ * (wdh_cache_append_rope), attends to it as a tree (wdh_cache_attention_tree), has the target's probabilities decide (wdh_verify_drafts)
+ * and keeps the accepted ones (wdh_cache_keep).  All can be recorded; whatever is int32 on the device is read there. */
+#define WDH_DRAFT_ROWS 1024   /* rows of a sequence that are verified at a time */
+
+/* Heads normed and rotated in one pass.  Head h of row r lies at X[x_offset + r x_stride + h x_head], d elements in a row; the
+ * first `heads` heads of a row are of one kind (queries), the `k_heads` behind them of another (keys).
+ *   norm (where QGamma, KGamma [d] is given):  x = x / sqrt(mean_d(x^2) + eps) * Gamma, rounded as wdh_rmsnorm rounds
+ *   rotation: the pairs (a, b) of the first `rotary` elements, (x[j], x[j + rotary / 2]) or, interleaved, (x[2j], x[2j + 1]), become
+ *     (a cos - b sin, b cos + a sin), cos and sin from row Positions[r] (0: row r) and column j of Cos and Sin [rows, rotary / 2].
+ * The other elements stay.  rotary is even, 0 to d (0: no rotation; Cos and Sin are 0 then); d is 1 to 1024.  Y may be X in the same
+ * layout; its heads must not overlap.  A row whose position is outside the tables gets NaN in place of its rotated elements. */
+int wdh_rope(wdh_buf X, int64_t x_offset, int64_t x_stride, int64_t x_head, wdh_buf Y, int64_t y_offset, int64_t y_stride,
+             int64_t y_head, wdh_buf QGamma, wdh_buf KGamma, wdh_buf Cos, wdh_buf Sin, wdh_buf Positions, int64_t tokens, int heads,
+             int k_heads, int d, int rotary, int rows, int interleaved, float eps);
+
+/* wdh_cache_append with the keys normed (KGamma [d], 0: not) and rotated on the way, as wdh_rope would have: the cache holds what the
+ * two calls leave, without the keys' way through memory.  Positions [tokens], or 0: a token's place in its sequence. */
+int wdh_cache_append_rope(wdh_buf K, int64_t k_offset, int64_t k_stride, wdh_buf V, int64_t v_offset, int64_t v_stride,
+                          wdh_buf KPages, wdh_buf KScales, wdh_buf VPages, wdh_buf VScales, wdh_buf Table, wdh_buf Lens,
+                          wdh_buf Starts, wdh_buf KGamma, wdh_buf Cos, wdh_buf Sin, wdh_buf Positions, int seqs, int tokens,
+                          int kv_heads, int d, int pages, int max_pages, int rotary, int rows, int interleaved, float eps);
+
+/* wdh_cache_attention for rows that do not follow one another: a row sees all tokens that its sequence had before the call's, and of
+ * the call's those whose bits are set in its mask: Mask [tokens, words] (int32), bit j % 32 of word j / 32 for row j of the same sequence (a
+ * tree's row sets the bits of its ancestors and its own).  Bits of rows that the sequence does not have count for nothing, rows beyond 32
+ * words are not seen.  A row that sees nothing gets 0.  words is 1 to 2^19.  All else as in wdh_cache_attention. */
+int wdh_cache_attention_tree(wdh_buf Q, int64_t q_offset, int64_t q_stride, wdh_buf KPages, wdh_buf KScales, wdh_buf VPages,
+                             wdh_buf VScales, wdh_buf Table, wdh_buf Lens, wdh_buf Starts, wdh_buf Mask, wdh_buf Y, int seqs,
+                             int tokens, int heads, int kv_heads, int d, int pages, int max_pages, int words, float alpha);
+
+/* Which drafted tokens the target accepts.  Rows Starts[s] .. Starts[s+1]-1 (at most WDH_DRAFT_ROWS) are sequence s's tree: the first
+ * is the token that is known already, each other one a drafted token (Tokens) that follows row Parents[r] of the same sequence, which
+ * comes before it (a row whose parent does not is never reached).  P [tokens, vocab] are the target's probabilities of what follows each
+ * row; Draft [tokens, vocab] those that a row's children were drawn from, independently of each other, or 0: children were chosen, not drawn.
+ * Uniform [tokens] are numbers from [0, 1): of a drafted row for its test, of a sequence's first row for the token drawn at the end.
+ * From the first row on, with t = 0, s = 1: the row's children in order; child c of token x is accepted where
+ *   Draft:  Uniform[c] s Draft[x] < max(P[x] - t Draft[x], 0);  if not, t += s, s = sum_x max(P[x] - t Draft[x], 0)
+ *   else:   Uniform[c] s < P[x] (0 for the token of a rejected sibling);  if not, s -= P[x]
+ * and the walk goes on from there.  Where none is accepted, Next[s] is the least token at which the running sum of what is left of
+ * P (max(P - t Draft, 0); without the rejected tokens; P itself where that is nothing) passes Uniform times the whole sum.  The
+ * distribution of the accepted tokens and the next one is the target's.  In 64 bits.  Count [seqs] is how many drafts are accepted;
+ * Path [tokens] has at Starts[s] + i which row of the sequence is the path's i-th (its first row's 0 first), -1 behind the path.
+ * Negative probabilities and NaN count as 0; a token outside the vocabulary is rejected; a row whose sum is 0 or infinite gives Next -1.
+ * Results of sequences without rows, or whose rows do not fit, are left as they are. */
+int wdh_verify_drafts(wdh_buf P, wdh_buf Draft, wdh_buf Tokens, wdh_buf Parents, wdh_buf Uniform, wdh_buf Starts, wdh_buf Next,
+                      wdh_buf Count, wdh_buf Path, int seqs, int tokens, int vocab);
+
+/* Keeps a path of each sequence's last rows in the cache: with `past` tokens before the call's rows (Lens[s] less the rows), slot
+ * past + i takes what slot past + Path[Starts[s] + i] holds, for i = 0 .. Count[s] (Count and Path of wdh_verify_drafts; paths go up).  The
+ * sequence then has past + 1 + Count[s] tokens: what lies behind is left as it is, for the next call to write over.  A page's scale grows
+ * where a token comes from a page of larger scale and needs it; earlier tokens are rounded again as in wdh_cache_append.  Count beyond
+ * the rows is cut, below 0 nothing is kept; a place of the path that goes down or out of the rows, or lies on a page outside the cache, leaves
+ * its slot as it is.  A sequence's pages from `past` on must be its own. */
+int wdh_cache_keep(wdh_buf KPages, wdh_buf KScales, wdh_buf VPages, wdh_buf VScales, wdh_buf Table, wdh_buf Lens, wdh_buf Starts,
+                   wdh_buf Path, wdh_buf Count, int seqs, int tokens, int kv_heads, int d, int pages, int max_pages);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,671 @@
+"""Positions and the operators for drafted tokens on the GPU against their definitions in 64 bits (drafts_ref): rotation with and without a norm of each
+head, appending with both on the way, attention of trees over the cache, verification, keeping; their refusals; and a serving step of them
+together, recorded and not."""
+import numpy as np
+import pytest
+
+import drafts_ref as D
+import fp8_ref as F
+import test_gpu_fp8_serving as S
+from webdnn_amd import capi
+from webdnn_amd import hostops as H
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+
+
+def up(ctx, *arrays):
+    return [None if a is None else ctx.move_tensor(np.ascontiguousarray(a)) for a in arrays]
+
+
+def refused(name, *args):
+    with pytest.raises(capi.HipError) as err:
+        H.call(name, *args)
+    assert err.value.code == -2, err.value
+
+
+# ---- rotation ----------------------------------------------------------------------------------
+SIZES = [(1, 1, 0, 2, 2), (3, 2, 1, 7, 6), (5, 3, 2, 32, 32), (4, 5, 1, 33, 20), (9, 4, 4, 64, 30), (17, 12, 3, 80, 36), (70, 8, 2, 128, 128), (2, 32, 8, 128, 64),
+         (3, 3, 0, 200, 198), (5, 1, 1, 256, 256), (2, 2, 1, 300, 100), (3, 1, 1, 512, 512), (2, 1, 0, 1000, 1000), (2, 1, 1, 1024, 6), (300, 40, 8, 128, 128),
+         (40, 3, 3, 1, 0), (6, 4, 2, 96, 0)]
+
+
+@pytest.mark.parametrize("tokens,heads,k_heads,d,rotary", SIZES)
+@pytest.mark.parametrize("norm", [(False, False), (True, True), (True, False)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope(ctx, tokens, heads, k_heads, d, rotary, norm, interleaved):
+    rng = np.random.default_rng(tokens * 1009 + d * 7 + rotary)
+    x = (rng.standard_normal((tokens, heads + k_heads, d)) * np.exp(rng.standard_normal((heads + k_heads, 1)))).astype(np.float32)
+    gammas = [rng.uniform(-2, 2, d).astype(np.float32) if n else None for n in norm]
+    cos, sin = D.tables(50, rotary) if rotary else (None, None)
+    positions = rng.integers(0, 50, tokens).astype(np.int32)
+    wide = np.full((tokens, x[0].size + 9), np.nan, np.float32)             # columns 5 .. of wider rows, at any address
+    wide[:, 5:5 + x[0].size] = x.reshape(tokens, -1)
+    place = np.full((tokens, x[0].size + 4), 7.5, np.float32)
+    dx, dc, ds, dp, gq, gk, out = up(ctx, wide, cos, sin, positions, *gammas, place)
+    H.rotary_embedding(ctx, dx, dc, ds, dp, heads, d, k_heads, gq, gk, interleaved, 1e-6, column=5, out=out, out_column=3)
+    got = out.get_data()
+    assert np.all(got[:, :3] == 7.5) and np.all(got[:, 3 + x[0].size:] == 7.5)
+    got = got[:, 3:3 + x[0].size].reshape(x.shape)
+    for part, gamma in ((slice(0, heads), gammas[0]), (slice(heads, None), gammas[1])):
+        want, bound = D.rope(x[:, part], gamma, cos, sin, positions, interleaved, 1e-6)
+        assert np.all(np.abs(got[:, part] - want) <= bound), float(np.max(np.abs(got[:, part] - want) - bound))
+        if gamma is None:
+            assert np.array_equal(got[:, part, rotary:], x[:, part, rotary:])
+    # in place, and without positions: the rows' own numbers
+    if tokens <= 50:
+        H.rotary_embedding(ctx, dx, dc, ds, None, heads, d, k_heads, gq, gk, interleaved, 1e-6, column=5, out=dx, out_column=5)
+        got = dx.get_data()
+        assert np.isnan(got[:, :5]).all() and np.isnan(got[:, 5 + x[0].size:]).all()
+        got = got[:, 5:5 + x[0].size].reshape(x.shape)
+        for part, gamma in ((slice(0, heads), gammas[0]), (slice(heads, None), gammas[1])):
+            want, bound = D.rope(x[:, part], gamma, cos, sin, np.arange(tokens), interleaved, 1e-6)
+            assert np.all(np.abs(got[:, part] - want) <= bound)
+
+
+def test_rope_of_heads_before_tokens(ctx):
+    """[heads, tokens, d] in, [tokens, heads, d] out, and back; one row read for all tokens."""
+    rng = np.random.default_rng(4)
+    tokens, heads, d = 6, 5, 48
+    x = rng.standard_normal((tokens, heads, d)).astype(np.float32)
+    cos, sin = D.tables(6, 16)
+    dx, dc, ds, y, z = up(ctx, x.transpose(1, 0, 2), cos, sin, np.zeros((tokens, heads, d), np.float32), np.zeros((heads, tokens, d), np.float32))
+    want, bound = D.rope(x, None, cos, sin, np.arange(6), False, 0.0)
+    tail = (0, 0, dc.handle, ds.handle, 0, tokens, heads, 0, d, 16, 6, 0, 0.0)
+    H.call("wdh_rope", dx.handle, 0, d, tokens * d, y.handle, 0, heads * d, d, *tail)
+    assert np.all(np.abs(y.get_data() - want) <= bound)
+    H.call("wdh_rope", dx.handle, 0, d, tokens * d, z.handle, 0, d, tokens * d, *tail)
+    assert np.array_equal(z.get_data().transpose(1, 0, 2), y.get_data())
+    H.call("wdh_rope", dx.handle, d, 0, tokens * d, y.handle, 0, heads * d, d, *tail)
+    want, bound = D.rope(np.repeat(x[1:2], tokens, 0), None, cos, sin, np.arange(6), False, 0.0)
+    assert np.all(np.abs(y.get_data() - want) <= bound)
+
+
+def test_rope_of_extreme_rows_and_positions(ctx):
+    """Heads of zeros, of squares beyond and below fp32's range, with an infinity or a NaN; positions outside the tables."""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((8, 1, 64)).astype(np.float32)
+    x[0], x[1], x[2] = 0, x[1] * np.float32(1e25), x[2] * np.float32(1e-30)
+    x[3, 0, 60], x[4, 0, 61] = np.inf, np.nan
+    cos, sin = D.tables(9, 32)
+    positions = np.array([1, 8, 3, 4, 5, 9, -1, 1 << 30], np.int32)
+    gamma = rng.uniform(0.5, 1.5, 64).astype(np.float32)
+    dx, dc, ds, dp, dg = up(ctx, x.reshape(8, 64), cos, sin, positions, gamma)
+    got = H.rotary_embedding(ctx, dx, dc, ds, dp, 1, 64, q_scale=dg, epsilon=0.0).get_data().reshape(x.shape)
+    want, bound = D.rope(x, gamma, cos, sin, positions, False, 0.0)
+    for r in (1, 2):
+        assert np.all(np.abs(got[r] - want[r]) <= bound[r]), r
+    assert np.isnan(got[0]).all() and np.isnan(got[4]).all()
+    assert np.isnan(got[3, 0, 60]) and np.all(got[3, 0, np.arange(64) != 60] == 0)
+    for r in (5, 6, 7):
+        assert np.isnan(got[r, 0, :32]).all() and np.all(np.abs(got[r, 0, 32:] - want[r, 0, 32:]) <= bound[r, 0, 32:])
+
+
+def test_rope_without_rows(ctx):
+    y = H.rotary_embedding(ctx, ctx.empty_tensor([0, 64]), None, None, None, 2, 32)
+    assert y.get_data().shape == (0, 64)
+    y = H.rotary_embedding(ctx, ctx.empty_tensor([3, 64]), None, None, None, 0, 32)
+    assert y.get_data().shape == (3, 0)
+
+
+# ---- append ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,d,rotary", [(1, 32, 32), (3, 64, 22), (2, 128, 128), (2, 128, 0)])
+@pytest.mark.parametrize("new,past", S.MIXES)
+@pytest.mark.parametrize("norm,interleaved,given", [(True, False, False), (False, True, True), (True, True, True)])
+def test_append_rope(ctx, heads, d, rotary, new, past, norm, interleaved, given):
+    """What wdh_rope and wdh_cache_append leave, bit for bit."""
+    rng = np.random.default_rng(sum(new) * 131 + d)
+    table, lens, starts, pages = S.layout(rng, new, past)
+    n, width = int(starts[-1]), heads * d
+    c = F.Cache(pages, heads, d)
+    one, two = S.on_device(ctx, c), S.on_device(ctx, c)
+    begin = np.concatenate([[0], np.cumsum(past)]).astype(np.int32)
+    old = rng.standard_normal((int(begin[-1]), width)).astype(np.float32)
+    dt, dl, ds = up(ctx, table, lens, starts)
+    for device in (one, two):
+        H.cache_append(ctx, device, *up(ctx, old, old[::-1]), dt, *up(ctx, np.array(past, np.int32), begin))
+    kv = rng.standard_normal((n, 2 * width + 8)).astype(np.float32) * np.float32(5)
+    if n > 2:
+        kv[n // 2, 5], kv[n // 3, width + 9] = np.inf, np.nan
+    place = np.concatenate([np.arange(p, p + m) for m, p in zip(new, past)]).astype(np.int32)
+    at = rng.integers(-1, 250, n).astype(np.int32) if given else place
+    cos, sin = D.tables(400, rotary) if rotary else (None, None)
+    gamma = rng.uniform(0.5, 2, d).astype(np.float32) if norm else None
+    dkv, dp, dc, dn, dg = up(ctx, kv, at, cos, sin, gamma)
+    H.cache_append_rotary(ctx, one, dkv, dkv, dt, dl, ds, dc, dn, dp if given else None, dg, interleaved, 1e-6, k_column=4, v_column=8 + width)
+    turned = H.rotary_embedding(ctx, dkv, dc, dn, dp, heads, d, 0, dg, None, interleaved, 1e-6, column=4)
+    H.cache_append(ctx, two, turned, dkv, dt, dl, ds, v_column=8 + width)
+    for a, b in ((one.k, two.k), (one.k_scales, two.k_scales), (one.v, two.v), (one.v_scales, two.v_scales)):
+        assert np.array_equal(a.get_data(), b.get_data(), equal_nan=True)
+
+
+# ---- attention of trees --------------------------------------------------------------------------
+def attend_tree(ctx, c, q, table, lens, starts, mask, alpha, out=None, wide=0):
+    n, heads, d = q.shape
+    rows = np.full((n, heads * d + 2 * wide), np.nan, np.float32)
+    rows[:, wide:wide + heads * d] = q.reshape(n, -1)
+    dq, dt, dl, ds, dm = up(ctx, rows, table, lens, starts, mask)
+    y = H.cache_attention_tree(ctx, S.on_device(ctx, c), dq, heads, alpha, dt, dl, ds, dm, q_column=wide, out=out)
+    return y.get_data().reshape(n, heads, d)
+
+
+def masks(rng, new, words, kind):
+    rows = []
+    for n in new:
+        if kind == "tree":
+            m = D.unpack(H.tree_mask(D.tree(rng, n, 3), np.array([0, n])), n)[:, :n]
+        elif kind == "random":
+            m = rng.random((n, n)) < 0.3
+        else:
+            m = np.zeros((n, n), bool)
+        rows += list(m)
+    return rows, D.pack(rows, words)
+
+
+@pytest.mark.parametrize("heads,kv,d", [(1, 1, 32), (8, 1, 64), (6, 2, 128), (4, 4, 128), (40, 2, 64), (3, 1, 128)])
+@pytest.mark.parametrize("new,past", [([1], [0]), ([5, 1, 3], [0, 63, 500]), ([7, 12, 2], [61, 64, 700]), ([100, 1, 65, 7], [0, 130, 64, 1000]), ([33], [3000]),
+                                      ([32, 31], [32, 33]), ([130], [190])])
+@pytest.mark.parametrize("kind", ["tree", "random"])
+def test_attention_of_trees(ctx, heads, kv, d, new, past, kind):
+    rng = np.random.default_rng(heads * 1009 + sum(past) + d)
+    c, table, lens, starts = S.filled(rng, new, past, kv, d)
+    q = rng.standard_normal((int(starts[-1]), heads, d)).astype(np.float32)
+    sees, mask = masks(rng, new, -(-max(new) // 32) + len(new) % 2, kind)
+    alpha = np.float32(d ** -0.5)
+    want, bound = D.attention(c, q, table, lens, starts, sees, float(alpha))
+    got = attend_tree(ctx, c, q, table, lens, starts, mask, alpha, wide=4 * (len(new) % 2))
+    assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) - bound))
+
+
+# (calls with enough rows for the forms that share pages: many tokens, many heads, a long past)
+@pytest.mark.parametrize("heads,kv,d,new,past", [(32, 2, 128, [64], [9000]), (64, 2, 64, [130, 40], [100, 900]), (32, 8, 128, [32] * 10, list(range(0, 1000, 100))),
+                                                (64, 4, 32, [64] * 8, [65] * 8), (16, 4, 64, [8] * 40, list(range(0, 400, 10))), (8, 8, 128, [60] * 6, [500] * 6),
+                                                (64, 4, 128, [64] * 6, [100, 0, 64, 1, 300, 20])])
+def test_attention_of_large_trees(ctx, heads, kv, d, new, past):
+    rng = np.random.default_rng(heads + sum(past) + d)
+    c, table, lens, starts = S.filled(rng, new, past, kv, d)
+    q = rng.standard_normal((int(starts[-1]), heads, d)).astype(np.float32)
+    sees, mask = masks(rng, new, -(-max(new) // 32), "tree")
+    want, bound = D.attention(c, q, table, lens, starts, sees, 0.1)
+    got = attend_tree(ctx, c, q, table, lens, starts, mask, 0.1)
+    assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) - bound))
+
+
+@pytest.mark.parametrize("heads,new,past", [(4, [5, 40, 3], [0, 0, 70]), (32, [200, 100], [0, 64])])
+def test_masks_that_leave_nothing_or_name_rows_that_are_not_there(ctx, heads, new, past):
+    """Empty masks, bits behind a sequence's rows, and rows beyond the masks' words."""
+    rng = np.random.default_rng(8)
+    c, table, lens, starts = S.filled(rng, new, past, 2, 64)
+    q = rng.standard_normal((sum(new), heads, 64)).astype(np.float32)
+    sees, _ = masks(rng, new, 1, "none")
+    got = attend_tree(ctx, c, q, table, lens, starts, D.pack(sees, 2), 0.125)
+    want, bound = D.attention(c, q, table, lens, starts, sees, 0.125)
+    assert np.all(np.abs(got - want) <= bound)
+    for s in range(len(new)):
+        if past[s] == 0:
+            assert np.all(got[starts[s]:starts[s + 1]] == 0)
+    got = attend_tree(ctx, c, q, table, lens, starts, np.full((sum(new), 1), -1, np.int32), 0.125)     # the first 32 rows, whoever they are
+    for n, at in zip(new, starts):
+        for r in range(n):
+            sees[at + r] = np.arange(n) < 32
+    want, bound = D.attention(c, q, table, lens, starts, sees, 0.125)
+    assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("heads,new", [(4, [50]), (32, [200])])
+def test_nan_in_rows_that_are_not_seen(ctx, heads, new):
+    """Tokens of the tree whose keys or values hold NaN: rows that do not see them are what they are without."""
+    rng = np.random.default_rng(9)
+    kv, d, past = 2, 64, 30
+    c, table, lens, starts = S.filled(rng, new, [past], kv, d)
+    q = rng.standard_normal((new[0], heads, d)).astype(np.float32)
+    sees, mask = masks(rng, new, -(-new[0] // 32), "tree")
+    want, bound = D.attention(c, q, table, lens, starts, sees, 0.125)
+    hit = 7
+    page, slot = table[0, (past + hit) // 64], (past + hit) % 64
+    c.v[page, 0, 5, slot] = 0x7f
+    c.k[page, 1, slot, 9] = 0xff
+    got = attend_tree(ctx, c, q, table, lens, starts, mask, 0.125)
+    sure = np.array([row[hit] for row in sees])
+    assert sure.any() and not sure.all()
+    assert np.all(np.abs(got - want)[~sure] <= bound[~sure])
+    group = heads // kv
+    assert np.isnan(got[sure][:, :group, 5]).all() and np.isnan(got[sure][:, group:]).all()
+    rest = np.arange(d) != 5
+    assert np.all((np.abs(got - want) <= bound)[sure][:, :group][..., rest])
+
+
+@pytest.mark.parametrize("heads,new", [(4, [50]), (32, [200])])
+@pytest.mark.parametrize("scale", [None, 0.0, np.inf, np.nan])
+def test_a_page_without_a_place_or_a_scale(ctx, heads, new, scale):
+    """A page of the tree: rows that see none of its tokens are what they are without; all rows for a page of the past."""
+    rng = np.random.default_rng(10)
+    c, table, lens, starts = S.filled(rng, new, [100], 1, 64)
+    q = rng.standard_normal((new[0], heads, 64)).astype(np.float32)
+    sees, mask = masks(rng, new, -(-new[0] // 32), "random")
+    for r in range(0, new[0], 2):
+        sees[r][28:] = False                                              # tokens 128 .. are page 2
+    mask = D.pack(sees, mask.shape[1])
+    want, bound = D.attention(c, q, table, lens, starts, sees, 0.125)
+    which = 2
+    if scale is None:
+        table[0, which] = 1 << 20
+    else:
+        c.vs[table[0, which], 0] = scale
+    got = attend_tree(ctx, c, q, table, lens, starts, mask, 0.125)
+    sure = np.array([np.asarray(row)[28:92].any() for row in sees])
+    assert sure.any() and not sure.all()
+    assert np.isnan(got[sure]).all() and np.all(np.abs(got - want)[~sure] <= bound[~sure])
+    table[0, 0] = -1
+    assert np.isnan(attend_tree(ctx, c, q, table, lens, starts, mask, 0.125)).all()
+
+
+def test_rows_of_no_sequence_stay_as_they_are(ctx):
+    rng = np.random.default_rng(12)
+    c, table, lens, starts = S.filled(rng, [1, 4, 2, 3], [70, 0, 9, 64], 2, 32)
+    starts = np.concatenate([starts, [starts[-1]]]).astype(np.int32)
+    table, lens = np.concatenate([table, table[:1]]), np.append(lens, 0).astype(np.int32)
+    q = rng.standard_normal((16, 4, 32)).astype(np.float32)
+    sees = [np.arange(4) <= 1] * 16
+    want, bound = D.attention(c, q[:10], table, lens, starts, sees, 0.2)
+    lens[1], lens[3] = 3, 1000
+    got = attend_tree(ctx, c, q, table, lens, starts, D.pack(sees, 1), 0.2, out=ctx.move_tensor(np.full((16, 4 * 32), 7.5, np.float32)))
+    for a, b in ((0, 1), (5, 7)):
+        assert np.all(np.abs(got[a:b] - want[a:b]) <= bound[a:b])
+    for a, b in ((1, 5), (7, 16)):
+        assert np.all(got[a:b] == 7.5)
+
+
+def test_a_chain_is_causal_attention(ctx):
+    """Masks of chains give what wdh_cache_attention gives, within both bounds."""
+    rng = np.random.default_rng(13)
+    c, table, lens, starts = S.filled(rng, [20, 70], [100, 5], 2, 128)
+    q = rng.standard_normal((90, 8, 128)).astype(np.float32)
+    mask = H.tree_mask(np.concatenate([np.arange(-1, 19), np.arange(-1, 69)]), starts)
+    want, bound = c.attention(q, table, lens, starts, 0.1)
+    got = attend_tree(ctx, c, q, table, lens, starts, mask, 0.1)
+    assert np.all(np.abs(got - want) <= bound)
+
+
+# ---- verification ----------------------------------------------------------------------------------
+def drafts(rng, new, vocab, most_children, drawn, near=0.7):
+    """Trees of tokens with the probabilities they are verified with."""
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    parents = np.concatenate([D.tree(rng, n, most_children) if n else np.zeros(0, np.int32) for n in new])
+    rows = len(parents)
+    soft = lambda x: np.exp(x) / np.exp(x).sum(1, keepdims=True)
+    logits = rng.standard_normal((rows, vocab)) * 2
+    p, draft = soft(logits).astype(np.float32), soft(logits + rng.standard_normal((rows, vocab)) * near).astype(np.float32)
+    tokens = np.zeros(rows, np.int32)
+    taken = {}
+    for s in range(len(new)):
+        for r in range(1, int(new[s])):
+            row, above = starts[s] + r, starts[s] + parents[starts[s] + r]
+            if drawn:
+                tokens[row] = min(np.searchsorted(np.cumsum(draft[above].astype(np.float64)), rng.random()), vocab - 1)
+            else:
+                order = np.argsort(-draft[above], kind="stable")
+                tokens[row] = order[taken.setdefault(above, 0) % vocab]
+                taken[above] += 1
+    return p, draft, tokens, parents, rng.random(rows).astype(np.float32), starts
+
+
+def check_verify(ctx, p, draft, tokens, parents, uniform, starts):
+    want = D.verify(p, draft, tokens, parents, uniform, starts)
+    dp, dt, da, du, ds, dd = up(ctx, p, tokens, parents, uniform, starts, draft)
+    seqs = len(starts) - 1
+    out = up(ctx, *(np.full(n, -7, np.int32) for n in (seqs, seqs, len(tokens))))
+    H.verify_drafts(ctx, dp, dt, da, du, ds, dd, out)
+    got = [t.get_data() for t in out]
+    for name, g, w in zip(("next", "count", "path"), got, want):
+        assert np.array_equal(g, w), (name, g, w)
+    return got
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 5, 255, 256, 1000, 4097, 30522])
+@pytest.mark.parametrize("new,most_children", [([1], 1), ([2], 1), ([5, 1, 8], 1), ([9, 33, 2], 3), ([70, 129, 3, 1], 4), ([30] * 20, 2)])
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify(ctx, vocab, new, most_children, drawn):
+    rng = np.random.default_rng(vocab * 31 + sum(new))
+    p, draft, *rest = drafts(rng, new, vocab, most_children, drawn)
+    check_verify(ctx, p, draft if drawn else None, *rest)
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify_where_all_or_none_pass(ctx, drawn):
+    rng = np.random.default_rng(3)
+    p, draft, tokens, parents, uniform, starts = drafts(rng, [12, 20], 5000, 3, drawn)
+    first = [0, 12]
+    for u in (0.0, 1 - 2.0 ** -24):
+        numbers = np.full(32, u, np.float32)
+        numbers[first] = (0.0, 1 - 2.0 ** -24)                                # the first token that can be drawn, and the last
+        next_, count, path = check_verify(ctx, p, draft if drawn else None, tokens, parents, numbers, starts)
+        if u == 0:
+            depth = lambda s, r: 0 if r <= 0 else 1 + depth(s, parents[starts[s] + r])
+            assert all(depth(s, int(path[starts[s] + count[s]])) == count[s] > 0 for s in range(2))
+    same = check_verify(ctx, p, p if drawn else None, tokens, parents, uniform, starts)   # drafts from the target itself
+    if drawn:
+        assert np.all(same[1] > 0)
+
+
+def test_verify_of_exact_sums(ctx):
+    """Probabilities that are powers of two: tests and draws that fall on their borders."""
+    p = np.zeros((6, 8), np.float32)
+    p[:] = [0.25, 0, 0.125, 0.125, 0.25, 0, 0.25, 0]
+    draft = np.full((6, 8), 0.125, np.float32)
+    parents, tokens = np.array([-1, 0, 0, 0, 1, 2], np.int32), np.array([0, 2, 1, 4, 6, 0], np.int32)
+    for numbers in ([0.25, 0.99, 0, 0.5, 0, 0], [0.5, 1 - 2.0 ** -24, 0.0, 0.999, 0, 0], [0.75, 0.125, 0.5, 0.25, 0.5, 0], [0.0, 0.25, 0, 0, 0.25, 0],
+                    [0.625, 0.875, 0.5, 0.5, 0.9, 0.9], [1 - 2.0 ** -24, 0.125, 0.9, 0.9, 0.25, 0.9]):
+        u = np.array(numbers, np.float32)
+        for d in (draft, None):
+            check_verify(ctx, p, d, tokens, parents, u, np.array([0, 6], np.int32))
+    # the same token twice among siblings, and rows that nothing is left of
+    twice = np.array([0, 2, 2, 2, 6, 0], np.int32)
+    one = np.zeros((6, 8), np.float32)
+    one[:, 2] = 1
+    for table in (p, one):
+        for d in (draft, one, None):
+            for u in (0.05, 0.2, 0.999):
+                check_verify(ctx, table, d, twice, parents, np.full(6, u, np.float32), np.array([0, 6], np.int32))
+
+
+def test_verify_of_what_is_no_probability(ctx):
+    """Negative numbers and NaN count as 0; a row of zeros or with an infinity gives -1; tokens outside the vocabulary and rows that do not follow an
+    earlier one are never accepted; sequences without rows, with too many or outside the call are left out."""
+    rng = np.random.default_rng(6)
+    p, draft, tokens, parents, uniform, starts = drafts(rng, [3, 3, 1, 1, 6, 4], 700, 2, False)
+    uniform[:] = 0.3
+    p[starts[0]:starts[1], ::3] = -1
+    p[starts[1]:starts[2], ::3] = np.nan
+    p[starts[2]], p[starts[3], 5] = 0, np.inf
+    tokens[starts[4] + 1:starts[4] + 4] = (-1, 700, 1 << 30)
+    parents[starts[5] + 1:starts[5] + 4] = (1, 3, -5)
+    got = check_verify(ctx, p, None, tokens, parents, uniform, starts)
+    assert got[0][2] == -1 and got[0][3] == -1 and got[1][5] == 0
+    dp, dt, da, du = up(ctx, p, tokens, parents, uniform)
+    odd = np.array([0, 3, 3, 2, 100, -4, 5], np.int32)                        # whole; empty; backwards; beyond; back; from before the call
+    out = up(ctx, *(np.full(n, -7, np.int32) for n in (6, 6, len(tokens))))
+    H.verify_drafts(ctx, dp, dt, da, du, *up(ctx, odd), out=out)
+    next_, count, path = (t.get_data() for t in out)
+    assert next_[0] == got[0][0] and np.all(next_[1:] == -7) and np.all(count[1:] == -7)
+    assert np.array_equal(path[:3], got[2][:3]) and np.all(path[3:] == -7)
+    # the most rows that a sequence may have, and one more
+    n = 1024
+    p, draft, tokens, parents, uniform, _ = drafts(rng, [2 * n + 1], 40, 6, False)
+    parents[n:] = np.concatenate([[-1], parents[1:n + 1]])
+    starts = np.array([0, n, 2 * n + 1], np.int32)
+    want = D.verify(p[:n], None, tokens[:n], parents[:n], uniform[:n], starts[:2])
+    out = up(ctx, *(np.full(k, -7, np.int32) for k in (2, 2, len(tokens))))
+    H.verify_drafts(ctx, *up(ctx, p, tokens, parents, uniform, starts), out=out)
+    got = [t.get_data() for t in out]
+    assert got[0][0] == want[0][0] and got[1][0] == want[1][0] and np.array_equal(got[2][:n], want[2])
+    assert got[0][1] == -7 and got[1][1] == -7 and np.all(got[2][n:] == -7)
+
+
+# ---- keeping -----------------------------------------------------------------------------------------
+def random_path(rng, parents):
+    """A path of rows from the first one on, and how many drafts it has."""
+    node, walk = 0, [0]
+    while True:
+        below = [i for i in range(len(parents)) if parents[i] == node]
+        if not below or (len(walk) > 1 and rng.random() < 0.1):
+            return walk
+        node = below[rng.integers(0, len(below))]
+        walk.append(node)
+
+
+@pytest.mark.parametrize("heads,d", [(1, 32), (3, 64), (2, 128)])
+@pytest.mark.parametrize("new,past", [([1], [0]), ([4], [63]), ([7, 1, 12], [0, 62, 200]), ([130, 9, 64, 5], [0, 0, 64, 61]), ([9] * 70, list(range(0, 140, 2))), ([150], [33])])
+@pytest.mark.parametrize("most_children", [1, 3])
+def test_keep(ctx, heads, d, new, past, most_children):
+    rng = np.random.default_rng(sum(new) * 17 + d)
+    table, lens, starts, pages = S.layout(rng, new, past)
+    c = F.Cache(pages, heads, d)
+    for ls, st, n in ((np.array(past, np.int32), np.concatenate([[0], np.cumsum(past)]), sum(past)), (lens, starts, sum(new))):
+        k, v = (rng.standard_normal((n, heads, d)).astype(np.float32) * 2.0 ** rng.integers(-6, 6, (n, 1, 1)).astype(np.float32) for _ in range(2))
+        c.append(k.astype(np.float32), v.astype(np.float32), table, ls, st)
+    device = S.on_device(ctx, c)
+    path, count = np.full(sum(new), -1, np.int32), np.zeros(len(new), np.int32)
+    for s, n in enumerate(new):
+        walk = random_path(rng, D.tree(rng, n, most_children))
+        path[starts[s]:starts[s] + len(walk)], count[s] = walk, len(walk) - 1
+    H.cache_keep(ctx, device, *up(ctx, table, lens, starts, path, count))
+    D.keep(c, table, lens, starts, path, count)
+    S.check_cache(device, c)
+
+
+def test_keep_of_what_does_not_fit(ctx):
+    """Paths that go down or out of the rows, pages outside the cache, counts below 0 and beyond the rows, sequences that do not fit."""
+    rng = np.random.default_rng(3)
+    new, past = [10, 70, 5, 6, 4, 3], [60, 20, 0, 0, 64, 10]
+    table, lens, starts, pages = S.layout(rng, new, past)
+    c = F.Cache(pages, 2, 64)
+    for ls, st, n in ((np.array(past, np.int32), np.concatenate([[0], np.cumsum(past)]), sum(past)), (lens, starts, sum(new))):
+        c.append(*(rng.standard_normal((n, 2, 64)).astype(np.float32) * np.float32(9) ** rng.integers(-1, 2, (n, 1, 1)).astype(np.float32) for _ in range(2)), table, ls, st)
+    device = S.on_device(ctx, c)
+    path, count = np.full(sum(new), -1, np.int32), np.array([4, 30, -1, 100, 2, 2], np.int32)
+    path[:5] = (0, 3, 2, 12, 9)                       # (row 2 stays, row 12 is not there)
+    path[10:41] = np.sort(rng.choice(np.arange(1, 70), 31, replace=False))
+    path[starts[2]:starts[2] + 5] = (0, 3, 4, -1, -1)
+    path[starts[3]:starts[3] + 6] = (0, 2, 4, 5, -1, 1 << 30)
+    path[starts[4]:starts[4] + 3] = (0, 2, 3)
+    path[starts[5]:starts[5] + 3] = (1, 2, 2)
+    bad = table.copy()
+    bad[1, 1] = pages + 5                             # the second sequence's tokens from its slot 64 on
+    bad[4, 1] = -3
+    lens = lens.copy()
+    lens[5] = 2                                       # fewer tokens than rows
+    H.cache_keep(ctx, device, *up(ctx, bad, lens, starts, path, count))
+    count[2], count[5] = -1, -1
+    D.keep(c, bad, lens, starts, path, count)
+    S.check_cache(device, c)
+
+
+def test_keep_of_the_largest_numbers(ctx):
+    """Keys near fp32's largest, whose e4m3 values stand for more than that, move to a page of smaller ones."""
+    k = np.full((66, 1, 32), 1.0, np.float32)
+    k[65] = np.float32(3.4e38)
+    table, lens, starts = np.array([[0, 1]], np.int32), np.array([66], np.int32), np.array([0, 66], np.int32)
+    c = F.Cache(2, 1, 32)
+    c.append(k, k, table, lens, starts)
+    device = S.on_device(ctx, c)
+    lens, starts, path, count = lens, np.array([0, 4], np.int32), np.array([0, 3, -1, -1], np.int32), np.array([1], np.int32)
+    H.cache_keep(ctx, device, *up(ctx, table, lens, starts, path, count))
+    D.keep(c, table, lens, starts, path, count)
+    S.check_cache(device, c)
+
+
+# ---- refusals -----------------------------------------------------------------------------------
+def test_refusals(ctx):
+    f, i, e = lambda *s: ctx.empty_tensor(s), lambda *s: ctx.empty_tensor(s, "int32"), lambda *s: ctx.empty_tensor(s, "float8e4m3fn")
+    h = lambda t: t.handle
+    x, y, cos, sin, at, gamma = f(4, 128), f(4, 128), f(9, 32), f(9, 32), i(4), f(64)
+
+    def rope(X=x, xo=0, xs=128, xh=64, Y=y, yo=0, ys=128, yh=64, qg=0, kg=0, c=h(cos), s=h(sin), p=h(at), tokens=4, heads=1, k_heads=1, d=64, rotary=64, rows=9,
+             inter=0, eps=1e-6):
+        return h(X), xo, xs, xh, h(Y), yo, ys, yh, qg, kg, c, s, p, tokens, heads, k_heads, d, rotary, rows, inter, eps
+
+    H.call("wdh_rope", *rope())
+    for bad in (dict(tokens=5), dict(tokens=-1), dict(heads=-1), dict(d=0), dict(d=1025), dict(rotary=63), dict(rotary=66), dict(rotary=-2), dict(c=0), dict(s=0),
+                dict(rotary=0), dict(rows=10), dict(rows=-1), dict(eps=-1.0), dict(eps=float("nan")), dict(xs=-128), dict(yo=-1), dict(yo=1), dict(xo=1), dict(ys=127),
+                dict(yh=63), dict(yh=0), dict(ys=0), dict(X=y, xo=0, xs=128, xh=0), dict(X=y, yo=0, xo=64), dict(qg=h(y)), dict(qg=h(at)), dict(kg=12345678), dict(p=h(y)),
+                dict(tokens=1 << 40), dict(heads=1 << 20), dict(xs=1 << 60), dict(p=h(i(3)))):
+        refused("wdh_rope", *rope(**bad))
+
+    cache = H.KvCache.empty(ctx, 4, 2, 64)
+    table, lens, starts, k = i(3, 2), i(3), i(4), f(5, 128)
+    kv = [h(t) for t in (cache.k, cache.k_scales, cache.v, cache.v_scales, table, lens, starts)]
+    tail = (3, 5, 2, 64, 4, 2)
+
+    def append(g=0, c=h(cos), s=h(sin), p=0, rotary=64, rows=9, eps=1e-6, kx=h(k), tail=tail):
+        return (kx, 0, 128, h(k), 0, 128, *kv, g, c, s, p, *tail, rotary, rows, 0, eps)
+
+    for t in (table, lens, starts):
+        t.set_data(np.zeros(t.dims, np.int32))
+    H.call("wdh_cache_append_rope", *append())
+    for bad in (dict(g=h(f(63))), dict(c=0), dict(rotary=0), dict(rotary=66), dict(rotary=7), dict(rows=10), dict(rows=-1), dict(eps=float("nan")), dict(p=h(i(4))),
+                dict(g=kv[1]), dict(c=kv[1], rows=0), dict(kx=h(f(4, 128))), dict(tail=(3, 5, 2, 48, 4, 2)), dict(tail=(4, 5, 2, 64, 4, 2)), dict(tail=(3, 5, 2, 64, 5, 2))):
+        refused("wdh_cache_append_rope", *append(**bad))
+
+    q, yy, mask = f(5, 256), f(5, 256), i(5, 2)
+
+    def tree(m=h(mask), out=h(yy), heads=4, words=2, seqs=3, tokens=5):
+        return (h(q), 0, 256, *kv, m, out, seqs, tokens, heads, 2, 64, 4, 2, words, 1.0)
+
+    H.call("wdh_cache_attention_tree", *tree())
+    for bad in (dict(words=3), dict(words=0), dict(words=-1), dict(words=1 << 20), dict(m=0), dict(m=h(yy)), dict(out=h(mask)), dict(out=h(q)), dict(heads=5), dict(heads=0),
+                dict(seqs=4), dict(tokens=6)):
+        refused("wdh_cache_attention_tree", *tree(**bad))
+
+    p, d, u, t, par, st, nx, co, pa = f(6, 50), f(6, 50), f(6), i(6), i(6), i(3), i(2), i(2), i(6)
+    st.set_data(np.zeros(3, np.int32))
+
+    def verify(P=h(p), Dr=h(d), T=h(t), A=h(par), U=h(u), St=h(st), N=h(nx), C=h(co), Pa=h(pa), seqs=2, tokens=6, vocab=50):
+        return P, Dr, T, A, U, St, N, C, Pa, seqs, tokens, vocab
+
+    H.call("wdh_verify_drafts", *verify())
+    for bad in (dict(P=0), dict(vocab=51), dict(vocab=0), dict(vocab=-1), dict(tokens=7), dict(tokens=-1), dict(seqs=3), dict(seqs=-1), dict(N=h(co)), dict(Pa=h(t)),
+                dict(C=h(st)), dict(U=h(nx)), dict(Dr=h(f(5, 50))), dict(A=0), dict(N=0), dict(vocab=(1 << 30) + 1), dict(tokens=(1 << 24) + 1)):
+        refused("wdh_verify_drafts", *verify(**bad))
+
+    path, count = i(5), i(3)
+    path.set_data(np.zeros(5, np.int32))
+    count.set_data(np.zeros(3, np.int32))
+
+    def keep(Pa=h(path), C=h(count), KS=kv[1], seqs=3, tokens=5, d=64, pages=4, most=2):
+        return (kv[0], KS, *kv[2:], Pa, C, seqs, tokens, 2, d, pages, most)
+
+    H.call("wdh_cache_keep", *keep())
+    for bad in (dict(Pa=0), dict(C=0), dict(Pa=kv[1]), dict(KS=kv[3]), dict(tokens=6), dict(seqs=4), dict(d=48), dict(pages=5), dict(most=3), dict(tokens=-1),
+                dict(C=h(i(2)))):
+        refused("wdh_cache_keep", *keep(**bad))
+
+
+# ---- together ------------------------------------------------------------------------------------
+class Layer:
+    """Attention of a serving step with drafts: one projection's rows in, the heads' results out."""
+
+    def __init__(self, ctx, rng, heads, kv, d, positions):
+        self.ctx, self.heads, self.kv, self.d = ctx, heads, kv, d
+        self.cos, self.sin = up(ctx, *D.tables(positions, d))
+        self.gq, self.gk = up(ctx, *(rng.uniform(0.5, 1.5, d).astype(np.float32) for _ in range(2)))
+
+    def run(self, qkv, cache, table, lens, starts, positions, mask):
+        ctx, hd = self.ctx, self.heads * self.d
+        q = H.rotary_embedding(ctx, qkv, self.cos, self.sin, positions, self.heads, self.d, q_scale=self.gq, epsilon=1e-6)
+        H.cache_append_rotary(ctx, cache, qkv, qkv, table, lens, starts, self.cos, self.sin, positions, self.gk, epsilon=1e-6, k_column=hd,
+                              v_column=hd + self.kv * self.d)
+        return H.cache_attention_tree(ctx, cache, q, self.heads, self.d ** -0.5, table, lens, starts, mask)
+
+
+def step(ctx, layer, s, cache):
+    """Append and attend, verify, keep, and the next step's lengths and positions, all on the device."""
+    y = layer.run(s["qkv"], cache, s["table"], s["lens"], s["starts"], s["positions"], s["mask"])
+    token, count, path = H.verify_drafts(ctx, s["p"], s["tokens"], s["parents"], s["uniform"], s["starts"], s["draft"], s.get("out"))
+    H.cache_keep(ctx, cache, s["table"], s["lens"], s["starts"], path, count)
+    more = H.binary(ctx, "Add", s["lens"], count)                      # lens - n + 1 + count tokens are kept, and n come next
+    lens = H.binary(ctx, "Add", more, s["one"])
+    positions = H.binary(ctx, "Add", H.gather(ctx, H.binary(ctx, "Sub", lens, s["rows"]), s["row_seq"]), s["depth"])
+    return y, token, count, path, lens, positions
+
+
+def start(ctx, rng, layer, new, past, vocab, drawn):
+    seqs, n = len(new), sum(new)
+    table, lens, starts, pages = S.layout(rng, [m + 60 for m in new], past)
+    lens = (lens - 60).astype(np.int32)
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    parents = np.concatenate([D.tree(rng, m, 2) for m in new])
+    depth = np.zeros(n, np.int32)
+    row_seq = np.repeat(np.arange(seqs), new).astype(np.int32)
+    for r in range(n):
+        if parents[r] >= 0:
+            depth[r] = depth[starts[row_seq[r]] + parents[r]] + 1
+    host = dict(table=table, lens=lens, starts=starts, parents=parents, depth=depth, row_seq=row_seq, one=np.ones(seqs, np.int32), rows=np.array(new, np.int32),
+                positions=(np.array(past)[row_seq] + depth).astype(np.int32), mask=H.tree_mask(parents, starts))
+    return host, pages
+
+
+def fresh_rows(rng, layer, host, vocab, drawn):
+    n = len(host["parents"])
+    p, draft, tokens, _, uniform, _ = drafts(rng, np.diff(host["starts"]), vocab, 2, drawn, near=0.3)
+    tokens = rng.integers(0, vocab, n).astype(np.int32)
+    tokens[rng.random(n) < 0.6] = 0
+    p[:, 0] += 2
+    p /= p.sum(1, keepdims=True)
+    return dict(qkv=rng.standard_normal((n, (layer.heads + 2 * layer.kv) * layer.d)).astype(np.float32), p=p, draft=draft if drawn else None, tokens=tokens, uniform=uniform)
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+def test_steps_with_drafts(ctx, drawn):
+    """Three steps over two sequences' trees: each operator against its definition, on what the one before it left."""
+    rng = np.random.default_rng(40)
+    layer = Layer(ctx, rng, 4, 2, 64, 400)
+    host, pages = start(ctx, rng, layer, [12, 7], [120, 50], 300, drawn)
+    c = F.Cache(pages, layer.kv, layer.d)
+    old = rng.standard_normal((170, layer.kv, layer.d)).astype(np.float32)
+    c.append(old, old, host["table"], np.array([120, 50]), np.array([0, 120, 170]))
+    cache = S.on_device(ctx, c)
+    accepted = 0
+    for turn in range(3):
+        host.update(fresh_rows(rng, layer, host, 300, drawn))
+        s = {k: up(ctx, v)[0] for k, v in host.items()}
+        n, hd, kd = len(host["parents"]), layer.heads * layer.d, layer.kv * layer.d
+        y, token, count, path, lens, positions = (t.get_data() for t in step(ctx, layer, s, cache))
+        rows = host["qkv"]
+        cos, sin = layer.cos.get_data(), layer.sin.get_data()
+        q, _ = D.rope(rows[:, :hd].reshape(n, layer.heads, layer.d), layer.gq.get_data(), cos, sin, host["positions"], False, 1e-6)
+        turned = H.rotary_embedding(ctx, s["qkv"], layer.cos, layer.sin, s["positions"], layer.kv, layer.d, q_scale=layer.gk, epsilon=1e-6, column=hd)
+        k, _ = D.rope(rows[:, hd:hd + kd].reshape(n, layer.kv, layer.d), layer.gk.get_data(), cos, sin, host["positions"], False, 1e-6)
+        assert np.all(np.abs(turned.get_data().reshape(k.shape) - k) <= 8 * E * (np.abs(k).max(-1, keepdims=True) * 2))   # (a rotated pair is as long as it was)
+        c.append(turned.get_data().reshape(k.shape), rows[:, hd + kd:].reshape(n, layer.kv, layer.d), host["table"], host["lens"], host["starts"])
+        q32 = H.rotary_embedding(ctx, s["qkv"], layer.cos, layer.sin, s["positions"], layer.heads, layer.d, q_scale=layer.gq, epsilon=1e-6).get_data()
+        want, bound = D.attention(c, q32.reshape(q.shape), host["table"], host["lens"], host["starts"], D.unpack(host["mask"], n), layer.d ** -0.5)
+        assert np.all(np.abs(y.reshape(want.shape) - want) <= bound)
+        found = D.verify(host["p"], host["draft"], host["tokens"], host["parents"], host["uniform"], host["starts"])
+        for got, w in zip((token, count, path), found):
+            assert np.array_equal(got, w)
+        D.keep(c, host["table"], host["lens"], host["starts"], path, count)
+        S.check_cache(cache, c)
+        assert np.array_equal(lens, host["lens"] + 1 + count)
+        host.update(lens=lens, positions=positions)
+        assert np.array_equal(positions, (lens - host["rows"])[host["row_seq"]] + host["depth"])
+        accepted += int(count.sum())
+    assert accepted > 0
+
+
+def test_a_recorded_step_follows_its_sequences(ctx):
+    """Recorded once, replayed with other rows, probabilities and lengths in the same buffers; every replay against the call-by-call run."""
+    rng = np.random.default_rng(41)
+    layer = Layer(ctx, rng, 8, 2, 128, 2000)
+    host, pages = start(ctx, rng, layer, [20, 9, 15], [900, 62, 130], 3000, True)
+    caches = []
+    old = rng.standard_normal((1092, layer.kv * layer.d)).astype(np.float32)
+    for _ in range(2):
+        caches.append(S.on_device(ctx, F.Cache(pages, layer.kv, layer.d)))
+        H.cache_append(ctx, caches[-1], *up(ctx, old, old, host["table"], np.array([900, 62, 130], np.int32), np.array([0, 900, 962, 1092], np.int32)))
+    host.update(fresh_rows(rng, layer, host, 3000, True))
+    s = {k: up(ctx, v)[0] for k, v in host.items()}
+    spare = S.on_device(ctx, F.Cache(pages, layer.kv, layer.d))
+    for t in step(ctx, layer, s, spare):                              # (the first run fills the pool)
+        t.dispose()
+    ctx.sync()
+    ctx.graph_begin()
+    out = step(ctx, layer, s, caches[0])
+    graph = ctx.graph_end()
+    try:
+        for turn in range(4):
+            host.update(fresh_rows(rng, layer, host, 3000, True))
+            for name in ("qkv", "p", "draft", "tokens", "uniform", "lens", "positions"):
+                s[name].set_data(host[name])
+            ctx.graph_launch(graph)
+            got = [t.get_data() for t in out]
+            want = step(ctx, layer, s, caches[1])
+            for a, b in zip(got, want):
+                assert np.array_equal(a, b.get_data()), turn
+                b.dispose()
+            for a, b in zip(vars(caches[0]).items(), vars(caches[1]).items()):
+                if isinstance(a[1], H.HipTensor):
+                    assert np.array_equal(a[1].get_data(), b[1].get_data(), equal_nan=True), (turn, a[0])
+            host.update(lens=got[4], positions=got[5])
+    finally:
+        ctx.graph_destroy(graph)

@@ -82,6 +82,11 @@ SIGNATURES = {
     "wdh_gemm_fp8": (_c.c_int, [c_buf] * 6 + [_c.c_int64, _c.c_int, _c.c_int, _c.c_int, c_buf]),
     "wdh_cache_append": (_c.c_int, [c_buf, _c.c_int64, _c.c_int64, c_buf, _c.c_int64, _c.c_int64] + [c_buf] * 7 + [_c.c_int] * 6),
     "wdh_cache_attention": (_c.c_int, [c_buf, _c.c_int64, _c.c_int64] + [c_buf] * 8 + [_c.c_int] * 7 + [_c.c_float]),
+    "wdh_rope": (_c.c_int, [c_buf, _c.c_int64, _c.c_int64, _c.c_int64] * 2 + [c_buf] * 5 + [_c.c_int64] + [_c.c_int] * 6 + [_c.c_float]),
+    "wdh_cache_append_rope": (_c.c_int, [c_buf, _c.c_int64, _c.c_int64] * 2 + [c_buf] * 11 + [_c.c_int] * 9 + [_c.c_float]),
+    "wdh_cache_attention_tree": (_c.c_int, [c_buf, _c.c_int64, _c.c_int64] + [c_buf] * 9 + [_c.c_int] * 8 + [_c.c_float]),
+    "wdh_verify_drafts": (_c.c_int, [c_buf] * 9 + [_c.c_int] * 3),
+    "wdh_cache_keep": (_c.c_int, [c_buf] * 9 + [_c.c_int] * 6),
 }
 
 

@@ -1,0 +1,403 @@
+// What comes after a forward pass over drafted tokens: which of them the target's probabilities accept, and keeping those in the cache.
+//
+// The reference has no such operators.
+//
+// Verification.  A sequence's rows are a tree, parents first; p_c is the target's distribution behind row c, and its children's tokens were
+// drawn one by one and independently from q_c.  At node c the first child is accepted with probability min(1, p/q) of its token, and
+// after each rejection p gives way to its normed part above q.  Since max(max(a, 0) - b, 0) = max(a - b, 0) for b >= 0, what is left of p after k
+// rejections is
+//   r_k(x) = max(p(x) - t_k q(x), 0),  s_k = sum_x r_k(x),  t_0 = 0, s_0 = 1, t_{k+1} = t_k + s_k:
+// one number for all of a row's history, so that a test needs two elements (u s_k q(x) < r_k(x)), and a rejection one pass over two rows.
+// Drafts that were chosen, not drawn (no q), are accepted with their share of what is left, u s < p(x); a rejected one is taken out: s -= p(x).
+// Where no child is accepted a token is drawn from what is left, by its cumulative sum.  A token so found has the target's distribution.
+// All of it in 64 bits, sums in a fixed order: the token drawn goes by where a sum passes a number.
+#include "common.h"
+#include "fp8.h"
+#include "kv_cache.h"
+
+namespace {
+
+using namespace wdh::fp8;
+using namespace wdh::kv;
+using wdh::fail;
+
+constexpr int MOST_ROWS = WDH_DRAFT_ROWS;
+
+struct VerifyParams {
+  const float *P, *Q, *U;
+  const int *tokens, *parents, *starts;
+  int *next, *count, *path;
+  int seqs, rows, vocab;
+};
+
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+// Sums over the lanes up to and with each.
+__device__ __forceinline__ double wave_scan_d(double v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const double below = __shfl_up(v, off, 64);
+    if (lane >= off) v += below;
+  }
+  return v;
+}
+
+// What is left of a row: of elements idx .. idx+3, 0 behind `end`.  Negative numbers and NaN count as 0.
+struct Rest {
+  const float *p, *q;      // (q null: nothing but the taken-out tokens is missing)
+  double t;
+  const int *out;          // tokens that are taken out
+  int outs, vocab;
+};
+__device__ __forceinline__ void rest4(const Rest &r, int idx, int end, double (&v)[4]) {
+  const f32x4 p = load4(r.p, idx, end);
+  const f32x4 q = r.q ? load4(r.q, idx, end) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = fmax((double)p[e] - r.t * (double)q[e], 0.0);
+  for (int i = 0; i < r.outs; i++) {
+    const int at = r.out[i] - idx;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (at == e) v[e] = 0.0;
+  }
+}
+// Sum of elements lo .. hi-1, by a wavefront.
+__device__ __forceinline__ double wave_rest(const Rest &r, int lo, int hi) {
+  double sum = 0.0;
+#pragma unroll 4
+  for (int idx = lo + 4 * (int)(threadIdx.x & 63); idx < hi; idx += 256) {
+    double v[4];
+    rest4(r, idx, hi, v);
+    sum += (v[0] + v[1]) + (v[2] + v[3]);
+  }
+  return wave_sum_d(sum);
+}
+
+constexpr int WAVES = 16;
+// The sixteenth of lo .. hi-1 that is `i`'s, in whole turns of a wavefront.
+__device__ __forceinline__ int part_begin(int lo, int hi, int i) {
+  const int each = ((hi - lo + WAVES - 1) / WAVES + 255) / 256 * 256;
+  const long long at = lo + (long long)each * i;
+  return at < hi ? (int)at : hi;
+}
+// The sums of all sixteen; their sum in order.
+__device__ __forceinline__ double parts_of(const Rest &r, int lo, int hi, double *sums) {
+  const int wave = threadIdx.x >> 6;
+  const double mine = wave_rest(r, part_begin(lo, hi, wave), part_begin(lo, hi, wave + 1));
+  __syncthreads();  // (who still reads the sums before)
+  if ((threadIdx.x & 63) == 0) sums[wave] = mine;
+  __syncthreads();
+  double total = 0.0;
+#pragma unroll
+  for (int i = 0; i < WAVES; i++) total += sums[i];
+  return total;
+}
+// The part in which the running sum, `base` before the first, passes `target`, else the last that is not empty; base moves on.
+__device__ __forceinline__ int part_of(const double *sums, double target, double &base) {
+  int last = 0;
+  double before = base, last_before = base;
+  for (int i = 0; i < WAVES; i++) {
+    if (sums[i] > 0.0) last = i, last_before = before;
+    if (before + sums[i] > target) break;
+    before += sums[i];
+  }
+  base = last_before;
+  return last;
+}
+
+// A workgroup to a sequence.  Bound: the pass over a row of one workgroup.
+__global__ __launch_bounds__(64 * WAVES) void verify_drafts(VerifyParams a) {
+  __shared__ int parent[MOST_ROWS], token[MOST_ROWS], path[MOST_ROWS], out[MOST_ROWS];
+  __shared__ float px[MOST_ROWS], qx[MOST_ROWS], us[MOST_ROWS];
+  __shared__ double sums[WAVES];
+  __shared__ int found;
+  const int seq = blockIdx.x, row0 = a.starts[seq], tid = threadIdx.x, lane = tid & 63;
+  const long long rows = (long long)a.starts[seq + 1] - row0;
+  if (row0 < 0 || rows <= 0 || rows > MOST_ROWS || row0 + rows > a.rows) return;
+  const int n = (int)rows;
+  for (int i = tid; i < MOST_ROWS; i += 64 * WAVES) {
+    const int up = i < n ? a.parents[row0 + i] : -1, x = i < n ? a.tokens[row0 + i] : 0;
+    const bool below = i > 0 && up >= 0 && up < i, real = below && x >= 0 && x < a.vocab;
+    const long long at = ((long long)row0 + (real ? up : 0)) * a.vocab + (real ? x : 0);
+    parent[i] = below ? up : -1;
+    token[i] = x;
+    px[i] = real ? a.P[at] : 0.0f;
+    qx[i] = real && a.Q ? a.Q[at] : 0.0f;
+    us[i] = i < n ? a.U[row0 + i] : 0.0f;
+  }
+  __syncthreads();
+  // All wavefronts take the same walk.
+  int node = 0, taken = 0;
+  Rest rest;
+  double mass;
+  bool summed;
+  for (bool walking = true; walking;) {
+    if (tid == 0) path[taken] = node;
+    rest = Rest{a.P + ((long long)row0 + node) * a.vocab, nullptr, 0.0, out, 0, a.vocab};
+    mass = 1.0;
+    summed = false;
+    walking = false;
+    for (int base = node / 64 * 64; base < n && !walking; base += 64) {
+      unsigned long long children = __ballot(parent[base + lane] == node);
+      while (children) {
+        const int child = base + __ffsll(children) - 1;
+        children &= children - 1;
+        const double u = us[child], likely = a.Q ? (double)qx[child] : 1.0;
+        double left = fmax((double)px[child] - rest.t * likely, 0.0);
+        if (!a.Q) {
+          left = fmax((double)px[child], 0.0);
+          for (int i = 0; i < rest.outs; i++)
+            if (out[i] == token[child]) left = 0.0;
+        }
+        if (u * mass * likely < left) {
+          node = child;
+          taken++;
+          walking = true;
+          break;
+        }
+        if (a.Q) {
+          rest.q = a.Q + ((long long)row0 + node) * a.vocab;
+          rest.t += mass;
+          mass = parts_of(rest, 0, a.vocab, sums);
+          summed = true;
+        } else {
+          mass -= left;
+          __syncthreads();  // (who still reads the list)
+          if (tid == 0) out[rest.outs] = token[child];
+          rest.outs++;
+          __syncthreads();
+        }
+      }
+    }
+  }
+  // a token from what is left of the last row, or, if that is nothing, from the row
+  double total = summed ? mass : parts_of(rest, 0, a.vocab, sums);
+  if (!(total > 0.0) && (rest.outs || rest.q)) {
+    rest.outs = 0;
+    rest.q = nullptr;
+    rest.t = 0.0;
+    total = parts_of(rest, 0, a.vocab, sums);
+  }
+  if (tid == 0) found = -1;
+  __syncthreads();
+  if (total > 0.0 && total <= DBL_MAX) {
+    const double target = (double)us[0] * total;
+    double base = 0.0;
+    int part = part_of(sums, target, base);
+    int lo = part_begin(0, a.vocab, part), hi = part_begin(0, a.vocab, part + 1);
+    parts_of(rest, lo, hi, sums);
+    part = part_of(sums, target, base);
+    const int begin = part_begin(lo, hi, part), end = part_begin(lo, hi, part + 1);
+    if (tid < 64) {
+      int at = -1;
+      bool done = false;
+      for (int turn = begin; turn < end && !done; turn += 256) {
+        const int idx = turn + 4 * lane;
+        double v[4] = {0.0, 0.0, 0.0, 0.0};
+        if (idx < end) rest4(rest, idx, end, v);
+        const double mine = (v[0] + v[1]) + (v[2] + v[3]), upto = wave_scan_d(mine);
+        double before = base + (upto - mine);
+        int first = -1, last = -1;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          before += v[e];
+          if (v[e] > 0.0) {
+            last = idx + e;
+            if (first < 0 && before > target) first = idx + e;
+          }
+        }
+        const unsigned long long passed = __ballot(first >= 0), some = __ballot(last >= 0);
+        if (passed) {
+          at = __shfl(first, __ffsll(passed) - 1, 64);
+          done = true;
+        } else if (some) {
+          at = __shfl(last, 63 - __clzll(some), 64);  // (the last so far: what is found if rounding leaves the sum short)
+        }
+        base += __shfl(upto, 63, 64);
+      }
+      if (lane == 0) found = at;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += 64 * WAVES) a.path[row0 + i] = i <= taken ? path[i] : -1;
+  if (tid == 0) {
+    a.next[seq] = found;
+    a.count[seq] = taken;
+  }
+}
+
+// ---- keeping accepted tokens -------------------------------------------------------------------
+struct KeepParams {
+  Sequences q;
+  const int *path, *count;
+  unsigned char *KP, *VP;
+  float *KS, *VS;
+  int heads;
+};
+
+// Tokens of a path go behind each other: slot past + i takes what slot past + path[i] holds, which is never before it.  So a workgroup has a
+// sequence's pages of one head, keys (blockIdx.z 0) or values, and goes over them in order; what a page takes is in registers before any of
+// it is written, and what later pages take lies behind.  Bound: latency.
+template <int D>
+__global__ __launch_bounds__(256) void cache_keep(KeepParams p) {
+  constexpr int NP = PAGE * D / 4 / 256, PPT = D / 4;
+  __shared__ float part[4], scale_of[PAGE];
+  __shared__ long long from[PAGE];   // where a slot's token comes from: page cell * 64 + slot
+  const Place s = sequence(p.q, blockIdx.x);
+  if (s.n == 0) return;
+  const int given = p.count[s.seq], kept = given < 0 ? 0 : given < s.n - 1 ? given + 1 : s.n, past = s.len - s.n;
+  if (kept == 0) return;
+  const bool values = blockIdx.z;
+  const int head = blockIdx.y, t = threadIdx.x;
+  unsigned char *pages = values ? p.VP : p.KP;
+  float *scales = values ? p.VS : p.KS;
+  const int *table = p.q.table + (long long)s.seq * p.q.max_pages;
+  for (int pi = past / PAGE; pi <= (past + kept - 1) / PAGE; pi++) {
+    const int id = table[pi];
+    if (id < 0 || id >= p.q.pages) continue;
+    const long long at = (long long)id * p.heads + head;
+    const int first = past > pi * PAGE ? past - pi * PAGE : 0, last = past + kept - pi * PAGE < PAGE ? past + kept - pi * PAGE : PAGE;
+    bool moves = false;
+    __syncthreads();  // (the page before is done with the list)
+    if (t < PAGE) {
+      long long cell = at;
+      int slot = t;
+      if (t >= first && t < last) {
+        const int i = pi * PAGE + t - past, j = p.path[s.row0 + i];
+        if (j > i && j < s.n) {
+          const int there = table[(past + j) / PAGE];
+          if (there >= 0 && there < p.q.pages) {
+            cell = (long long)there * p.heads + head;
+            slot = (past + j) % PAGE;
+            moves = true;
+          }
+        }
+      }
+      from[t] = cell * PAGE + slot;
+      scale_of[t] = scales[cell];
+    }
+    if (!__syncthreads_or(moves)) continue;
+    unsigned char *page = pages + at * (PAGE * D);
+    f32x4 v[NP];
+    int old[NP];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int w = t + 256 * i, s0 = values ? w % (PAGE / 4) * 4 : w / PPT;
+      old[i] = s0 < last ? reinterpret_cast<const int *>(page)[w] : 0;
+      v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      int q = 0;
+      if (!values) {
+        if (s0 < first || s0 >= last) continue;
+        q = *reinterpret_cast<const int *>(pages + from[s0] * D + w % PPT * 4);
+      } else {
+        if (s0 + 4 <= first || s0 >= last) continue;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const long long f = from[s0 + e];
+          if (s0 + e >= first && s0 + e < last) q |= (int)pages[f / PAGE * (PAGE * D) + w / (PAGE / 4) * PAGE + f % PAGE] << (8 * e);
+        }
+      }
+      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(q, true);
+      v[i] = f32x4{a[0], a[1], b[0], b[1]};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {  // (a value that was rounded up may stand for more than fp32 holds; fmaxf passes NaN by)
+        const float x = fabsf(v[i][e] * scale_of[values ? s0 + e : s0]);
+        amax = fmaxf(amax, x > FLT_MAX ? FLT_MAX : x);
+      }
+    }
+    const float had = scales[at];
+    amax = wdh::rowmath::wave_max(amax);
+    if ((t & 63) == 0) part[t >> 6] = amax;
+    __syncthreads();
+    const float c = fmaxf(had, page_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])))), inv = 1.0f / c, factor = had / c;
+    const bool grown = c != had;
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int w = t + 256 * i, s0 = values ? w % (PAGE / 4) * 4 : w / PPT;
+      int *to = reinterpret_cast<int *>(page) + w;
+      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+      if (s0 < last)
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = v[i][e] * (scale_of[values ? s0 + e : s0] * inv);
+      if (!values) {
+        if (s0 >= first && s0 < last) *to = pack4(y, 1.0f);
+        else if (s0 < first && grown) *to = rescale4(old[i], factor);
+      } else if (s0 < last && (s0 + 4 > first || grown)) {
+        *to = merge4(old[i], pack4(y, 1.0f), first - s0, last - s0, grown, factor);
+      }
+    }
+    if (t == 0 && grown) scales[at] = c;
+  }
+}
+
+}  // namespace
+
+extern "C" int wdh_verify_drafts(wdh_buf hP, wdh_buf hDraft, wdh_buf hTokens, wdh_buf hParents, wdh_buf hUniform, wdh_buf hStarts, wdh_buf hNext,
+                                 wdh_buf hCount, wdh_buf hPath, int seqs, int tokens, int vocab) {
+  WDH_REQUIRE_INIT();
+  WDH_REQUIRE_COMPUTE_LANE();
+  if (seqs < 0 || tokens < 0 || vocab < 0) return fail(WDH_EINVAL, "wdh_verify_drafts: negative extent");
+  if (tokens > (1 << 24) || seqs > (1 << 20)) return fail(WDH_EINVAL, "wdh_verify_drafts: too many tokens or sequences");
+  if (vocab > (1 << 30)) return fail(WDH_EINVAL, "wdh_verify_drafts: a vocabulary of %d tokens (at most %d)", vocab, 1 << 30);
+  if (seqs == 0 || tokens == 0) return WDH_OK;
+  if (vocab == 0) return fail(WDH_EINVAL, "wdh_verify_drafts: an empty vocabulary");
+  void *pp, *pd = nullptr, *pt, *pa, *pu, *ps, *pn, *pc, *ph;
+  const size_t rows = (size_t)tokens * 4;
+  if (!wdh::operand(hP, rows * vocab, "wdh_verify_drafts: P", &pp)) return WDH_EINVAL;
+  if (hDraft && !wdh::operand(hDraft, rows * vocab, "wdh_verify_drafts: Draft", &pd)) return WDH_EINVAL;
+  if (!wdh::operand(hTokens, rows, "wdh_verify_drafts: Tokens", &pt) || !wdh::operand(hParents, rows, "wdh_verify_drafts: Parents", &pa) ||
+      !wdh::operand(hUniform, rows, "wdh_verify_drafts: Uniform", &pu) ||
+      !wdh::operand(hStarts, ((size_t)seqs + 1) * 4, "wdh_verify_drafts: Starts", &ps) ||
+      !wdh::operand(hNext, (size_t)seqs * 4, "wdh_verify_drafts: Next", &pn) ||
+      !wdh::operand(hCount, (size_t)seqs * 4, "wdh_verify_drafts: Count", &pc) || !wdh::operand(hPath, rows, "wdh_verify_drafts: Path", &ph))
+    return WDH_EINVAL;
+  const wdh_buf out[3] = {hNext, hCount, hPath}, in[6] = {hP, hDraft, hTokens, hParents, hUniform, hStarts};
+  for (int i = 0; i < 3; i++) {
+    for (wdh_buf h : in)
+      if (out[i] == h) return fail(WDH_EINVAL, "wdh_verify_drafts: a result aliases an input");
+    for (int j = 0; j < i; j++)
+      if (out[i] == out[j]) return fail(WDH_EINVAL, "wdh_verify_drafts: two results share a buffer");
+  }
+  const VerifyParams p = {(const float *)pp, (const float *)pd, (const float *)pu, (const int *)pt, (const int *)pa, (const int *)ps,
+                          (int *)pn, (int *)pc, (int *)ph, seqs, tokens, vocab};
+  hipLaunchKernelGGL(verify_drafts, dim3((unsigned)seqs), dim3(64 * WAVES), 0, wdh::stream(), p);
+  WDH_LAUNCH_CHECK();
+  return WDH_OK;
+}
+
+extern "C" int wdh_cache_keep(wdh_buf hKP, wdh_buf hKS, wdh_buf hVP, wdh_buf hVS, wdh_buf hTable, wdh_buf hLens, wdh_buf hStarts, wdh_buf hPath,
+                              wdh_buf hCount, int seqs, int tokens, int kv_heads, int d, int pages, int max_pages) {
+  WDH_REQUIRE_INIT();
+  WDH_REQUIRE_COMPUTE_LANE();
+  const char *who = "wdh_cache_keep";
+  if (int rc = check_cache(who, seqs, tokens, kv_heads, d, pages, max_pages)) return rc;
+  if (seqs == 0 || tokens == 0 || pages == 0 || max_pages == 0) return WDH_OK;
+  KeepParams p;
+  void *kp, *ks, *vp, *vs, *path, *count;
+  if (int rc = cache_operands(who, hKP, hKS, hVP, hVS, hTable, hLens, hStarts, seqs, kv_heads, d, pages, max_pages, &kp, &ks, &vp, &vs, &p.q)) return rc;
+  if (!wdh::operand(hPath, (size_t)tokens * 4, "wdh_cache_keep: Path", &path) || !wdh::operand(hCount, (size_t)seqs * 4, "wdh_cache_keep: Count", &count))
+    return WDH_EINVAL;
+  const wdh_buf out[4] = {hKP, hKS, hVP, hVS}, in[5] = {hTable, hLens, hStarts, hPath, hCount};
+  for (int i = 0; i < 4; i++) {
+    for (wdh_buf h : in)
+      if (out[i] == h) return fail(WDH_EINVAL, "%s: a part of the cache aliases an input", who);
+    for (int j = 0; j < i; j++)
+      if (out[i] == out[j]) return fail(WDH_EINVAL, "%s: two parts of the cache share a buffer", who);
+  }
+  p.q.tokens = tokens;
+  p.path = (const int *)path;
+  p.count = (const int *)count;
+  p.KP = (unsigned char *)kp; p.KS = (float *)ks; p.VP = (unsigned char *)vp; p.VS = (float *)vs;
+  p.heads = kv_heads;
+  const dim3 grid((unsigned)seqs, (unsigned)kv_heads, 2);
+  if (d == 32) hipLaunchKernelGGL((cache_keep<32>), grid, dim3(256), 0, wdh::stream(), p);
+  else if (d == 64) hipLaunchKernelGGL((cache_keep<64>), grid, dim3(256), 0, wdh::stream(), p);
+  else hipLaunchKernelGGL((cache_keep<128>), grid, dim3(256), 0, wdh::stream(), p);
+  WDH_LAUNCH_CHECK();
+  return WDH_OK;
+}

@@ -7,76 +7,17 @@
 // (what the second product of attention reads along is contiguous), each with one scale: element = e4m3 value * scale.
 // Scales are powers of two: when a later token outgrows its page, the earlier ones are scaled down without another rounding
 // (but for those that leave the range of normal e4m3 numbers).
-#include <stdio.h>
-
 #include "common.h"
 #include "fastdiv.h"
 #include "fp8.h"
+#include "kv_cache.h"
+#include "rope.h"
 
 namespace {
 
 using namespace wdh::fp8;
-
-constexpr int PAGE = 64;
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef int i32x2 __attribute__((ext_vector_type(2)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-
-// Which tokens of a call belong to which sequence, and where the sequences lie in the cache.
-struct Sequences {
-  const int *table;   // [seqs, max_pages]
-  const int *lens;    // [seqs], the tokens of the call counted
-  const int *starts;  // [seqs + 1]
-  int seqs, tokens, max_pages, pages;
-};
-struct Place {
-  int seq, row0, n, len, index;  // rows row0 .. row0+n-1 of the call are the last n of the sequence's len tokens
-};
-
-// A sequence's rows; n = 0 for one that has none, whose numbers do not fit the call or the table, or that is not there.
-__device__ __forceinline__ Place sequence(const Sequences &q, int s) {
-  Place p = {s, 0, 0, 0, 0};
-  if (s >= q.seqs) return p;
-  p.row0 = q.starts[s];
-  p.len = q.lens[s];
-  const long long n = (long long)q.starts[s + 1] - p.row0;
-  const bool fits = p.row0 >= 0 && n > 0 && p.row0 + n <= q.tokens && n <= p.len && p.len <= (long long)q.max_pages * PAGE;
-  p.n = fits ? (int)n : 0;
-  return p;
-}
-
-// Sums over the lanes up to and with each: shifts within rows of 16, then the last lanes of rows 0 and 2, and of row 1, into
-// those behind them.  They end at the largest int (sequences that contradict each other can claim more rows than the call has).
-__device__ __forceinline__ int add_sat(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ int dpp_add(int v) {
-  return add_sat(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false));
-}
-__device__ __forceinline__ int wave_scan(int v) {
-  v = dpp_add<0x111, 0xf>(v);
-  v = dpp_add<0x112, 0xf>(v);
-  v = dpp_add<0x114, 0xf>(v);
-  v = dpp_add<0x118, 0xf>(v);
-  v = dpp_add<wdh::rowmath::DPP_BCAST15, 0xa>(v);
-  return dpp_add<wdh::rowmath::DPP_BCAST31, 0xc>(v);
-}
-// The sequence that holds work item `item` when each has count(place) of them in turn, and which of its items that is; n = 0
-// behind the last.  Whole wavefronts call this: they look at 64 sequences side by side.
-template <class Count>
-__device__ __forceinline__ Place locate(const Sequences &q, int item, Count count) {
-  for (int i = 0; i < (q.seqs + 63) / 64; i++) {
-    const Place mine = sequence(q, 64 * i + (int)(threadIdx.x & 63));
-    const int items = mine.n ? count(mine) : 0, upto = wave_scan(items);
-    const unsigned long long has = __ballot(item < upto);
-    if (has) {
-      const int at = __ffsll(has) - 1;
-      return Place{__builtin_amdgcn_readlane(mine.seq, at), __builtin_amdgcn_readlane(mine.row0, at), __builtin_amdgcn_readlane(mine.n, at),
-                   __builtin_amdgcn_readlane(mine.len, at), item - __builtin_amdgcn_readlane(upto - items, at)};
-    }
-    item -= __builtin_amdgcn_readlane(upto, 63);
-  }
-  return Place{0, 0, 0, 0, 0};
-}
+using namespace wdh::kv;
+using wdh::fail;
 
 // ---- append --------------------------------------------------------------------------------
 struct AppendParams {
@@ -86,38 +27,18 @@ struct AppendParams {
   unsigned char *KP, *VP;
   float *KS, *VS;
   int heads;
+  // keys that are normed and rotated on the way
+  const float *gamma;    // (null: not normed)
+  const int *positions;  // (null: a token's place in its sequence)
+  wdh::rope::Rotation turn;
+  float eps;
 };
-
-// The least power of two c >= 2^-100 with amax <= 448 c (448 = 0.875 * 2^9).
-__device__ __forceinline__ float page_scale(float amax) {
-  const int bits = __float_as_int(amax);
-  int e = (bits >> 23) - 126;
-  e = (bits & 0x7fffff) <= 0x600000 ? e - 9 : e - 8;
-  return __int_as_float(((e > -100 ? e : -100) + 127) << 23);
-}
-
-// Four packed e4m3 values times a factor.
-__device__ __forceinline__ int rescale4(int q, float factor) {
-  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(q, true);
-  return pack4(f32x4{a[0], a[1], b[0], b[1]}, factor);
-}
-// Bytes first .. last-1 of four are taken from `fresh`, those below from `old` or, if the page's scale grew, from `old` scaled.
-__device__ __forceinline__ int merge4(int old, int fresh, int first, int last, bool grown, float factor) {
-  const int again = grown ? rescale4(old, factor) : old;
-  unsigned r = 0;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const unsigned from = e < first ? (unsigned)again : e < last ? (unsigned)fresh : (unsigned)old;
-    r |= from & (0xffu << (8 * e));
-  }
-  return (int)r;
-}
 
 // A workgroup owns a touched page of one head, keys (blockIdx.z 0) or values: nobody else reads or writes it, and its scale
 // needs the largest of the new elements before any of them is stored.  They stay in registers in between.
 // Bound: memory for prompts (6 of 100 to 2900 tokens, 8 heads of 128: 18.3 us, 5.0 TB/s), latency for single tokens (48: 6.6 us, a
 // call's own time 5.3).
-template <int D>
+template <int D, bool TURN>
 __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
   constexpr int NP = PAGE * D / 4 / 256;       // pieces of four elements a thread holds
   constexpr int PPT = D / 4;                   // pieces of a token
@@ -139,6 +60,33 @@ __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
     const int slot = (t + 256 * i) / PPT, d0 = (t + 256 * i) % PPT * 4;
     v[i] = slot >= first && slot < last ? *reinterpret_cast<const f32x4 *>(x + (row0 + slot) * stride + d0) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  if constexpr (TURN)
+    if (!values) {
+      // (a thread's pieces are the same elements of all its tokens)
+      const int d0 = t % PPT * 4;
+      const bool norm = p.gamma != nullptr;
+      const f32x4 one = {1.f, 1.f, 1.f, 1.f}, g = norm ? load4(p.gamma, d0, D) : one, og = norm ? wdh::rope::partners(p.turn, p.gamma, d0, D) : one;
+      f32x4 o[NP];
+      wdh::rope::Angles a[NP];
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        const int slot = (t + 256 * i) / PPT;
+        const bool mine = slot >= first && slot < last;
+        const int position = !mine ? 0 : p.positions ? p.positions[row0 + slot] : pi * PAGE + slot;
+        o[i] = mine ? wdh::rope::partners(p.turn, x + (row0 + slot) * stride, d0, D) : f32x4{0.f, 0.f, 0.f, 0.f};
+        a[i] = wdh::rope::angles(p.turn, position, mine ? d0 : D);
+      }
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        if (norm) {
+          const wdh::rowmath::RowFactor f = wdh::rowmath::row_factor(wdh::rope::group_sum<PPT>(wdh::rope::squares(v[i])) / (double)D, p.eps);
+          v[i] = wdh::rope::normed(v[i], f, g);
+          o[i] = wdh::rope::normed(o[i], f, og);
+        }
+        const int slot = (t + 256 * i) / PPT;
+        v[i] = slot >= first && slot < last ? wdh::rope::turn(p.turn, d0, v[i], o[i], a[i]) : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
   if (id < 0 || id >= p.q.pages) return;
   const long long at = (long long)id * p.heads + head;
   unsigned char *page = (values ? p.VP : p.KP) + at * (PAGE * D);
@@ -204,7 +152,16 @@ struct AttendParams {
   int wgs;         // workgroups for each head of the cache (0: one for each item, which works on the whole of it)
   float *partial;  // results [workgroup][2][kv head][16][D] of items that more than one workgroup works on (null: there are none),
   float *stats;    // and their tops and sums [workgroup][2][kv head][16][2]
+  const int *mask; // trees: [tokens][words], bit j: the row sees row j of its sequence
+  int words;
 };
+
+// Trees: which of 32 tokens from `at` on (counted from the sequence's first row; those before it are seen by all) a row sees, as bits.
+__device__ __forceinline__ unsigned tree_bits(const int *row, int words, int at) {
+  const int w = at >> 5;
+  auto word = [&](int i) { return i < 0 ? ~0u : i < words ? (unsigned)row[i] : 0u; };
+  return __builtin_amdgcn_alignbit(word(w + 1), word(w), at & 31);
+}
 
 // Work of attention: items of 16 rows (a row is a token and one of the queries that share a head of the cache), each as many units
 // of four pages (one for each wavefront of a workgroup) as its sequence has.  The units of all items stand in a row, and every
@@ -361,7 +318,7 @@ __device__ __forceinline__ void split2_f16(const float (&x)[8], f16x8 (&part)[2]
 // Bound: memory where rows are few (32 tokens behind 500 to 8500, 32 heads of 128 on 8: 56 us, 5.3 TB/s; a copy of this kernel that only
 // loads takes 55; pages brought line by line and turned in LDS: 61), so three exact parts cost nothing that two would not; with all rows in use, instructions (1.3 us for a page of each
 // wavefront, two workgroups to a CU).
-template <int D>
+template <int D, bool TREE>
 __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
   constexpr int STEPS = D / 32, CH = D >= 64 ? D / 64 : 1, DT = D / 16;
   constexpr int OP = D + 4;
@@ -399,9 +356,15 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
   // this lane's row
   const int flat = w.item * 16 + fresh(i16), token = wdh::fdiv(flat, p.group), sub = flat - token * group;
   const bool live = token < s.n;
-  const int limit = live ? s.len - s.n + token : -1;  // its last key
-  const int last_token = wdh::fdiv(w.item * 16 + 15, p.group), first_limit = s.len - s.n + wdh::fdiv(w.item * 16, p.group);
-  const int last_key = s.len - s.n + (last_token < s.n ? last_token : s.n - 1);
+  const int limit = live ? s.len - s.n + token : -1;  // its last key (trees: see `sees`)
+  const int last_token = wdh::fdiv(w.item * 16 + 15, p.group), first_limit = TREE ? s.len - s.n - 1 : s.len - s.n + wdh::fdiv(w.item * 16, p.group);
+  const int last_key = TREE ? s.len - 1 : s.len - s.n + (last_token < s.n ? last_token : s.n - 1);
+  // trees: which of the 16 keys from `key` on the lane's row sees
+  auto sees = [&](int key) {
+    const int behind = s.len - key;
+    const unsigned bits = tree_bits(p.mask + (long long)(s.row0 + (live ? token : 0)) * p.words, p.words, key - (s.len - s.n));
+    return live ? bits & (behind >= 16 ? 0xffffu : behind > 0 ? (1u << behind) - 1u : 0u) : 0u;
+  };
   const int seg_end = w.units - w.unit < units_end - unit ? w.units : w.unit + (units_end - unit);  // in units of the item
   const int begin = 4 * w.unit, seen = last_key / PAGE + 1, end = seen < 4 * seg_end ? seen : 4 * seg_end;
   const bool alone = w.unit == 0 && seg_end == w.units;  // the whole item is this workgroup's
@@ -484,7 +447,12 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     float x[16], most = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; e++) x[e] = sc[e >> 2][e & 3];
-    if (!whole) {
+    unsigned seen_bits = 0xffffu;
+    if (TREE && !whole) {
+      seen_bits = sees(pg * PAGE + 16 * g);
+#pragma unroll
+      for (int e = 0; e < 16; e++) most = fmaxf(most, (seen_bits >> e) & 1 ? x[e] * c : -INFINITY);
+    } else if (!whole) {
       const int ahead = limit - pg * PAGE - 16 * g;
 #pragma unroll
       for (int e = 0; e < 16; e++) most = fmaxf(most, e <= ahead ? x[e] * c : -INFINITY);
@@ -511,7 +479,10 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     }
 #pragma unroll
     for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -ref));
-    if (!whole) {
+    if (TREE && !whole) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) x[e] = (seen_bits >> e) & 1 ? x[e] : 0.0f;
+    } else if (!whole) {
       const int ahead = fresh(limit) - pg * PAGE - 16 * g;
 #pragma unroll
       for (int e = 0; e < 16; e++) x[e] = e <= ahead ? x[e] : 0.0f;
@@ -556,8 +527,8 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
 #pragma unroll 1
       for (int i = 0; i < 4 * DT; i++)
 #pragma unroll 1
-        for (int j = 0; j < PAGE && pg * PAGE + j <= limit; j++)
-          if ((vp[(16 * (i >> 2) + (i & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << i;
+        for (int j = 0; j < PAGE && pg * PAGE + j <= (TREE ? last_key : limit); j++)
+          if ((!TREE || (sees(pg * PAGE + j) & 1)) && (vp[(16 * (i >> 2) + (i & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << i;
 #pragma unroll
       for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -726,7 +697,7 @@ __device__ __forceinline__ Place many_item(const AttendParams &p, int rank, int 
 // Bound: instructions.  A page takes 64 matrix ones of 32 cycles a wavefront and about as long of others (conversions of keys and values,
 // powers, splitting weights), which alternate more than they overlap: matrix cores busy 41 % of the time (three prompts of 1200 to 4000
 // tokens, 16 heads of 128 on 4: 243 us, 469 TFLOP/s counted once).
-template <int D>
+template <int D, bool TREE>
 __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   constexpr int QN = D / 32, DT = D / 32;           // runs of 32 elements of d in a key; blocks of 32 rows of O^T
   constexpr int KPIECES = PAGE * D / 16 / 256 > 0 ? PAGE * D / 16 / 256 : 1;  // 16-byte pieces a thread brings of a page's keys, and of its values
@@ -742,12 +713,18 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   const int row0 = s.index * MANY, flat = row0 + 32 * wave + li, token = wdh::fdiv(flat, p.group), sub = flat - token * group;
   const bool live = token < s.n;
   const int limit = live ? past + token : -1;
-  const int first_limit = past + wdh::fdiv(row0, p.group);  // of the item's first row
-  const int last_token = wdh::fdiv(row0 + MANY - 1, p.group), last_key = past + (last_token < s.n ? last_token : s.n - 1);
+  const int first_limit = TREE ? past - 1 : past + wdh::fdiv(row0, p.group);  // of the item's first row
+  const int last_token = wdh::fdiv(row0 + MANY - 1, p.group), last_key = TREE ? s.len - 1 : past + (last_token < s.n ? last_token : s.n - 1);
   const int seen = last_key / PAGE + 1, begin = (int)((long long)seen * blockIdx.y / gridDim.y), end = (int)((long long)seen * (blockIdx.y + 1) / gridDim.y);
   // this wavefront's own pages end earlier
-  const int wave_token = wdh::fdiv(row0 + 32 * wave, p.group), wave_last = wdh::fdiv(row0 + 32 * wave + 31, p.group), wave_first = past + wave_token;
-  const int wave_end = wave_token < s.n ? (past + (wave_last < s.n ? wave_last : s.n - 1)) / PAGE + 1 : 0;
+  const int wave_token = wdh::fdiv(row0 + 32 * wave, p.group), wave_last = wdh::fdiv(row0 + 32 * wave + 31, p.group), wave_first = TREE ? past - 1 : past + wave_token;
+  const int wave_end = wave_token < s.n ? TREE ? seen : (past + (wave_last < s.n ? wave_last : s.n - 1)) / PAGE + 1 : 0;
+  // trees: which of the 32 keys from `key` on the lane's row sees
+  auto sees = [&](int key) {
+    const int behind = s.len - key;
+    const unsigned bits = tree_bits(p.mask + (long long)(s.row0 + (live ? token : 0)) * p.words, p.words, key - past);
+    return live ? bits & (behind >= 32 ? ~0u : behind > 0 ? (1u << behind) - 1u : 0u) : 0u;
+  };
   const int *table = p.q.table + (long long)s.seq * p.q.max_pages;
 
   struct Page { long long at; float ks, vs; bool known; };
@@ -861,6 +838,12 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   // What a row does not see counts for nothing; the largest of the rest.
   auto mask = [&](f32x16 &sc, int pg, int t) {
     if (pg * PAGE + PAGE - 1 <= wave_first) return;
+    if constexpr (TREE) {
+      const unsigned bits = sees(pg * PAGE + 32 * t + 16 * half);
+#pragma unroll
+      for (int r = 0; r < 16; r++) sc[r] = (bits >> r) & 1 ? sc[r] : -INFINITY;
+      return;
+    }
     const int ahead = limit - pg * PAGE - 32 * t - 16 * half;
 #pragma unroll
     for (int r = 0; r < 16; r++) sc[r] = r <= ahead ? sc[r] : -INFINITY;
@@ -957,13 +940,13 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 #pragma unroll 1
         for (int e = 0; e < 16; e++)
 #pragma unroll 1
-          for (int j = 0; j < PAGE && pg * PAGE + j <= limit; j++)
-            if ((vp[(32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << e;
+          for (int j = 0; j < PAGE && pg * PAGE + j <= (TREE ? last_key : limit); j++)
+            if ((!TREE || (sees(pg * PAGE + j) & 1)) && (vp[(32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << e;
 #pragma unroll
         for (int e = 0; e < 16; e++) o[i][e] = (nan >> e) & 1 ? NAN : o[i][e];
       }
     }
-    if (active && !now.known && limit >= pg * PAGE) sum = NAN;
+    if (active && !now.known && (TREE ? (sees(pg * PAGE) | sees(pg * PAGE + 32)) != 0 : limit >= pg * PAGE)) sum = NAN;
     now = then;
     then = after;
     after = later;
@@ -1036,7 +1019,8 @@ __global__ __launch_bounds__(256) void attend_many_join(AttendParams p, int part
 template <int D>
 int launch_many(const AttendParams &p, long long items, int parts) {
   hipStream_t st = wdh::stream();
-  hipLaunchKernelGGL((attend_many<D>), dim3((unsigned)(items * p.kv_heads), (unsigned)parts), dim3(256), 0, st, p);
+  if (p.mask) hipLaunchKernelGGL((attend_many<D, true>), dim3((unsigned)(items * p.kv_heads), (unsigned)parts), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((attend_many<D, false>), dim3((unsigned)(items * p.kv_heads), (unsigned)parts), dim3(256), 0, st, p);
   WDH_LAUNCH_CHECK();
   if (parts > 1) {
     hipLaunchKernelGGL((attend_many_join<D>), dim3((unsigned)items, (unsigned)p.kv_heads, MANY * D / 1024), dim3(256), 0, st, p, parts);
@@ -1048,7 +1032,9 @@ int launch_many(const AttendParams &p, long long items, int parts) {
 template <int D>
 int launch_attend(const AttendParams &p, long long items) {
   hipStream_t st = wdh::stream();
-  hipLaunchKernelGGL((attend_rows<D>), dim3((unsigned)(p.wgs ? p.wgs : items), (unsigned)p.kv_heads), dim3(256), 0, st, p);
+  const dim3 wgs((unsigned)(p.wgs ? p.wgs : items), (unsigned)p.kv_heads);
+  if (p.mask) hipLaunchKernelGGL((attend_rows<D, true>), wgs, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((attend_rows<D, false>), wgs, dim3(256), 0, st, p);
   WDH_LAUNCH_CHECK();
   if (p.partial) {
     // (an item of hundreds of shares is a wide workgroup's work, one of a few shares a small one's)
@@ -1061,68 +1047,62 @@ int launch_attend(const AttendParams &p, long long items) {
   return WDH_OK;
 }
 
-using wdh::fail;
-
-// What append and attention ask of their sequences and of the cache.
-int check_cache(const char *who, int seqs, int tokens, int kv_heads, int d, int pages, int max_pages) {
-  if (seqs < 0 || tokens < 0 || kv_heads < 0 || pages < 0 || max_pages < 0) return fail(WDH_EINVAL, "%s: negative extent", who);
-  if (d != 32 && d != 64 && d != 128) return fail(WDH_EINVAL, "%s: head dimension %d (32, 64 and 128 are built)", who, d);
-  if (kv_heads == 0 || kv_heads > 65535) return fail(WDH_EINVAL, "%s: %d heads of the cache (1 to 65535)", who, kv_heads);
-  if (max_pages > (1 << 24)) return fail(WDH_EINVAL, "%s: tables of %d pages (at most %d)", who, max_pages, 1 << 24);
-  if (tokens > (1 << 24) || seqs > (1 << 20)) return fail(WDH_EINVAL, "%s: too many tokens or sequences", who);
-  return WDH_OK;
+// `turn`: keys are normed and rotated on the way, as these say (no Positions: a token's place in its sequence).
+struct Turn {
+  wdh_buf gamma, cos, sin, positions;
+  int rotary, rows, interleaved;
+  float eps;
+};
+template <bool TURN>
+void launch_append(const AppendParams &p, int d, dim3 grid) {
+  if (d == 32) hipLaunchKernelGGL((cache_append<32, TURN>), grid, dim3(256), 0, wdh::stream(), p);
+  else if (d == 64) hipLaunchKernelGGL((cache_append<64, TURN>), grid, dim3(256), 0, wdh::stream(), p);
+  else hipLaunchKernelGGL((cache_append<128, TURN>), grid, dim3(256), 0, wdh::stream(), p);
 }
-int cache_operands(const char *who, wdh_buf hKP, wdh_buf hKS, wdh_buf hVP, wdh_buf hVS, wdh_buf hT, wdh_buf hL, wdh_buf hS, int seqs, int kv_heads,
-                   int d, int pages, int max_pages, void **kp, void **ks, void **vp, void **vs, Sequences *q) {
-  const size_t cells = (size_t)pages * kv_heads;
-  char what[64];
-  auto get = [&](wdh_buf h, size_t need, const char *name, void **out) {
-    snprintf(what, sizeof(what), "%s: %s", who, name);
-    return wdh::operand(h, need, what, out);
-  };
-  void *t, *l, *s;
-  if (!get(hKP, cells * PAGE * d, "KPages", kp) || !get(hKS, cells * 4, "KScales", ks) || !get(hVP, cells * PAGE * d, "VPages", vp) ||
-      !get(hVS, cells * 4, "VScales", vs) || !get(hT, (size_t)seqs * max_pages * 4, "Table", &t) || !get(hL, (size_t)seqs * 4, "Lens", &l) ||
-      !get(hS, ((size_t)seqs + 1) * 4, "Starts", &s))
-    return WDH_EINVAL;
-  q->table = (const int *)t;
-  q->lens = (const int *)l;
-  q->starts = (const int *)s;
-  q->seqs = seqs;
-  q->max_pages = max_pages;
-  q->pages = pages;
-  return WDH_OK;
-}
-// Rows of `width` elements, `stride` apart from element `offset` of the buffer on, that are read 16 bytes at a time.
-int check_rows(const char *who, const char *name, int64_t offset, int64_t stride, int64_t width) {
-  if (offset < 0 || stride < width || offset > (1LL << 46) || stride > (1LL << 22))
-    return fail(WDH_EINVAL, "%s: %s rows of %lld elements from %lld on, %lld apart", who, name, (long long)width, (long long)offset, (long long)stride);
-  if (offset % 4 || stride % 4) return fail(WDH_EINVAL, "%s: offset and stride of %s must be multiples of 4 elements", who, name);
-  return WDH_OK;
-}
-
-}  // namespace
-
-extern "C" int wdh_cache_append(wdh_buf hK, int64_t k_offset, int64_t k_stride, wdh_buf hV, int64_t v_offset, int64_t v_stride, wdh_buf hKP,
-                                wdh_buf hKS, wdh_buf hVP, wdh_buf hVS, wdh_buf hTable, wdh_buf hLens, wdh_buf hStarts, int seqs, int tokens,
-                                int kv_heads, int d, int pages, int max_pages) {
-  WDH_REQUIRE_INIT();
-  WDH_REQUIRE_COMPUTE_LANE();
-  const char *who = "wdh_cache_append";
+int append(const char *who, wdh_buf hK, int64_t k_offset, int64_t k_stride, wdh_buf hV, int64_t v_offset, int64_t v_stride, wdh_buf hKP, wdh_buf hKS,
+           wdh_buf hVP, wdh_buf hVS, wdh_buf hTable, wdh_buf hLens, wdh_buf hStarts, int seqs, int tokens, int kv_heads, int d, int pages,
+           int max_pages, const Turn *turn) {
   if (int rc = check_cache(who, seqs, tokens, kv_heads, d, pages, max_pages)) return rc;
   const int64_t width = (int64_t)kv_heads * d;
   if (int rc = check_rows(who, "K", k_offset, k_stride, width)) return rc;
   if (int rc = check_rows(who, "V", v_offset, v_stride, width)) return rc;
+  if (turn) {
+    if (turn->rotary < 0 || turn->rotary > d || turn->rotary % 2 || turn->rows < 0)
+      return fail(WDH_EINVAL, "%s: %d rotated elements of %d (an even number), tables of %d rows", who, turn->rotary, d, turn->rows);
+    if ((turn->rotary > 0) != (turn->cos != 0) || (turn->rotary > 0) != (turn->sin != 0))
+      return fail(WDH_EINVAL, "%s: Cos and Sin go with rotated elements", who);
+    if (!(turn->eps >= 0.0f)) return fail(WDH_EINVAL, "%s: epsilon %g", who, (double)turn->eps);
+  }
   if (seqs == 0 || tokens == 0 || pages == 0 || max_pages == 0) return WDH_OK;
   AppendParams p;
   void *pk, *pv, *kp, *ks, *vp, *vs;
-  if (!wdh::operand(hK, (size_t)(k_offset + (tokens - 1) * k_stride + width) * 4, "wdh_cache_append: K", &pk)) return WDH_EINVAL;
-  if (!wdh::operand(hV, (size_t)(v_offset + (tokens - 1) * v_stride + width) * 4, "wdh_cache_append: V", &pv)) return WDH_EINVAL;
+  auto get = [&](wdh_buf h, int64_t elements, const char *name, void **out) {
+    char what[64];
+    snprintf(what, sizeof(what), "%s: %s", who, name);
+    return wdh::operand(h, (size_t)elements * 4, what, out);
+  };
+  if (!get(hK, k_offset + (tokens - 1) * k_stride + width, "K", &pk) || !get(hV, v_offset + (tokens - 1) * v_stride + width, "V", &pv)) return WDH_EINVAL;
   if (int rc = cache_operands(who, hKP, hKS, hVP, hVS, hTable, hLens, hStarts, seqs, kv_heads, d, pages, max_pages, &kp, &ks, &vp, &vs, &p.q)) return rc;
-  const wdh_buf out[4] = {hKP, hKS, hVP, hVS}, in[5] = {hK, hV, hTable, hLens, hStarts};
+  p.gamma = nullptr;
+  p.positions = nullptr;
+  p.turn = wdh::rope::Rotation{nullptr, nullptr, 0, 0, 0};
+  p.eps = 0.0f;
+  if (turn) {
+    void *g = nullptr, *c = nullptr, *s = nullptr, *at = nullptr;
+    const int64_t table = (int64_t)turn->rows * (turn->rotary / 2);
+    if ((turn->gamma && !get(turn->gamma, d, "KGamma", &g)) || (turn->cos && !get(turn->cos, table, "Cos", &c)) ||
+        (turn->sin && !get(turn->sin, table, "Sin", &s)) || (turn->positions && !get(turn->positions, tokens, "Positions", &at)))
+      return WDH_EINVAL;
+    p.gamma = (const float *)g;
+    p.positions = (const int *)at;
+    p.turn = wdh::rope::Rotation{(const float *)c, (const float *)s, turn->rotary / 2, turn->rows, turn->interleaved != 0};
+    p.eps = turn->eps;
+  }
+  const wdh_buf out[4] = {hKP, hKS, hVP, hVS};
+  const wdh_buf in[9] = {hK, hV, hTable, hLens, hStarts, turn ? turn->gamma : 0, turn ? turn->cos : 0, turn ? turn->sin : 0, turn ? turn->positions : 0};
   for (int i = 0; i < 4; i++) {
     for (wdh_buf h : in)
-      if (out[i] == h) return fail(WDH_EINVAL, "%s: a part of the cache aliases an input", who);
+      if (h && out[i] == h) return fail(WDH_EINVAL, "%s: a part of the cache aliases an input", who);
     for (int j = 0; j < i; j++)
       if (out[i] == out[j]) return fail(WDH_EINVAL, "%s: two parts of the cache share a buffer", who);
   }
@@ -1136,32 +1116,42 @@ extern "C" int wdh_cache_append(wdh_buf hK, int64_t k_offset, int64_t k_stride, 
   // touched pages: each has a new token, and a sequence's are at most n / 64 + 2
   const long long bound = (long long)tokens / PAGE + 2LL * seqs, items = bound < tokens ? bound : tokens;
   const dim3 grid((unsigned)items, (unsigned)kv_heads, 2);
-  if (d == 32) hipLaunchKernelGGL((cache_append<32>), grid, dim3(256), 0, wdh::stream(), p);
-  else if (d == 64) hipLaunchKernelGGL((cache_append<64>), grid, dim3(256), 0, wdh::stream(), p);
-  else hipLaunchKernelGGL((cache_append<128>), grid, dim3(256), 0, wdh::stream(), p);
+  if (turn) launch_append<true>(p, d, grid);
+  else launch_append<false>(p, d, grid);
   WDH_LAUNCH_CHECK();
   return WDH_OK;
 }
 
-extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_stride, wdh_buf hKP, wdh_buf hKS, wdh_buf hVP, wdh_buf hVS,
-                                   wdh_buf hTable, wdh_buf hLens, wdh_buf hStarts, wdh_buf hY, int seqs, int tokens, int heads, int kv_heads,
-                                   int d, int pages, int max_pages, float alpha) {
-  WDH_REQUIRE_INIT();
-  WDH_REQUIRE_COMPUTE_LANE();
-  const char *who = "wdh_cache_attention";
+int attention(const char *who, wdh_buf hQ, int64_t q_offset, int64_t q_stride, wdh_buf hKP, wdh_buf hKS, wdh_buf hVP, wdh_buf hVS, wdh_buf hTable,
+              wdh_buf hLens, wdh_buf hStarts, const wdh_buf *hMask, int words, wdh_buf hY, int seqs, int tokens, int heads, int kv_heads, int d,
+              int pages, int max_pages, float alpha) {
   if (int rc = check_cache(who, seqs, tokens, kv_heads, d, pages, max_pages)) return rc;
   if (heads <= 0 || heads % kv_heads || heads > 65536) return fail(WDH_EINVAL, "%s: %d heads on %d of the cache", who, heads, kv_heads);
   const int64_t width = (int64_t)heads * d;
   if (int rc = check_rows(who, "Q", q_offset, q_stride, width)) return rc;
+  if (hMask && (words < 1 || words > (1 << 19))) return fail(WDH_EINVAL, "%s: masks of %d words (1 to %d)", who, words, 1 << 19);
   if (seqs == 0 || tokens == 0 || max_pages == 0) return WDH_OK;
   if (pages == 0) return fail(WDH_EINVAL, "%s: a cache without pages", who);
   AttendParams p;
   void *pq, *py, *kp, *ks, *vp, *vs;
-  if (!wdh::operand(hQ, (size_t)(q_offset + (tokens - 1) * q_stride + width) * 4, "wdh_cache_attention: Q", &pq)) return WDH_EINVAL;
-  if (!wdh::operand(hY, (size_t)tokens * width * 4, "wdh_cache_attention: Y", &py)) return WDH_EINVAL;
+  auto get = [&](wdh_buf h, size_t elements, const char *name, void **out) {
+    char what[64];
+    snprintf(what, sizeof(what), "%s: %s", who, name);
+    return wdh::operand(h, elements * 4, what, out);
+  };
+  if (!get(hQ, (size_t)(q_offset + (tokens - 1) * q_stride + width), "Q", &pq) || !get(hY, (size_t)tokens * width, "Y", &py)) return WDH_EINVAL;
   if (int rc = cache_operands(who, hKP, hKS, hVP, hVS, hTable, hLens, hStarts, seqs, kv_heads, d, pages, max_pages, &kp, &ks, &vp, &vs, &p.q)) return rc;
   for (wdh_buf h : {hQ, hKP, hKS, hVP, hVS, hTable, hLens, hStarts})
     if (h == hY) return fail(WDH_EINVAL, "%s: Y aliases an input", who);
+  p.mask = nullptr;
+  p.words = 0;
+  if (hMask) {
+    void *pm;
+    if (!get(*hMask, (size_t)tokens * words, "Mask", &pm)) return WDH_EINVAL;
+    if (*hMask == hY) return fail(WDH_EINVAL, "%s: Y aliases an input", who);
+    p.mask = (const int *)pm;
+    p.words = words;
+  }
   p.q.tokens = tokens;
   p.Q = (const float *)pq + q_offset;
   p.q_stride = q_stride;
@@ -1219,4 +1209,44 @@ extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_strid
   }
   if (work) (void)wdh_free(work);
   return rc;
+}
+
+}  // namespace
+
+extern "C" int wdh_cache_append(wdh_buf hK, int64_t k_offset, int64_t k_stride, wdh_buf hV, int64_t v_offset, int64_t v_stride, wdh_buf hKP,
+                                wdh_buf hKS, wdh_buf hVP, wdh_buf hVS, wdh_buf hTable, wdh_buf hLens, wdh_buf hStarts, int seqs, int tokens,
+                                int kv_heads, int d, int pages, int max_pages) {
+  WDH_REQUIRE_INIT();
+  WDH_REQUIRE_COMPUTE_LANE();
+  return append("wdh_cache_append", hK, k_offset, k_stride, hV, v_offset, v_stride, hKP, hKS, hVP, hVS, hTable, hLens, hStarts, seqs, tokens,
+                kv_heads, d, pages, max_pages, nullptr);
+}
+
+extern "C" int wdh_cache_append_rope(wdh_buf hK, int64_t k_offset, int64_t k_stride, wdh_buf hV, int64_t v_offset, int64_t v_stride, wdh_buf hKP,
+                                     wdh_buf hKS, wdh_buf hVP, wdh_buf hVS, wdh_buf hTable, wdh_buf hLens, wdh_buf hStarts, wdh_buf hKGamma,
+                                     wdh_buf hCos, wdh_buf hSin, wdh_buf hPositions, int seqs, int tokens, int kv_heads, int d, int pages,
+                                     int max_pages, int rotary, int rows, int interleaved, float eps) {
+  WDH_REQUIRE_INIT();
+  WDH_REQUIRE_COMPUTE_LANE();
+  const Turn turn = {hKGamma, hCos, hSin, hPositions, rotary, rows, interleaved, eps};
+  return append("wdh_cache_append_rope", hK, k_offset, k_stride, hV, v_offset, v_stride, hKP, hKS, hVP, hVS, hTable, hLens, hStarts, seqs, tokens,
+                kv_heads, d, pages, max_pages, &turn);
+}
+
+extern "C" int wdh_cache_attention(wdh_buf hQ, int64_t q_offset, int64_t q_stride, wdh_buf hKP, wdh_buf hKS, wdh_buf hVP, wdh_buf hVS,
+                                   wdh_buf hTable, wdh_buf hLens, wdh_buf hStarts, wdh_buf hY, int seqs, int tokens, int heads, int kv_heads,
+                                   int d, int pages, int max_pages, float alpha) {
+  WDH_REQUIRE_INIT();
+  WDH_REQUIRE_COMPUTE_LANE();
+  return attention("wdh_cache_attention", hQ, q_offset, q_stride, hKP, hKS, hVP, hVS, hTable, hLens, hStarts, nullptr, 0, hY, seqs, tokens, heads,
+                   kv_heads, d, pages, max_pages, alpha);
+}
+
+extern "C" int wdh_cache_attention_tree(wdh_buf hQ, int64_t q_offset, int64_t q_stride, wdh_buf hKP, wdh_buf hKS, wdh_buf hVP, wdh_buf hVS,
+                                        wdh_buf hTable, wdh_buf hLens, wdh_buf hStarts, wdh_buf hMask, wdh_buf hY, int seqs, int tokens, int heads,
+                                        int kv_heads, int d, int pages, int max_pages, int words, float alpha) {
+  WDH_REQUIRE_INIT();
+  WDH_REQUIRE_COMPUTE_LANE();
+  return attention("wdh_cache_attention_tree", hQ, q_offset, q_stride, hKP, hKS, hVP, hVS, hTable, hLens, hStarts, &hMask, words, hY, seqs, tokens,
+                   heads, kv_heads, d, pages, max_pages, alpha);
 }

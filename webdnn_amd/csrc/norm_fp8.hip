@@ -17,6 +17,8 @@
 namespace {
 
 using namespace wdh::fp8;
+using wdh::rowmath::RowFactor;
+using wdh::rowmath::row_factor;
 
 struct NormParams {
   const float *X, *R, *G;
@@ -32,17 +34,6 @@ __device__ __forceinline__ double wave_sum_d(double v) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
   return v;
-}
-
-// A row's factor as two: t, rounded, and a power of two, 1 for all but extreme rows.
-struct RowFactor {
-  float power, t;
-};
-__device__ __forceinline__ RowFactor row_factor(double mean, float eps) {
-  const double t = 1.0 / sqrt(mean + (double)eps);
-  if (t > 0x1p100) return RowFactor{0x1p60f, (float)(t * 0x1p-60)};
-  if (t < 0x1p-100) return RowFactor{0x1p-40f, (float)(t * 0x1p40)};
-  return RowFactor{1.0f, (float)t};
 }
 
 // One piece (elements idx .. idx+3 of `row`) on its way out; the 32 lanes of a half wavefront hold the 128 elements of a block.

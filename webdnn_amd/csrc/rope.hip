@@ -1,0 +1,148 @@
+// Positions of queries and keys: each head normed (or not) and rotated by the angles of its token's position, in one pass.
+//
+// The reference has no such operators; in its terms they are the chain of a norm (see norm_fp8.hip), Split, Neg, Concat, Mul, Add
+// (src/descriptor_runner/operators/cpu/operators/standard/binary7.ts:24-75, split.ts:12-87, concat.ts:21-84).
+//
+// Bound: memory.  A head stays in the registers of 8 to 64 lanes between its sum of squares and its use.
+#include "common.h"
+#include "fastdiv.h"
+#include "rope.h"
+
+namespace {
+
+using namespace wdh::rope;
+using wdh::fail;
+using wdh::rowmath::RowFactor;
+using wdh::rowmath::row_factor;
+
+struct RopeParams {
+  const float *X;
+  float *Y;
+  long long x_stride, x_head, y_stride, y_head;  // elements between tokens, and between a token's heads
+  const float *q_gamma, *k_gamma;
+  const int *positions;
+  Rotation r;
+  long long units;      // tokens * heads
+  wdh::FastDiv heads;   // q_heads of one kind, then those of the other
+  int q_heads, d;
+  float eps;
+};
+
+// LANES lanes to a head, NP pieces of four elements to a lane, UNROLL heads of a group of lanes on their way at a time.
+template <int LANES, int NP, int UNROLL>
+__global__ __launch_bounds__(256) void head_rope(RopeParams p) {
+  constexpr int GROUPS = 256 / LANES;
+  const int lane = threadIdx.x % LANES;
+  const long long unit0 = (long long)blockIdx.x * (GROUPS * UNROLL) + threadIdx.x / LANES;
+  f32x4 v[UNROLL][NP], o[UNROLL][NP], gamma[UNROLL][NP], other_gamma[UNROLL][NP];
+  Angles a[UNROLL][NP];
+  int token[UNROLL], head[UNROLL];
+#pragma unroll
+  for (int j = 0; j < UNROLL; j++) {
+    const int unit = (int)(unit0 + j * GROUPS < p.units ? unit0 + j * GROUPS : p.units - 1);  // (behind the last: the last once more, not stored)
+    token[j] = wdh::fdiv(unit, p.heads);
+    head[j] = unit - token[j] * p.heads.d;
+    const float *x = p.X + token[j] * p.x_stride + head[j] * p.x_head, *g = head[j] < p.q_heads ? p.q_gamma : p.k_gamma;
+    const int position = p.positions ? p.positions[token[j]] : token[j];
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int d0 = 4 * (lane + LANES * i);
+      v[j][i] = load4(x, d0, p.d);
+      o[j][i] = partners(p.r, x, d0, p.d);
+      if (g) {
+        gamma[j][i] = load4(g, d0, p.d);
+        other_gamma[j][i] = partners(p.r, g, d0, p.d);
+      }
+      a[j][i] = angles(p.r, position, d0);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < UNROLL; j++) {
+    if (head[j] < p.q_heads ? p.q_gamma : p.k_gamma) {
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < NP; i++) sum += squares(v[j][i]);
+      const RowFactor f = row_factor(group_sum<LANES>(sum) / (double)p.d, p.eps);
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        v[j][i] = normed(v[j][i], f, gamma[j][i]);
+        o[j][i] = normed(o[j][i], f, other_gamma[j][i]);
+      }
+    }
+    if (unit0 + j * GROUPS >= p.units) continue;
+    float *y = p.Y + token[j] * p.y_stride + head[j] * p.y_head;
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int d0 = 4 * (lane + LANES * i);
+      store4(y, d0, p.d, turn(p.r, d0, v[j][i], o[j][i], a[j][i]));
+    }
+  }
+}
+
+template <int LANES, int NP, int UNROLL>
+int launch(const RopeParams &p) {
+  constexpr int PER = 256 / LANES * UNROLL;
+  const long long wgs = (p.units + PER - 1) / PER;
+  if (wgs > 0xffffff) return fail(WDH_EINVAL, "wdh_rope: too many heads");  // (a launch has fewer than 2^32 threads)
+  hipLaunchKernelGGL((head_rope<LANES, NP, UNROLL>), dim3((unsigned)wgs), dim3(256), 0, wdh::stream(), p);
+  WDH_LAUNCH_CHECK();
+  return WDH_OK;
+}
+template <int LANES>
+int launch_lanes(const RopeParams &p) {
+  return launch<LANES, 1, 1>(p);
+}
+
+}  // namespace
+
+extern "C" int wdh_rope(wdh_buf hX, int64_t x_offset, int64_t x_stride, int64_t x_head, wdh_buf hY, int64_t y_offset, int64_t y_stride,
+                        int64_t y_head, wdh_buf hQGamma, wdh_buf hKGamma, wdh_buf hCos, wdh_buf hSin, wdh_buf hPositions, int64_t tokens,
+                        int heads, int k_heads, int d, int rotary, int rows, int interleaved, float eps) {
+  WDH_REQUIRE_INIT();
+  WDH_REQUIRE_COMPUTE_LANE();
+  if (tokens < 0 || heads < 0 || k_heads < 0 || rows < 0) return fail(WDH_EINVAL, "wdh_rope: negative extent");
+  if (d < 1 || d > 1024) return fail(WDH_EINVAL, "wdh_rope: heads of %d elements (1 to 1024)", d);
+  if (rotary < 0 || rotary > d || rotary % 2) return fail(WDH_EINVAL, "wdh_rope: %d rotated elements of %d (an even number)", rotary, d);
+  if ((rotary > 0) != (hCos != 0) || (rotary > 0) != (hSin != 0)) return fail(WDH_EINVAL, "wdh_rope: Cos and Sin go with rotated elements");
+  if (!(eps >= 0.0f)) return fail(WDH_EINVAL, "wdh_rope: epsilon %g", (double)eps);
+  if (heads > 65536 || k_heads > 65536) return fail(WDH_EINVAL, "wdh_rope: too many heads");
+  const int64_t all = (int64_t)heads + k_heads;
+  if (tokens == 0 || all == 0) return WDH_OK;
+  if (tokens > 0x7fffffffLL / all) return fail(WDH_EINVAL, "wdh_rope: too many heads");
+  const int64_t most = 1LL << 40;
+  for (int64_t v : {x_offset, x_stride, x_head, y_offset, y_stride, y_head})
+    if (v < 0 || v > most) return fail(WDH_EINVAL, "wdh_rope: an offset or a stride of %lld elements", (long long)v);
+  const int64_t x_last = (tokens - 1) * x_stride + (all - 1) * x_head, y_last = (tokens - 1) * y_stride + (all - 1) * y_head;
+  if (x_last > most || y_last > most) return fail(WDH_EINVAL, "wdh_rope: rows span too much");
+  const bool rows_of_heads = (all == 1 || y_head >= d) && (tokens == 1 || y_stride >= (all - 1) * y_head + d);
+  const bool heads_of_rows = (tokens == 1 || y_stride >= d) && (all == 1 || y_head >= (tokens - 1) * y_stride + d);
+  if (!rows_of_heads && !heads_of_rows) return fail(WDH_EINVAL, "wdh_rope: heads of Y overlap");
+  if (hX == hY && (x_offset != y_offset || x_stride != y_stride || x_head != y_head))
+    return fail(WDH_EINVAL, "wdh_rope: Y is X in another layout");
+  for (wdh_buf h : {hQGamma, hKGamma, hCos, hSin, hPositions})
+    if (h && h == hY) return fail(WDH_EINVAL, "wdh_rope: Y aliases an input");
+  void *px, *py, *qg = nullptr, *kg = nullptr, *pc = nullptr, *ps = nullptr, *pp = nullptr;
+  if (!wdh::operand(hX, (size_t)(x_offset + x_last + d) * 4, "wdh_rope: X", &px)) return WDH_EINVAL;
+  if (!wdh::operand(hY, (size_t)(y_offset + y_last + d) * 4, "wdh_rope: Y", &py)) return WDH_EINVAL;
+  if (hQGamma && !wdh::operand(hQGamma, (size_t)d * 4, "wdh_rope: QGamma", &qg)) return WDH_EINVAL;
+  if (hKGamma && !wdh::operand(hKGamma, (size_t)d * 4, "wdh_rope: KGamma", &kg)) return WDH_EINVAL;
+  const size_t table = (size_t)rows * (rotary / 2) * 4;
+  if (hCos && !wdh::operand(hCos, table, "wdh_rope: Cos", &pc)) return WDH_EINVAL;
+  if (hSin && !wdh::operand(hSin, table, "wdh_rope: Sin", &ps)) return WDH_EINVAL;
+  if (hPositions && !wdh::operand(hPositions, (size_t)tokens * 4, "wdh_rope: Positions", &pp)) return WDH_EINVAL;
+  RopeParams p;
+  p.X = (const float *)px + x_offset;
+  p.Y = (float *)py + y_offset;
+  p.x_stride = x_stride; p.x_head = x_head; p.y_stride = y_stride; p.y_head = y_head;
+  p.q_gamma = (const float *)qg; p.k_gamma = (const float *)kg;
+  p.positions = (const int *)pp;
+  p.r = Rotation{(const float *)pc, (const float *)ps, rotary / 2, rows, interleaved != 0};
+  p.units = tokens * all;
+  p.heads = wdh::make_fastdiv(all);
+  p.q_heads = heads; p.d = d; p.eps = eps;
+  if (d <= 32) return launch_lanes<8>(p);
+  if (d <= 64) return launch_lanes<16>(p);
+  if (d <= 128) return launch_lanes<32>(p);
+  if (d <= 256) return launch_lanes<64>(p);
+  return d <= 512 ? launch<64, 2, 1>(p) : launch<64, 4, 1>(p);
+}

@@ -1,6 +1,6 @@
 // Cross-lane reductions and the exponential shared by the row kernels (Softmax,
 // LayerNormalization) and the fused attention kernel, so that the fused and the
-// unfused softmax round alike.
+// unfused softmax round alike; the factor of the root-mean-square norms.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -51,6 +51,17 @@ __device__ __forceinline__ float exp_f32(float x) {
   float r = __builtin_fmaf(x, log2e_hi, -n);
   r = __builtin_fmaf(x, log2e_lo, r);
   return __builtin_ldexpf(__builtin_amdgcn_exp2f(r), (int)n);
+}
+
+// The factor of a root-mean-square norm's row, 1 / sqrt(mean + eps), as two: t, rounded, and a power of two, 1 for all but extreme rows.
+struct RowFactor {
+  float power, t;
+};
+__device__ __forceinline__ RowFactor row_factor(double mean, float eps) {
+  const double t = 1.0 / sqrt(mean + (double)eps);
+  if (t > 0x1p100) return RowFactor{0x1p60f, (float)(t * 0x1p-60)};
+  if (t < 0x1p-100) return RowFactor{0x1p-40f, (float)(t * 0x1p40)};
+  return RowFactor{1.0f, (float)t};
 }
 
 }  // namespace rowmath

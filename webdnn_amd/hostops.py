@@ -1002,3 +1002,128 @@ def cache_attention(ctx, cache, q, heads, alpha, table, lens, starts, q_column=0
     call("wdh_cache_attention", q.handle, q_column, stride, cache.k.handle, cache.k_scales.handle, cache.v.handle, cache.v_scales.handle,
          table.handle, lens.handle, starts.handle, y.handle, seqs, tokens, heads, cache.heads, cache.d, cache.pages, most, float(alpha))
     return y
+
+
+# ---- positions and drafted tokens (include/webdnn_hip.h) ------------------------------------------------
+def _rotation(what, d, cos, sin, positions, tokens):
+    """(rotated elements, rows of the tables) of cos and sin [rows, rotary / 2]; positions [tokens] or None."""
+    _require_f32(cos, sin)
+    if (cos is None) != (sin is None):
+        raise OperatorError("%s: cos and sin go together" % what)
+    if positions is not None:
+        _require("%s: positions" % what, positions, [tokens], "int32")
+    if cos is None:
+        return 0, 0
+    if cos.ndim != 2 or cos.dims != sin.dims or cos.dims[1] < 1 or 2 * cos.dims[1] > d:
+        raise OperatorError("%s: tables %s and %s for heads of %d elements" % (what, cos.dims, sin.dims, d))
+    if cos.dims[0] > INT32_MAX:
+        _too_large(what, cos.dims[0])
+    return 2 * cos.dims[1], cos.dims[0]
+
+
+def rotary_embedding(ctx, x, cos, sin, positions, heads, d, k_heads=0, q_scale=None, k_scale=None, interleaved=False, epsilon=1e-5, column=0,
+                     out=None, out_column=0):
+    """Heads of x's rows ([tokens, (heads + k_heads) * d], or columns column.. of wider rows) rotated by the angles of their positions (rows of
+    cos and sin [positions, rotary / 2]; positions None: a row's own number), after a root-mean-square norm of each head where q_scale (the first
+    `heads`) or k_scale (the others) [d] is given.  cos and sin None: the norm alone.  out: rows for the result, from column out_column on (x itself
+    with the same column: in place)."""
+    if min(heads, k_heads) < 0 or d < 1 or max(heads, k_heads, d) > INT32_MAX:
+        raise OperatorError("rotary_embedding: %d + %d heads of %d" % (heads, k_heads, d))
+    width = (heads + k_heads) * d
+    stride, tokens = _rows_at("rotary_embedding: x", x, column, width)
+    rotary, rows = _rotation("rotary_embedding", d, cos, sin, positions, tokens)
+    for what, t in (("q_scale", q_scale), ("k_scale", k_scale)):
+        if t is not None:
+            _require("rotary_embedding: %s" % what, t, [d])
+    y = ctx.empty_tensor([tokens, width]) if out is None else out
+    y_stride, y_tokens = _rows_at("rotary_embedding: out", y, out_column, width)
+    if y_tokens != tokens:
+        raise OperatorError("rotary_embedding: %d rows for %d" % (y_tokens, tokens))
+    call("wdh_rope", x.handle, column, stride, d, y.handle, out_column, y_stride, d, _handle(q_scale), _handle(k_scale), _handle(cos), _handle(sin),
+         _handle(positions), tokens, heads, k_heads, d, rotary, rows, int(interleaved), epsilon)
+    return y
+
+
+def cache_append_rotary(ctx, cache, k, v, table, lens, starts, cos, sin, positions=None, k_scale=None, interleaved=False, epsilon=1e-5, k_column=0,
+                        v_column=0):
+    """cache_append with the keys normed (k_scale [d]) and rotated on the way, as rotary_embedding would have.  positions None: a token's
+    place in its sequence."""
+    seqs, most = _sequences(table, lens, starts)
+    width = cache.heads * cache.d
+    (ks, tokens), (vs, v_tokens) = _rows_at("cache_append: k", k, k_column, width), _rows_at("cache_append: v", v, v_column, width)
+    if tokens != v_tokens:
+        raise OperatorError("cache_append: %d keys and %d values" % (tokens, v_tokens))
+    rotary, rows = _rotation("cache_append", cache.d, cos, sin, positions, tokens)
+    if k_scale is not None:
+        _require("cache_append: k_scale", k_scale, [cache.d])
+    call("wdh_cache_append_rope", k.handle, k_column, ks, v.handle, v_column, vs, cache.k.handle, cache.k_scales.handle, cache.v.handle,
+         cache.v_scales.handle, table.handle, lens.handle, starts.handle, _handle(k_scale), _handle(cos), _handle(sin), _handle(positions), seqs, tokens,
+         cache.heads, cache.d, cache.pages, most, rotary, rows, int(interleaved), epsilon)
+
+
+def cache_attention_tree(ctx, cache, q, heads, alpha, table, lens, starts, mask, q_column=0, out=None):
+    """cache_attention for rows that see the tokens before the call's and, of their sequence's own rows, those whose bits are set in
+    mask [tokens, words] (int32; bit j % 32 of word j / 32 for row j)."""
+    seqs, most = _sequences(table, lens, starts)
+    if heads <= 0 or not cache.heads or heads % cache.heads:
+        raise OperatorError("cache_attention: %d heads on %d of the cache" % (heads, cache.heads))
+    stride, tokens = _rows_at("cache_attention: q", q, q_column, heads * cache.d)
+    if mask.ndim != 2 or mask.dims[1] < 1 or mask.dims[1] > INT32_MAX:
+        raise OperatorError("cache_attention: mask is [tokens, words]")
+    _require("cache_attention: mask", mask, [tokens, mask.dims[1]], "int32")
+    y = _result(ctx, out, [tokens, heads * cache.d])
+    call("wdh_cache_attention_tree", q.handle, q_column, stride, cache.k.handle, cache.k_scales.handle, cache.v.handle, cache.v_scales.handle,
+         table.handle, lens.handle, starts.handle, mask.handle, y.handle, seqs, tokens, heads, cache.heads, cache.d, cache.pages, most, mask.dims[1],
+         float(alpha))
+    return y
+
+
+def tree_mask(parents, starts):
+    """The mask of cache_attention_tree for trees given by each row's parent (a row of its own sequence, -1 for none): numpy int32
+    [tokens, words], rows that see their ancestors and themselves.  parents and starts are host arrays."""
+    parents, starts = np.asarray(parents), np.asarray(starts)
+    most = int(np.diff(starts).max(initial=1))
+    mask = np.zeros((len(parents), max(1, -(-most // 32))), np.uint32)
+    for first, end in zip(starts[:-1], starts[1:]):
+        for r in range(int(first), int(end)):
+            up, place = int(parents[r]), r - int(first)
+            if not -1 <= up < place:
+                raise OperatorError("tree_mask: row %d follows row %d of its sequence" % (place, up))
+            if up >= 0:
+                mask[r] = mask[int(first) + up]
+            mask[r, place // 32] |= np.uint32(1 << (place % 32))
+    return mask.view(np.int32)
+
+
+def verify_drafts(ctx, probabilities, tokens, parents, uniform, starts, draft=None, out=None):
+    """Which drafted tokens the target's probabilities [rows, vocabulary] accept: (next token, accepted drafts) of each sequence and the path
+    [rows].  tokens, parents [rows] and starts [sequences + 1] are int32 tensors, uniform [rows] numbers from [0, 1); draft [rows, vocabulary]: what
+    each row's children were drawn from (None: they were chosen).  out = (next, count, path)."""
+    _require_f32(probabilities, uniform, draft)
+    if probabilities.ndim != 2 or starts.ndim != 1 or starts.dims[0] < 1:
+        raise OperatorError("verify_drafts: probabilities are [rows, vocabulary], starts [sequences + 1]")
+    (rows, vocab), seqs = probabilities.dims, starts.dims[0] - 1
+    if max(rows, vocab, seqs) > INT32_MAX:
+        _too_large("verify_drafts", rows, vocab, seqs)
+    if draft is not None:
+        _require("verify_drafts: draft", draft, [rows, vocab])
+    for what, t in (("tokens", tokens), ("parents", parents)):
+        _require("verify_drafts: %s" % what, t, [rows], "int32")
+    _require("verify_drafts: uniform", uniform, [rows])
+    _require("verify_drafts: starts", starts, [seqs + 1], "int32")
+    token, count, path = out if out is not None else (None, None, None)
+    token, count, path = _result(ctx, token, [seqs], "int32"), _result(ctx, count, [seqs], "int32"), _result(ctx, path, [rows], "int32")
+    call("wdh_verify_drafts", probabilities.handle, _handle(draft), tokens.handle, parents.handle, uniform.handle, starts.handle, token.handle,
+         count.handle, path.handle, seqs, rows, vocab)
+    return token, count, path
+
+
+def cache_keep(ctx, cache, table, lens, starts, path, count):
+    """Of the rows that were appended last (lens with them counted), each sequence keeps the path that verify_drafts found: 1 + count tokens."""
+    seqs, most = _sequences(table, lens, starts)
+    if path.ndim != 1 or path.dims[0] > INT32_MAX:
+        raise OperatorError("cache_keep: path is [rows]")
+    _require("cache_keep: path", path, path.dims, "int32")
+    _require("cache_keep: count", count, [seqs], "int32")
+    call("wdh_cache_keep", cache.k.handle, cache.k_scales.handle, cache.v.handle, cache.v_scales.handle, table.handle, lens.handle, starts.handle,
+         path.handle, count.handle, seqs, path.dims[0], cache.heads, cache.d, cache.pages, most)

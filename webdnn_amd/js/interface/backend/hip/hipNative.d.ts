@@ -100,4 +100,24 @@ export interface HipNative {
   cacheAttention(Q: Handle, qOffset: number, qStride: number, KPages: Handle, KScales: Handle, VPages: Handle, VScales: Handle,
                  Table: Handle, Lens: Handle, Starts: Handle, Y: Handle, seqs: number, tokens: number, heads: number,
                  kvHeads: number, d: number, pages: number, maxPages: number, alpha: number): void;
+  // ---- positions and drafted tokens (0 = absent) ----
+  /** heads of rows normed (QGamma for the first `heads`, KGamma for the kHeads behind them) and rotated by their positions' rows of Cos and Sin */
+  rope(X: Handle, xOffset: number, xStride: number, xHead: number, Y: Handle, yOffset: number, yStride: number, yHead: number, QGamma: Handle,
+       KGamma: Handle, Cos: Handle, Sin: Handle, Positions: Handle, tokens: number, heads: number, kHeads: number, d: number, rotary: number,
+       rows: number, interleaved: number, epsilon: number): void;
+  /** cacheAppend with the keys normed and rotated on the way */
+  cacheAppendRope(K: Handle, kOffset: number, kStride: number, V: Handle, vOffset: number, vStride: number, KPages: Handle, KScales: Handle,
+                  VPages: Handle, VScales: Handle, Table: Handle, Lens: Handle, Starts: Handle, KGamma: Handle, Cos: Handle, Sin: Handle,
+                  Positions: Handle, seqs: number, tokens: number, kvHeads: number, d: number, pages: number, maxPages: number, rotary: number,
+                  rows: number, interleaved: number, epsilon: number): void;
+  /** cacheAttention for rows that see, of their sequence's own rows, those whose bits are set in Mask [tokens, words] */
+  cacheAttentionTree(Q: Handle, qOffset: number, qStride: number, KPages: Handle, KScales: Handle, VPages: Handle, VScales: Handle,
+                     Table: Handle, Lens: Handle, Starts: Handle, Mask: Handle, Y: Handle, seqs: number, tokens: number, heads: number,
+                     kvHeads: number, d: number, pages: number, maxPages: number, words: number, alpha: number): void;
+  /** Next, Count [seqs] and Path [tokens] of the drafts that P (and Draft, what they were drawn from) accept */
+  verifyDrafts(P: Handle, Draft: Handle, Tokens: Handle, Parents: Handle, Uniform: Handle, Starts: Handle, Next: Handle, Count: Handle,
+               Path: Handle, seqs: number, tokens: number, vocab: number): void;
+  /** keeps each sequence's path of its last rows */
+  cacheKeep(KPages: Handle, KScales: Handle, VPages: Handle, VScales: Handle, Table: Handle, Lens: Handle, Starts: Handle, Path: Handle,
+            Count: Handle, seqs: number, tokens: number, kvHeads: number, d: number, pages: number, maxPages: number): void;
 }

@@ -21,7 +21,7 @@
 
 #include "webdnn_hip.h"
 
-#define MAX_ARGS 24
+#define MAX_ARGS 28
 
 static napi_value throw_last(napi_env env, const char *fn, int rc) {
   char msg[640];
@@ -454,6 +454,63 @@ FN(js_cache_attention) { /* (Q, qOffset, qStride, KPages, KScales, VPages, VScal
   return make_undefined(env);
 }
 
+/* Integers up to `count` into a; those that are C ints (bits of `ints`) are not cut to their low bits. */
+static int to_ints(napi_env env, const char *fn, napi_value *argv, int count, uint32_t ints, int64_t *a) {
+  for (int i = 0; i < count; i++) {
+    if (!to_i64(env, argv[i], &a[i])) return throw_arg(env, fn, "integer argument expected"), 0;
+    if ((ints >> i & 1) && a[i] != (int32_t)a[i]) return throw_arg(env, fn, "an extent does not fit 32 bits"), 0;
+  }
+  return 1;
+}
+
+FN(js_rope) { /* (X, xOffset, xStride, xHead, Y, yOffset, yStride, yHead, QGamma, KGamma, Cos, Sin, Positions, tokens, ...) */
+  ARGS("wdh_rope", 21);
+  int64_t a[20];
+  if (!to_ints(env, FNAME, argv, 20, 0xfc000u, a)) return NULL;
+  F64(20, eps);
+  CHECK(wdh_rope(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], a[13], (int)a[14], (int)a[15],
+                 (int)a[16], (int)a[17], (int)a[18], (int)a[19], (float)eps));
+  return make_undefined(env);
+}
+
+FN(js_cache_append_rope) { /* (K, kOffset, kStride, V, vOffset, vStride, KPages, KScales, VPages, VScales, Table, Lens, Starts, KGamma, ...) */
+  ARGS("wdh_cache_append_rope", 27);
+  int64_t a[26];
+  if (!to_ints(env, FNAME, argv, 26, 0x3fe0000u, a)) return NULL;
+  F64(26, eps);
+  CHECK(wdh_cache_append_rope(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[15], a[16],
+                              (int)a[17], (int)a[18], (int)a[19], (int)a[20], (int)a[21], (int)a[22], (int)a[23], (int)a[24],
+                              (int)a[25], (float)eps));
+  return make_undefined(env);
+}
+
+FN(js_cache_attention_tree) { /* (Q, qOffset, qStride, KPages, KScales, VPages, VScales, Table, Lens, Starts, Mask, Y, ..., alpha) */
+  ARGS("wdh_cache_attention_tree", 21);
+  int64_t a[20];
+  if (!to_ints(env, FNAME, argv, 20, 0xff000u, a)) return NULL;
+  F64(20, alpha);
+  CHECK(wdh_cache_attention_tree(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], (int)a[12], (int)a[13],
+                                 (int)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19], (float)alpha));
+  return make_undefined(env);
+}
+
+FN(js_verify_drafts) { /* (P, Draft, Tokens, Parents, Uniform, Starts, Next, Count, Path, seqs, tokens, vocab) */
+  ARGS("wdh_verify_drafts", 12);
+  int64_t a[12];
+  if (!to_ints(env, FNAME, argv, 12, 0xe00u, a)) return NULL;
+  CHECK(wdh_verify_drafts(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], (int)a[9], (int)a[10], (int)a[11]));
+  return make_undefined(env);
+}
+
+FN(js_cache_keep) { /* (KPages, KScales, VPages, VScales, Table, Lens, Starts, Path, Count, ...) */
+  ARGS("wdh_cache_keep", 15);
+  int64_t a[15];
+  if (!to_ints(env, FNAME, argv, 15, 0x7e00u, a)) return NULL;
+  CHECK(wdh_cache_keep(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], (int)a[9], (int)a[10], (int)a[11], (int)a[12], (int)a[13],
+                       (int)a[14]));
+  return make_undefined(env);
+}
+
 FN(js_reduce_mean) {
   ARGS("wdh_reduce_mean", 4);
   I64(0, X); I64(1, Y); I64(2, outer); I64(3, len);
@@ -568,7 +625,8 @@ static napi_value init_module(napi_env env, napi_value exports) {
       {"gemm", js_gemm}, {"gemmEx", js_gemm_ex}, {"linearGroup", js_linear_group}, {"conv2d", js_conv2d}, {"conv2dEx", js_conv2d_ex}, {"binary", js_binary}, {"unary", js_unary},
       {"softmax", js_softmax}, {"attention", js_attention}, {"layernorm", js_layernorm}, {"layernormAdd", js_layernorm_add}, {"reduceMean", js_reduce_mean}, {"reduceAxis", js_reduce_axis},
       {"rmsnorm", js_rmsnorm}, {"quantizeFp8", js_quantize_fp8}, {"gemmFp8", js_gemm_fp8}, {"cacheAppend", js_cache_append},
-      {"cacheAttention", js_cache_attention},
+      {"cacheAttention", js_cache_attention}, {"rope", js_rope}, {"cacheAppendRope", js_cache_append_rope},
+      {"cacheAttentionTree", js_cache_attention_tree}, {"verifyDrafts", js_verify_drafts}, {"cacheKeep", js_cache_keep},
       {"maxpool2d", js_maxpool2d}, {"globalAvgpool", js_global_avgpool},
       {"transpose", js_transpose}, {"gather", js_gather}, {"cast", js_cast},
       {"stridedCopy", js_strided_copy}, {"graphBegin", js_graph_begin}, {"graphEnd", js_graph_end},
