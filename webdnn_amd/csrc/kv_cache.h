@@ -4,6 +4,7 @@
 #include <stdio.h>
 
 #include "common.h"
+#include "fastdiv.h"
 #include "fp8.h"
 
 namespace wdh {
@@ -72,6 +73,117 @@ __device__ __forceinline__ Place locate(const Sequences &q, int item, Count coun
   return Place{0, 0, 0, 0, 0};
 }
 
+// ---- attention -------------------------------------------------------------------------------
+struct AttendParams {
+  Sequences q;
+  const float *Q;
+  long long q_stride;
+  const unsigned char *KP, *VP;
+  const float *KS, *VS;
+  float *Y;
+  int heads, kv_heads;
+  FastDiv group;  // queries that share a head of the cache
+  float scale;     // alpha * log2(e): powers are taken of two
+  int wgs;         // workgroups for each head of the cache (0: one for each item, which works on the whole of it)
+  float *partial;  // results [workgroup][2][kv head][ROWS][D] of items that more than one workgroup works on (null: there are none),
+  float *stats;    // and their tops and sums [workgroup][2][kv head][ROWS][2]
+  const int *mask; // trees: [tokens][words], bit j: the row sees row j of its sequence
+  int words;
+};
+
+// Work of attention: items of ROWS rows (a row is a token and one of the queries that share a head of the cache), each as many units
+// of UNIT pages (one for each wavefront of a workgroup, or for some that share it) as its sequence has.  The units of all items stand in a row, and every
+// workgroup takes `share` neighbouring ones: all end at the same time, whatever the sequences' lengths.
+constexpr int MOST_UNITS = 1 << 30;
+struct Work {
+  Place s;
+  int item, unit, units;  // the item, the unit of it that was asked for, and how many it has
+  int before;             // units in front of the item
+  int ordinal;            // items in front of it (where that is asked for)
+  int share, total;
+};
+template <int ROWS>
+__device__ __forceinline__ int items_of(const Place &s, int group) { return s.n ? (int)(((long long)s.n * group + ROWS - 1) / ROWS) : 0; }
+template <int UNIT>
+__device__ __forceinline__ int units_of(const Place &s) { return (s.len + UNIT * PAGE - 1) / (UNIT * PAGE); }
+// 64 sequences side by side, a lane to each; upto: units of these up to and with the lane's.
+struct Look {
+  Place mine;
+  int items, units, upto;
+};
+template <int ROWS, int UNIT>
+__device__ __forceinline__ Look look(const AttendParams &p, int round) {
+  Look l;
+  l.mine = sequence(p.q, 64 * round + fresh(threadIdx.x & 63));
+  l.items = items_of<ROWS>(l.mine, p.group.d);
+  l.units = units_of<UNIT>(l.mine);
+  l.upto = wave_scan(l.items * l.units);
+  return l;
+}
+template <int ROWS, int UNIT>
+__device__ __forceinline__ int total_units(const AttendParams &p, const Look &first) {
+  int total = __builtin_amdgcn_readlane(first.upto, 63);
+  for (int i = 1; i < (p.q.seqs + 63) / 64; i++) total = add_sat(total, __builtin_amdgcn_readlane(look<ROWS, UNIT>(p, i).upto, 63));
+  return total <= MOST_UNITS ? total : 0;  // (more than the host allows: numbers that contradict each other)
+}
+// The item that holds unit number `index` of all (or, by_item, item number `index`); s.n = 0 behind the last.
+template <int ROWS, int UNIT, bool ORDINAL = false>
+__device__ __forceinline__ Work locate_work(const AttendParams &p, const Look &first, int index, bool by_item) {
+  Work w;
+  int before = 0, before_items = 0;
+  Look l = first;
+  for (int i = 0; i < (p.q.seqs + 63) / 64; i++) {
+    if (i) l = look<ROWS, UNIT>(p, i);
+    const int upto = add_sat(before, l.upto), upto_items = by_item || ORDINAL ? add_sat(before_items, wave_scan(l.items)) : 0;
+    const unsigned long long has = __ballot(index < (by_item ? upto_items : upto));
+    if (has) {
+      const int at = __ffsll(has) - 1;
+      w.s.seq = __builtin_amdgcn_readlane(l.mine.seq, at);
+      w.s.row0 = __builtin_amdgcn_readlane(l.mine.row0, at);
+      w.s.n = __builtin_amdgcn_readlane(l.mine.n, at);
+      w.s.len = __builtin_amdgcn_readlane(l.mine.len, at);
+      w.units = __builtin_amdgcn_readlane(l.units, at);
+      const int begin = __builtin_amdgcn_readlane(upto - l.items * l.units, at);
+      w.item = by_item ? index - __builtin_amdgcn_readlane(upto_items - l.items, at) : (index - begin) / w.units;
+      w.before = begin + w.item * w.units;
+      w.unit = by_item ? 0 : index - w.before;
+      if constexpr (ORDINAL) w.ordinal = __builtin_amdgcn_readlane(upto_items - l.items, at) + w.item;
+      return w;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+    before_items = __builtin_amdgcn_readlane(upto_items, 63);
+  }
+  w.s = Place{0, 0, 0, 0, 0};
+  return w;
+}
+
+// All items of a call (where there are units at all).
+template <int ROWS, int UNIT>
+__device__ __forceinline__ int total_items(const AttendParams &p, const Look &first) {
+  int total = __builtin_amdgcn_readlane(wave_scan(first.items), 63);
+  for (int i = 1; i < (p.q.seqs + 63) / 64; i++) total = add_sat(total, __builtin_amdgcn_readlane(wave_scan(look<ROWS, UNIT>(p, i).items), 63));
+  return total;
+}
+
+// Element `at`, the same for the whole wavefront, of something no kernel writes meanwhile: through the scalar cache, past the
+// queue of vector loads (which come back in order: behind a page's worth of them this one number would wait for all).
+template <class T>
+__device__ __forceinline__ T scalar(const T *from, long long at) {
+  typedef const __attribute__((address_space(4))) T *constant;
+  return *(constant)(uintptr_t)(from + at);
+}
+
+// A number that all lanes have alike, in a scalar register.
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+
+// Trees: which of 32 tokens from `at` on (counted from the sequence's first row; those before it are seen by all) a row sees, as bits.
+__device__ __forceinline__ unsigned tree_bits(const int *row, int words, int at) {
+  const int w = at >> 5;
+  auto word = [&](int i) { return i < 0 ? ~0u : i < words ? (unsigned)row[i] : 0u; };
+  return __builtin_amdgcn_alignbit(word(w + 1), word(w), at & 31);
+}
+
+// ---- bytes of pages ----------------------------------------------------------------------------
 // The least power of two c >= 2^-100 with amax <= 448 c (448 = 0.875 * 2^9).
 __device__ __forceinline__ float page_scale(float amax) {
   const int bits = __float_as_int(amax);
@@ -134,6 +246,9 @@ inline int check_rows(const char *who, const char *name, int64_t offset, int64_t
   if (offset % 4 || stride % 4) return fail(WDH_EINVAL, "%s: offset and stride of %s must be multiples of 4 elements", who, name);
   return WDH_OK;
 }
+
+// Attention of trees (kv_tree.hip): rows of p.mask.
+int attend_trees(const char *who, AttendParams &p, int d);
 
 }  // namespace kv
 }  // namespace wdh

@@ -139,100 +139,7 @@ __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
 }
 
 // ---- attention -------------------------------------------------------------------------------
-struct AttendParams {
-  Sequences q;
-  const float *Q;
-  long long q_stride;
-  const unsigned char *KP, *VP;
-  const float *KS, *VS;
-  float *Y;
-  int heads, kv_heads;
-  wdh::FastDiv group;  // queries that share a head of the cache
-  float scale;     // alpha * log2(e): powers are taken of two
-  int wgs;         // workgroups for each head of the cache (0: one for each item, which works on the whole of it)
-  float *partial;  // results [workgroup][2][kv head][16][D] of items that more than one workgroup works on (null: there are none),
-  float *stats;    // and their tops and sums [workgroup][2][kv head][16][2]
-  const int *mask; // trees: [tokens][words], bit j: the row sees row j of its sequence
-  int words;
-};
-
-// Trees: which of 32 tokens from `at` on (counted from the sequence's first row; those before it are seen by all) a row sees, as bits.
-__device__ __forceinline__ unsigned tree_bits(const int *row, int words, int at) {
-  const int w = at >> 5;
-  auto word = [&](int i) { return i < 0 ? ~0u : i < words ? (unsigned)row[i] : 0u; };
-  return __builtin_amdgcn_alignbit(word(w + 1), word(w), at & 31);
-}
-
-// Work of attention: items of 16 rows (a row is a token and one of the queries that share a head of the cache), each as many units
-// of four pages (one for each wavefront of a workgroup) as its sequence has.  The units of all items stand in a row, and every
-// workgroup takes `share` neighbouring ones: all end at the same time, whatever the sequences' lengths.
-constexpr int MOST_UNITS = 1 << 30;
 constexpr float LARGE_SCORE = 0x1p22f;  // from here on (as powers of two) half a step of fp32 is a quarter of an exponent and more
-struct Work {
-  Place s;
-  int item, unit, units;  // the item, the unit of it that was asked for, and how many it has
-  int before;             // units in front of the item
-  int share, total;
-};
-__device__ __forceinline__ int items_of(const Place &s, int group) { return s.n ? (int)(((long long)s.n * group + 15) / 16) : 0; }
-__device__ __forceinline__ int units_of(const Place &s) { return (s.len + 4 * PAGE - 1) / (4 * PAGE); }
-// 64 sequences side by side, a lane to each; upto: units of these up to and with the lane's.
-struct Look {
-  Place mine;
-  int items, units, upto;
-};
-__device__ __forceinline__ Look look(const AttendParams &p, int round) {
-  Look l;
-  l.mine = sequence(p.q, 64 * round + fresh(threadIdx.x & 63));
-  l.items = items_of(l.mine, p.group.d);
-  l.units = units_of(l.mine);
-  l.upto = wave_scan(l.items * l.units);
-  return l;
-}
-__device__ __forceinline__ int total_units(const AttendParams &p, const Look &first) {
-  int total = __builtin_amdgcn_readlane(first.upto, 63);
-  for (int i = 1; i < (p.q.seqs + 63) / 64; i++) total = add_sat(total, __builtin_amdgcn_readlane(look(p, i).upto, 63));
-  return total <= MOST_UNITS ? total : 0;  // (more than the host allows: numbers that contradict each other)
-}
-// The item that holds unit number `index` of all (or, by_item, item number `index`); s.n = 0 behind the last.
-__device__ __forceinline__ Work locate_work(const AttendParams &p, const Look &first, int index, bool by_item) {
-  Work w;
-  int before = 0, before_items = 0;
-  Look l = first;
-  for (int i = 0; i < (p.q.seqs + 63) / 64; i++) {
-    if (i) l = look(p, i);
-    const int upto = add_sat(before, l.upto), upto_items = by_item ? add_sat(before_items, wave_scan(l.items)) : 0;
-    const unsigned long long has = __ballot(index < (by_item ? upto_items : upto));
-    if (has) {
-      const int at = __ffsll(has) - 1;
-      w.s.seq = __builtin_amdgcn_readlane(l.mine.seq, at);
-      w.s.row0 = __builtin_amdgcn_readlane(l.mine.row0, at);
-      w.s.n = __builtin_amdgcn_readlane(l.mine.n, at);
-      w.s.len = __builtin_amdgcn_readlane(l.mine.len, at);
-      w.units = __builtin_amdgcn_readlane(l.units, at);
-      const int begin = __builtin_amdgcn_readlane(upto - l.items * l.units, at);
-      w.item = by_item ? index - __builtin_amdgcn_readlane(upto_items - l.items, at) : (index - begin) / w.units;
-      w.before = begin + w.item * w.units;
-      w.unit = by_item ? 0 : index - w.before;
-      return w;
-    }
-    before = __builtin_amdgcn_readlane(upto, 63);
-    before_items = __builtin_amdgcn_readlane(upto_items, 63);
-  }
-  w.s = Place{0, 0, 0, 0, 0};
-  return w;
-}
-
-// Element `at`, the same for the whole wavefront, of something no kernel writes meanwhile: through the scalar cache, past the
-// queue of vector loads (which come back in order: behind a page's worth of them this one number would wait for all).
-template <class T>
-__device__ __forceinline__ T scalar(const T *from, long long at) {
-  typedef const __attribute__((address_space(4))) T *constant;
-  return *(constant)(uintptr_t)(from + at);
-}
-
-// A number that all lanes have alike, in a scalar register.
-__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 
 // Over the four lanes that share lane % 16: a swap of a register with itself leaves both halves' values side by side.
 template <class Op>
@@ -318,7 +225,7 @@ __device__ __forceinline__ void split2_f16(const float (&x)[8], f16x8 (&part)[2]
 // Bound: memory where rows are few (32 tokens behind 500 to 8500, 32 heads of 128 on 8: 56 us, 5.3 TB/s; a copy of this kernel that only
 // loads takes 55; pages brought line by line and turned in LDS: 61), so three exact parts cost nothing that two would not; with all rows in use, instructions (1.3 us for a page of each
 // wavefront, two workgroups to a CU).
-template <int D, bool TREE>
+template <int D>
 __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
   constexpr int STEPS = D / 32, CH = D >= 64 ? D / 64 : 1, DT = D / 16;
   constexpr int OP = D + 4;
@@ -329,16 +236,16 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, g = lane >> 4;
   const unsigned k_lane = (16 * (i16 >> 2) + (i16 & 3)) * D + (D >= 64 ? 16 : 8) * g, v_lane = i16 * PAGE + 16 * g;  // (of a page)
   const int head = blockIdx.y;
-  const Look first = look(p, 0);
+  const Look first = look<16, 4>(p, 0);
   const Minus minus = minus_one();
   Work w;
   int unit, units_end;
   if (p.wgs) {
-    const int total = total_units(p, first), share = (total + p.wgs - 1) / p.wgs;
+    const int total = total_units<16, 4>(p, first), share = (total + p.wgs - 1) / p.wgs;
     unit = blockIdx.x * share;
     units_end = total - unit < share ? total : unit + share;
   } else {
-    w = locate_work(p, first, gridDim.x - 1 - blockIdx.x, true);  // (a prompt's last items are its longest)
+    w = locate_work<16, 4>(p, first, gridDim.x - 1 - blockIdx.x, true);  // (a prompt's last items are its longest)
     unit = w.before;
     units_end = w.s.n ? w.before + w.units : unit;
   }
@@ -349,22 +256,16 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     w.before = unit;
     w.unit = 0;
   } else if (p.wgs) {
-    w = locate_work(p, first_segment ? first : look(p, 0), unit, false);
+    w = locate_work<16, 4>(p, first_segment ? first : look<16, 4>(p, 0), unit, false);
     if (w.s.n == 0) return;  // (numbers that contradict each other)
   }
   const Place s = w.s;
   // this lane's row
   const int flat = w.item * 16 + fresh(i16), token = wdh::fdiv(flat, p.group), sub = flat - token * group;
   const bool live = token < s.n;
-  const int limit = live ? s.len - s.n + token : -1;  // its last key (trees: see `sees`)
-  const int last_token = wdh::fdiv(w.item * 16 + 15, p.group), first_limit = TREE ? s.len - s.n - 1 : s.len - s.n + wdh::fdiv(w.item * 16, p.group);
-  const int last_key = TREE ? s.len - 1 : s.len - s.n + (last_token < s.n ? last_token : s.n - 1);
-  // trees: which of the 16 keys from `key` on the lane's row sees
-  auto sees = [&](int key) {
-    const int behind = s.len - key;
-    const unsigned bits = tree_bits(p.mask + (long long)(s.row0 + (live ? token : 0)) * p.words, p.words, key - (s.len - s.n));
-    return live ? bits & (behind >= 16 ? 0xffffu : behind > 0 ? (1u << behind) - 1u : 0u) : 0u;
-  };
+  const int limit = live ? s.len - s.n + token : -1;  // its last key
+  const int last_token = wdh::fdiv(w.item * 16 + 15, p.group), first_limit = s.len - s.n + wdh::fdiv(w.item * 16, p.group);
+  const int last_key = s.len - s.n + (last_token < s.n ? last_token : s.n - 1);
   const int seg_end = w.units - w.unit < units_end - unit ? w.units : w.unit + (units_end - unit);  // in units of the item
   const int begin = 4 * w.unit, seen = last_key / PAGE + 1, end = seen < 4 * seg_end ? seen : 4 * seg_end;
   const bool alone = w.unit == 0 && seg_end == w.units;  // the whole item is this workgroup's
@@ -447,12 +348,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     float x[16], most = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; e++) x[e] = sc[e >> 2][e & 3];
-    unsigned seen_bits = 0xffffu;
-    if (TREE && !whole) {
-      seen_bits = sees(pg * PAGE + 16 * g);
-#pragma unroll
-      for (int e = 0; e < 16; e++) most = fmaxf(most, (seen_bits >> e) & 1 ? x[e] * c : -INFINITY);
-    } else if (!whole) {
+    if (!whole) {
       const int ahead = limit - pg * PAGE - 16 * g;
 #pragma unroll
       for (int e = 0; e < 16; e++) most = fmaxf(most, e <= ahead ? x[e] * c : -INFINITY);
@@ -479,10 +375,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
     }
 #pragma unroll
     for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -ref));
-    if (TREE && !whole) {
-#pragma unroll
-      for (int e = 0; e < 16; e++) x[e] = (seen_bits >> e) & 1 ? x[e] : 0.0f;
-    } else if (!whole) {
+    if (!whole) {
       const int ahead = fresh(limit) - pg * PAGE - 16 * g;
 #pragma unroll
       for (int e = 0; e < 16; e++) x[e] = e <= ahead ? x[e] : 0.0f;
@@ -527,8 +420,8 @@ __global__ __launch_bounds__(256, 2) void attend_rows(AttendParams p) {
 #pragma unroll 1
       for (int i = 0; i < 4 * DT; i++)
 #pragma unroll 1
-        for (int j = 0; j < PAGE && pg * PAGE + j <= (TREE ? last_key : limit); j++)
-          if ((!TREE || (sees(pg * PAGE + j) & 1)) && (vp[(16 * (i >> 2) + (i & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << i;
+        for (int j = 0; j < PAGE && pg * PAGE + j <= limit; j++)
+          if ((vp[(16 * (i >> 2) + (i & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << i;
 #pragma unroll
       for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -592,9 +485,9 @@ __global__ __launch_bounds__(THREADS) void attend_join(AttendParams p) {
   constexpr int LANES = D / 4, SIDE = THREADS / LANES;
   __shared__ __attribute__((aligned(16))) f32x4 results[SIDE][LANES];
   __shared__ float totals[SIDE], tops[SIDE];
-  const Look first = look(p, 0);
-  const int head = blockIdx.y, total_u = total_units(p, first), share = (total_u + p.wgs - 1) / p.wgs;
-  const Work w = locate_work(p, first, blockIdx.x, true);
+  const Look first = look<16, 4>(p, 0);
+  const int head = blockIdx.y, total_u = total_units<16, 4>(p, first), share = (total_u + p.wgs - 1) / p.wgs;
+  const Work w = locate_work<16, 4>(p, first, blockIdx.x, true);
   if (w.s.n == 0 || share == 0) return;
   const int from_wg = w.before / share, to_wg = (w.before + w.units - 1) / share;
   if (from_wg == to_wg) return;
@@ -697,7 +590,7 @@ __device__ __forceinline__ Place many_item(const AttendParams &p, int rank, int 
 // Bound: instructions.  A page takes 64 matrix ones of 32 cycles a wavefront and about as long of others (conversions of keys and values,
 // powers, splitting weights), which alternate more than they overlap: matrix cores busy 41 % of the time (three prompts of 1200 to 4000
 // tokens, 16 heads of 128 on 4: 243 us, 469 TFLOP/s counted once).
-template <int D, bool TREE>
+template <int D>
 __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   constexpr int QN = D / 32, DT = D / 32;           // runs of 32 elements of d in a key; blocks of 32 rows of O^T
   constexpr int KPIECES = PAGE * D / 16 / 256 > 0 ? PAGE * D / 16 / 256 : 1;  // 16-byte pieces a thread brings of a page's keys, and of its values
@@ -713,18 +606,12 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   const int row0 = s.index * MANY, flat = row0 + 32 * wave + li, token = wdh::fdiv(flat, p.group), sub = flat - token * group;
   const bool live = token < s.n;
   const int limit = live ? past + token : -1;
-  const int first_limit = TREE ? past - 1 : past + wdh::fdiv(row0, p.group);  // of the item's first row
-  const int last_token = wdh::fdiv(row0 + MANY - 1, p.group), last_key = TREE ? s.len - 1 : past + (last_token < s.n ? last_token : s.n - 1);
+  const int first_limit = past + wdh::fdiv(row0, p.group);  // of the item's first row
+  const int last_token = wdh::fdiv(row0 + MANY - 1, p.group), last_key = past + (last_token < s.n ? last_token : s.n - 1);
   const int seen = last_key / PAGE + 1, begin = (int)((long long)seen * blockIdx.y / gridDim.y), end = (int)((long long)seen * (blockIdx.y + 1) / gridDim.y);
   // this wavefront's own pages end earlier
-  const int wave_token = wdh::fdiv(row0 + 32 * wave, p.group), wave_last = wdh::fdiv(row0 + 32 * wave + 31, p.group), wave_first = TREE ? past - 1 : past + wave_token;
-  const int wave_end = wave_token < s.n ? TREE ? seen : (past + (wave_last < s.n ? wave_last : s.n - 1)) / PAGE + 1 : 0;
-  // trees: which of the 32 keys from `key` on the lane's row sees
-  auto sees = [&](int key) {
-    const int behind = s.len - key;
-    const unsigned bits = tree_bits(p.mask + (long long)(s.row0 + (live ? token : 0)) * p.words, p.words, key - past);
-    return live ? bits & (behind >= 32 ? ~0u : behind > 0 ? (1u << behind) - 1u : 0u) : 0u;
-  };
+  const int wave_token = wdh::fdiv(row0 + 32 * wave, p.group), wave_last = wdh::fdiv(row0 + 32 * wave + 31, p.group), wave_first = past + wave_token;
+  const int wave_end = wave_token < s.n ? (past + (wave_last < s.n ? wave_last : s.n - 1)) / PAGE + 1 : 0;
   const int *table = p.q.table + (long long)s.seq * p.q.max_pages;
 
   struct Page { long long at; float ks, vs; bool known; };
@@ -838,12 +725,6 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
   // What a row does not see counts for nothing; the largest of the rest.
   auto mask = [&](f32x16 &sc, int pg, int t) {
     if (pg * PAGE + PAGE - 1 <= wave_first) return;
-    if constexpr (TREE) {
-      const unsigned bits = sees(pg * PAGE + 32 * t + 16 * half);
-#pragma unroll
-      for (int r = 0; r < 16; r++) sc[r] = (bits >> r) & 1 ? sc[r] : -INFINITY;
-      return;
-    }
     const int ahead = limit - pg * PAGE - 32 * t - 16 * half;
 #pragma unroll
     for (int r = 0; r < 16; r++) sc[r] = r <= ahead ? sc[r] : -INFINITY;
@@ -940,13 +821,13 @@ __global__ __launch_bounds__(256, 2) void attend_many(AttendParams p) {
 #pragma unroll 1
         for (int e = 0; e < 16; e++)
 #pragma unroll 1
-          for (int j = 0; j < PAGE && pg * PAGE + j <= (TREE ? last_key : limit); j++)
-            if ((!TREE || (sees(pg * PAGE + j) & 1)) && (vp[(32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << e;
+          for (int j = 0; j < PAGE && pg * PAGE + j <= limit; j++)
+            if ((vp[(32 * i + 8 * (e >> 2) + 4 * half + (e & 3)) * PAGE + j] & 0x7f) == 0x7f) nan |= 1u << e;
 #pragma unroll
         for (int e = 0; e < 16; e++) o[i][e] = (nan >> e) & 1 ? NAN : o[i][e];
       }
     }
-    if (active && !now.known && (TREE ? (sees(pg * PAGE) | sees(pg * PAGE + 32)) != 0 : limit >= pg * PAGE)) sum = NAN;
+    if (active && !now.known && limit >= pg * PAGE) sum = NAN;
     now = then;
     then = after;
     after = later;
@@ -1019,8 +900,7 @@ __global__ __launch_bounds__(256) void attend_many_join(AttendParams p, int part
 template <int D>
 int launch_many(const AttendParams &p, long long items, int parts) {
   hipStream_t st = wdh::stream();
-  if (p.mask) hipLaunchKernelGGL((attend_many<D, true>), dim3((unsigned)(items * p.kv_heads), (unsigned)parts), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((attend_many<D, false>), dim3((unsigned)(items * p.kv_heads), (unsigned)parts), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((attend_many<D>), dim3((unsigned)(items * p.kv_heads), (unsigned)parts), dim3(256), 0, st, p);
   WDH_LAUNCH_CHECK();
   if (parts > 1) {
     hipLaunchKernelGGL((attend_many_join<D>), dim3((unsigned)items, (unsigned)p.kv_heads, MANY * D / 1024), dim3(256), 0, st, p, parts);
@@ -1032,9 +912,7 @@ int launch_many(const AttendParams &p, long long items, int parts) {
 template <int D>
 int launch_attend(const AttendParams &p, long long items) {
   hipStream_t st = wdh::stream();
-  const dim3 wgs((unsigned)(p.wgs ? p.wgs : items), (unsigned)p.kv_heads);
-  if (p.mask) hipLaunchKernelGGL((attend_rows<D, true>), wgs, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((attend_rows<D, false>), wgs, dim3(256), 0, st, p);
+  hipLaunchKernelGGL((attend_rows<D>), dim3((unsigned)(p.wgs ? p.wgs : items), (unsigned)p.kv_heads), dim3(256), 0, st, p);
   WDH_LAUNCH_CHECK();
   if (p.partial) {
     // (an item of hundreds of shares is a wide workgroup's work, one of a few shares a small one's)
@@ -1159,6 +1037,7 @@ int attention(const char *who, wdh_buf hQ, int64_t q_offset, int64_t q_stride, w
   p.Y = (float *)py;
   p.heads = heads; p.kv_heads = kv_heads; p.group = wdh::make_fastdiv(heads / kv_heads);
   p.scale = alpha * 1.44269504088896341f;
+  if (p.mask) return attend_trees(who, p, d);
   // items of 16 or 128 rows: a sequence of n tokens has ceil(n group / rows); whichever bound of their number is lower
   auto items_of_rows = [&](int rows) {
     const long long loose = (long long)tokens * p.group.d / rows + seqs, tight = (long long)tokens * ((p.group.d + rows - 1) / rows);
