@@ -18,6 +18,7 @@ using namespace wdh::fp8;
 using namespace wdh::kv;
 using wdh::fail;
 
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
@@ -71,6 +72,23 @@ __device__ __forceinline__ float both_halves(float v, float (*op)(float, float))
   auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+// The largest of the LANES neighbouring lanes that share a row, in all of them.
+template <int CTRL>
+__device__ __forceinline__ unsigned max_with(unsigned v) {
+  const unsigned other = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+  return v > other ? v : other;
+}
+template <int LANES>
+__device__ __forceinline__ unsigned lanes_max(unsigned v) {
+  using namespace wdh::rowmath;
+  v = max_with<DPP_HALF_MIRROR>(max_with<DPP_XOR2>(max_with<DPP_XOR1>(v)));
+  if constexpr (LANES > 8) v = max_with<DPP_MIRROR>(v);
+  if constexpr (LANES > 16) {
+    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = b[0] > b[1] ? b[0] : b[1];
+  }
+  return v;
+}
 __device__ __forceinline__ float max2(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float add2(float a, float b) { return a + b; }
 
@@ -105,9 +123,9 @@ struct Joint {
 template <int D, int RB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParams p, Joint *joints, int most_joints) {
   constexpr int STEPS = D / 16, VT = D / 32, S = WAVES / RB, ROWS = 32 * RB, OP = D + 4;
-  // Pages pass through LDS: in operand order a page's rows are 16-byte pieces of 32 lines to a load, and wavefronts that each ask for them
-  // fill the L1 cache's time with looking up lines.  Four blocks have two places for a page, and a barrier a page; two have one place, and two barriers; a
-  // block's own wavefront needs none.
+  // Pages pass through LDS, from where all blocks of rows read them: in operand order a page's rows are 16-byte pieces of 32 lines to a load, and where every
+  // wavefront asked for them itself the L1 cache looked up lines 85 % of the time.  (That took as long, but left no registers to load ahead.)
+  // Four blocks have two places for a page, and a barrier a page; two have one place, and two barriers; a block's own wavefront needs none.
   constexpr int BUFS = RB == 4 ? 2 : 1;
   constexpr int CHUNKS = PAGE * D / 1024;          // what a wavefront brings of a page at a time
   struct Input { f16x8 q[RB][STEPS][2][64]; unsigned char keys[S][BUFS][PAGE * D], values[S][BUFS][PAGE * D]; };
@@ -161,39 +179,48 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
     return live ? bits & (behind >= 16 ? 0xffffu : behind > 0 ? (1u << behind) - 1u : 0u) : 0u;
   };
 
-  // (asked for first: the way to the first page takes three rounds of loads)
-  float x[STEPS][8];
-  {
-    const float *qrow = p.Q + (long long)(s.row0 + (live ? token : 0)) * p.q_stride + (long long)(head * group + sub) * D;
-#pragma unroll
-    for (int i = 0; i < STEPS; i++) {
-      const int d0 = 32 * (i / 2) + 16 * half + 8 * (i & 1);
-      const f32x4 a = *reinterpret_cast<const f32x4 *>(qrow + d0), b = *reinterpret_cast<const f32x4 *>(qrow + d0 + 4);
-#pragma unroll
-      for (int e = 0; e < 4; e++) x[i][e] = a[e], x[i][4 + e] = b[e];
-    }
-  }
   // The wavefront's pages, 64 at a time, a lane to each: numbers and scales come in two rounds of loads, and none is waited for in between (scalar loads
   // would be, with every read of LDS: both are counted alike, and scalar ones return in any order).
   int held_id = 0, taken = 0;
   float held_ks = 0.0f, held_vs = 0.0f;
   struct Page { long long at; float ks, vs; };
+  auto number_of = [&](int i) {  // (behind the last: the last once more, which is loaded and not used: no branch about registers)
+    const int at = begin + stream + S * i;
+    return table[at < end ? at : end - 1];
+  };
+  auto cell_of = [&](int i) { return (long long)__builtin_amdgcn_readlane(held_id, i) * p.kv_heads + head; };
+  auto hold = [&](int id) {
+    const bool known = id >= 0 && id < p.q.pages;
+    held_id = known ? id : 0;
+    held_ks = p.KS[(long long)held_id * p.kv_heads + head];
+    held_vs = p.VS[(long long)held_id * p.kv_heads + head];
+    if (!known) held_vs = 0.0f;
+  };
+  // (a page that is not there, or has no scale, makes its rows NaN, at the end of its turn)
+  auto check_held = [&]() {
+    if (!(held_ks > 0.0f && held_ks <= FLT_MAX) || !(held_vs > 0.0f && held_vs <= FLT_MAX)) held_ks = FLT_MIN, held_vs = 0.0f;
+  };
   auto next_page = [&]() {
     const int which = taken++ & 63;
-    if (which == 0) {
-      const int at = begin + stream + S * (taken - 1 + lane);
-      const int id = table[at < end ? at : end - 1];  // (behind the last: the last once more, which is loaded and not used: no branch about registers)
-      const bool known = id >= 0 && id < p.q.pages;
-      const long long cell = (long long)(known ? id : 0) * p.kv_heads + head;
-      held_ks = p.KS[cell];
-      held_vs = p.VS[cell];
-      // (a page that is not there, or has no scale, makes its rows NaN, at the end of its turn)
-      if (!known || !(held_ks > 0.0f && held_ks <= FLT_MAX) || !(held_vs > 0.0f && held_vs <= FLT_MAX)) held_ks = FLT_MIN, held_vs = 0.0f;
-      held_id = known ? id : 0;
+    if (which == 0 && taken > 1) {
+      hold(number_of(taken - 1 + lane));
+      check_held();
     }
-    return Page{(long long)__builtin_amdgcn_readlane(held_id, which) * p.kv_heads + head, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held_ks), which)),
-                __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held_vs), which))};
+    return Page{cell_of(which), __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held_ks), which)),
+              __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held_vs), which))};
   };
+  // The way to the first page: its number, and the queries at the same time, a row to D / 4 lanes.
+  const int at_lane = fresh(lane), first_id = number_of(at_lane);
+  constexpr int LANES = D / 4, Q_ROWS = 64 / LANES, Q_LOADS = 32 / S / Q_ROWS;
+  f32x4 x[Q_LOADS];
+#pragma unroll
+  for (int i = 0; i < Q_LOADS; i++) {
+    const int flat_q = row0 + stream * (32 / S) + Q_ROWS * i + at_lane / LANES, t = wdh::fdiv(flat_q, p.group), tk = t < s.n ? t : 0;
+    x[i] = *reinterpret_cast<const f32x4 *>(p.Q + (long long)(s.row0 + tk) * p.q_stride + (long long)(head * group + flat_q - t * group) * D + 4 * (at_lane % LANES));
+  }
+  hold(first_id);
+  // (lanes that write a row's elements would meet in one bank, 16 at a time: they write them two at a time; 16 sequences of 32 nodes 109 -> 106 us)
+  auto query_place = [](int block, int half, int row) { return 32 * half + (row ^ (2 * block + half)); };
   // A row's 16-byte pieces change places in LDS, so that rows of a tile lie on different banks.  Loads go there directly, a lane's 16 bytes behind the
   // lane's before it: so it is the pieces' addresses in memory that change.
   auto key_piece = [](int row, int piece) { return D == 128 ? piece ^ (row & 7) : D == 64 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1); };
@@ -209,42 +236,40 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
   auto bring_keys = [&](long long at, int buf) { bring(p.KP + at * (PAGE * D) + k_from, lds.in.keys[stream][buf]); };
   auto bring_values = [&](long long at, int buf) { bring(p.VP + at * (PAGE * D) + v_from, lds.in.values[stream][buf]); };
   int pg = begin + stream;
-  Page now = next_page(), then = next_page();
-  bring_keys(now.at, 0);
-  bring_values(now.at, 0);
+  bring_keys(cell_of(0), 0);
+  bring_values(cell_of(0), 0);
   if (lane < 2) bad_values[stream][lane] = 0;
 
   // Queries times alpha log2(e) in two float16 parts, a row brought to [2^14, 2^15) by a power of two: what two parts leave out is at most 2^-23 of an
   // element, or 2^-39 of the row's largest one.
-  float row_scale;
-  {
-    float most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < STEPS; i++)
+  for (int i = 0; i < Q_LOADS; i++) {
+    unsigned most = 0;  // (numbers without their signs, as integers)
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        x[i][e] *= p.scale;
-        most = fmaxf(most, finite_abs(x[i][e]));
-      }
-    const int exponent = exponent_of(both_halves(most, max2));  // (of zeros and of subnormal rows: -127)
+    for (int e = 0; e < 4; e++) {
+      x[i][e] *= p.scale;
+      most = max(most, __float_as_uint(fabsf(x[i][e])));  // (not finite: so are its scores, whatever the others')
+    }
+    const int exponent = exponent_of(__uint_as_float(lanes_max<LANES>(most)));  // (of zeros and of subnormal rows: -127)
     const int up = 14 - exponent < 126 ? 14 - exponent : 126;
-    row_scale = power_of_two(-up);
+    const int r = stream * (32 / S) + Q_ROWS * i + at_lane / LANES, d = 4 * (at_lane % LANES);
+    union { f16x2 h[2]; f16x4 v; } parts[2];
 #pragma unroll
-    for (int i = 0; i < STEPS; i++)
-      if (i % S == stream) {
-        f16x8 parts[2];
+    for (int e = 0; e < 2; e++) {
+      const f32x2 y = {x[i][2 * e] * power_of_two(up), x[i][2 * e + 1] * power_of_two(up)};
+      parts[0].h[e] = __builtin_convertvector(y, f16x2);
+      parts[1].h[e] = __builtin_convertvector(f32x2{less_low(y[0], parts[0].h[e]), less_high(y[1], parts[0].h[e])}, f16x2);
+    }
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float y = x[i][e] * power_of_two(up);
-          parts[0][e] = (_Float16)y;
-          parts[1][e] = (_Float16)(y - (float)parts[0][e]);
-        }
-        lds.in.q[rb][i][0][lane] = parts[0];
-        lds.in.q[rb][i][1][lane] = parts[1];
-      }
+    for (int part = 0; part < 2; part++)
+      reinterpret_cast<f16x4 *>(&lds.in.q[rb][2 * (d / 32) + (d >> 3 & 1)][part][query_place(d / 32, d >> 4 & 1, r)])[d >> 2 & 1] = parts[part].v;
+    if (d == 0) tops[rb][r] = power_of_two(-up);
   }
+  check_held();
+  Page now = next_page(), then = next_page();
   loads_left<0>();
   __syncthreads();
+  const float row_scale = tops[rb][li];
 
   f32x16 o[VT];
 #pragma unroll
@@ -297,7 +322,8 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
     // place beside them, and not in a branch on the way.)
     for (; HAS_ROWS;) {
       // (the queries' place hidden from the compiler, which would hold them all in registers that the loop has better use for)
-      const f16x8 *q = &lds.in.q[rb][0][0][0] + fresh(lane);
+      const int hidden = fresh(lane), hidden_row = hidden & 31;
+      auto query = [&](int i, int part) { return lds.in.q[rb][i][part][query_place(i / 2, hidden >> 5, hidden_row)]; };
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -306,7 +332,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
       i32x4 piece[2];
 #pragma unroll
       for (int t = 0; t < 2; t++) piece[t] = key_at(t, 0);
-      f16x8 q_low = q[64], q_high = q[0], kw[2];
+      f16x8 q_low = query(0, 1), q_high = query(0, 0), kw[2];
 #pragma unroll
       for (int t = 0; t < 2; t++) kw[t] = widen_f16(piece[t][0], piece[t][1]);
       __builtin_amdgcn_sched_barrier(0);
@@ -315,7 +341,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
         f16x8 next_low, next_high, next_kw[2];
         i32x4 next_piece[2];
         if (i + 1 < STEPS) {
-          next_low = q[64 * (2 * i + 3)], next_high = q[64 * (2 * i + 2)];
+          next_low = query(i + 1, 1), next_high = query(i + 1, 0);
 #pragma unroll
           for (int t = 0; t < 2; t++) {
             if (i % 2 == 0 && i + 2 < STEPS) next_piece[t] = key_at(t, i / 2 + 1);
@@ -344,7 +370,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
       if constexpr (TAIL)
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const unsigned bits = bits_now[t];
+          const unsigned bits = fresh(bits_now[t]);  // (not tested before the loop, into more scalar registers than there are)
 #pragma unroll
           for (int e = 0; e < 16; e++) sc[t][e] = (bits >> e) & 1 ? sc[t][e] : -INFINITY;
         }
@@ -489,40 +515,36 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
     sums[wave][li] = sum;
   }
   __syncthreads();
-  for (int cell = threadIdx.x; cell < ROWS * (D / 4); cell += 64 * WAVES) {
-    const int row = cell / (D / 4), d = cell % (D / 4) * 4, block = row / 32, r = row % 32;
-    const int flat_row = w.item * ROWS + row, tk = wdh::fdiv(flat_row, p.group);
-    if (tk >= s.n) continue;
-    float most = -INFINITY;
+  const int thread = fresh(threadIdx.x);  // (what is computed of it is computed here, and holds no registers before)
+  const long long place = ((2LL * blockIdx.x + (first_segment ? 0 : 1)) * p.kv_heads + head) * ROWS;  // (an item of several workgroups is the first or the last of each)
+  if (thread < ROWS) {
+    const int block = thread / 32, r = thread % 32;
+    float most = -INFINITY, total = 0.0f;
 #pragma unroll
     for (int i = 0; i < S; i++) most = fmaxf(most, tops[block + RB * i][r]);
     const float ref = most == -INFINITY ? 0.0f : most;
-    float weight[S], total = 0.0f;
 #pragma unroll
-    for (int i = 0; i < S; i++) {
-      weight[i] = sums[block + RB * i][r] * __builtin_amdgcn_exp2f(tops[block + RB * i][r] - ref);
-      total += weight[i];
-    }
-    const float part = total == 0.0f ? 0.0f : 1.0f / total;
+    for (int i = 0; i < S; i++) total += sums[block + RB * i][r] *= __builtin_amdgcn_exp2f(tops[block + RB * i][r] - ref);
+    tops[block][r] = total == 0.0f ? 0.0f : 1.0f / total;
+    if (!alone && p.partial) *reinterpret_cast<f32x2 *>(p.stats + 2 * (place + thread)) = f32x2{most, total};
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int cell = thread; cell < ROWS * LANES; cell += 64 * WAVES) {
+    const int row = cell / LANES, d = 4 * (cell % LANES), block = row / 32, r = row % 32;
+    const int flat_row = w.item * ROWS + row, tk = wdh::fdiv(flat_row, p.group);
+    const float part = tops[block][r];
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < S; i++) {
       const f32x4 x = *reinterpret_cast<const f32x4 *>(&lds.outs[block + RB * i][r * OP + d]);
-      const float f = weight[i] * part;
+      const float f = sums[block + RB * i][r] * part;
 #pragma unroll
       for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(f, x[e], y[e]);
     }
-    if (alone) {
-      *reinterpret_cast<f32x4 *>(p.Y + ((long long)(s.row0 + tk) * p.heads + head * group + (flat_row - tk * group)) * D + d) = y;
-    } else if (p.partial) {
-      // (an item that more than one workgroup works on is the first or the last of each)
-      const long long at = ((2LL * blockIdx.x + (first_segment ? 0 : 1)) * p.kv_heads + head) * ROWS + row;
-      *reinterpret_cast<f32x4 *>(p.partial + at * D + d) = y;
-      if (d == 0) {
-        p.stats[2 * at] = most;
-        p.stats[2 * at + 1] = total;
-      }
-    }
+    if (tk >= s.n) continue;
+    if (alone) *reinterpret_cast<f32x4 *>(p.Y + ((long long)(s.row0 + tk) * p.heads + head * group + (flat_row - tk * group)) * D + d) = y;
+    else if (p.partial) *reinterpret_cast<f32x4 *>(p.partial + (place + row) * D + d) = y;
   }
   if (joints && threadIdx.x == 0 && w.unit == 0 && w.ordinal < most_joints)
     joints[w.ordinal * p.kv_heads + head] =
@@ -580,15 +602,18 @@ __global__ __launch_bounds__(256) void tree_join(AttendParams p, const Joint *jo
 }
 
 template <int D, int RB, int WAVES>
-int launch(const char *who, AttendParams &p) {
+int launch(const char *who, AttendParams &p, long long rows) {
   constexpr int ROWS = 32 * RB, UNIT = WAVES / RB;
   const long long tokens = p.q.tokens, loose = tokens * p.group.d / ROWS + p.q.seqs, tight = tokens * ((p.group.d + ROWS - 1) / ROWS);
   const long long items = loose < tight ? loose : tight, most_units = (p.q.max_pages + UNIT - 1) / UNIT, units = items * most_units;
   if (items * p.kv_heads > 0xffffffLL / 2 || units > MOST_UNITS) return fail(WDH_EINVAL, "%s: too many rows of tables so wide", who);
-  // as many workgroups as the chip holds at a time, or as there can be units
-  const long long resident = 8LL / WAVES * wdh::compute_units() / p.kv_heads;
+  // As many workgroups as the chip holds at a time, or as there can be units.  Or one to each item, where the chip is full of them: the longest item's turns,
+  // less those that a share of all would be, have to be worth the join and the second item that a share has parts of (four turns or so).  Heads of 64 with
+  // 8 nodes and 500 to 1500 tokens each, shares / items: 64 sequences 25.2 / 21.6 us, with three times as many tokens 36.3 / 44.4, then 128 sequences 67 / 54.
+  const long long chip = 8LL / WAVES * wdh::compute_units(), resident = chip / p.kv_heads;
+  const long long likely = p.q.seqs * ((rows + ROWS - 1) / ROWS) * p.kv_heads, idle = (likely + chip - 1) / chip * chip - likely;
   p.wgs = (int)(units < resident ? units : resident > 0 ? resident : 1);
-  if (most_units <= 2 || most_units * 16 <= items * p.kv_heads) p.wgs = 0;
+  if (most_units == 1 || most_units * idle <= 4 * chip) p.wgs = 0;
   wdh_buf work = 0;
   Joint *joints = nullptr;
   if (p.wgs > 1) {  // (items of one unit are never cut)
@@ -614,9 +639,13 @@ int launch(const char *who, AttendParams &p) {
 template <int D>
 int launch_rows(const char *who, AttendParams &p) {
   const long long rows = ((long long)p.q.tokens * p.group.d + p.q.seqs - 1) / p.q.seqs;  // (of a sequence, on average)
-  if (rows <= 32) return launch<D, 1, D == 128 ? 8 : 4>(who, p);
-  if (rows <= 64) return launch<D, 2, 8>(who, p);
-  return launch<D, 4, 8>(who, p);
+  // More rows to an item read the cache fewer times, and are fewer and longer items.  32, 64 and 128 rows to an item (us), heads of 128, 4 of them in the cache:
+  //   32 sequences behind 1500 tokens: of 32 rows 22 / 28 / 34, of 64 rows 28 / 30 / 46, of 128 rows 52 / 36 / 50, of 192 rows 93 / 73 / 60
+  //   and one sequence of 512 rows, 2 heads: behind 6400 30 / 24 / 30, behind 25600 49 / 47 / 49, behind 102400 135 / 120 / 118
+  if (rows <= 32) return launch<D, 1, D == 128 ? 8 : 4>(who, p, rows);
+  const long long pages = p.q.seqs * ((rows + 127) / 128) * p.kv_heads * p.q.max_pages;  // for items of 128 rows, at most
+  if (rows <= 64 || pages < 20LL * wdh::compute_units()) return launch<D, 2, 8>(who, p, rows);
+  return launch<D, 4, 8>(who, p, rows);
 }
 
 }  // namespace
