@@ -95,6 +95,7 @@ def verify(p, draft, tokens, parents, uniform, starts):
     seqs = len(starts) - 1
     token, count, path = np.full(seqs, -7, np.int32), np.full(seqs, -7, np.int32), np.full(len(tokens), -7, np.int32)
     weigh = lambda x: np.where(x > 0, x.astype(np.float64), 0.0)
+    draft = None if draft is None else weigh(draft)
     for s in range(seqs):
         lo, n = int(starts[s]), int(starts[s + 1] - starts[s])
         if n <= 0:
@@ -113,7 +114,7 @@ def verify(p, draft, tokens, parents, uniform, starts):
                     follow = child
                     break
                 if draft is not None:
-                    left = weigh(left - mass * draft[lo + node].astype(np.float64))
+                    left = weigh(left - mass * draft[lo + node])
                     mass = left.sum()
                 elif real:
                     mass -= left[x]

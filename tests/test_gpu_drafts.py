@@ -331,6 +331,34 @@ def test_verify(ctx, vocab, new, most_children, drawn):
     check_verify(ctx, p, draft if drawn else None, *rest)
 
 
+@pytest.mark.parametrize("vocab,new,most_children", [(33279, [1], 1), (33280, [1], 1), (33281, [7], 1), (50001, [33], 3), (40003, [5, 1, 8], 1), (40962, [9, 33, 2], 3),
+                                                     (128000, [4, 6], 2)])
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify_of_long_rows(ctx, vocab, new, most_children, drawn):
+    """Rows that several workgroups sum."""
+    rng = np.random.default_rng(vocab + 7 * sum(new))
+    p, draft, tokens, parents, uniform, starts = drafts(rng, new, vocab, most_children, drawn)
+    for u in (uniform, np.zeros_like(uniform), np.full_like(uniform, 0.5), np.full_like(uniform, 1 - 2.0 ** -24)):
+        check_verify(ctx, p, draft if drawn else None, tokens, parents, u, starts)
+
+
+@pytest.mark.parametrize("vocab", [7, 40000])
+def test_verify_where_little_is_left(ctx, vocab):
+    """Rows of one token, of no number and of none, with drafts that leave all, one or nothing of them."""
+    n = 5
+    p, draft = np.zeros((3 * n, vocab), np.float32), np.zeros((3 * n, vocab), np.float32)
+    last = vocab - 1
+    p[:n, last] = 1                                                           # all in the last token
+    p[n:2 * n, 3], p[n:2 * n, 4] = np.nan, -np.inf                            # nothing
+    p[2 * n:, 2] = p[2 * n:, last] = 0.5
+    draft[:, 2] = draft[:, 4] = 0.5
+    parents, tokens = np.array([-1, 0, 0, 0, 1] * 3, np.int32), np.array([0, 2, 4, last, 2] * 3, np.int32)
+    starts = np.array([0, n, 2 * n, 3 * n], np.int32)
+    for d in (draft, p, None):
+        for u in (0.0, 0.25, 0.5, 0.75, 1 - 2.0 ** -24):
+            check_verify(ctx, p, d, tokens, parents, np.full(3 * n, u, np.float32), starts)
+
+
 @pytest.mark.parametrize("drawn", [True, False])
 def test_verify_where_all_or_none_pass(ctx, drawn):
     rng = np.random.default_rng(3)

@@ -46,7 +46,9 @@ __device__ __forceinline__ double wave_scan_d(double v) {
   return v;
 }
 
-// What is left of a row: of elements idx .. idx+3, 0 behind `end`.  Negative numbers and NaN count as 0.
+// What is left of an element.  Negative probabilities and NaN count as 0.
+__device__ __forceinline__ double left_of(float p, float q, double t) { return fmax(__builtin_fma(-t, (double)fmaxf(q, 0.0f), (double)fmaxf(p, 0.0f)), 0.0); }
+// What is left of a row: of elements idx .. idx+3, 0 behind `end`.
 struct Rest {
   const float *p, *q;      // (q null: nothing but the taken-out tokens is missing)
   double t;
@@ -57,7 +59,7 @@ __device__ __forceinline__ void rest4(const Rest &r, int idx, int end, double (&
   const f32x4 p = load4(r.p, idx, end);
   const f32x4 q = r.q ? load4(r.q, idx, end) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = fmax((double)p[e] - r.t * (double)q[e], 0.0);
+  for (int e = 0; e < 4; e++) v[e] = left_of(p[e], q[e], r.t);
   for (int i = 0; i < r.outs; i++) {
     const int at = r.out[i] - idx;
 #pragma unroll
@@ -65,19 +67,54 @@ __device__ __forceinline__ void rest4(const Rest &r, int idx, int end, double (&
       if (at == e) v[e] = 0.0;
   }
 }
-// Sum of elements lo .. hi-1, by a wavefront.
+// Sum of elements lo .. hi-1, by a wavefront: AT_ONCE turns of it are on their way together.  Behind the row's end its last four elements are loaded once more;
+// what is not counted is put to 0 before it becomes a number of 64 bits, whose instructions are what bounds this on one compute unit.
+constexpr int AT_ONCE = 4;
+template <bool DRAFT>
 __device__ __forceinline__ double wave_rest(const Rest &r, int lo, int hi) {
+  const int lane = threadIdx.x & 63;
   double sum = 0.0;
-#pragma unroll 4
-  for (int idx = lo + 4 * (int)(threadIdx.x & 63); idx < hi; idx += 256) {
-    double v[4];
-    rest4(r, idx, hi, v);
-    sum += (v[0] + v[1]) + (v[2] + v[3]);
+  for (int turn = lo; turn < hi; turn += 256 * AT_ONCE) {
+    f32x4 p[AT_ONCE], q[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; i++) {
+      const int idx = turn + 256 * i + 4 * lane, at = idx < r.vocab - 4 ? idx : r.vocab - 4;
+      p[i] = *reinterpret_cast<const f32x4_any *>(r.p + at);
+      if constexpr (DRAFT) q[i] = *reinterpret_cast<const f32x4_any *>(r.q + at);
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; i++) {
+      const int from = turn + 256 * i, idx = from + 4 * lane, at = idx < r.vocab - 4 ? idx : r.vocab - 4;
+      if (from >= hi) break;
+      if (from + 256 > hi)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (at + e < idx || at + e >= hi) {
+            p[i][e] = 0.0f;
+            if constexpr (DRAFT) q[i][e] = 0.0f;
+          }
+      if constexpr (!DRAFT)
+        for (int j = 0; j < r.outs; j++) {
+          const int gone = r.out[j];
+          if (gone >= from && gone < from + 256)
+#pragma unroll
+            for (int e = 0; e < 4; e++) p[i][e] = at + e == gone ? 0.0f : p[i][e];
+        }
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum += DRAFT ? left_of(p[i][e], q[i][e], r.t) : (double)fmaxf(p[i][e], 0.0f);
+    }
   }
   return wave_sum_d(sum);
 }
+__device__ __forceinline__ double wave_rest(const Rest &r, int lo, int hi) {
+  if (r.vocab >= 4) return r.q ? wave_rest<true>(r, lo, hi) : wave_rest<false>(r, lo, hi);
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+  if (lo == 0 && hi > 0 && (threadIdx.x & 63) == 0) rest4(r, 0, hi, v);
+  return wave_sum_d((v[0] + v[1]) + (v[2] + v[3]));
+}
 
 constexpr int WAVES = 16;
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 // The sixteenth of lo .. hi-1 that is `i`'s, in whole turns of a wavefront.
 __device__ __forceinline__ int part_begin(int lo, int hi, int i) {
   const int each = ((hi - lo + WAVES - 1) / WAVES + 255) / 256 * 256;
@@ -86,7 +123,7 @@ __device__ __forceinline__ int part_begin(int lo, int hi, int i) {
 }
 // The sums of all sixteen; their sum in order.
 __device__ __forceinline__ double parts_of(const Rest &r, int lo, int hi, double *sums) {
-  const int wave = threadIdx.x >> 6;
+  const int wave = wave_of();
   const double mine = wave_rest(r, part_begin(lo, hi, wave), part_begin(lo, hi, wave + 1));
   __syncthreads();  // (who still reads the sums before)
   if ((threadIdx.x & 63) == 0) sums[wave] = mine;
@@ -109,124 +146,192 @@ __device__ __forceinline__ int part_of(const double *sums, double target, double
   return last;
 }
 
-// A workgroup to a sequence.  Bound: the pass over a row of one workgroup.
-__global__ __launch_bounds__(64 * WAVES) void verify_drafts(VerifyParams a) {
+// Long rows are summed by sixteen workgroups, in a launch of its own, which more sequences take longer to be through with.  One launch / two (us): a tree of
+// 33 chosen drafts over 16000 tokens 9.6 / 10.0, over 32000 11.3 / 10.1, over 50001 13.5 / 10.5, over 128000 22 / 11.5; 32 sequences of 5 drawn in a row over 32000
+// 10.1 / 12.2, over 50001 13.6 / 12.9, over 128000 20 / 14.4; 64 sequences of 8 drawn over 50001 20 / 26; trees of 33 drawn, 8 of them, over 50001 23 / 24
+// (later sums of a tree are one workgroup's either way).
+bool in_two(int seqs, int vocab) { return vocab >= 32768 + 512LL * seqs; }
+
+// Where a walk has come to: the node, how many drafts were accepted, the last child that was rejected (-1: none), and t.
+struct Walk {
+  int node, taken, tried;
+  double t;
+};
+// What the first of two launches leaves for the second, for each sequence.
+struct Halfway {
+  Walk walk;
+  double sums[WAVES][WAVES];  // of the parts' parts
+};
+
+// ALL: a workgroup to a sequence.  FIRST and SECOND: sixteen, which all take the walk to the first sum that it needs (or to its end) and have a part
+// of that sum each, and one that goes on from there.  Bound: latency (of a row that one workgroup reads, its rate).
+enum Stage { ALL, FIRST, SECOND };
+template <int STAGE>
+__global__ __launch_bounds__(64 * WAVES, STAGE == FIRST ? 8 : 4) void verify_drafts(VerifyParams a, Halfway *halfway) {
   __shared__ int parent[MOST_ROWS], token[MOST_ROWS], path[MOST_ROWS], out[MOST_ROWS];
   __shared__ float px[MOST_ROWS], qx[MOST_ROWS], us[MOST_ROWS];
-  __shared__ double sums[WAVES];
-  __shared__ int found;
+  __shared__ double sums[WAVES], sums_of[WAVES][WAVES];
+  __shared__ int found, outs_found;
   const int seq = blockIdx.x, row0 = a.starts[seq], tid = threadIdx.x, lane = tid & 63;
   const long long rows = (long long)a.starts[seq + 1] - row0;
   if (row0 < 0 || rows <= 0 || rows > MOST_ROWS || row0 + rows > a.rows) return;
   const int n = (int)rows;
   for (int i = tid; i < MOST_ROWS; i += 64 * WAVES) {
-    const int up = i < n ? a.parents[row0 + i] : -1, x = i < n ? a.tokens[row0 + i] : 0;
-    const bool below = i > 0 && up >= 0 && up < i, real = below && x >= 0 && x < a.vocab;
-    const long long at = ((long long)row0 + (real ? up : 0)) * a.vocab + (real ? x : 0);
-    parent[i] = below ? up : -1;
-    token[i] = x;
-    px[i] = real ? a.P[at] : 0.0f;
-    qx[i] = real && a.Q ? a.Q[at] : 0.0f;
+    const int up = i < n ? a.parents[row0 + i] : -1;
+    parent[i] = i > 0 && up >= 0 && up < i ? up : -1;
+    token[i] = i < n ? a.tokens[row0 + i] : 0;
     us[i] = i < n ? a.U[row0 + i] : 0.0f;
   }
-  __syncthreads();
-  // All wavefronts take the same walk.
-  int node = 0, taken = 0;
-  Rest rest;
-  double mass;
-  bool summed;
-  for (bool walking = true; walking;) {
-    if (tid == 0) path[taken] = node;
-    rest = Rest{a.P + ((long long)row0 + node) * a.vocab, nullptr, 0.0, out, 0, a.vocab};
-    mass = 1.0;
-    summed = false;
-    walking = false;
-    for (int base = node / 64 * 64; base < n && !walking; base += 64) {
-      unsigned long long children = __ballot(parent[base + lane] == node);
-      while (children) {
-        const int child = base + __ffsll(children) - 1;
-        children &= children - 1;
-        const double u = us[child], likely = a.Q ? (double)qx[child] : 1.0;
-        double left = fmax((double)px[child] - rest.t * likely, 0.0);
-        if (!a.Q) {
-          left = fmax((double)px[child], 0.0);
-          for (int i = 0; i < rest.outs; i++)
-            if (out[i] == token[child]) left = 0.0;
-        }
-        if (u * mass * likely < left) {
-          node = child;
-          taken++;
-          walking = true;
-          break;
-        }
-        if (a.Q) {
-          rest.q = a.Q + ((long long)row0 + node) * a.vocab;
-          rest.t += mass;
-          mass = parts_of(rest, 0, a.vocab, sums);
-          summed = true;
-        } else {
-          mass -= left;
-          __syncthreads();  // (who still reads the list)
-          if (tid == 0) out[rest.outs] = token[child];
-          rest.outs++;
-          __syncthreads();
-        }
-      }
+  auto fetch = [&]() {  // the elements that tests need
+    for (int i = tid; i < n; i += 64 * WAVES) {
+      const int up = parent[i], x = token[i];
+      const bool real = up >= 0 && x >= 0 && x < a.vocab;
+      const long long at = ((long long)row0 + (real ? up : 0)) * a.vocab + (real ? x : 0);
+      px[i] = real ? a.P[at] : 0.0f;
+      qx[i] = real && a.Q ? a.Q[at] : 0.0f;
     }
-  }
-  // a token from what is left of the last row, or, if that is nothing, from the row
-  double total = summed ? mass : parts_of(rest, 0, a.vocab, sums);
-  if (!(total > 0.0) && (rest.outs || rest.q)) {
-    rest.outs = 0;
-    rest.q = nullptr;
-    rest.t = 0.0;
-    total = parts_of(rest, 0, a.vocab, sums);
-  }
-  if (tid == 0) found = -1;
-  __syncthreads();
-  if (total > 0.0 && total <= DBL_MAX) {
-    const double target = (double)us[0] * total;
-    double base = 0.0;
-    int part = part_of(sums, target, base);
-    int lo = part_begin(0, a.vocab, part), hi = part_begin(0, a.vocab, part + 1);
-    parts_of(rest, lo, hi, sums);
-    part = part_of(sums, target, base);
-    const int begin = part_begin(lo, hi, part), end = part_begin(lo, hi, part + 1);
-    if (tid < 64) {
-      int at = -1;
-      bool done = false;
-      for (int turn = begin; turn < end && !done; turn += 256) {
-        const int idx = turn + 4 * lane;
-        double v[4] = {0.0, 0.0, 0.0, 0.0};
-        if (idx < end) rest4(rest, idx, end, v);
-        const double mine = (v[0] + v[1]) + (v[2] + v[3]), upto = wave_scan_d(mine);
-        double before = base + (upto - mine);
-        int first = -1, last = -1;
+    __syncthreads();
+  };
+  Walk walk = {0, 0, -1, 0.0};
+  double mass = 1.0;
+  int outs = 0;
+  bool summed = false, fine = false;  // mass is the sum of `sums`; and those are sums of `sums_of`
+  if constexpr (STAGE == SECOND) {
+    const Halfway &from = halfway[seq];
+    walk = from.walk;
+    if (tid < WAVES * WAVES) sums_of[tid / WAVES][tid % WAVES] = from.sums[tid / WAVES][tid % WAVES];
+    if (tid == 0) outs_found = 0;
+    __syncthreads();
+    if (tid < WAVES) {
+      double sum = 0.0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          before += v[e];
-          if (v[e] > 0.0) {
-            last = idx + e;
-            if (first < 0 && before > target) first = idx + e;
-          }
-        }
-        const unsigned long long passed = __ballot(first >= 0), some = __ballot(last >= 0);
-        if (passed) {
-          at = __shfl(first, __ffsll(passed) - 1, 64);
-          done = true;
-        } else if (some) {
-          at = __shfl(last, 63 - __clzll(some), 64);  // (the last so far: what is found if rounding leaves the sum short)
-        }
-        base += __shfl(upto, 63, 64);
+      for (int i = 0; i < WAVES; i++) sum += sums_of[tid][i];
+      sums[tid] = sum;
+    }
+    if (!a.Q && walk.tried >= 0)  // chosen drafts: the walk is at its end, the node's children have all been taken out
+      for (int i = tid; i < n; i += 64 * WAVES)
+        if (parent[i] == walk.node) out[atomicAdd(&outs_found, 1)] = token[i];
+    __syncthreads();
+    outs = outs_found;
+    mass = 0.0;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) mass += sums[i];
+    summed = fine = true;
+  } else {
+    if (tid == 0) path[0] = 0;
+    fetch();
+  }
+  const int known = walk.taken;
+  auto rest_of = [&]() {
+    const long long row = ((long long)row0 + walk.node) * a.vocab;
+    return Rest{a.P + row, a.Q && walk.tried >= 0 ? a.Q + row : nullptr, walk.t, out, outs, a.vocab};
+  };
+  // All wavefronts take the same walk.
+  bool fetched = STAGE != SECOND;
+  for (;;) {
+    int child = -1;
+    if (STAGE != SECOND || a.Q)
+      for (int base = (walk.tried < 0 ? walk.node : walk.tried) / 64 * 64; base < n && child < 0; base += 64) {
+        const unsigned long long children = __ballot(parent[base + lane] == walk.node && base + lane > walk.tried);
+        if (children) child = base + __ffsll(children) - 1;
       }
-      if (lane == 0) found = at;
+    if (child < 0) break;
+    if (!fetched) {
+      fetch();
+      fetched = true;
+    }
+    const double u = us[child], likely = a.Q ? (double)fmaxf(qx[child], 0.0f) : 1.0;
+    double left = left_of(px[child], qx[child], walk.t);  // (t is 0 where drafts were chosen)
+    if (!a.Q) {
+      for (int i = 0; i < outs; i++)
+        if (out[i] == token[child]) left = 0.0;
+    }
+    if (u * mass * likely < left) {
+      walk = Walk{child, walk.taken + 1, -1, 0.0};
+      if (tid == 0) path[walk.taken] = child;
+      mass = 1.0;
+      outs = 0;
+      summed = fine = false;
+      continue;
+    }
+    walk.tried = child;
+    if (a.Q) {
+      walk.t += mass;
+      if constexpr (STAGE == FIRST) break;
+      mass = parts_of(rest_of(), 0, a.vocab, sums);
+      summed = true;
+      fine = false;
+    } else {
+      mass -= left;
+      __syncthreads();  // (who still reads the list)
+      if (tid == 0) out[outs] = token[child];
+      outs++;
+      __syncthreads();
+    }
+  }
+  Rest rest = rest_of();
+  if constexpr (STAGE == FIRST) {
+    const int lo = part_begin(0, a.vocab, blockIdx.y), hi = part_begin(0, a.vocab, blockIdx.y + 1);
+    const double mine = wave_rest(rest, part_begin(lo, hi, wave_of()), part_begin(lo, hi, wave_of() + 1));
+    if (lane == 0) halfway[seq].sums[blockIdx.y][wave_of()] = mine;
+    if (blockIdx.y) return;
+    if (tid == 0) halfway[seq].walk = walk;
+  } else {
+    // a token from what is left of the last row, or, if that is nothing, from the row
+    double total = summed ? mass : parts_of(rest, 0, a.vocab, sums);
+    if (!(total > 0.0) && (rest.outs || rest.q)) {
+      rest.outs = 0;
+      rest.q = nullptr;
+      rest.t = 0.0;
+      total = parts_of(rest, 0, a.vocab, sums);
+      fine = false;
+    }
+    if (tid == 0) found = -1;
+    __syncthreads();
+    if (total > 0.0 && total <= DBL_MAX) {
+      const double target = (double)us[0] * total;
+      double base = 0.0;
+      int part = part_of(sums, target, base);
+      const int lo = part_begin(0, a.vocab, part), hi = part_begin(0, a.vocab, part + 1);
+      if (!fine) parts_of(rest, lo, hi, sums);
+      part = part_of(fine ? sums_of[part] : sums, target, base);
+      const int begin = part_begin(lo, hi, part), end = part_begin(lo, hi, part + 1);
+      if (tid < 64) {
+        int at = -1;
+        bool done = false;
+        for (int turn = begin; turn < end && !done; turn += 256) {
+          const int idx = turn + 4 * lane;
+          double v[4] = {0.0, 0.0, 0.0, 0.0};
+          if (idx < end) rest4(rest, idx, end, v);
+          const double mine = (v[0] + v[1]) + (v[2] + v[3]), upto = wave_scan_d(mine);
+          double before = base + (upto - mine);
+          int first = -1, last = -1;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            before += v[e];
+            if (v[e] > 0.0) {
+              last = idx + e;
+              if (first < 0 && before > target) first = idx + e;
+            }
+          }
+          const unsigned long long passed = __ballot(first >= 0), some = __ballot(last >= 0);
+          if (passed) {
+            at = __shfl(first, __ffsll(passed) - 1, 64);
+            done = true;
+          } else if (some) {
+            at = __shfl(last, 63 - __clzll(some), 64);  // (the last so far: what is found if rounding leaves the sum short)
+          }
+          base += __shfl(upto, 63, 64);
+        }
+        if (lane == 0) found = at;
+      }
     }
   }
   __syncthreads();
-  for (int i = tid; i < n; i += 64 * WAVES) a.path[row0 + i] = i <= taken ? path[i] : -1;
-  if (tid == 0) {
+  for (int i = tid + (STAGE == SECOND ? known + 1 : 0); i < (STAGE == SECOND ? walk.taken + 1 : n); i += 64 * WAVES) a.path[row0 + i] = i <= walk.taken ? path[i] : -1;
+  if (STAGE != FIRST && tid == 0) {
     a.next[seq] = found;
-    a.count[seq] = taken;
+    a.count[seq] = walk.taken;
   }
 }
 
@@ -365,7 +470,18 @@ extern "C" int wdh_verify_drafts(wdh_buf hP, wdh_buf hDraft, wdh_buf hTokens, wd
   }
   const VerifyParams p = {(const float *)pp, (const float *)pd, (const float *)pu, (const int *)pt, (const int *)pa, (const int *)ps,
                           (int *)pn, (int *)pc, (int *)ph, seqs, tokens, vocab};
-  hipLaunchKernelGGL(verify_drafts, dim3((unsigned)seqs), dim3(64 * WAVES), 0, wdh::stream(), p);
+  hipStream_t st = wdh::stream();
+  if (!in_two(seqs, vocab)) {
+    hipLaunchKernelGGL(verify_drafts<ALL>, dim3((unsigned)seqs), dim3(64 * WAVES), 0, st, p, nullptr);
+  } else {
+    const wdh_buf work = wdh_alloc((size_t)seqs * sizeof(Halfway));
+    if (!work) return WDH_ENOMEM;
+    size_t have;
+    Halfway *halfway = (Halfway *)wdh::resolve(work, &have);
+    hipLaunchKernelGGL(verify_drafts<FIRST>, dim3((unsigned)seqs, WAVES), dim3(64 * WAVES), 0, st, p, halfway);
+    hipLaunchKernelGGL(verify_drafts<SECOND>, dim3((unsigned)seqs), dim3(64 * WAVES), 0, st, p, halfway);
+    (void)wdh_free(work);
+  }
   WDH_LAUNCH_CHECK();
   return WDH_OK;
 }
