@@ -38,10 +38,15 @@ struct AppendParams {
 // needs the largest of the new elements before any of them is stored.  They stay in registers in between.
 // Bound: memory for prompts (6 of 100 to 2900 tokens, 8 heads of 128: 18.3 us, 5.0 TB/s), latency for single tokens (48: 6.6 us, a
 // call's own time 5.3).
-template <int D, bool TURN>
+// TURN: keys are normed and rotated on the way, and which pairs are; where they face each other, a thread's pieces are partners in turn, and nothing is loaded
+// twice.  Rotation goes over two pieces of a thread at a time, and not over those without new tokens.  8 heads of 128 (us): one token of 48 sequences 12.0 with all
+// pieces at a time, 8.2 so, 8.0 facing (6.6 without rotation); six prompts of 100 to 2900 tokens 44 / 40 / 23 (18 without; neighbours 28).
+constexpr int AS_IT_IS = -1;
+template <int D, int TURN>
 __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
   constexpr int NP = PAGE * D / 4 / 256;       // pieces of four elements a thread holds
   constexpr int PPT = D / 4;                   // pieces of a token
+  constexpr int AT_ONCE = 2;                   // pieces of a thread that are rotated together
   __shared__ float part[4];
   __shared__ int turn[PAGE * (D / 4 + 1)];     // values on their way from [token][d] to [d][token], four to a word
   const Place s = locate(p.q, blockIdx.x, [](const Place &s) { return (s.len - 1) / PAGE - (s.len - s.n) / PAGE + 1; });
@@ -54,37 +59,60 @@ __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
   // (token `slot` of the page is row row0 + slot of the call)
   const float *x = (values ? p.V : p.K) + head * D;
   const long long row0 = (long long)s.row0 + (long long)pi * PAGE - before;
+  // piece i of a thread: which token, and elements of it
+  const bool facing = TURN == wdh::rope::FACING && !values;
+  auto slot_of = [&](int i) { return facing ? t / (PPT / 2) + 512 / PPT * (i / 2) : (t + 256 * i) / PPT; };
+  auto d0_of = [&](int i) { return facing ? t % (PPT / 2) * 4 + i % 2 * (D / 2) : t % PPT * 4; };
+  auto word_of = [&](int i) { return facing ? slot_of(i) * PPT + d0_of(i) / 4 : t + 256 * i; };
   f32x4 v[NP];
 #pragma unroll
   for (int i = 0; i < NP; i++) {
-    const int slot = (t + 256 * i) / PPT, d0 = (t + 256 * i) % PPT * 4;
+    const int slot = slot_of(i), d0 = d0_of(i);
     v[i] = slot >= first && slot < last ? *reinterpret_cast<const f32x4 *>(x + (row0 + slot) * stride + d0) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if constexpr (TURN)
+  if constexpr (TURN != AS_IT_IS)
     if (!values) {
       // (a thread's pieces are the same elements of all its tokens)
-      const int d0 = t % PPT * 4;
+      constexpr int GROUP = TURN == wdh::rope::FACING ? PPT / 2 : PPT, EACH = TURN == wdh::rope::FACING ? 2 : 1;  // lanes to a token, and pieces of it to a lane
+      const int d0 = d0_of(0);
       const bool norm = p.gamma != nullptr;
-      const f32x4 one = {1.f, 1.f, 1.f, 1.f}, g = norm ? load4(p.gamma, d0, D) : one, og = norm ? wdh::rope::partners(p.turn, p.gamma, d0, D) : one;
-      f32x4 o[NP];
-      wdh::rope::Angles a[NP];
+      const f32x4 one = {1.f, 1.f, 1.f, 1.f}, g = norm ? load4(p.gamma, d0, D) : one;
+      const f32x4 og = !norm || TURN == wdh::rope::NEIGHBOURS ? one : TURN == wdh::rope::FACING ? load4(p.gamma, d0 + D / 2, D) : wdh::rope::partners(p.turn, p.gamma, d0, D);
+      constexpr int SLOTS = 256 / PPT;  // tokens of a round of pieces: rounds without new ones are left out
 #pragma unroll
-      for (int i = 0; i < NP; i++) {
-        const int slot = (t + 256 * i) / PPT;
-        const bool mine = slot >= first && slot < last;
-        const int position = !mine ? 0 : p.positions ? p.positions[row0 + slot] : pi * PAGE + slot;
-        o[i] = mine ? wdh::rope::partners(p.turn, x + (row0 + slot) * stride, d0, D) : f32x4{0.f, 0.f, 0.f, 0.f};
-        a[i] = wdh::rope::angles(p.turn, position, mine ? d0 : D);
-      }
+      for (int round = 0; round < NP; round += AT_ONCE) {
+        if (SLOTS * round >= last || SLOTS * (round + AT_ONCE) <= first) continue;
+        f32x4 o[AT_ONCE];
+        wdh::rope::Angles a[AT_ONCE];
 #pragma unroll
-      for (int i = 0; i < NP; i++) {
-        if (norm) {
-          const wdh::rowmath::RowFactor f = wdh::rowmath::row_factor(wdh::rope::group_sum<PPT>(wdh::rope::squares(v[i])) / (double)D, p.eps);
-          v[i] = wdh::rope::normed(v[i], f, g);
-          o[i] = wdh::rope::normed(o[i], f, og);
+        for (int i = 0; i < AT_ONCE; i += EACH) {
+          const int slot = slot_of(round + i);
+          const bool mine = slot >= first && slot < last;
+          const int position = !mine ? 0 : p.positions ? p.positions[row0 + slot] : pi * PAGE + slot;
+          if constexpr (TURN == wdh::rope::ANYWHERE)
+            o[i] = mine ? wdh::rope::partners(p.turn, x + (row0 + slot) * stride, d0, D) : f32x4{0.f, 0.f, 0.f, 0.f};
+          a[i] = wdh::rope::angles<TURN>(p.turn, position, d0);
         }
-        const int slot = (t + 256 * i) / PPT;
-        v[i] = slot >= first && slot < last ? wdh::rope::turn(p.turn, d0, v[i], o[i], a[i]) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i += EACH) {
+          f32x4 &own = v[round + i], &other = TURN == wdh::rope::FACING ? v[round + i + 1] : o[i];
+          if (norm) {
+            double sum = wdh::rope::squares(own);
+            if constexpr (TURN == wdh::rope::FACING) sum += wdh::rope::squares(other);
+            const wdh::rowmath::RowFactor f = wdh::rope::head_factor(wdh::rope::group_sum<GROUP>(sum) / (double)D, p.eps);
+            own = wdh::rope::normed(own, f, g);
+            if constexpr (TURN != wdh::rope::NEIGHBOURS) other = wdh::rope::normed(other, f, og);
+          }
+          const int slot = slot_of(round + i);
+          const bool mine = slot >= first && slot < last;
+          const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (TURN == wdh::rope::FACING) {
+            wdh::rope::turn_facing(own, other, a[i]);
+            if (!mine) own = other = none;
+          } else {
+            own = !mine ? none : TURN == wdh::rope::NEIGHBOURS ? wdh::rope::turn_neighbours(p.turn, d0, own, a[i]) : wdh::rope::turn(p.turn, d0, own, other, a[i]);
+          }
+        }
       }
     }
   if (id < 0 || id >= p.q.pages) return;
@@ -114,8 +142,8 @@ __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
   if (!values) {
 #pragma unroll
     for (int i = 0; i < NP; i++) {
-      const int slot = (t + 256 * i) / PPT;
-      int *to = reinterpret_cast<int *>(page) + t + 256 * i;
+      const int slot = slot_of(i);
+      int *to = reinterpret_cast<int *>(page) + word_of(i);
       if (slot >= first && slot < last) *to = pack4(v[i], inv);
       else if (slot < first && grown) *to = rescale4(*to, factor);
     }
@@ -931,7 +959,7 @@ struct Turn {
   int rotary, rows, interleaved;
   float eps;
 };
-template <bool TURN>
+template <int TURN>
 void launch_append(const AppendParams &p, int d, dim3 grid) {
   if (d == 32) hipLaunchKernelGGL((cache_append<32, TURN>), grid, dim3(256), 0, wdh::stream(), p);
   else if (d == 64) hipLaunchKernelGGL((cache_append<64, TURN>), grid, dim3(256), 0, wdh::stream(), p);
@@ -963,7 +991,7 @@ int append(const char *who, wdh_buf hK, int64_t k_offset, int64_t k_stride, wdh_
   if (int rc = cache_operands(who, hKP, hKS, hVP, hVS, hTable, hLens, hStarts, seqs, kv_heads, d, pages, max_pages, &kp, &ks, &vp, &vs, &p.q)) return rc;
   p.gamma = nullptr;
   p.positions = nullptr;
-  p.turn = wdh::rope::Rotation{nullptr, nullptr, 0, 0, 0};
+  p.turn = wdh::rope::Rotation{nullptr, nullptr, 0, 0};
   p.eps = 0.0f;
   if (turn) {
     void *g = nullptr, *c = nullptr, *s = nullptr, *at = nullptr;
@@ -973,7 +1001,7 @@ int append(const char *who, wdh_buf hK, int64_t k_offset, int64_t k_stride, wdh_
       return WDH_EINVAL;
     p.gamma = (const float *)g;
     p.positions = (const int *)at;
-    p.turn = wdh::rope::Rotation{(const float *)c, (const float *)s, turn->rotary / 2, turn->rows, turn->interleaved != 0};
+    p.turn = wdh::rope::Rotation{(const float *)c, (const float *)s, turn->rotary / 2, turn->rows};
     p.eps = turn->eps;
   }
   const wdh_buf out[4] = {hKP, hKS, hVP, hVS};
@@ -994,8 +1022,10 @@ int append(const char *who, wdh_buf hK, int64_t k_offset, int64_t k_stride, wdh_
   // touched pages: each has a new token, and a sequence's are at most n / 64 + 2
   const long long bound = (long long)tokens / PAGE + 2LL * seqs, items = bound < tokens ? bound : tokens;
   const dim3 grid((unsigned)items, (unsigned)kv_heads, 2);
-  if (turn) launch_append<true>(p, d, grid);
-  else launch_append<false>(p, d, grid);
+  if (!turn) launch_append<AS_IT_IS>(p, d, grid);
+  else if (turn->interleaved || turn->rotary == 0) launch_append<wdh::rope::NEIGHBOURS>(p, d, grid);
+  else if (turn->rotary == d) launch_append<wdh::rope::FACING>(p, d, grid);
+  else launch_append<wdh::rope::ANYWHERE>(p, d, grid);
   WDH_LAUNCH_CHECK();
   return WDH_OK;
 }

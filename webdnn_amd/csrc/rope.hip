@@ -3,7 +3,7 @@
 // The reference has no such operators; in its terms they are the chain of a norm (see norm_fp8.hip), Split, Neg, Concat, Mul, Add
 // (src/descriptor_runner/operators/cpu/operators/standard/binary7.ts:24-75, split.ts:12-87, concat.ts:21-84).
 //
-// Bound: memory.  A head stays in the registers of 8 to 64 lanes between its sum of squares and its use.
+// A head stays in the registers of 8 to 64 lanes between its sum of squares and its use.  Bound: memory, then instructions.
 #include "common.h"
 #include "fastdiv.h"
 #include "rope.h"
@@ -13,7 +13,6 @@ namespace {
 using namespace wdh::rope;
 using wdh::fail;
 using wdh::rowmath::RowFactor;
-using wdh::rowmath::row_factor;
 
 struct RopeParams {
   const float *X;
@@ -25,72 +24,72 @@ struct RopeParams {
   long long units;      // tokens * heads
   wdh::FastDiv heads;   // q_heads of one kind, then those of the other
   int q_heads, d;
+  double of_d;          // 1 / d
   float eps;
 };
 
-// LANES lanes to a head, NP pieces of four elements to a lane, UNROLL heads of a group of lanes on their way at a time.
-template <int LANES, int NP, int UNROLL>
+// LANES lanes to a head, NP pieces of four elements to a lane.  FACING: a head of 8 LANES elements is rotated whole, by halves, so that a lane's two pieces
+// are each other's partners.  A lane has two pieces wherever there are as many, for it is instructions that bound this: 8192 tokens of 40 heads of 128 take
+// 86 us with one piece to a lane, 62 so.  (More heads to a lane take longer: 2 95 us, 4 121.)
+template <int LANES, int NP, int PAIRS>
 __global__ __launch_bounds__(256) void head_rope(RopeParams p) {
-  constexpr int GROUPS = 256 / LANES;
   const int lane = threadIdx.x % LANES;
-  const long long unit0 = (long long)blockIdx.x * (GROUPS * UNROLL) + threadIdx.x / LANES;
-  f32x4 v[UNROLL][NP], o[UNROLL][NP], gamma[UNROLL][NP], other_gamma[UNROLL][NP];
-  Angles a[UNROLL][NP];
-  int token[UNROLL], head[UNROLL];
+  const long long at = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int unit = (int)(at < p.units ? at : p.units - 1);  // (behind the last: the last once more, not stored)
+  const int token = wdh::fdiv(unit, p.heads), head = unit - token * p.heads.d, d = PAIRS == FACING ? 8 * LANES : p.d;
+  const float *x = p.X + token * p.x_stride + head * p.x_head, *g = head < p.q_heads ? p.q_gamma : p.k_gamma;
+  const int position = p.positions ? p.positions[token] : token;
+  f32x4 v[NP], o[NP], gamma[NP], other_gamma[NP];
+  Angles a[NP];
 #pragma unroll
-  for (int j = 0; j < UNROLL; j++) {
-    const int unit = (int)(unit0 + j * GROUPS < p.units ? unit0 + j * GROUPS : p.units - 1);  // (behind the last: the last once more, not stored)
-    token[j] = wdh::fdiv(unit, p.heads);
-    head[j] = unit - token[j] * p.heads.d;
-    const float *x = p.X + token[j] * p.x_stride + head[j] * p.x_head, *g = head[j] < p.q_heads ? p.q_gamma : p.k_gamma;
-    const int position = p.positions ? p.positions[token[j]] : token[j];
+  for (int i = 0; i < NP; i++) {
+    const int d0 = 4 * (lane + LANES * i);
+    v[i] = load4(x, d0, d);
+    if (g) gamma[i] = load4(g, d0, d);
+    if constexpr (PAIRS == ANYWHERE) {
+      o[i] = partners(p.r, x, d0, d);
+      if (g) other_gamma[i] = partners(p.r, g, d0, d);
+    }
+    if (PAIRS != FACING || i == 0) a[i] = angles<PAIRS>(p.r, position, d0);
+  }
+  if (g) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < NP; i++) sum += squares(v[i]);
+    const RowFactor f = head_factor(group_sum<LANES>(sum) * p.of_d, p.eps);
 #pragma unroll
     for (int i = 0; i < NP; i++) {
-      const int d0 = 4 * (lane + LANES * i);
-      v[j][i] = load4(x, d0, p.d);
-      o[j][i] = partners(p.r, x, d0, p.d);
-      if (g) {
-        gamma[j][i] = load4(g, d0, p.d);
-        other_gamma[j][i] = partners(p.r, g, d0, p.d);
-      }
-      a[j][i] = angles(p.r, position, d0);
+      v[i] = normed(v[i], f, gamma[i]);
+      if constexpr (PAIRS == ANYWHERE) o[i] = normed(o[i], f, other_gamma[i]);
     }
   }
+  if (at >= p.units) return;
+  if constexpr (PAIRS == FACING) turn_facing(v[0], v[1], a[0]);
+  float *y = p.Y + token * p.y_stride + head * p.y_head;
 #pragma unroll
-  for (int j = 0; j < UNROLL; j++) {
-    if (head[j] < p.q_heads ? p.q_gamma : p.k_gamma) {
-      double sum = 0.0;
-#pragma unroll
-      for (int i = 0; i < NP; i++) sum += squares(v[j][i]);
-      const RowFactor f = row_factor(group_sum<LANES>(sum) / (double)p.d, p.eps);
-#pragma unroll
-      for (int i = 0; i < NP; i++) {
-        v[j][i] = normed(v[j][i], f, gamma[j][i]);
-        o[j][i] = normed(o[j][i], f, other_gamma[j][i]);
-      }
-    }
-    if (unit0 + j * GROUPS >= p.units) continue;
-    float *y = p.Y + token[j] * p.y_stride + head[j] * p.y_head;
-#pragma unroll
-    for (int i = 0; i < NP; i++) {
-      const int d0 = 4 * (lane + LANES * i);
-      store4(y, d0, p.d, turn(p.r, d0, v[j][i], o[j][i], a[j][i]));
-    }
+  for (int i = 0; i < NP; i++) {
+    const int d0 = 4 * (lane + LANES * i);
+    if constexpr (PAIRS == ANYWHERE) v[i] = turn(p.r, d0, v[i], o[i], a[i]);
+    if constexpr (PAIRS == NEIGHBOURS) v[i] = turn_neighbours(p.r, d0, v[i], a[i]);
+    store4(y, d0, d, v[i]);
   }
 }
 
-template <int LANES, int NP, int UNROLL>
+template <int LANES, int NP, int PAIRS>
 int launch(const RopeParams &p) {
-  constexpr int PER = 256 / LANES * UNROLL;
+  constexpr int PER = 256 / LANES;
   const long long wgs = (p.units + PER - 1) / PER;
   if (wgs > 0xffffff) return fail(WDH_EINVAL, "wdh_rope: too many heads");  // (a launch has fewer than 2^32 threads)
-  hipLaunchKernelGGL((head_rope<LANES, NP, UNROLL>), dim3((unsigned)wgs), dim3(256), 0, wdh::stream(), p);
+  hipLaunchKernelGGL((head_rope<LANES, NP, PAIRS>), dim3((unsigned)wgs), dim3(256), 0, wdh::stream(), p);
   WDH_LAUNCH_CHECK();
   return WDH_OK;
 }
-template <int LANES>
-int launch_lanes(const RopeParams &p) {
-  return launch<LANES, 1, 1>(p);
+template <int LANES, int NP>
+int launch_pairs(const RopeParams &p, bool neighbours) {
+  if (neighbours) return launch<LANES, NP, NEIGHBOURS>(p);
+  if constexpr (NP == 2)
+    if (p.r.half == 4 * LANES) return launch<LANES, 2, FACING>(p);
+  return launch<LANES, NP, ANYWHERE>(p);
 }
 
 }  // namespace
@@ -136,13 +135,14 @@ extern "C" int wdh_rope(wdh_buf hX, int64_t x_offset, int64_t x_stride, int64_t 
   p.x_stride = x_stride; p.x_head = x_head; p.y_stride = y_stride; p.y_head = y_head;
   p.q_gamma = (const float *)qg; p.k_gamma = (const float *)kg;
   p.positions = (const int *)pp;
-  p.r = Rotation{(const float *)pc, (const float *)ps, rotary / 2, rows, interleaved != 0};
+  p.r = Rotation{(const float *)pc, (const float *)ps, rotary / 2, rows};
   p.units = tokens * all;
   p.heads = wdh::make_fastdiv(all);
-  p.q_heads = heads; p.d = d; p.eps = eps;
-  if (d <= 32) return launch_lanes<8>(p);
-  if (d <= 64) return launch_lanes<16>(p);
-  if (d <= 128) return launch_lanes<32>(p);
-  if (d <= 256) return launch_lanes<64>(p);
-  return d <= 512 ? launch<64, 2, 1>(p) : launch<64, 4, 1>(p);
+  p.q_heads = heads; p.d = d; p.of_d = 1.0 / d; p.eps = eps;
+  const bool neighbours = interleaved || rotary == 0;  // (no pairs: none that need others)
+  if (d <= 32) return launch_pairs<8, 1>(p, neighbours);
+  if (d <= 64) return launch_pairs<8, 2>(p, neighbours);
+  if (d <= 128) return launch_pairs<16, 2>(p, neighbours);
+  if (d <= 256) return launch_pairs<32, 2>(p, neighbours);
+  return d <= 512 ? launch_pairs<64, 2>(p, neighbours) : launch_pairs<64, 4>(p, neighbours);
 }
