@@ -346,97 +346,119 @@ struct KeepParams {
 
 // Tokens of a path go behind each other: slot past + i takes what slot past + path[i] holds, which is never before it.  So a workgroup has a
 // sequence's pages of one head, keys (blockIdx.z 0) or values, and goes over them in order; what a page takes is in registers before any of
-// it is written, and what later pages take lies behind.  Bound: latency.
+// it is written, and what later pages take lies behind.  Bound: latency, of five rounds of loads after each other (numbers of rows; path; tables; scales and
+// elements; and words to be kept).  The ways to two pages are found at a time, and threads go to the words that are written: with a way and all words for each page
+// 16 sequences of 32 rows took 10.8 us, 200 of 9 rows 14.2; so 5.6 and 7.1.
 template <int D>
 __global__ __launch_bounds__(256) void cache_keep(KeepParams p) {
   constexpr int NP = PAGE * D / 4 / 256, PPT = D / 4;
-  __shared__ float part[4], scale_of[PAGE];
-  __shared__ long long from[PAGE];   // where a slot's token comes from: page cell * 64 + slot
+  __shared__ float part[2][4], scales_of[2][PAGE], had_of[2];
+  __shared__ long long froms[2][PAGE], at_of[2];   // where a slot's token comes from, and the page's own cell
+  __shared__ int moves_of[2];
+  const int given = p.count[blockIdx.x];
   const Place s = sequence(p.q, blockIdx.x);
   if (s.n == 0) return;
-  const int given = p.count[s.seq], kept = given < 0 ? 0 : given < s.n - 1 ? given + 1 : s.n, past = s.len - s.n;
+  const int kept = given < 0 ? 0 : given < s.n - 1 ? given + 1 : s.n, past = s.len - s.n;
   if (kept == 0) return;
   const bool values = blockIdx.z;
   const int head = blockIdx.y, t = threadIdx.x;
   unsigned char *pages = values ? p.VP : p.KP;
   float *scales = values ? p.VS : p.KS;
   const int *table = p.q.table + (long long)s.seq * p.q.max_pages;
-  for (int pi = past / PAGE; pi <= (past + kept - 1) / PAGE; pi++) {
-    const int id = table[pi];
-    if (id < 0 || id >= p.q.pages) continue;
-    const long long at = (long long)id * p.heads + head;
-    const int first = past > pi * PAGE ? past - pi * PAGE : 0, last = past + kept - pi * PAGE < PAGE ? past + kept - pi * PAGE : PAGE;
-    bool moves = false;
-    __syncthreads();  // (the page before is done with the list)
-    if (t < PAGE) {
+  const int end = (past + kept - 1) / PAGE + 1;
+  for (int two = past / PAGE; two < end; two += 2) {
+    __syncthreads();  // (the pages before are done with the lists)
+    float scale = 0.0f;
+    if (t < 2 * PAGE) {
+      const int page = two + t / PAGE, i = page * PAGE + t % PAGE - past, id = page < end ? table[page] : -1;
+      const int j = page < end && i >= 0 && i < kept ? p.path[s.row0 + i] : -1;
+      const bool known = id >= 0 && id < p.q.pages;
+      const long long at = known ? (long long)id * p.heads + head : 0;
       long long cell = at;
-      int slot = t;
-      if (t >= first && t < last) {
-        const int i = pi * PAGE + t - past, j = p.path[s.row0 + i];
-        if (j > i && j < s.n) {
-          const int there = table[(past + j) / PAGE];
-          if (there >= 0 && there < p.q.pages) {
-            cell = (long long)there * p.heads + head;
-            slot = (past + j) % PAGE;
-            moves = true;
-          }
+      int slot = t % PAGE;
+      bool moves = false;
+      if (known && j > i && j < s.n) {
+        const int there = table[(past + j) / PAGE];
+        if (there >= 0 && there < p.q.pages) {
+          cell = (long long)there * p.heads + head;
+          slot = (past + j) % PAGE;
+          moves = true;
         }
       }
-      from[t] = cell * PAGE + slot;
-      scale_of[t] = scales[cell];
-    }
-    if (!__syncthreads_or(moves)) continue;
-    unsigned char *page = pages + at * (PAGE * D);
-    f32x4 v[NP];
-    int old[NP];
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NP; i++) {
-      const int w = t + 256 * i, s0 = values ? w % (PAGE / 4) * 4 : w / PPT;
-      old[i] = s0 < last ? reinterpret_cast<const int *>(page)[w] : 0;
-      v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      int q = 0;
-      if (!values) {
-        if (s0 < first || s0 >= last) continue;
-        q = *reinterpret_cast<const int *>(pages + from[s0] * D + w % PPT * 4);
-      } else {
-        if (s0 + 4 <= first || s0 >= last) continue;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const long long f = from[s0 + e];
-          if (s0 + e >= first && s0 + e < last) q |= (int)pages[f / PAGE * (PAGE * D) + w / (PAGE / 4) * PAGE + f % PAGE] << (8 * e);
-        }
+      scale = scales[cell];
+      froms[t / PAGE][t % PAGE] = cell * (PAGE * D) + (values ? slot : slot * D);
+      const unsigned long long any = __ballot(moves);
+      if (t % PAGE == 0) {
+        moves_of[t / PAGE] = any != 0;
+        at_of[t / PAGE] = at;
+        had_of[t / PAGE] = scales[at];
       }
-      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(q, true);
-      v[i] = f32x4{a[0], a[1], b[0], b[1]};
-#pragma unroll
-      for (int e = 0; e < 4; e++) {  // (a value that was rounded up may stand for more than fp32 holds; fmaxf passes NaN by)
-        const float x = fabsf(v[i][e] * scale_of[values ? s0 + e : s0]);
-        amax = fmaxf(amax, x > FLT_MAX ? FLT_MAX : x);
-      }
+      scales_of[t / PAGE][t % PAGE] = scale;
     }
-    const float had = scales[at];
-    amax = wdh::rowmath::wave_max(amax);
-    if ((t & 63) == 0) part[t >> 6] = amax;
     __syncthreads();
-    const float c = fmaxf(had, page_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])))), inv = 1.0f / c, factor = had / c;
-    const bool grown = c != had;
+#pragma unroll 1
+    for (int which = 0; which < 2; which++) {
+      if (!moves_of[which]) continue;
+      const int page0 = (two + which) * PAGE, first = past > page0 ? past - page0 : 0, last = past + kept - page0 < PAGE ? past + kept - page0 : PAGE;
+      const long long *from = froms[which];
+      const float *scale_of = scales_of[which];
+      unsigned char *page = pages + at_of[which] * (PAGE * D);
+      // the words that are written: keys: all of the new tokens'; values: those of each element that a new token is in
+      const int word0 = first / 4, each = (last + 3) / 4 - word0, words = values ? D * each : (last - first) * PPT;
+      const int inverse = (65536 + each - 1) / each;  // (exact for numbers up to 2048)
+      auto word_of = [&](int k) { return values ? (k * inverse >> 16) * (PAGE / 4) + word0 + k - (k * inverse >> 16) * each : first * PPT + k; };
+      f32x4 v[NP];
+      int old[NP];
+      float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NP; i++) {
-      const int w = t + 256 * i, s0 = values ? w % (PAGE / 4) * 4 : w / PPT;
-      int *to = reinterpret_cast<int *>(page) + w;
-      f32x4 y = {0.f, 0.f, 0.f, 0.f};
-      if (s0 < last)
+      for (int i = 0; i < NP; i++) {
+        if (256 * i >= words) break;
+        const int k = t + 256 * i, w = word_of(k), s0 = values ? w % (PAGE / 4) * 4 : w / PPT;
+        v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        old[i] = 0;
+        if (k >= words) continue;
+        int q = 0;
+        if (!values) {
+          q = *reinterpret_cast<const int *>(pages + from[s0] + w % PPT * 4);
+        } else {
+          old[i] = reinterpret_cast<const int *>(page)[w];
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (s0 + e >= first && s0 + e < last) q |= (int)pages[from[s0 + e] + w / (PAGE / 4) * PAGE] << (8 * e);
+        }
+        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(q, true);
+        v[i] = f32x4{a[0], a[1], b[0], b[1]};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {  // (a value that was rounded up may stand for more than fp32 holds; fmaxf passes NaN by)
+          const float x = fabsf(v[i][e] * scale_of[values ? s0 + e : s0]);
+          amax = fmaxf(amax, x > FLT_MAX ? FLT_MAX : x);
+        }
+      }
+      const float had = had_of[which];
+      amax = wdh::rowmath::wave_max(amax);
+      if ((t & 63) == 0) part[which][t >> 6] = amax;
+      __syncthreads();
+      const float *pt = part[which], c = fmaxf(had, page_scale(fmaxf(fmaxf(pt[0], pt[1]), fmaxf(pt[2], pt[3])))), inv = 1.0f / c, factor = had / c;
+      const bool grown = c != had;
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        if (256 * i >= words) break;
+        const int k = t + 256 * i, w = word_of(k), s0 = values ? w % (PAGE / 4) * 4 : w / PPT;
+        if (k >= words) continue;
+        f32x4 y;
 #pragma unroll
         for (int e = 0; e < 4; e++) y[e] = v[i][e] * (scale_of[values ? s0 + e : s0] * inv);
-      if (!values) {
-        if (s0 >= first && s0 < last) *to = pack4(y, 1.0f);
-        else if (s0 < first && grown) *to = rescale4(old[i], factor);
-      } else if (s0 < last && (s0 + 4 > first || grown)) {
-        *to = merge4(old[i], pack4(y, 1.0f), first - s0, last - s0, grown, factor);
+        reinterpret_cast<int *>(page)[w] = values ? merge4(old[i], pack4(y, 1.0f), first - s0, last - s0, grown, factor) : pack4(y, 1.0f);
+      }
+      if (grown) {  // the tokens before
+        for (int w = t; w < PAGE * D / 4; w += 256) {
+          if (values ? w % (PAGE / 4) >= word0 : w >= first * PPT) continue;
+          int *to = reinterpret_cast<int *>(page) + w;
+          *to = rescale4(*to, factor);
+        }
+        if (t == 0) scales[at_of[which]] = c;
       }
     }
-    if (t == 0 && grown) scales[at] = c;
   }
 }
 
