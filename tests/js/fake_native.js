@@ -299,6 +299,27 @@ const native = {
     }
   },
 
+  rope(X, xOffset, xStride, xHead, Y, yOffset, yStride, yHead, QGamma, KGamma, Cos, Sin, Positions, tokens, heads, kHeads, d, rotary, rows, interleaved, eps) {
+    count("rope");
+    if (QGamma || KGamma || kHeads) throw new Error("fake rope: heads of one kind, without a norm");
+    if (tokens === 0 || heads === 0) return;
+    const last = (tokens - 1) * xStride + (heads - 1) * xHead + d, half = rotary / 2;
+    need(X, (xOffset + last) * 4, "wdh_rope: X"); need(Y, (yOffset + (tokens - 1) * yStride + (heads - 1) * yHead + d) * 4, "wdh_rope: Y");
+    need(Cos, rows * half * 4, "wdh_rope: Cos"); need(Sin, rows * half * 4, "wdh_rope: Sin");
+    if (Positions) need(Positions, tokens * 4, "wdh_rope: Positions");
+    const x = f32(X), y = f32(Y), cos = f32(Cos), sin = f32(Sin), pos = Positions ? i32(Positions) : null;
+    for (let r = 0; r < tokens; r++) for (let h = 0; h < heads; h++) {
+      const from = xOffset + r * xStride + h * xHead, to = yOffset + r * yStride + h * yHead, at = pos ? pos[r] : r;
+      for (let i = rotary; i < d; i++) y[to + i] = x[from + i];
+      for (let j = 0; j < half; j++) {
+        const a = interleaved ? 2 * j : j, b = interleaved ? 2 * j + 1 : j + half, known = at >= 0 && at < rows;
+        const c = known ? cos[at * half + j] : NaN, s = known ? sin[at * half + j] : NaN, xa = x[from + a], xb = x[from + b];
+        y[to + a] = xa * c - Math.fround(xb * s);
+        y[to + b] = xb * c + Math.fround(xa * s);
+      }
+    }
+  },
+
   quantizeFp8(X, Q, QScale, rows, cols, blockRows) {
     count("quantizeFp8");
     if (blockRows !== 1) throw new Error("fake quantizeFp8: rows only");
@@ -439,7 +460,7 @@ const native = {
 // Like the library: between graphBegin and graphEnd compute calls are recorded, not executed;
 // alloc/free work, but a buffer freed meanwhile keeps its storage for the graph's lifetime;
 // calls that need device data on the host throw and spoil the capture.
-const RECORDED = ["copy", "gemm", "gemmEx", "linearGroup", "conv2d", "conv2dEx", "binary", "unary", "softmax", "attention", "layernorm", "layernormAdd", "rmsnorm", "quantizeFp8", "gemmFp8", "reduceMean", "reduceAxis", "maxpool2d",
+const RECORDED = ["copy", "gemm", "gemmEx", "linearGroup", "conv2d", "conv2dEx", "binary", "unary", "softmax", "attention", "layernorm", "layernormAdd", "rmsnorm", "rope", "quantizeFp8", "gemmFp8", "reduceMean", "reduceAxis", "maxpool2d",
   "globalAvgpool", "transpose", "gather", "cast", "stridedCopy"];
 const REFUSED = ["write", "read", "sync", "trim", "eventRecord", "eventElapsedMs"];
 const graphs = new Map();

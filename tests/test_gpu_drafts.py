@@ -260,6 +260,41 @@ def test_a_page_without_a_place_or_a_scale(ctx, heads, new, scale):
     assert np.isnan(attend_tree(ctx, c, q, table, lens, starts, mask, 0.125)).all()
 
 
+@pytest.mark.parametrize("heads,new", [(4, [50, 3]), (16, [64, 20]), (32, [200, 7])])
+def test_scales_of_all_sizes(ctx, heads, new):
+    """Pages whose scales are far apart, no powers of two, or next to the ends of fp32; scores beyond 2^20 among them."""
+    rng = np.random.default_rng(heads)
+    c, table, lens, starts = S.filled(rng, new, [900, 640], 2, 64)
+    q = rng.standard_normal((int(starts[-1]), heads, 64)).astype(np.float32)
+    sees, mask = masks(rng, new, -(-max(new) // 32), "tree")
+    for k_scale, v_scale in ((lambda n: 2.0 ** rng.integers(-6, 3, n), lambda n: 2.0 ** rng.integers(-30, 10, n)),
+                             (lambda n: rng.uniform(0.01, 0.2, n), lambda n: rng.uniform(0.01, 5, n)),
+                             (lambda n: np.full(n, 2.0 ** -100), lambda n: np.full(n, 2.0 ** -100)),
+                             (lambda n: rng.uniform(1, 2, n) * 2.0 ** rng.integers(-40, 0, n), lambda n: rng.uniform(1, 2, n) * 2.0 ** 110),
+                             (lambda n: rng.uniform(500, 4000, n), lambda n: rng.uniform(1, 2, n)),
+                             (lambda n: rng.uniform(1, 2, n) * 2.0 ** 17, lambda n: rng.uniform(1, 2, n) * 2.0 ** rng.integers(-20, 20, n))):
+        c.ks[:] = np.asarray(k_scale(c.ks.size), np.float32).reshape(c.ks.shape)
+        c.vs[:] = np.asarray(v_scale(c.vs.size), np.float32).reshape(c.vs.shape)
+        want, bound = D.attention(c, q, table, lens, starts, sees, 0.125)
+        got = attend_tree(ctx, c, q, table, lens, starts, mask, 0.125)
+        assert np.all(np.abs(got - want) <= bound), float(np.max((np.abs(got - want) - bound) / bound))
+
+
+@pytest.mark.parametrize("d,heads,kv", [(32, 16, 1), (64, 32, 4), (128, 8, 8), (128, 32, 2)])
+@pytest.mark.parametrize("seqs,new,past", [(1, 5, 30000), (1, 70, 9000), (3, 40, 5000), (64, 3, 200), (150, 2, 70), (300, 1, 0)])
+def test_attention_of_many_lengths(ctx, d, heads, kv, seqs, new, past):
+    """Sequences of one token to tens of thousands in one call, so that items are cut anywhere, and in every number of rows to an item."""
+    rng = np.random.default_rng(seqs * 31 + d)
+    lengths = [int(n) for n in np.linspace(new, 1, seqs).round()]
+    before = [int(n) for n in np.linspace(past, 0, seqs)]
+    c, table, lens, starts = S.filled(rng, lengths, before, kv, d)
+    q = (rng.standard_normal((int(starts[-1]), heads, d)) * 3).astype(np.float32)
+    sees, mask = masks(rng, lengths, -(-max(lengths) // 32), "tree")
+    want, bound = D.attention(c, q, table, lens, starts, sees, 0.2)
+    got = attend_tree(ctx, c, q, table, lens, starts, mask, 0.2)
+    assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) - bound))
+
+
 def test_rows_of_no_sequence_stay_as_they_are(ctx):
     rng = np.random.default_rng(12)
     c, table, lens, starts = S.filled(rng, [1, 4, 2, 3], [70, 0, 9, 64], 2, 32)

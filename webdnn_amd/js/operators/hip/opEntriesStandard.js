@@ -17,6 +17,7 @@ const { getOpEntries: getOpEntriesoperatorsstandardmaxpool } = require("./operat
 const { getOpEntries: getOpEntriesoperatorsstandardreducemean } = require("./operators/standard/reducemean");
 const { getOpEntries: getOpEntriesoperatorsstandardreshape5 } = require("./operators/standard/reshape5");
 const { getOpEntries: getOpEntriesoperatorsstandardrmsnormalization } = require("./operators/standard/rmsnormalization");
+const { getOpEntries: getOpEntriesoperatorsstandardrotaryembedding } = require("./operators/standard/rotaryembedding");
 const { getOpEntries: getOpEntriesoperatorsstandardslice } = require("./operators/standard/slice");
 const { getOpEntries: getOpEntriesoperatorsstandardsoftmax } = require("./operators/standard/softmax");
 const { getOpEntries: getOpEntriesoperatorsstandardsplit } = require("./operators/standard/split");
@@ -43,6 +44,7 @@ function getOpEntries() {
   entries.push(...getOpEntriesoperatorsstandardreducemean());
   entries.push(...getOpEntriesoperatorsstandardreshape5());
   entries.push(...getOpEntriesoperatorsstandardrmsnormalization());
+  entries.push(...getOpEntriesoperatorsstandardrotaryembedding());
   entries.push(...getOpEntriesoperatorsstandardslice());
   entries.push(...getOpEntriesoperatorsstandardsoftmax());
   entries.push(...getOpEntriesoperatorsstandardsplit());
