@@ -272,6 +272,8 @@ def test_scales_of_all_sizes(ctx, heads, new):
                              (lambda n: np.full(n, 2.0 ** -100), lambda n: np.full(n, 2.0 ** -100)),
                              (lambda n: rng.uniform(1, 2, n) * 2.0 ** rng.integers(-40, 0, n), lambda n: rng.uniform(1, 2, n) * 2.0 ** 110),
                              (lambda n: rng.uniform(500, 4000, n), lambda n: rng.uniform(1, 2, n)),
+                             (lambda n: np.ones(n) / 64, lambda n: rng.choice([2.0 ** -100, 2.0 ** -100, 1e-20, 0.01, 1.0, 2.0 ** 60, 2.0 ** 110], n)),
+                             (lambda n: np.ones(n) / 64, lambda n: np.where(np.arange(n) % 4 < 2, 2.0 ** -100, 0.25)),
                              (lambda n: rng.uniform(1, 2, n) * 2.0 ** 17, lambda n: rng.uniform(1, 2, n) * 2.0 ** rng.integers(-20, 20, n))):
         c.ks[:] = np.asarray(k_scale(c.ks.size), np.float32).reshape(c.ks.shape)
         c.vs[:] = np.asarray(v_scale(c.vs.size), np.float32).reshape(c.vs.shape)

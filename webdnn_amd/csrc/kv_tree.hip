@@ -110,8 +110,10 @@ __device__ __forceinline__ i32x4 seen_values(i32x4 v, int behind, bool &bad) {
 // pass 2^14, beyond which float16 parts end.  What two parts leave out of a weight is at most 2^-23 of it or 2^-25, 2^-32 of the row's largest.
 constexpr float AIM = 8.0f, MOST = 14.0f;
 constexpr float LARGE_SCORE = 0x1p20f;  // from here on offsets are scores themselves: larger ones are whole numbers with more than 1 between them
-// Values are widened times a power of two that their page's scale asks for: 2^VALUE_AT for the first page.
-constexpr int VALUE_AT = -4, VALUE_LEAST = -15, VALUE_MOST = 7;
+// Values are widened times a power of two that their page's scale asks for: 2^VALUE_AT for the first page.  Units of results follow that scale down to 2^-BELOW
+// of the largest one so far (so that nothing overflows on the way); scales below have their weights lowered, by up to 2^BELOW again, and what that
+// leaves out of a row is at most 2^-BELOW of the largest values that it might have seen.
+constexpr int VALUE_AT = -4, VALUE_LEAST = -15, VALUE_MOST = 7, BELOW = 60;
 
 // What the join has to know of an item.
 struct Joint {
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
     for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
   float sum = 0.0f, offset = 0.0f;
   bool has_seen = false;
-  int unit_of_o = __builtin_amdgcn_frexp_expf(now.vs) - VALUE_AT;  // o is in units of 2^unit_of_o
+  int largest_ve = now.vs > 0.0f ? __builtin_amdgcn_frexp_expf(now.vs) : -126, unit_of_o = largest_ve - VALUE_AT;  // o is in units of 2^unit_of_o
   // Between wavefronts that share pages; a block's own wavefront has to wait for its own reads of LDS alone.
   auto sync = [] {
     if constexpr (RB > 1) __syncthreads();
@@ -306,7 +308,9 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
     // The values' scale: a power of two that goes with their widening, and what is left, between 1/2 and 1, which goes into the weights' exponents (and
     // out of their sum).  Where that power is out of reach of float16, o changes its units.
     const bool known = now.vs > 0.0f, even = (__float_as_uint(now.ks) & 0x7fffffu) == 0;
-    const int ve = known ? __builtin_amdgcn_frexp_expf(now.vs) : unit_of_o + VALUE_AT;
+    const int own_ve = known ? __builtin_amdgcn_frexp_expf(now.vs) : unit_of_o + VALUE_AT;
+    largest_ve = own_ve > largest_ve ? own_ve : largest_ve;
+    const int ve = own_ve > largest_ve - BELOW ? own_ve : largest_ve - BELOW, lowered = ve - own_ve < BELOW ? ve - own_ve : BELOW;
     const float rest = known ? __builtin_amdgcn_frexp_mantf(now.vs) : 0.5f;
     auto key_at = [&](int t, int j) {
       const int row = 32 * t + key_row;
@@ -427,7 +431,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
           for (int e = 0; e < 16; e++) sc[t][e] *= factor;
         c = 1.0f;
       }
-      const float v_power = power_of_two(ve - unit_of_o), from = offset + __builtin_amdgcn_logf(rest), rest_inverse = __builtin_amdgcn_rcpf(rest);
+      const float v_power = power_of_two(ve - unit_of_o), from = offset + __builtin_amdgcn_logf(rest) - (float)lowered, rest_inverse = __builtin_amdgcn_rcpf(rest) * power_of_two(lowered);
 #pragma unroll
       for (int t = 0; t < 2; t++) {
         i32x4 vp[VT];
