@@ -297,6 +297,24 @@ def test_attention_of_many_lengths(ctx, d, heads, kv, seqs, new, past):
     assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) - bound))
 
 
+@pytest.mark.parametrize("heads,new", [(4, [5, 3]), (16, [40, 20]), (32, [200, 7])])
+def test_queries_that_are_not_finite(ctx, heads, new):
+    """Such a row is NaN, unless it sees nothing; the others are what they are."""
+    rng = np.random.default_rng(heads)
+    c, table, lens, starts = S.filled(rng, new, [0, 70], 2, 64)
+    q = rng.standard_normal((int(starts[-1]), heads, 64)).astype(np.float32)
+    sees, mask = masks(rng, new, -(-max(new) // 32), "random")
+    sees[1], mask[1] = np.zeros(new[0], bool), 0
+    want, bound = D.attention(c, q, table, lens, starts, sees, 0.125)
+    bad = np.zeros(q.shape[:2], bool)
+    for r, h, value in ((1, 0, np.inf), (1, 1, np.nan), (3, 1, np.inf), (4, 2, -np.inf), (4, 3, np.nan), (new[0] + 1, 0, -np.inf), (new[0] + 2, 3, np.nan)):
+        q[r, h, rng.integers(0, 64)] = value
+        bad[r, h] = np.any(sees[r]) or r >= new[0]
+    got = attend_tree(ctx, c, q, table, lens, starts, mask, 0.125)
+    assert np.all(np.isnan(got[bad])) and np.all(got[1] == 0)
+    assert np.all(np.abs(got - want)[~bad] <= bound[~bad])
+
+
 def test_rows_of_no_sequence_stay_as_they_are(ctx):
     rng = np.random.default_rng(12)
     c, table, lens, starts = S.filled(rng, [1, 4, 2, 3], [70, 0, 9, 64], 2, 32)
@@ -734,3 +752,42 @@ def test_a_recorded_step_follows_its_sequences(ctx):
             host.update(lens=got[4], positions=got[5])
     finally:
         ctx.graph_destroy(graph)
+
+
+def test_recordings_with_workspaces_of_their_own(ctx):
+    """Two recordings of calls that share out pages and rows among workgroups, replayed in turn with other operands, and eager calls in between."""
+    rng = np.random.default_rng(43)
+    cases = []
+    for new, past in (([33], [5000]), ([9, 20, 3], [3000, 100, 1500])):
+        c, table, lens, starts = S.filled(rng, new, past, 2, 64)
+        n, vocab = int(starts[-1]), 40000
+        mask = masks(rng, new, -(-max(new) // 32), "tree")[1]
+        p, draft, tokens, parents, uniform, starts32 = drafts(rng, new, vocab, 2, True)
+        dq, dt, dl, ds, dm, dp, dd, dk, da, du = up(ctx, np.zeros((n, 16 * 64), np.float32), table, lens, starts32, mask, p, draft, tokens, parents, uniform)
+        cache, seqs = S.on_device(ctx, c), len(new)
+        run = lambda cache=cache, dq=dq, dt=dt, dl=dl, ds=ds, dm=dm, dp=dp, dd=dd, dk=dk, da=da, du=du: (
+            H.cache_attention_tree(ctx, cache, dq, 16, 0.125, dt, dl, ds, dm), *H.verify_drafts(ctx, dp, dk, da, du, ds, dd))
+        for t in run():                                                       # (the first run fills the pool)
+            t.dispose()
+        cases.append((run, dq, du))
+    ctx.sync()
+    recorded = []
+    try:
+        for run, *_ in cases:
+            ctx.graph_begin()
+            out = run()
+            recorded.append((ctx.graph_end(), out))
+        for turn in range(4):
+            for run, dq, du in cases:
+                dq.set_data(rng.standard_normal(dq.dims).astype(np.float32))
+                du.set_data(rng.random(du.dims).astype(np.float32))
+            for graph, _ in recorded:
+                ctx.graph_launch(graph)
+            for (run, *_), (_, out) in zip(cases, recorded):
+                want = run()
+                for a, b in zip(out, want):
+                    assert np.array_equal(a.get_data(), b.get_data()), turn
+                    b.dispose()
+    finally:
+        for graph, _ in recorded:
+            ctx.graph_destroy(graph)

@@ -250,15 +250,16 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       x[i][e] *= p.scale;
-      most = max(most, __float_as_uint(fabsf(x[i][e])));  // (not finite: so are its scores, whatever the others')
+      most = max(most, __float_as_uint(fabsf(x[i][e])));
     }
     const int exponent = exponent_of(__uint_as_float(lanes_max<LANES>(most)));  // (of zeros and of subnormal rows: -127)
     const int up = 14 - exponent < 126 ? 14 - exponent : 126;
+    const float times = exponent < 128 ? power_of_two(up) : NAN;  // (a row that is not finite has no scores that are)
     const int r = stream * (32 / S) + Q_ROWS * i + at_lane / LANES, d = 4 * (at_lane % LANES);
     union { f16x2 h[2]; f16x4 v; } parts[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      const f32x2 y = {x[i][2 * e] * power_of_two(up), x[i][2 * e + 1] * power_of_two(up)};
+      const f32x2 y = {x[i][2 * e] * times, x[i][2 * e + 1] * times};
       parts[0].h[e] = __builtin_convertvector(y, f16x2);
       parts[1].h[e] = __builtin_convertvector(f32x2{less_low(y[0], parts[0].h[e]), less_high(y[1], parts[0].h[e])}, f16x2);
     }
