@@ -101,6 +101,27 @@ def test_rope_of_extreme_rows_and_positions(ctx):
         assert np.isnan(got[r, 0, :32]).all() and np.all(np.abs(got[r, 0, 32:] - want[r, 0, 32:]) <= bound[r, 0, 32:])
 
 
+@pytest.mark.parametrize("d,rotary,interleaved", [(64, 64, False), (128, 128, False), (256, 256, False), (512, 512, False), (64, 64, True), (96, 30, True), (700, 700, True),
+                                                  (96, 96, False), (64, 24, False)])
+def test_rope_of_extreme_rows_in_every_form(ctx, d, rotary, interleaved):
+    """The same for pairs that a lane holds and for those that it does not; in place as well."""
+    rng = np.random.default_rng(d)
+    x = rng.standard_normal((9, 2, d)).astype(np.float32)
+    x[0, 0], x[1], x[2] = 0, x[1] * np.float32(1e25), x[2] * np.float32(1e-30)
+    x[3, 0, 1], x[4, 1, d - 1], x[8, 0, 0] = np.inf, np.nan, 3e38
+    cos, sin = D.tables(9, rotary)
+    positions = np.array([1, 8, 3, 4, 5, 9, -1, 1 << 30, 0], np.int32)
+    gamma = rng.uniform(0.5, 1.5, d).astype(np.float32)
+    dx, dc, ds, dp, dg = up(ctx, x.reshape(9, -1), cos, sin, positions, gamma)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        want, bound = D.rope(x, gamma, cos, sin, positions, interleaved, 0.0)
+    for out in (None, dx):
+        got = H.rotary_embedding(ctx, dx, dc, ds, dp, 2, d, q_scale=dg, interleaved=interleaved, epsilon=0.0, out=out).get_data().reshape(x.shape)
+        known = np.isfinite(want)
+        assert np.array_equal(np.isnan(got), ~known)
+        assert np.all(np.abs(got - want)[known] <= bound[known])
+
+
 def test_rope_without_rows(ctx):
     y = H.rotary_embedding(ctx, ctx.empty_tensor([0, 64]), None, None, None, 2, 32)
     assert y.get_data().shape == (0, 64)
