@@ -102,7 +102,7 @@ def test_rope_of_extreme_rows_and_positions(ctx):
 
 
 @pytest.mark.parametrize("d,rotary,interleaved", [(64, 64, False), (128, 128, False), (256, 256, False), (512, 512, False), (64, 64, True), (96, 30, True), (700, 700, True),
-                                                  (96, 96, False), (64, 24, False)])
+                                                  (96, 96, False), (64, 24, False), (80, 32, False), (33, 16, False), (300, 64, False), (1000, 64, False), (20, 8, False), (32, 32, False)])
 def test_rope_of_extreme_rows_in_every_form(ctx, d, rotary, interleaved):
     """The same for pairs that a lane holds and for those that it does not; in place as well."""
     rng = np.random.default_rng(d)

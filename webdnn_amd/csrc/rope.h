@@ -17,8 +17,8 @@ struct Rotation {
   int half, rows;
 };
 // Which pairs there are: (x[2j], x[2j + 1]), in a lane's four elements both; (x[j], x[j + half]) of a whole head, where a lane has four elements of the lower half
-// and their partners; or anywhere in the head.
-enum Pairs { NEIGHBOURS, FACING, ANYWHERE };
+// and their partners; the same with partners in a lane that differs in one bit of its number; or anywhere in the head.
+enum Pairs { NEIGHBOURS, FACING, EXCHANGED, ANYWHERE };
 typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
 
 // The partners, ANYWHERE, of elements d0 .. d0+3 of `from` (a head, or what it is multiplied with), 0 where there are none.

@@ -30,7 +30,7 @@ struct RopeParams {
 
 // LANES lanes to a head, NP pieces of four elements to a lane.  FACING: a head of 8 LANES elements is rotated whole, by halves, so that a lane's two pieces
 // are each other's partners.  A lane has two pieces wherever there are as many, for it is instructions that bound this: 8192 tokens of 40 heads of 128 take
-// 86 us with one piece to a lane, 62 so.  (More heads to a lane take longer: 2 95 us, 4 121.)
+// 86 us with one piece to a lane, 62 so.  EXCHANGED: halves of a part of the head; 64 of 128 elements 73 us with partners loaded again, 65 so.  (More heads to a lane take longer: 2 95 us, 4 121.)
 template <int LANES, int NP, int PAIRS>
 __global__ __launch_bounds__(256) void head_rope(RopeParams p) {
   const int lane = threadIdx.x % LANES;
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void head_rope(RopeParams p) {
       o[i] = partners(p.r, x, d0, d);
       if (g) other_gamma[i] = partners(p.r, g, d0, d);
     }
-    if (PAIRS != FACING || i == 0) a[i] = angles<PAIRS>(p.r, position, d0);
+    if ((PAIRS != FACING && PAIRS != EXCHANGED) || i == 0) a[i] = angles<PAIRS>(p.r, position, d0);
   }
   if (g) {
     double sum = 0.0;
@@ -62,6 +62,11 @@ __global__ __launch_bounds__(256) void head_rope(RopeParams p) {
       v[i] = normed(v[i], f, gamma[i]);
       if constexpr (PAIRS == ANYWHERE) o[i] = normed(o[i], f, other_gamma[i]);
     }
+  }
+  if constexpr (PAIRS == EXCHANGED) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[0][e] = __shfl_xor(v[0][e], p.r.half / 4, LANES);
+    v[0] = turn(p.r, 4 * lane, v[0], o[0], a[0]);
   }
   if (at >= p.units) return;
   if constexpr (PAIRS == FACING) turn_facing(v[0], v[1], a[0]);
@@ -89,6 +94,8 @@ int launch_pairs(const RopeParams &p, bool neighbours) {
   if (neighbours) return launch<LANES, NP, NEIGHBOURS>(p);
   if constexpr (NP == 2)
     if (p.r.half == 4 * LANES) return launch<LANES, 2, FACING>(p);
+  // (a power of two of four elements, within the lanes' first pieces)
+  if (p.r.half >= 4 && (p.r.half & (p.r.half - 1)) == 0 && p.r.half <= 2 * LANES) return launch<LANES, NP, EXCHANGED>(p);
   return launch<LANES, NP, ANYWHERE>(p);
 }
 
