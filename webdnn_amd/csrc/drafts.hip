@@ -344,6 +344,13 @@ struct KeepParams {
   int heads;
 };
 
+// What takes elements of a page of scale `scale` to one of scale 1 / inv.  The new scale holds 1/448 of each element, the least of which is 2^-9: more than 2^18 is
+// for zeros alone, which an infinite ratio (scales of 2^28 and 2^-100) would make NaN.  A scale that is no number leaves none.
+__device__ __forceinline__ float to_scale(float scale, float inv) {
+  const float ratio = scale * inv;
+  return ratio > 0x1p18f && scale <= FLT_MAX ? 0x1p18f : ratio;
+}
+
 // Tokens of a path go behind each other: slot past + i takes what slot past + path[i] holds, which is never before it.  So a workgroup has a
 // sequence's pages of one head, keys (blockIdx.z 0) or values, and goes over them in order; what a page takes is in registers before any of
 // it is written, and what later pages take lies behind.  Bound: latency, of five rounds of loads after each other (numbers of rows; path; tables; scales and
@@ -447,7 +454,7 @@ __global__ __launch_bounds__(256) void cache_keep(KeepParams p) {
         if (k >= words) continue;
         f32x4 y;
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = v[i][e] * (scale_of[values ? s0 + e : s0] * inv);
+        for (int e = 0; e < 4; e++) y[e] = v[i][e] * to_scale(scale_of[values ? s0 + e : s0], inv);
         reinterpret_cast<int *>(page)[w] = values ? merge4(old[i], pack4(y, 1.0f), first - s0, last - s0, grown, factor) : pack4(y, 1.0f);
       }
       if (grown) {  // the tokens before
