@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
   if constexpr (TURN != AS_IT_IS)
     if (!values) {
       // (a thread's pieces are the same elements of all its tokens)
-      constexpr int GROUP = TURN == wdh::rope::FACING ? PPT / 2 : PPT, EACH = TURN == wdh::rope::FACING ? 2 : 1;  // lanes to a token, and pieces of it to a lane
+      constexpr int EACH = TURN == wdh::rope::FACING ? 2 : 1;  // pieces of a token to a lane
       const int d0 = d0_of(0);
       const bool norm = p.gamma != nullptr;
       const f32x4 one = {1.f, 1.f, 1.f, 1.f}, g = norm ? load4(p.gamma, d0, D) : one;
@@ -97,9 +97,10 @@ __global__ __launch_bounds__(256) void cache_append(AppendParams p) {
         for (int i = 0; i < AT_ONCE; i += EACH) {
           f32x4 &own = v[round + i], &other = TURN == wdh::rope::FACING ? v[round + i + 1] : o[i];
           if (norm) {
-            double sum = wdh::rope::squares(own);
-            if constexpr (TURN == wdh::rope::FACING) sum += wdh::rope::squares(other);
-            const wdh::rowmath::RowFactor f = wdh::rope::head_factor(wdh::rope::group_sum<GROUP>(sum) / (double)D, p.eps);
+            double sum;
+            if constexpr (TURN == wdh::rope::FACING) sum = wdh::rope::head_squares<D>(own, other);
+            else sum = wdh::rope::head_squares<D>(own);
+            const wdh::rowmath::RowFactor f = wdh::rope::head_factor(sum / (double)D, p.eps);
             own = wdh::rope::normed(own, f, g);
             if constexpr (TURN != wdh::rope::NEIGHBOURS) other = wdh::rope::normed(other, f, og);
           }

@@ -89,6 +89,8 @@ __device__ __forceinline__ void turn_facing(f32x4 &low, f32x4 &high, Angles a) {
   }
 }
 
+constexpr int DPP_ROTATE8 = 0x128;  // lanes of a row of 16 that are 8 apart
+
 // Sums over groups of LANES neighbouring lanes, in all of them.
 template <int CTRL>
 __device__ __forceinline__ double dpp_add_d(double v) {
@@ -112,6 +114,21 @@ __device__ __forceinline__ double squares(f32x4 v) {
 #pragma unroll
   for (int e = 0; e < 4; e++) sum = fma((double)v[e], (double)v[e], sum);
   return sum;
+}
+// A head's sum of squares in the order in which wdh_rope adds it, whose lanes have the pieces of both halves of a head of 64 or 128 (of 32: one of eight pieces), for
+// lanes that have one of its pieces each, and for those that have two which face each other: the factor's bits, and with them those of the
+// cache, may hang on it.
+template <int D>
+__device__ __forceinline__ double head_squares(f32x4 own) {
+  const double v = squares(own);
+  if constexpr (D == 32) return group_sum<8>(v);
+  else if constexpr (D == 64) return group_sum<8>(dpp_add_d<DPP_ROTATE8>(v));
+  else return group_sum<16>(v + __shfl_xor(v, 16, 64));
+}
+template <int D>
+__device__ __forceinline__ double head_squares(f32x4 low, f32x4 high) {
+  if constexpr (D == 32) return group_sum<4>(squares(low)) + group_sum<4>(squares(high));
+  else return group_sum<D / 8>(squares(low) + squares(high));
 }
 // What a head's elements are multiplied with, from the mean of their squares.  Division and root of 64 bits are some 40 instructions for a number that is
 // rounded to 32; instead the instruction's root, good to 2^-26 or so, and one step of Newton's, y + y (1 - m y^2) / 2, which leaves 1.5 of that
