@@ -571,8 +571,9 @@ int wdh_cache_append_rope(wdh_buf K, int64_t k_offset, int64_t k_stride, wdh_buf
 /* wdh_cache_attention for rows that do not follow one another: a row sees all tokens that its sequence had before the call's, and of
  * the call's those whose bits are set in its mask: Mask [tokens, words] (int32), bit j % 32 of word j / 32 for row j of the same sequence (a
  * tree's row sets the bits of its ancestors and its own).  Bits of rows that the sequence does not have count for nothing, rows beyond 32
- * words are not seen.  A row that sees nothing gets 0.  words is 1 to 2^19.  All else as in wdh_cache_attention, except that values of pages
- * whose scale is below 2^-60 of the largest one among the sequence's pages may count as 0. */
+ * words are not seen.  A row that sees nothing gets 0.  words is 1 to 2^19.  All else as in wdh_cache_attention, except that a token whose weight
+ * times its page's scale is below 2^-32 of the row's largest such product may be missing among the values, not in the sum of weights (n of
+ * them take n 2^-32 of the largest share from a result). */
 int wdh_cache_attention_tree(wdh_buf Q, int64_t q_offset, int64_t q_stride, wdh_buf KPages, wdh_buf KScales, wdh_buf VPages,
                              wdh_buf VScales, wdh_buf Table, wdh_buf Lens, wdh_buf Starts, wdh_buf Mask, wdh_buf Y, int seqs,
                              int tokens, int heads, int kv_heads, int d, int pages, int max_pages, int words, float alpha);

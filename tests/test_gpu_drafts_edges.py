@@ -1,5 +1,5 @@
 """The operators for drafted tokens at operands where a definition and a shortcut part: zeros kept from pages of large scales; norms beside the
-middle of two fp32 numbers."""
+middle of two fp32 numbers; attention of trees over pages whose values differ in size, and at scores of any size."""
 import math
 from fractions import Fraction
 
@@ -9,6 +9,7 @@ import pytest
 import drafts_ref as D
 import fp8_ref as F
 import test_gpu_drafts as T
+import test_gpu_fp8_edges as X
 import test_gpu_fp8_serving as S
 from webdnn_amd import hostops as H
 
@@ -112,3 +113,124 @@ def test_append_rope_adds_squares_as_rope_does(ctx, d, rotary, interleaved):
     assert np.any(first <= 272) and np.any(first > 272)                       # (the rows are on both sides of the middle)
     assert np.array_equal(one.k_scales.get_data(), two.k_scales.get_data())
     assert np.array_equal(one.k.get_data(), two.k.get_data())
+
+
+# ---- attention over pages whose values differ in size ----------------------------------------------
+def chain(n):
+    return H.tree_mask(np.arange(-1, n - 1), np.array([0, n]))
+
+
+@pytest.mark.parametrize("octaves", [0, 16, 30, 60, 82])
+@pytest.mark.parametrize("new,heads,kv,d,large", [(1, 4, 2, 64, [0]), (7, 4, 1, 128, [3, 4]), (90, 4, 2, 64, [2]), (30, 4, 2, 32, [9]), (650, 64, 2, 64, [0]),
+                                                  (650, 64, 2, 64, [3, 7]), (650, 64, 2, 64, [11]), (700, 32, 4, 128, [1]), (1300, 64, 2, 32, [0, 9])])
+def test_values_of_pages_that_differ_in_size(ctx, new, heads, kv, d, large, octaves):
+    """As of wdh_cache_attention, with its bound: rows of chains."""
+    rng = np.random.default_rng(octaves)
+    past = 640
+    c, table, lens, starts, q = X.sized_pages(rng, new, past, heads, kv, d, large, octaves)
+    want = X.attention(c, q, table[0], int(lens[0]), d ** -0.5)
+    got = T.attend_tree(ctx, c, q, table, lens, starts, chain(new), np.float32(d ** -0.5))
+    assert X.relative(got, want) <= 2.0 ** -20, (X.relative(got, want) * 2 ** 20)
+
+
+@pytest.mark.parametrize("small,large,nats", [(-90, 110, 320), (-90, 110, 40), (-90, 110, 7), (-30, 100, 160), (0, 70, 60), (-95, -30, 30), (-20, 40, 0), (0, 50, 22)])
+@pytest.mark.parametrize("new,heads,kv,d,pages", [(2, 4, 2, 64, [0]), (2, 4, 2, 64, [9]), (9, 4, 1, 128, [4, 5]), (50, 4, 2, 64, [0, 3]), (90, 4, 2, 32, [2]), (650, 64, 2, 64, [0, 5]),
+                                                  (650, 64, 2, 64, [8])])
+def test_pages_of_all_sizes_count_by_their_shares(ctx, new, heads, kv, d, pages, small, large, nats):
+    """Some pages hold values of 2^large, the others of 2^small; the former's keys are `nats` below the latter's.  Which of them a row rests on goes by weight
+    times value, and its sum of weights by the weights alone.
+
+    The bound for scores of size one: see test_gpu_fp8_edges.test_values_of_pages_that_differ_in_size.  Here one product of a score is `nats`, alike for all keys of
+    a page, so that what it is off shows in all of a row: 2^-23 by its query's parts, 2^-24 each by alpha, alpha log2(e) and the query times that (3 / 2^23 together), and
+    2^-23 by each of the 2 d / 16 instructions that add to it (their additions need not round to nearest); in all nats (3 + d / 8) 2^-23 of a weight."""
+    rng = np.random.default_rng(large - small)
+    past = 640
+    table, lens, starts, count = S.layout(rng, [new], [past])
+    n = int(lens[0])
+    k, v = (rng.standard_normal((n, kv, d)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((new, heads, d)).astype(np.float32)
+    k[:, :, 0], q[:, :, 0] = 0, 16
+    octave = np.full(n, small)
+    for page in pages:
+        at = slice(64 * page, 64 * page + 64)
+        k[at, :, 0], octave[at] = -nats / 16 / d ** -0.5, large
+    v *= np.float32(2) ** octave.astype(np.float32)[:, None, None]
+    c = F.Cache(count, kv, d)
+    c.append(k, v, table, lens, np.array([0, n]))
+    want = X.attention(c, q, table[0], n, d ** -0.5)
+    got = T.attend_tree(ctx, c, q, table, lens, starts, chain(new), np.float32(d ** -0.5))
+    assert X.relative(got, want) <= 2.0 ** -20 + nats * (3 + d / 8) * 2.0 ** -23, (X.relative(got, want) * 2 ** 20)
+
+
+@pytest.mark.parametrize("new,past,heads,kv,d", [(1, 900, 8, 2, 64), (60, 100, 4, 2, 128), (3, 3000, 2, 1, 128), (650, 100, 64, 2, 64), (700, 0, 32, 4, 128), (40, 200, 2, 2, 32)])
+@pytest.mark.parametrize("size", [1e2, 3e3, 1e4, 1e5, 1e7, 1e9, 1e14])
+def test_scores_of_any_size(ctx, new, past, heads, kv, d, size):
+    """Where neighbouring fp32 numbers are further apart than the powers of two that weights are, rows rest on their largest score: the others
+    are left far behind (rows whose two largest scores are not further apart than their errors are left out), on pages whose values are 2^5 times as
+    large too (2^10 times what is 30 nats below: 2^-33)."""
+    rng = np.random.default_rng(new)
+    table, lens, starts, pages = S.layout(rng, [new], [past])
+    n = int(lens[0])
+    k, v = (rng.standard_normal((n, kv, d)).astype(np.float32) for _ in range(2))
+    c = F.Cache(pages, kv, d)
+    c.append(k * np.float32(size), v, table, lens, np.array([0, n]))
+    c.ks *= rng.uniform(0.5, 1, c.ks.shape).astype(np.float32)
+    c.vs *= rng.uniform(0.5, 1, c.vs.shape).astype(np.float32) * np.float32(2) ** rng.integers(-5, 6, c.vs.shape).astype(np.float32)
+    q = (rng.standard_normal((new, heads, d)) * size).astype(np.float32)
+    keys, values = c.tokens(table[0], n)
+    got = T.attend_tree(ctx, c, q, table, lens, starts, chain(new), 0.125)
+    tried = 0
+    for h in range(heads):
+        kv_head = h // (heads // kv)
+        t = q[:, h].astype(np.float64) @ keys[kv_head].T * 0.125
+        t[np.arange(n) > np.arange(new)[:, None] + past] = -np.inf
+        order = np.sort(t, 1)
+        far = np.ones(new, bool) if n == 1 else order[:, -1] - order[:, -2] > 2.0 ** -15 * np.abs(q[:, h]).sum(1) * size * 0.125 + 30
+        if past == 0:
+            far[0] = True
+        best = t.argmax(1)
+        scale = c.vs[table[0][best // 64], kv_head].astype(np.float64)
+        assert np.all((np.abs(got[:, h] - values[kv_head][best]) <= 2.0 ** -20 * 448 * scale[:, None])[far]), h
+        tried += far.sum()
+    assert tried > 0.5 * heads * new
+
+
+@pytest.mark.parametrize("new,heads,kv,d", [(2, 4, 2, 64), (50, 4, 2, 64), (90, 4, 2, 128), (650, 64, 2, 32)])
+@pytest.mark.parametrize("size", [1.0, 1e3, 3e4, 1e6])
+def test_equal_scores_of_any_size_share_a_row(ctx, new, heads, kv, d, size):
+    """All keys alike, whatever the values' scales: rows are the average of what they see.  Weights are equal numbers, so what is off is the sums, of 2^-23 an
+    addition at most, and values' products."""
+    rng = np.random.default_rng(int(size))
+    past = 448
+    table, lens, starts, pages = S.layout(rng, [new], [past])
+    n = int(lens[0])
+    k = np.repeat(rng.standard_normal((1, kv, d)).astype(np.float32), n, 0) * np.float32(size)
+    v = rng.standard_normal((n, kv, d)).astype(np.float32)
+    c = F.Cache(pages, kv, d)
+    c.append(k, v, table, lens, np.array([0, n]))
+    c.vs *= np.float32(2) ** rng.integers(-9, 9, c.vs.shape).astype(np.float32)
+    q = (rng.standard_normal((new, heads, d)) * size).astype(np.float32)
+    _, values = c.tokens(table[0], n)
+    upto = np.cumsum(values, 1)[:, past:] / np.arange(past + 1, n + 1)[None, :, None]
+    want = np.repeat(upto, heads // kv, 0).transpose(1, 0, 2)
+    got = T.attend_tree(ctx, c, q, table, lens, starts, chain(new), 1.0)
+    assert X.relative(got, want) <= 2.0 ** -20, (X.relative(got, want) * 2 ** 20)
+
+
+@pytest.mark.parametrize("new,heads,kv,d", [(2, 4, 2, 64), (30, 4, 2, 128), (90, 4, 2, 32)])
+@pytest.mark.parametrize("octaves", [24, 31, 34])
+def test_many_small_weights_beside_a_large_one(ctx, new, heads, kv, d, octaves):
+    """20000 tokens with weights of 2^-octaves, whose values do not cancel: 2^-20 as above, and no more than 2^-32 of the largest share for each of them."""
+    rng = np.random.default_rng(octaves)
+    past = 20000
+    table, lens, starts, pages = S.layout(rng, [new], [past])
+    n = int(lens[0])
+    k, v = np.zeros((n, kv, d), np.float32), rng.uniform(1, 2, (n, kv, d)).astype(np.float32)
+    k[:, :, 0], k[3, :, 0] = -octaves * np.log(2) / 16 / d ** -0.5, 0
+    q = np.zeros((new, heads, d), np.float32)
+    q[:, :, 0] = 16
+    c = F.Cache(pages, kv, d)
+    c.append(k, v, table, lens, np.array([0, n]))
+    want = X.attention(c, q, table[0], n, d ** -0.5)
+    got = T.attend_tree(ctx, c, q, table, lens, starts, chain(new), np.float32(d ** -0.5))
+    assert np.all(np.abs(got - want) <= 2 * (2.0 ** -20 + n * 2.0 ** -32))

@@ -22,15 +22,6 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-// Eight e4m3 values times a power of two from 2^-15 to 2^7 as float16: exact, whatever the value.
-__device__ __forceinline__ f16x8 widen_times(int lo, int hi, float power) {
-  union { f16x2 h[4]; f16x8 v; } u;
-  u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)lo, power, false);
-  u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)lo, power, true);
-  u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)hi, power, false);
-  u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)hi, power, true);
-  return u.v;
-}
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 0xff) - 127; }  // (of 0 and subnormal numbers: -127)
 
@@ -106,14 +97,15 @@ __device__ __forceinline__ i32x4 seen_values(i32x4 v, int behind, bool &bad) {
   return v;
 }
 
-// Weights are held as 2^(score + offset): the largest of a row is brought to 2^7 .. 2^8 when it is first seen, and again only when a larger one would
-// pass 2^14, beyond which float16 parts end.  What two parts leave out of a weight is at most 2^-23 of it or 2^-25, 2^-32 of the row's largest.
-constexpr float AIM = 8.0f, MOST = 14.0f;
-constexpr float LARGE_SCORE = 0x1p20f;  // from here on offsets are scores themselves: larger ones are whole numbers with more than 1 between them
-// Values are widened times a power of two that their page's scale asks for: 2^VALUE_AT for the first page.  Units of results follow that scale down to 2^-BELOW
-// of the largest one so far (so that nothing overflows on the way); scales below have their weights lowered, by up to 2^BELOW again, and what that
-// leaves out of a row is at most 2^-BELOW of the largest values that it might have seen.
-constexpr int VALUE_AT = -4, VALUE_LEAST = -15, VALUE_MOST = 7, BELOW = 60;
+// A row's weights go into the second product times their pages' scales (a power of two and a rest between 1/2 and 1), as 2^(score + ref + shift) rest with
+// shift = lift + the power's exponent.  lift brings the largest share so far to 2^7 .. 2^9 when the row first sees something, and again only when a larger one might
+// pass 2^15, beyond which float16 parts end.  What two parts leave out of a share is at most 2^-23 of it or 2^-25, 2^-32 of the row's largest, whatever the scales of
+// pages that count for less.  The sum of weights is in units of 2^-ref, in which the first page's largest weight is 1/2 to 1, and none passes 2^MOST_WEIGHT: shares and
+// weights may be far apart (values of 2^110 behind weights of 2^-200, beside values of 2^-100).  Where a page's shares are so far below others' that its weights
+// would leave fp32 on the way to their sum, LEAST_SHIFT keeps them from that, with which they are still nothing to float16.
+constexpr float AIM = 9.0f, MOST = 15.0f, MOST_WEIGHT = 50.0f, LEAST_SHIFT = -80.0f;
+static_assert(MOST_WEIGHT + LEAST_SHIFT < -25.0f, "half of float16's least number");
+constexpr float LARGE_SCORE = 0x1p20f;  // from here on fp32 numbers are too far apart for ref and shift to be added first
 
 // What the join has to know of an item.
 struct Joint {
@@ -283,9 +275,8 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
   for (int i = 0; i < VT; i++)
 #pragma unroll
     for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
-  float sum = 0.0f, offset = 0.0f;
-  bool has_seen = false;
-  int largest_ve = now.vs > 0.0f ? __builtin_amdgcn_frexp_expf(now.vs) : -126, unit_of_o = largest_ve - VALUE_AT;  // o is in units of 2^unit_of_o
+  float sum = 0.0f, ref = 0.0f, lift = 0.0f;  // o is in units of 2^-(ref + lift), the sum of 2^-ref
+  bool has_seen = false, far = false;                  // far: some row's ref is a LARGE_SCORE
   // Between wavefronts that share pages; a block's own wavefront has to wait for its own reads of LDS alone.
   auto sync = [] {
     if constexpr (RB > 1) __syncthreads();
@@ -310,13 +301,9 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
     if constexpr (TAIL)
 #pragma unroll
       for (int t = 0; t < 2; t++) bits_of[t] = sees_in(pg + S, 32 * t + 16 * half);
-    // The values' scale: a power of two that goes with their widening, and what is left, between 1/2 and 1, which goes into the weights' exponents (and
-    // out of their sum).  Where that power is out of reach of float16, o changes its units.
+    // The values' scale: a power of two and what is left, between 1/2 and 1; both go into the weights' exponents, and out of their sum.
     const bool known = now.vs > 0.0f, even = (__float_as_uint(now.ks) & 0x7fffffu) == 0;
-    const int own_ve = known ? __builtin_amdgcn_frexp_expf(now.vs) : unit_of_o + VALUE_AT;
-    largest_ve = own_ve > largest_ve ? own_ve : largest_ve;
-    const int ve = own_ve > largest_ve - BELOW ? own_ve : largest_ve - BELOW, lowered = ve - own_ve < BELOW ? ve - own_ve : BELOW;
-    const float rest = known ? __builtin_amdgcn_frexp_mantf(now.vs) : 0.5f;
+    const float ve = known ? (float)__builtin_amdgcn_frexp_expf(now.vs) : 0.0f, rest = known ? __builtin_amdgcn_frexp_mantf(now.vs) : 0.5f;
     auto key_at = [&](int t, int j) {
       const int row = 32 * t + key_row;
       return *reinterpret_cast<const i32x4 *>(keys + row * D + 16 * key_piece(row, 2 * j + half));
@@ -326,9 +313,10 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
       bring_values(then.at, buf ^ 1);
     }
     f32x16 sc[2];
-    float c;
+    float c, shift;
     // (Where what is there has to be brought to other units, rarely, the page is begun again, so that the accumulators change in its products, in one
-    // place beside them, and not in a branch on the way.)
+    // place beside them, and not in a branch on the way; once, after which its own shares and weights are in range.)
+    bool again = false;
     for (; HAS_ROWS;) {
       // (the queries' place hidden from the compiler, which would hold them all in registers that the loop has better use for)
       const int hidden = fresh(lane), hidden_row = hidden & 31;
@@ -388,21 +376,29 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
 #pragma unroll
       for (int e = 1; e < 32; e++) most = fmaxf(most, sc[e / 16][e % 16]);
       most = both_halves(most, max2) * c;
-      const float top = ceilf(most), wanted = fabsf(top) < LARGE_SCORE ? AIM - top : -top;
-      if (!has_seen && most > -INFINITY) {
-        offset = wanted;
-        has_seen = true;
+      if (__any(!has_seen && most > -INFINITY)) {
+        if (!has_seen && most > -INFINITY) {
+          ref = -ceilf(most);
+          lift = AIM - ve;
+          has_seen = true;
+        }
+        far = __any(fabsf(ref) >= LARGE_SCORE);
       }
-      const bool passes = most + offset > MOST, moves = ve - unit_of_o < VALUE_LEAST || ve - unit_of_o > VALUE_MOST;
-      if (!__any(passes) && !moves) break;
-      const float to = passes ? wanted : offset;
-      float scaled = __builtin_amdgcn_exp2f(to - offset);
-      sum *= scaled;
-      offset = to;
-      if (moves) {
-        scaled = __builtin_amdgcn_ldexpf(scaled, unit_of_o - (ve - VALUE_AT));
-        unit_of_o = ve - VALUE_AT;
+      float above = most + ref;
+      shift = fmaxf(ve + lift, LEAST_SHIFT);
+      if (!__any(above > MOST_WEIGHT || above + shift > MOST)) break;
+      float to = ref, by = lift;
+      if (above > MOST_WEIGHT) {  // (o's units stay)
+        to = -ceilf(most);
+        by += ref - to;
+        above = most + to;
       }
+      if (above + ve + by > MOST) by = AIM - ceilf(above) - ve;
+      const float scaled = __builtin_amdgcn_exp2f((to - ref) + (by - lift));
+      sum *= __builtin_amdgcn_exp2f(to - ref);
+      ref = to;
+      lift = by;
+      far = __any(fabsf(ref) >= LARGE_SCORE);
 #pragma unroll
       for (int i = 0; i < VT; i++)
 #pragma unroll
@@ -427,16 +423,26 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
       bad_values[stream][~n & 1] = 0;  // (read a turn ago, written in the next: there is a barrier on both sides)
     }
     if constexpr (HAS_ROWS) {
-      // A scale that is no power of two rounds products with it: the largest was rounded before it became the offset, so are the others.
-      if (!even) {
+      // A scale that is no power of two rounds products with it: the largest was rounded before ref was taken from it, so are the others.
+      float from = ref;
+      if (!even || far) {
         const float factor = rarely(c);
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
           for (int e = 0; e < 16; e++) sc[t][e] *= factor;
         c = 1.0f;
+        if (far) {
+          const float less = rarely(ref);
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[t][e] += less;
+          from = 0.0f;
+        }
       }
-      const float v_power = power_of_two(ve - unit_of_o), from = offset + __builtin_amdgcn_logf(rest) - (float)lowered, rest_inverse = __builtin_amdgcn_rcpf(rest) * power_of_two(lowered);
+      const float scale = shift + __builtin_amdgcn_logf(rest), of_sum = __builtin_amdgcn_exp2f(-scale);
+      from += scale;
 #pragma unroll
       for (int t = 0; t < 2; t++) {
         i32x4 vp[VT];
@@ -447,7 +453,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
         float added = sc[t][0];
 #pragma unroll
         for (int e = 1; e < 16; e++) added += sc[t][e];
-        sum = __builtin_fmaf(added, rest_inverse, sum);
+        sum = __builtin_fmaf(added, of_sum, sum);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
           float x[8];
@@ -457,7 +463,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
           split2(x, pr);
 #pragma unroll
           for (int i = 0; i < VT; i++) {
-            const f16x8 vw = widen_times(vp[i][2 * u], vp[i][2 * u + 1], v_power);
+            const f16x8 vw = widen_f16(vp[i][2 * u], vp[i][2 * u + 1]);
 #pragma unroll
             for (int part = 1; part >= 0; part--) o[i] = mfma32(vw, pr[part], o[i]);
           }
@@ -516,11 +522,11 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
     for (int a = 0; a < 4; a++) {
       f32x4 y;
 #pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_ldexpf(o[i][4 * a + e] * inverse, unit_of_o);
+      for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_ldexpf(o[i][4 * a + e] * inverse, -(int)lift);
       *reinterpret_cast<f32x4 *>(&lds.outs[wave][li * OP + 32 * i + 8 * a + 4 * half]) = y;
     }
   if (half == 0) {
-    tops[wave][li] = sum == 0.0f ? -INFINITY : -offset;
+    tops[wave][li] = sum == 0.0f ? -INFINITY : -ref;
     sums[wave][li] = sum;
   }
   __syncthreads();
