@@ -1,16 +1,18 @@
 """The operators for drafted tokens at operands where a definition and a shortcut part: zeros kept from pages of large scales; norms beside the
-middle of two fp32 numbers; attention of trees over pages whose values differ in size, and at scores of any size."""
+middle of two fp32 numbers; attention of trees over pages whose values differ in size, at scores of any size, and in 2-norm in every form."""
 import math
 from fractions import Fraction
 
 import numpy as np
 import pytest
+import torch
 
 import drafts_ref as D
 import fp8_ref as F
 import test_gpu_drafts as T
 import test_gpu_fp8_edges as X
 import test_gpu_fp8_serving as S
+import tree_plan
 from webdnn_amd import hostops as H
 
 pytestmark = pytest.mark.gpu
@@ -234,3 +236,43 @@ def test_many_small_weights_beside_a_large_one(ctx, new, heads, kv, d, octaves):
     want = X.attention(c, q, table[0], n, d ** -0.5)
     got = T.attend_tree(ctx, c, q, table, lens, starts, chain(new), np.float32(d ** -0.5))
     assert np.all(np.abs(got - want) <= 2 * (2.0 ** -20 + n * 2.0 ** -32))
+
+
+# ---- precision ----------------------------------------------------------------------------------------
+def any_cache(rng, new, past, kv, d):
+    """A cache of normally distributed elements, its scales any numbers of a size."""
+    table, lens, starts, pages = S.layout(rng, new, past)
+    c = F.Cache(pages, kv, d)
+    pool = F.encode(rng.standard_normal(4099) * 64)
+    c.k[:], c.v[:] = (rng.choice(pool, x.shape) for x in (c.k, c.v))
+    for s in (c.ks, c.vs):
+        s[:] = rng.uniform(0.7, 1.4, s.shape) / 64
+    return c, table, lens, starts
+
+
+def attention_of_trees(c, q, table, lens, starts, mask, alpha):
+    out = np.empty(q.shape)
+    group = q.shape[1] // c.heads
+    for s, length in enumerate(lens):
+        a, b = starts[s], starts[s + 1]
+        n, past = b - a, length - (b - a)
+        k, v = (torch.from_numpy(t) for t in c.tokens(table[s], int(length)))
+        sees = torch.ones((n, int(length)), dtype=torch.bool)
+        sees[:, past:] = torch.from_numpy(D.unpack(mask[a:b], n)[:, :n])
+        for h in range(q.shape[1]):
+            t = torch.from_numpy(q[a:b, h].astype(np.float64)) @ k[h // group].T * alpha
+            out[a:b, h] = (torch.softmax(t.masked_fill(~sees, -np.inf), 1) @ v[h // group]).numpy()
+    return out
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("new,past,heads,kv", tree_plan.CASES)
+def test_attention_in_2_norm(ctx, new, past, heads, kv, d):
+    """In every form of items.  (The bound: see test_gpu_fp8_edges.test_values_of_pages_that_differ_in_size.)"""
+    rng = np.random.default_rng(sum(new) + d)
+    c, table, lens, starts = any_cache(rng, new, past, kv, d)
+    q = rng.standard_normal((sum(new), heads, d)).astype(np.float32)
+    mask = H.tree_mask(np.concatenate([D.tree(rng, n, 3) for n in new]), starts)
+    want = attention_of_trees(c, q, table, lens, starts, mask, d ** -0.5)
+    got = T.attend_tree(ctx, c, q, table, lens, starts, mask, np.float32(d ** -0.5))
+    assert X.relative(got, want) <= 2.0 ** -20, X.relative(got, want) * 2.0 ** 20
