@@ -599,8 +599,8 @@ int wdh_verify_drafts(wdh_buf P, wdh_buf Draft, wdh_buf Tokens, wdh_buf Parents,
  * past + i takes what slot past + Path[Starts[s] + i] holds, for i = 0 .. Count[s] (Count and Path of wdh_verify_drafts; paths go up).  The
  * sequence then has past + 1 + Count[s] tokens: what lies behind is left as it is, for the next call to write over.  A page's scale grows
  * where a token comes from a page of larger scale and needs it; earlier tokens are rounded again as in wdh_cache_append.  Count beyond
- * the rows is cut, below 0 nothing is kept; a place of the path that goes down or out of the rows, or lies on a page outside the cache, leaves
- * its slot as it is.  A sequence's pages from `past` on must be its own. */
+ * the rows is cut, below 0 nothing is kept; where the path's place i is below i or out of the rows, or lies on a page outside the cache,
+ * the slot stays as it is.  A sequence's pages from `past` on must be its own. */
 int wdh_cache_keep(wdh_buf KPages, wdh_buf KScales, wdh_buf VPages, wdh_buf VScales, wdh_buf Table, wdh_buf Lens, wdh_buf Starts,
                    wdh_buf Path, wdh_buf Count, int seqs, int tokens, int kv_heads, int d, int pages, int max_pages);
 

@@ -308,7 +308,7 @@ void launch_few(const ProductParams &p, bool aligned) {
 // last eight of them, on both sides alike).  A slab is multiplied by quarters, the next one's fragments on their way from LDS
 // meanwhile (8192^3: 1032 to 1080 us from run to run, 1018 to 1065 TFLOP/s; fragments of the whole slab at a time 1146).
 // Bound: the matrix cores, the conversions and the way through LDS alternate more than they overlap (without the loads of slabs that
-// product takes 890 us, without their way into LDS either 800; library products of bfloat16 operands of that size take 954).
+// product takes 890 us, without their way into LDS either 800; library products of bfloat16 operands of that size take 890 in ten calls in a row, 776 in long runs).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <int NW, int MW, int TN, int TM>

@@ -115,7 +115,8 @@ struct Joint {
 
 // RB blocks of 32 rows to an item, WAVES / RB wavefronts to a block, which take the item's pages in turn.
 // Bound: matrix instructions, which take 50 % of the time, and what they leave half of theirs to, conversions and the softmax: 64 rows of 16 heads on 2
-// of 128 take 87 us for each 102400 tokens behind them, 1230 TFLOP/s with the second parts (a large library product has 1155).  Beside its pages an item
+// of 128 take 89 us for each 102400 tokens behind them, 1210 TFLOP/s with the second parts (a large library product has 1240 in ten calls in a row, 1417 in
+// long runs).  Pages' scales in the weights' exponents take as long as they did in the widening of values.  Beside its pages an item
 // costs a workgroup 13 us, 3.5 of them a page's instructions on their first way into the cache.  The pages' order in a workgroup is fixed, no sum
 // depends on another workgroup's time.
 template <int D, int RB, int WAVES>
@@ -657,6 +658,8 @@ int launch_rows(const char *who, AttendParams &p) {
   // More rows to an item read the cache fewer times, and are fewer and longer items.  32, 64 and 128 rows to an item (us), heads of 128, 4 of them in the cache:
   //   32 sequences behind 1500 tokens: of 32 rows 22 / 28 / 34, of 64 rows 28 / 30 / 46, of 128 rows 52 / 36 / 50, of 192 rows 93 / 73 / 60
   //   and one sequence of 512 rows, 2 heads: behind 6400 30 / 24 / 30, behind 25600 49 / 47 / 49, behind 102400 135 / 120 / 118
+  // For 33 to 64 rows, 4 heads of 128, items of 64 are the faster ones in 42 of 48 kinds of calls measured (32 / 64 rows to an item: 32 sequences behind 500 25.1 / 22.7, 64 behind
+  // 1500 57 / 43, 128 behind 700 90 / 54, one behind 25600 28 / 23); not for 32 sequences behind 1500 (27.6 / 30.6) or one of heads of 64 behind 1500 (12.9 / 14.0).
   if (rows <= 32) return launch<D, 1, D == 128 ? 8 : 4>(who, p, rows);
   const long long pages = p.q.seqs * ((rows + 127) / 128) * p.kv_heads * p.q.max_pages;  // for items of 128 rows, at most
   if (rows <= 64 || pages < 20LL * wdh::compute_units()) return launch<D, 2, 8>(who, p, rows);

@@ -2,8 +2,8 @@
 //
 // Element pairs (a, b) of the first 2 half elements, (x[j], x[j + half]) or (x[2j], x[2j + 1]), become
 //   (a cos_j - b sin_j, b cos_j + a sin_j),  cos_j and sin_j from the position's rows of two tables;
-// the elements behind them stay.  A lane needs the partners of its four elements too: where it does not hold them, they are loaded again, from cache, rather
-// than exchanged, so that pairs may lie anywhere in the head.
+// the elements behind them stay.  A lane needs the partners of its four elements too.  Where it does not hold them, they come from the lane that does, if that is a
+// bit of the lane's number away (wdh_rope alone); else they are loaded again, from cache, so that pairs may lie anywhere in the head.
 #pragma once
 #include "fp8.h"
 
