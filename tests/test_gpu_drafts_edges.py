@@ -276,3 +276,34 @@ def test_attention_in_2_norm(ctx, new, past, heads, kv, d):
     want = attention_of_trees(c, q, table, lens, starts, mask, d ** -0.5)
     got = T.attend_tree(ctx, c, q, table, lens, starts, mask, np.float32(d ** -0.5))
     assert X.relative(got, want) <= 2.0 ** -20, X.relative(got, want) * 2.0 ** 20
+
+
+# ---- shares beside the largest that float16 parts take ------------------------------------------------
+@pytest.mark.parametrize("low,high", [(-96, -92), (60, 64), (-30, -27), (-96, -91), (3, 7)])
+@pytest.mark.parametrize("seqs,new,heads,kv,d,pages", [(60, 3, 8, 4, 64, 16), (60, 3, 8, 4, 128, 16), (32, 50, 8, 8, 64, 16), (32, 32, 32, 8, 128, 24)])
+def test_shares_beside_the_largest(ctx, seqs, new, heads, kv, d, pages, low, high):
+    """Pages of scale 2^low with scores of 0, then pages of 2^high with a score s at which their shares cross 2^15 in the units that the first ones set (with
+    2^9 for their own), s a few steps of fp32 apart from row to row: whether a row changes its units hangs on how sums of s, exponents and units round, and all that
+    ask for it have to agree.  A row is the average of two averages; s is off by (3 + d / 8) 2^-23 of itself, as above, and 2^-18 is more than that and 2^-20."""
+    assert not tree_plan.form_of([new] * seqs, [64 * pages] * seqs, heads, kv, d)[1]   # (a workgroup goes through all pages of an item)
+    rng = np.random.default_rng(high - low)
+    c = F.Cache(pages + seqs, kv, d)
+    second = np.arange(pages + seqs) >= pages // 2
+    c.k[:], c.k[second, ..., 0] = 0, F.encode(1.0)
+    c.v[:] = rng.choice(F.encode(rng.standard_normal(4099) * 64), c.v.shape)
+    c.ks[:] = 1
+    c.vs[:] = np.where(second, 2.0 ** high, 2.0 ** low)[:, None]
+    table = np.concatenate([np.tile(np.arange(pages), (seqs, 1)), pages + np.arange(seqs)[:, None]], 1).astype(np.int32)
+    lens, starts = np.full(seqs, 64 * pages + new, np.int32), (new * np.arange(seqs + 1)).astype(np.int32)
+    target = 15 - (9 + high - low)                                            # of s, a power of two's exponent
+    q = np.zeros((seqs * new, heads, d), np.float32)
+    steps = np.arange(seqs * new * heads).reshape(seqs * new, heads) % 128 - 64
+    q[:, :, 0] = target / np.log2(np.e) * (1 + steps * 2.0 ** -23)
+    s = q[:, :, 0].astype(np.float64) * np.log2(np.e)
+    assert s.min() < target < s.max()
+    values = np.repeat(np.moveaxis(F.decode(c.v[:pages]), 3, 2), heads // kv, 1)   # [pages, heads, tokens, d]
+    first, rest = (values[part].mean((0, 2)) * scale for part, scale in ((slice(0, pages // 2), 2.0 ** low), (slice(pages // 2, None), 2.0 ** high)))
+    weight = (2.0 ** s / (1 + 2.0 ** s))[:, :, None]
+    want = (1 - weight) * first + weight * rest
+    got = T.attend_tree(ctx, c, q, table, lens, starts, np.zeros((seqs * new, 2), np.int32), 1.0)
+    assert X.relative(got, want) <= 2.0 ** -18, X.relative(got, want) * 2.0 ** 20

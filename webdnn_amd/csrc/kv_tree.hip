@@ -387,14 +387,15 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void attend_tree(AttendParam
       }
       float above = most + ref;
       shift = fmaxf(ve + lift, LEAST_SHIFT);
-      if (!__any(above > MOST_WEIGHT || above + shift > MOST)) break;
+      if (again || !__any(above > MOST_WEIGHT || above + shift > MOST)) break;
+      again = true;
       float to = ref, by = lift;
       if (above > MOST_WEIGHT) {  // (o's units stay)
         to = -ceilf(most);
         by += ref - to;
         above = most + to;
       }
-      if (above + ve + by > MOST) by = AIM - ceilf(above) - ve;
+      if (above + fmaxf(ve + by, LEAST_SHIFT) > MOST) by = AIM - ceilf(above) - ve;
       const float scaled = __builtin_amdgcn_exp2f((to - ref) + (by - lift));
       sum *= __builtin_amdgcn_exp2f(to - ref);
       ref = to;
